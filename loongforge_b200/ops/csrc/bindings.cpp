@@ -10,6 +10,7 @@
 #include <cstdint>
 #include "elementwise.h"
 #include "gemm_sm100.h"
+#include "linear_attn.h"
 #include "wait_budget.h"
 #ifdef LF_HAVE_ATTN
 #include "attention_sm100.h"
@@ -945,6 +946,440 @@ void indexer_topk(const at::Tensor& q, const at::Tensor& k, const at::Tensor& w,
 }
 #endif  // LF_HAVE_DSA
 
+// ------------------------------------------------------------------------------------------------ linear attention
+
+// [rows, heads, d] with unit inner stride and 16-byte rows, as the linear-attention kernels read their inputs.
+void check_heads(const at::Tensor& t, const char* name, const at::Tensor& like) {
+  check_bf16_cuda(t, name);
+  TORCH_CHECK(t.dim() == 3 && t.device() == like.device(), name, " must be [rows, heads, dim] on one device with the others");
+  TORCH_CHECK(t.size(0) == like.size(0), name, " must have as many rows as q");
+  TORCH_CHECK(t.numel() == 0 || (t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+                                 reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0),
+              name, " must have a unit inner stride and 16-byte aligned rows");
+}
+
+void check_gate(const at::Tensor& t, const char* name, const at::Tensor& v) {
+  TORCH_CHECK(t.is_cuda() && t.device() == v.device() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.dim() == 2 &&
+                  t.size(0) == v.size(0) && t.size(1) == v.size(1),
+              name, " must be contiguous fp32 [rows, value heads] on v's device");
+}
+
+void check_state(const at::Tensor& t, const char* name, int64_t N, const at::Tensor& q, const at::Tensor& v) {
+  TORCH_CHECK(t.is_cuda() && t.device() == v.device() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.dim() == 4 &&
+                  (N < 0 || t.size(0) == N) && t.size(1) == v.size(1) && t.size(2) == q.size(2) && t.size(3) == v.size(2) &&
+                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              name, " must be contiguous fp32 [sequences, value heads, dk, dv] on v's device, 16-byte aligned");
+}
+
+void check_status(const at::Tensor& status, const at::Tensor& like) {
+  TORCH_CHECK(status.is_cuda() && status.device() == like.device() && status.scalar_type() == at::kInt && status.numel() >= 1,
+              "status must be an int32 word on the inputs' device");
+}
+
+// Row boundaries as the kernels use them (clamped to [0, T], non-decreasing) and every sequence's first chunk.
+std::vector<at::Tensor> delta_plan(const at::Tensor& cu, int64_t T, const at::Tensor& status) {
+  TORCH_CHECK(cu.is_cuda() && cu.scalar_type() == at::kInt && cu.is_contiguous() && cu.dim() == 1 && cu.numel() >= 2,
+              "cu_seqlens must be contiguous int32 [sequences + 1]");
+  TORCH_CHECK(T <= INT32_MAX && cu.numel() <= (1 << 30), "more than 2^31 - 1 tokens");
+  check_status(status, cu);
+  c10::cuda::CUDAGuard guard(cu.device());
+  at::Tensor bounds = at::empty_like(cu), first = at::empty_like(cu);
+  const int rc = lf::delta_plan(cu.data_ptr<int>(), static_cast<int>(cu.numel() - 1), T, bounds.data_ptr<int>(),
+                                first.data_ptr<int>(), status.data_ptr<int>(), cur_stream());
+  TORCH_CHECK(rc == 0, "lf::delta_plan failed with code ", rc);
+  ++g_launches;
+  return {bounds, first};
+}
+
+lf::DeltaArgs delta_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, const at::Tensor& beta,
+                         const c10::optional<at::Tensor>& bounds, const c10::optional<at::Tensor>& first, double scale, bool l2norm) {
+  check_heads(q, "q", q);
+  check_heads(k, "k", q);
+  check_heads(v, "v", q);
+  TORCH_CHECK(q.size(1) == k.size(1) && q.size(2) == k.size(2), "q and k must have the same heads");
+  TORCH_CHECK(q.size(1) > 0 && v.size(1) > 0 && v.size(1) % q.size(1) == 0, "the value heads must be a multiple of the key heads");
+  check_gate(g, "g", v);
+  check_gate(beta, "beta", v);
+  TORCH_CHECK(q.size(0) <= INT32_MAX, "more than 2^31 - 1 tokens");
+  lf::DeltaArgs a;
+  a.q = q.data_ptr(); a.q_ts = q.stride(0); a.q_hs = q.stride(1);
+  a.k = k.data_ptr(); a.k_ts = k.stride(0); a.k_hs = k.stride(1);
+  a.v = v.data_ptr(); a.v_ts = v.stride(0); a.v_hs = v.stride(1);
+  a.g = g.data_ptr<float>();
+  a.beta = beta.data_ptr<float>();
+  a.T = q.size(0);
+  a.Hk = static_cast<int>(q.size(1));
+  a.Hv = static_cast<int>(v.size(1));
+  a.dk = static_cast<int>(q.size(2));
+  a.dv = static_cast<int>(v.size(2));
+  a.scale = static_cast<float>(scale);
+  a.l2norm = l2norm ? 1 : 0;
+  a.NC = (a.T + lf::DELTA_CHUNK - 1) / lf::DELTA_CHUNK;
+  TORCH_CHECK(bounds.has_value() == first.has_value());
+  if (bounds.has_value()) {
+    TORCH_CHECK(bounds->is_cuda() && bounds->device() == q.device() && first->device() == q.device() && bounds->scalar_type() == at::kInt &&
+                    first->scalar_type() == at::kInt && bounds->is_contiguous() && first->is_contiguous() &&
+                    bounds->numel() >= 2 && bounds->numel() == first->numel(), "bad sequence plan");
+    a.cu = bounds->data_ptr<int>();
+    a.cbase = first->data_ptr<int>();
+    a.N = static_cast<int>(bounds->numel() - 1);
+    a.NC = a.T / lf::DELTA_CHUNK + a.N;  // sum of the sequences' chunk counts is at most this
+  }
+  return a;
+}
+
+// {o, final state or empty}, and with `keep` what the backward pass reads: {past, memory, its remainder, U, its remainder,
+// chunk states, A / P, factors} (see DeltaArgs).
+std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
+                                  const at::Tensor& beta, c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first,
+                                  double scale, bool l2norm, c10::optional<at::Tensor> s_in, bool want_state, bool keep) {
+  c10::cuda::CUDAGuard guard(q.device());
+  lf::DeltaArgs a = delta_args(q, k, v, g, beta, bounds, first, scale, l2norm);
+  auto bf = v.options(), fl = g.options();
+  at::Tensor o = at::empty({a.T, a.Hv, a.dv}, bf);
+  at::Tensor s_out = want_state ? at::empty({a.N, a.Hv, a.dk, a.dv}, fl) : at::empty({0}, fl);
+  at::Tensor ap = at::empty({a.NC, a.Hv, lf::DELTA_AP}, bf), vec = at::empty({a.NC, a.Hv, lf::DELTA_VEC}, fl);
+  a.o = o.data_ptr();
+  a.ap = ap.data_ptr();
+  a.vec = vec.data_ptr<float>();
+  if (s_in.has_value()) {
+    check_state(*s_in, "initial_state", a.N, q, v);
+    a.s_in = s_in->data_ptr<float>();
+  }
+  if (want_state) a.s_out = s_out.data_ptr<float>();
+  std::vector<at::Tensor> out = {o, s_out};
+  if (keep) {
+    at::Tensor past = at::empty({a.T, a.Hv, a.dv}, fl);
+    at::Tensor mem = at::empty_like(o), mem_lo = at::empty_like(o), u = at::empty_like(o), u_lo = at::empty_like(o);
+    at::Tensor states = at::empty({a.NC, a.Hv, 2, a.dv, a.dk}, bf);
+    a.past = past.data_ptr<float>();
+    a.mem = mem.data_ptr();
+    a.mem_lo = mem_lo.data_ptr();
+    a.u = u.data_ptr();
+    a.u_lo = u_lo.data_ptr();
+    a.states = states.data_ptr();
+    out.insert(out.end(), {past, mem, mem_lo, u, u_lo, states, ap, vec});
+  }
+  const int rc = lf::delta_forward(a, cur_stream());
+  TORCH_CHECK(rc == 0, "lf::delta_forward failed with code ", rc, " (dk = ", a.dk, ", dv = ", a.dv, ")");
+  g_launches += a.NC > 0 ? 2 : 1;
+  if (a.cu) {
+    lf::ZeroRows z;
+    z.n = 1;
+    z.p[0] = a.o;
+    z.row_bytes[0] = 2LL * a.Hv * a.dv;
+    lf::delta_zero_uncovered(z, a.cu, a.N, a.T, cur_stream());
+    ++g_launches;
+  }
+  return out;
+}
+
+// {dq, dk, dv, dg, dbeta, gradient of the initial state or empty}
+std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tensor> ds_out, const at::Tensor& q, const at::Tensor& k,
+                                  const at::Tensor& v, const at::Tensor& g, const at::Tensor& beta,
+                                  c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first, double scale, bool l2norm,
+                                  bool want_ds, const at::Tensor& past, const at::Tensor& mem, const at::Tensor& mem_lo,
+                                  const at::Tensor& u, const at::Tensor& u_lo, const at::Tensor& states, const at::Tensor& ap,
+                                  const at::Tensor& vec) {
+  c10::cuda::CUDAGuard guard(q.device());
+  lf::DeltaArgs a = delta_args(q, k, v, g, beta, bounds, first, scale, l2norm);
+  check_heads(dout, "dout", q);
+  for (const at::Tensor* t : {&dout, &mem, &mem_lo, &u, &u_lo})
+    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kBFloat16 && t->is_contiguous() &&
+                    t->numel() == a.T * a.Hv * a.dv, "the outputs' gradient must be contiguous bf16 [T, value heads, dv]");
+  TORCH_CHECK(past.device() == q.device() && past.scalar_type() == at::kFloat && past.is_contiguous() && past.numel() == a.T * a.Hv * a.dv);
+  TORCH_CHECK(states.device() == q.device() && states.scalar_type() == at::kBFloat16 && states.numel() == a.NC * a.Hv * 2 * a.dk * a.dv &&
+              ap.scalar_type() == at::kBFloat16 && ap.numel() == a.NC * a.Hv * lf::DELTA_AP && vec.scalar_type() == at::kFloat &&
+              vec.numel() == a.NC * a.Hv * lf::DELTA_VEC, "what the forward pass kept does not fit these inputs");
+  auto bf = v.options(), fl = g.options();
+  at::Tensor dq = at::empty(q.sizes(), bf), dk = at::empty(k.sizes(), bf), dv = at::empty(v.sizes(), bf);
+  at::Tensor dg = at::empty_like(g), dbeta = at::empty_like(beta);
+  at::Tensor ds_in = want_ds ? at::empty({a.N, a.Hv, a.dk, a.dv}, fl) : at::empty({0}, fl);
+  at::Tensor dstates = at::empty({a.NC, a.Hv, a.dv, a.dk}, bf);
+  at::Tensor rowdots = at::empty({a.NC, a.Hv, a.dv / 16, 3, 64}, fl), sdots = at::empty({a.NC, a.Hv, a.dv / 16}, fl);
+  a.dout = dout.data_ptr();
+  if (ds_out.has_value()) {
+    check_state(*ds_out, "the final state's gradient", a.N, q, v);
+    a.ds_out = ds_out->data_ptr<float>();
+  }
+  if (want_ds) a.ds_in = ds_in.data_ptr<float>();
+  a.past = past.data_ptr<float>();
+  a.mem = mem.data_ptr();
+  a.mem_lo = mem_lo.data_ptr();
+  a.u = u.data_ptr();
+  a.u_lo = u_lo.data_ptr();
+  a.states = states.data_ptr();
+  a.ap = ap.data_ptr();
+  a.vec = vec.data_ptr<float>();
+  a.dstates = dstates.data_ptr();
+  a.rowdots = rowdots.data_ptr<float>();
+  a.sdots = sdots.data_ptr<float>();
+  a.dq = dq.data_ptr();
+  a.dkey = dk.data_ptr();
+  a.dv_ = dv.data_ptr();
+  a.dg = dg.data_ptr<float>();
+  a.dbeta = dbeta.data_ptr<float>();
+  const int rc = lf::delta_backward(a, cur_stream());
+  TORCH_CHECK(rc == 0, "lf::delta_backward failed with code ", rc, " (dk = ", a.dk, ", dv = ", a.dv, ")");
+  g_launches += a.NC > 0 ? 3 : 1;
+  if (a.cu) {
+    lf::ZeroRows z;
+    z.n = 5;
+    void* p[5] = {a.dq, a.dkey, a.dv_, a.dg, a.dbeta};
+    const long long b[5] = {2LL * a.Hk * a.dk, 2LL * a.Hk * a.dk, 2LL * a.Hv * a.dv, 4LL * a.Hv, 4LL * a.Hv};
+    for (int i = 0; i < 5; ++i) {
+      z.p[i] = p[i];
+      z.row_bytes[i] = b[i];
+    }
+    lf::delta_zero_uncovered(z, a.cu, a.N, a.T, cur_stream());
+    ++g_launches;
+  }
+  return {dq, dk, dv, dg, dbeta, ds_in};
+}
+
+// One token per row; `state` [slots, value heads, dk, dv] is updated in place.
+at::Tensor delta_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g, const at::Tensor& beta,
+                      at::Tensor state, c10::optional<at::Tensor> index, double scale, bool l2norm, const at::Tensor& status) {
+  c10::cuda::CUDAGuard guard(q.device());
+  const lf::DeltaArgs d = delta_args(q, k, v, g, beta, c10::nullopt, c10::nullopt, scale, l2norm);
+  check_state(state, "state", -1, q, v);
+  check_status(status, q);
+  lf::DeltaStepArgs a;
+  a.q = d.q; a.q_ts = d.q_ts; a.q_hs = d.q_hs;
+  a.k = d.k; a.k_ts = d.k_ts; a.k_hs = d.k_hs;
+  a.v = d.v; a.v_ts = d.v_ts; a.v_hs = d.v_hs;
+  a.g = d.g;
+  a.beta = d.beta;
+  a.state = state.data_ptr<float>();
+  a.slots = state.size(0);
+  a.B = static_cast<int>(d.T);
+  a.Hk = d.Hk; a.Hv = d.Hv; a.dk = d.dk; a.dv = d.dv;
+  a.scale = d.scale;
+  a.l2norm = d.l2norm;
+  a.status = status.data_ptr<int>();
+  if (index.has_value()) {
+    TORCH_CHECK(index->is_cuda() && index->device() == q.device() && index->scalar_type() == at::kInt && index->is_contiguous() &&
+                    index->numel() == a.B, "state_indices must be contiguous int32 [rows]");
+    a.index = index->data_ptr<int>();
+  } else {
+    TORCH_CHECK(a.slots >= a.B, "state has fewer slots than there are rows");
+  }
+  at::Tensor o = at::empty({d.T, d.Hv, d.dv}, v.options());
+  a.o = o.data_ptr();
+  const int rc = lf::delta_step(a, cur_stream());
+  TORCH_CHECK(rc == 0, "lf::delta_step failed with code ", rc, " (dk = ", a.dk, ", dv = ", a.dv, ")");
+  ++g_launches;
+  return o;
+}
+
+lf::ConvArgs conv_args(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias,
+                       const c10::optional<at::Tensor>& cu, bool silu) {
+  check_bf16_cuda(x, "x");
+  check_bf16_cuda(w, "weight");
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && w.size(0) == x.size(1) && w.device() == x.device() && w.is_contiguous(),
+              "weight must be contiguous [channels, taps] on x's device");
+  TORCH_CHECK(x.numel() == 0 || (x.stride(1) == 1 && x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0),
+              "x must have a unit inner stride and 16-byte aligned rows");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0, "weight must be 16-byte aligned");
+  lf::ConvArgs a;
+  a.x = x.data_ptr();
+  a.x_ts = x.stride(0);
+  a.w = w.data_ptr();
+  a.T = x.size(0);
+  a.C = static_cast<int>(x.size(1));
+  a.K = static_cast<int>(w.size(1));
+  a.silu = silu ? 1 : 0;
+  if (bias.has_value()) {
+    check_bf16_cuda(*bias, "bias");
+    TORCH_CHECK(bias->numel() == a.C && bias->is_contiguous() && bias->device() == x.device(), "bias must be contiguous [channels]");
+    a.bias = bias->data_ptr();
+  }
+  if (cu.has_value()) {
+    TORCH_CHECK(cu->is_cuda() && cu->device() == x.device() && cu->scalar_type() == at::kInt && cu->is_contiguous() && cu->numel() >= 2,
+                "bad sequence boundaries");
+    a.cu = cu->data_ptr<int>();
+    a.N = static_cast<int>(cu->numel() - 1);
+  }
+  return a;
+}
+
+at::Tensor conv1d_fwd(const at::Tensor& x, const at::Tensor& w, c10::optional<at::Tensor> bias, c10::optional<at::Tensor> cu, bool silu) {
+  c10::cuda::CUDAGuard guard(x.device());
+  lf::ConvArgs a = conv_args(x, w, bias, cu, silu);
+  at::Tensor y = at::empty({a.T, a.C}, x.options());
+  a.y = y.data_ptr();
+  const int rc = lf::conv_fwd(a, cur_stream());
+  TORCH_CHECK(rc == 0, "lf::conv_fwd failed with code ", rc);
+  ++g_launches;
+  return y;
+}
+
+// {dx, dweight, dbias or empty}
+std::vector<at::Tensor> conv1d_bwd(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& w, c10::optional<at::Tensor> bias,
+                                   c10::optional<at::Tensor> cu, bool silu) {
+  c10::cuda::CUDAGuard guard(x.device());
+  lf::ConvArgs a = conv_args(x, w, bias, cu, silu);
+  check_bf16_cuda(dy, "dy");
+  TORCH_CHECK(dy.is_contiguous() && dy.dim() == 2 && dy.size(0) == a.T && dy.size(1) == a.C && dy.device() == x.device() &&
+                  reinterpret_cast<uintptr_t>(dy.data_ptr()) % 16 == 0, "dy must match y");
+  at::Tensor dx = at::empty({a.T, a.C}, x.options()), dw = at::empty_like(w), db = at::empty({bias.has_value() ? a.C : 0}, w.options());
+  at::Tensor partial = at::empty({lf::conv_blocks(a.T, a.C), a.K + 1, a.C}, x.options().dtype(at::kFloat));
+  a.dy = dy.data_ptr();
+  a.dx = dx.data_ptr();
+  a.partial = partial.data_ptr<float>();
+  a.dw = dw.data_ptr();
+  a.db = bias.has_value() ? db.data_ptr() : nullptr;
+  const int rc = lf::conv_bwd(a, cur_stream());
+  TORCH_CHECK(rc == 0, "lf::conv_bwd failed with code ", rc);
+  g_launches += 2;
+  return {dx, dw, db};
+}
+
+// One token per row; `state` [slots, channels, taps - 1] is shifted in place.
+at::Tensor conv1d_step(const at::Tensor& x, at::Tensor state, const at::Tensor& w, c10::optional<at::Tensor> bias,
+                       c10::optional<at::Tensor> index, bool silu, const at::Tensor& status) {
+  c10::cuda::CUDAGuard guard(x.device());
+  const lf::ConvArgs c = conv_args(x, w, bias, c10::nullopt, silu);
+  check_status(status, x);
+  TORCH_CHECK(state.is_cuda() && state.device() == x.device() && state.scalar_type() == at::kBFloat16 && state.is_contiguous() &&
+                  state.dim() == 3 && state.size(1) == c.C && state.size(2) == c.K - 1 &&
+                  reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0,
+              "state must be contiguous bf16 [slots, channels, taps - 1] on x's device");
+  TORCH_CHECK(c.T <= INT32_MAX);
+  lf::ConvStepArgs a;
+  a.x = c.x; a.x_ts = c.x_ts; a.w = c.w; a.bias = c.bias;
+  a.state = state.data_ptr();
+  a.slots = state.size(0);
+  a.B = static_cast<int>(c.T);
+  a.C = c.C; a.K = c.K; a.silu = c.silu;
+  a.status = status.data_ptr<int>();
+  if (index.has_value()) {
+    TORCH_CHECK(index->is_cuda() && index->device() == x.device() && index->scalar_type() == at::kInt && index->is_contiguous() &&
+                    index->numel() == a.B, "state_indices must be contiguous int32 [rows]");
+    a.index = index->data_ptr<int>();
+  } else {
+    TORCH_CHECK(a.slots >= a.B, "state has fewer slots than there are rows");
+  }
+  at::Tensor y = at::empty({a.B, a.C}, x.options());
+  a.y = y.data_ptr();
+  const int rc = lf::conv_step(a, cur_stream());
+  TORCH_CHECK(rc == 0, "lf::conv_step failed with code ", rc);
+  ++g_launches;
+  return y;
+}
+
+// ------------------------------------------------------------------------- per-head norm + rotation of queries and keys
+
+lf::QkNormRopeArgs qk_args(const at::Tensor& x, int64_t G, int64_t R, bool gated, const at::Tensor& qw, const at::Tensor& kw,
+                           const c10::optional<at::Tensor>& freqs, const c10::optional<at::Tensor>& inv_freq,
+                           const c10::optional<at::Tensor>& pos, const c10::optional<at::Tensor>& axis, int64_t rot_dim, bool interleaved,
+                           double mscale, double eps, double w_offset, const at::Tensor& status) {
+  check_bf16_cuda(x, "qkv");
+  check_bf16_cuda(qw, "q_weight");
+  check_bf16_cuda(kw, "k_weight");
+  check_status(status, x);
+  lf::QkNormRopeArgs a;
+  a.G = static_cast<int>(G);
+  a.R = static_cast<int>(R);
+  a.P = static_cast<int>(gated ? 2 * R + 2 : R + 2);
+  TORCH_CHECK(x.dim() == 2 && G > 0 && R > 0 && x.size(1) % (G * a.P) == 0, "qkv must be [T, groups * heads of a group * D]");
+  a.D = static_cast<int>(x.size(1) / (G * a.P));
+  TORCH_CHECK(a.D == 64 || a.D == 128 || a.D == 256, "qk_norm_rope: head dim ", a.D, " is not covered");
+  TORCH_CHECK(x.stride(1) == 1 && x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0,
+              "qkv must have a unit inner stride and 16-byte aligned rows");
+  for (const at::Tensor* w : {&qw, &kw})
+    TORCH_CHECK(w->numel() == a.D && w->is_contiguous() && w->device() == x.device() &&
+                    reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0, "norm weights must be contiguous [D], 16-byte aligned");
+  const int64_t half = rot_dim / 2;
+  TORCH_CHECK(rot_dim > 0 && rot_dim <= a.D && (interleaved ? rot_dim % 8 == 0 : rot_dim % 16 == 0),
+              "qk_norm_rope: rot_dim ", rot_dim, " is not covered");
+  TORCH_CHECK(freqs.has_value() != inv_freq.has_value(), "give either freqs or inv_freq");
+  a.x = x.data_ptr();
+  a.x_ts = x.stride(0);
+  a.T = x.size(0);
+  a.rot_dim = static_cast<int>(rot_dim);
+  a.interleaved = interleaved ? 1 : 0;
+  a.qw = qw.data_ptr();
+  a.kw = kw.data_ptr();
+  auto words = [&](const at::Tensor& t, at::ScalarType ty, const char* name) {
+    TORCH_CHECK(t.is_cuda() && t.device() == x.device() && t.scalar_type() == ty && t.is_contiguous(), name, " has a wrong type, device or layout");
+  };
+  if (pos.has_value()) {
+    words(*pos, at::kInt, "pos_ids");
+    a.pos = pos->data_ptr<int>();
+  }
+  if (freqs.has_value()) {
+    words(*freqs, at::kFloat, "freqs");
+    TORCH_CHECK(freqs->dim() == 2 && freqs->size(1) == half, "freqs must be [positions, rot_dim / 2]");
+    TORCH_CHECK(pos.has_value() ? pos->numel() == a.T : freqs->size(0) >= a.T, "freqs or pos_ids do not cover the tokens");
+    a.freqs = freqs->data_ptr<float>();
+    a.freq_rows = freqs->size(0);
+  } else {
+    words(*inv_freq, at::kFloat, "inv_freq");
+    TORCH_CHECK(inv_freq->numel() == half, "inv_freq must be [rot_dim / 2]");
+    TORCH_CHECK(pos.has_value() && (pos->dim() == 1 || pos->dim() == 2) && pos->size(-1) == a.T, "pos_ids must be [T] or [axes, T]");
+    a.inv_freq = inv_freq->data_ptr<float>();
+    a.axes = pos->dim() == 2 ? static_cast<int>(pos->size(0)) : 1;
+    TORCH_CHECK(a.axes >= 1 && (a.axes == 1 || axis.has_value()), "several position axes need `axis`");
+    if (axis.has_value()) {
+      words(*axis, at::kInt, "axis");
+      TORCH_CHECK(axis->numel() == half, "axis must be [rot_dim / 2]");
+      a.axis = axis->data_ptr<int>();
+    }
+  }
+  a.eps = static_cast<float>(eps);
+  a.w_offset = static_cast<float>(w_offset);
+  a.mscale = static_cast<float>(mscale);
+  a.status = status.data_ptr<int>();
+  return a;
+}
+
+std::vector<at::Tensor> qk_norm_rope_fwd(const at::Tensor& x, int64_t G, int64_t R, bool gated, const at::Tensor& qw, const at::Tensor& kw,
+                                         c10::optional<at::Tensor> freqs, c10::optional<at::Tensor> inv_freq, c10::optional<at::Tensor> pos,
+                                         c10::optional<at::Tensor> axis, int64_t rot_dim, bool interleaved, double mscale, double eps,
+                                         double w_offset, const at::Tensor& status) {
+  c10::cuda::CUDAGuard guard(x.device());
+  lf::QkNormRopeArgs a = qk_args(x, G, R, gated, qw, kw, freqs, inv_freq, pos, axis, rot_dim, interleaved, mscale, eps, w_offset, status);
+  at::Tensor q = at::empty({a.T, G * R, a.D}, x.options()), k = at::empty({a.T, G, a.D}, x.options());
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  const int rc = lf::qk_norm_rope_fwd(a, cur_stream());
+  TORCH_CHECK(rc == 0, "lf::qk_norm_rope_fwd failed with code ", rc);
+  ++g_launches;
+  return {q, k};
+}
+
+// {gradient of the packed row, of q_weight, of k_weight}
+std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const at::Tensor& dk, const at::Tensor& dv, c10::optional<at::Tensor> dgate,
+                                         const at::Tensor& x, int64_t G, int64_t R, bool gated, const at::Tensor& qw, const at::Tensor& kw,
+                                         c10::optional<at::Tensor> freqs, c10::optional<at::Tensor> inv_freq, c10::optional<at::Tensor> pos,
+                                         c10::optional<at::Tensor> axis, int64_t rot_dim, bool interleaved, double mscale, double eps,
+                                         double w_offset, const at::Tensor& status) {
+  c10::cuda::CUDAGuard guard(x.device());
+  lf::QkNormRopeArgs a = qk_args(x, G, R, gated, qw, kw, freqs, inv_freq, pos, axis, rot_dim, interleaved, mscale, eps, w_offset, status);
+  TORCH_CHECK(gated == dgate.has_value());
+  auto grad = [&](const at::Tensor& t, int64_t n, const char* name) {
+    check_bf16_cuda(t, name);
+    TORCH_CHECK(t.device() == x.device() && t.is_contiguous() && t.numel() == n && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+                name, " must be contiguous and match its output");
+    return t.data_ptr();
+  };
+  a.dq = grad(dq, a.T * G * R * a.D, "dq");
+  a.dk = grad(dk, a.T * G * a.D, "dk");
+  a.dv = grad(dv, a.T * G * a.D, "dv");
+  if (gated) a.dgate = grad(*dgate, a.T * G * R * a.D, "dgate");
+  at::Tensor dx = at::empty({a.T, x.size(1)}, x.options()), dqw = at::empty_like(qw), dkw = at::empty_like(kw);
+  at::Tensor partial = at::empty({lf::qk_norm_rope_bwd_grid(a.T), 2, a.D}, x.options().dtype(at::kFloat));
+  a.dx = dx.data_ptr();
+  a.partial = partial.data_ptr<float>();
+  a.dqw = dqw.data_ptr();
+  a.dkw = dkw.data_ptr();
+  const int rc = lf::qk_norm_rope_bwd(a, cur_stream());
+  TORCH_CHECK(rc == 0, "lf::qk_norm_rope_bwd failed with code ", rc);
+  g_launches += 2;
+  return {dx, dqw, dkw};
+}
+
 // Budget of the device-side waits on flags written by other GPUs, in milliseconds (see wait_budget.h).
 void set_peer_wait_budget_ms(double ms) { lf::set_peer_wait_budget_ms(ms); }
 double peer_wait_budget_ms() { return lf::peer_wait_budget_ms(); }
@@ -1002,6 +1437,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sparse_mla_probs", &sparse_mla_probs);
   m.def("indexer_topk", &indexer_topk);
 #endif
+  m.def("delta_plan", &delta_plan);
+  m.def("delta_fwd", &delta_fwd);
+  m.def("delta_bwd", &delta_bwd);
+  m.def("delta_step", &delta_step);
+  m.def("conv1d_fwd", &conv1d_fwd);
+  m.def("conv1d_bwd", &conv1d_bwd);
+  m.def("conv1d_step", &conv1d_step);
+  m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd);
+  m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd);
   m.def("router_fwd", &router_fwd);
   m.def("router_bwd", &router_bwd);
   m.def("set_peer_wait_budget_ms", &set_peer_wait_budget_ms);

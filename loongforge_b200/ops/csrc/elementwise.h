@@ -35,6 +35,28 @@ void master_join(const void* w, const void* lo, float* master, long long n, cuda
 int sumsq_partials(long long n);
 void sumsq(const void* x, int is_bf16, long long n, float* out, float* partial, cudaStream_t s);
 
+// Per-head RMS norm of queries and keys with the rotation in the same pass (qk_norm_rope.cu). Heads of a group lie as
+// [R query heads | R gate heads if P = 2 R + 2 | key | value] in the packed row.
+struct QkNormRopeArgs {
+  const void* x = nullptr;  // bf16 [T, G * P * D], row stride x_ts
+  long long x_ts = 0, T = 0, freq_rows = 0;
+  int G = 0, R = 0, P = 0, D = 0, rot_dim = 0, interleaved = 0, axes = 1;
+  const void *qw = nullptr, *kw = nullptr;  // bf16 [D]
+  const float* freqs = nullptr;     // [freq_rows, rot_dim / 2] angles; token t takes row pos[t] (or t)
+  const float* inv_freq = nullptr;  // or [rot_dim / 2]: angle = pos[axis[i], t] * inv_freq[i]
+  const int *pos = nullptr, *axis = nullptr;
+  float eps = 0.f, w_offset = 0.f, mscale = 1.f;
+  void *q = nullptr, *k = nullptr;  // bf16 [T, G * R, D], [T, G, D]
+  const void *dq = nullptr, *dk = nullptr, *dv = nullptr, *dgate = nullptr;
+  void* dx = nullptr;          // bf16 [T, G * P * D]
+  float* partial = nullptr;    // fp32 [qk_norm_rope_bwd_grid(T), 2, D]
+  void *dqw = nullptr, *dkw = nullptr;  // bf16 [D]
+  int* status = nullptr;
+};
+int qk_norm_rope_bwd_grid(long long T);
+int qk_norm_rope_fwd(const QkNormRopeArgs& a, cudaStream_t s);  // 0, or negative for shapes that are not covered
+int qk_norm_rope_bwd(const QkNormRopeArgs& a, cudaStream_t s);
+
 // MoE router (router.cu). score: 0 softmax over the selected k, 1 softmax over all experts then top-k, 2 sigmoid.
 struct RouterArgs {
   const void* logits = nullptr;  // [T, E] fp32 or bf16

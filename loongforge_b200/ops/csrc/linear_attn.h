@@ -1,0 +1,100 @@
+// Host launchers of the linear-attention kernels: the gated delta rule (gated_delta_sm100.cu, gated_delta_step.cu)
+// and the depthwise causal convolution in front of it (causal_conv.cu). Raw pointers + stream; strides in elements.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace lf {
+
+constexpr int DELTA_CHUNK = 64;      // tokens of one chunk
+constexpr int DELTA_VEC = 11 * 64;   // fp32 words of one chunk's per-token factors (see the prepare kernel)
+constexpr int DELTA_AP = 4 * 64 * 64;  // bf16 words of one chunk's inverse and score matrix (high and low parts)
+
+struct DeltaArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;  // bf16 [T, Hk, dk], [T, Hk, dk], [T, Hv, dv]
+  long long q_ts = 0, q_hs = 0, k_ts = 0, k_hs = 0, v_ts = 0, v_hs = 0;
+  const float *g = nullptr, *beta = nullptr;  // fp32 [T, Hv]
+  // Sequence plan: cu [N + 1] (clamped, non-decreasing) and first chunk of every sequence [N + 1]; null = one sequence.
+  const int *cu = nullptr, *cbase = nullptr;
+  int N = 1, Hk = 0, Hv = 0, dk = 0, dv = 0;
+  long long T = 0, NC = 0;  // NC: upper bound of the number of chunks
+  float scale = 1.f;
+  int l2norm = 1;
+  const float* s_in = nullptr;  // [N, Hv, dk, dv] or null (zero)
+  float* s_out = nullptr;       // [N, Hv, dk, dv] or null
+  void *o = nullptr;            // bf16 [T, Hv, dv]
+  // Kept for the backward pass (all or none), [T, Hv, dv]: what o owes to earlier tokens (fp32), the memory read at each
+  // token and U (bf16 with the remainder of the rounding); and the state in front of every chunk.
+  float* past = nullptr;
+  void *mem = nullptr, *mem_lo = nullptr, *u = nullptr, *u_lo = nullptr, *states = nullptr;
+  void* ap = nullptr;    // bf16 [NC, Hv, DELTA_AP]
+  float* vec = nullptr;  // fp32 [NC, Hv, DELTA_VEC]
+  // backward
+  const void* dout = nullptr;   // bf16 [T, Hv, dv], contiguous
+  const float* ds_out = nullptr;  // gradient of s_out or null
+  float* ds_in = nullptr;         // gradient of s_in or null
+  void* dstates = nullptr;      // bf16 fragments of the state gradients, half the size of `states`
+  float* rowdots = nullptr;     // fp32 [NC, Hv, dv / 16, 3, 64]
+  float* sdots = nullptr;       // fp32 [NC, Hv, dv / 16]
+  void *dq = nullptr, *dkey = nullptr, *dv_ = nullptr;  // bf16, contiguous
+  float *dg = nullptr, *dbeta = nullptr;                // fp32 [T, Hv]
+  int* status = nullptr;
+};
+
+// 0 on success; negative when the shape is not covered (dk, dv in {64, 128}).
+int delta_plan(const int* cu_in, int N, long long T, int* cu, int* cbase, int* status, cudaStream_t s);
+int delta_forward(const DeltaArgs& a, cudaStream_t s);
+int delta_backward(const DeltaArgs& a, cudaStream_t s);
+// Zeroes the rows [0, cu[0]) and [cu[N], T) of up to six row-major buffers.
+struct ZeroRows {
+  void* p[6] = {};
+  long long row_bytes[6] = {};
+  int n = 0;
+};
+void delta_zero_uncovered(const ZeroRows& z, const int* cu, int N, long long T, cudaStream_t s);
+
+struct DeltaStepArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;  // bf16 [B, Hk, dk], [B, Hk, dk], [B, Hv, dv]
+  long long q_ts = 0, q_hs = 0, k_ts = 0, k_hs = 0, v_ts = 0, v_hs = 0;
+  const float *g = nullptr, *beta = nullptr;  // [B, Hv]
+  float* state = nullptr;                     // [slots, Hv, dk, dv], updated in place
+  const int* index = nullptr;                 // [B] slot of each row, negative = no row; null = row b uses slot b
+  void* o = nullptr;                          // bf16 [B, Hv, dv]
+  int B = 0, Hk = 0, Hv = 0, dk = 0, dv = 0;
+  long long slots = 0;
+  float scale = 1.f;
+  int l2norm = 1;
+  int* status = nullptr;
+};
+int delta_step(const DeltaStepArgs& a, cudaStream_t s);
+
+struct ConvArgs {
+  const void* x = nullptr;  // bf16 [T, C], row stride x_ts
+  long long x_ts = 0;
+  const void *w = nullptr, *bias = nullptr;  // bf16 [C, K], [C] or null
+  const int* cu = nullptr;                   // [N + 1] or null
+  int N = 1, C = 0, K = 0, silu = 1;
+  long long T = 0;
+  void* y = nullptr;            // bf16 [T, C]
+  const void* dy = nullptr;     // bf16 [T, C]
+  void* dx = nullptr;           // bf16 [T, C]
+  float* partial = nullptr;     // fp32 [conv_blocks(T, C), K + 1, C]
+  void *dw = nullptr, *db = nullptr;  // bf16
+};
+int conv_blocks(long long T, int C);
+int conv_fwd(const ConvArgs& a, cudaStream_t s);
+int conv_bwd(const ConvArgs& a, cudaStream_t s);
+
+struct ConvStepArgs {
+  const void* x = nullptr;  // bf16 [B, C], row stride x_ts
+  long long x_ts = 0;
+  const void *w = nullptr, *bias = nullptr;
+  void* state = nullptr;       // bf16 [slots, C, K - 1], updated in place
+  const int* index = nullptr;  // [B] or null
+  void* y = nullptr;           // bf16 [B, C]
+  int B = 0, C = 0, K = 0, silu = 1;
+  long long slots = 0;
+  int* status = nullptr;
+};
+int conv_step(const ConvStepArgs& a, cudaStream_t s);
+
+}  // namespace lf

@@ -305,6 +305,126 @@ def rope(x: torch.Tensor, freqs: torch.Tensor, *, pos_ids: Optional[torch.Tensor
     return torch.cat([rot, xg[:, :, rope_in_group:]], dim=2).reshape(shape)
 
 
+# ----------------------------------------------------------------------------- per-head norm + RoPE of q and k
+
+
+def _rot_angles(T, freqs, inv_freq, axis, pos_ids):
+    """Angles [T, rot_dim / 2]: rows of the table, or position times frequency of each frequency's axis."""
+    if freqs is not None:
+        return freqs[:T] if pos_ids is None else freqs[pos_ids.long()]
+    pos = pos_ids if pos_ids.dim() == 2 else pos_ids[None]
+    ax = torch.zeros(inv_freq.numel(), dtype=torch.long, device=pos.device) if axis is None else axis.long()
+    return (pos.double()[ax].t() * inv_freq.double()).float()
+
+
+def qk_norm_rope_ref(qkv, groups, q_per_group, q_weight, k_weight, *, freqs=None, inv_freq=None, axis=None, pos_ids=None,
+                     rot_dim=None, interleaved=False, mscale=1.0, eps=1e-6, w_offset=0.0, gated=False):
+    """PyTorch form of `qk_norm_rope` (same arguments)."""
+    T = qkv.shape[0]
+    x = qkv.unflatten(1, (groups, 2 * q_per_group + 2 if gated else q_per_group + 2, -1))
+    D = x.shape[-1]
+    ang = _rot_angles(T, freqs, inv_freq, axis, pos_ids)
+
+    def one(t, w):
+        n = t.float()
+        n = n * torch.rsqrt(n.pow(2).mean(-1, keepdim=True) + eps) * (w.float() + w_offset)
+        return rope_ref(n, ang, D if rot_dim is None else rot_dim, 0, interleaved, mscale).to(qkv.dtype)
+
+    out = (one(x[:, :, :q_per_group].reshape(T, groups * q_per_group, D), q_weight), one(x[:, :, -2], k_weight), x[:, :, -1])
+    return out + ((x[:, :, q_per_group:2 * q_per_group],) if gated else ())
+
+
+class _QKNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, qw, kw, G, R, gated, freqs, inv_freq, pos, axis, rot_dim, interleaved, mscale, eps, w_offset):
+        ctx.cfg = (G, R, gated), (rot_dim, interleaved, mscale, eps, w_offset)
+        ctx.save_for_backward(qkv, qw, kw, freqs, inv_freq, pos, axis)
+        q, k = _C().qk_norm_rope_fwd(qkv, G, R, gated, qw, kw, freqs, inv_freq, pos, axis, *ctx.cfg[1],
+                                     _ext.status_tensor(qkv.device))
+        x = qkv.unflatten(1, (G, 2 * R + 2 if gated else R + 2, -1))
+        return (q, k, x[:, :, -1]) + ((x[:, :, R:2 * R],) if gated else ())
+
+    @staticmethod
+    def backward(ctx, *grads):
+        qkv, qw, kw, freqs, inv_freq, pos, axis = ctx.saved_tensors
+        (G, R, gated), rot = ctx.cfg
+        d = [g if g.data_ptr() % 16 == 0 else g.clone() for g in (g.contiguous() for g in grads)]
+        dx, dqw, dkw = _C().qk_norm_rope_bwd(d[0], d[1], d[2], d[3] if gated else None, qkv, G, R, gated, qw, kw, freqs,
+                                             inv_freq, pos, axis, *rot, _ext.status_tensor(qkv.device))
+        return (dx, dqw, dkw) + (None,) * 12
+
+
+def qk_norm_rope_supported(qkv, groups: int, q_per_group: int, q_weight, rot_dim: Optional[int] = None, *,
+                           interleaved: bool = False, gated: bool = False) -> bool:
+    """Whether the one-pass kernel covers this call: bf16 on a GPU, head dim 64, 128 or 256, rotated span a multiple of 16
+    (8 for interleaved pairs)."""
+    if not (qkv.is_cuda and qkv.dtype == q_weight.dtype == torch.bfloat16 and qkv.dim() == 2):
+        return False
+    heads = groups * (2 * q_per_group + 2 if gated else q_per_group + 2)
+    D = qkv.shape[1] // heads
+    r = D if rot_dim is None else rot_dim
+    return (qkv.shape[1] == heads * D and D in (64, 128, 256) and 0 < r <= D and r % (8 if interleaved else 16) == 0)
+
+
+def qk_norm_rope(qkv: torch.Tensor, groups: int, q_per_group: int, q_weight: torch.Tensor, k_weight: torch.Tensor, *,
+                 freqs: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None,
+                 axis: Optional[torch.Tensor] = None, pos_ids: Optional[torch.Tensor] = None,
+                 rot_dim: Optional[int] = None, interleaved: bool = False, mscale: float = 1.0, eps: float = 1e-6,
+                 w_offset: float = 0.0, gated: bool = False):
+    """RMSNorm of every query and key head followed by the rotary embedding, in one pass over the packed projection.
+
+    ``qkv [T, G * P * D]`` holds G groups of ``[q_0..q_{R-1}, k, v]`` heads (``gated``: ``[q.., gate_0..gate_{R-1}, k, v]``).
+    Returns ``q [T, G*R, D]``, ``k [T, G, D]``, and views of `qkv`: ``v [T, G, D]`` and, when gated, ``gate [T, G, R, D]``;
+    the gradient of the packed row is written in one pass too. Weights ``[D]``, ``y = x * rstd * (w + w_offset)``.
+
+    Angles: either ``freqs`` (fp32 ``[P, rot_dim/2]``; token t uses row ``pos_ids[t]``, or row t), or ``inv_freq``
+    (fp32 ``[rot_dim/2]``) with ``pos_ids [T]`` or ``[axes, T]`` and ``axis [rot_dim/2]`` naming each frequency's position
+    axis (time / height / width of images and video): angle i of token t is ``pos_ids[axis[i], t] * inv_freq[i]``. The
+    first `rot_dim` elements of a head rotate, pairs ``(i, i + rot_dim/2)`` or, interleaved, ``(2i, 2i + 1)``; cosine and
+    sine are scaled by `mscale`. On a GPU a table row or an axis out of range turns by zero and sets the status word.
+    """
+    if (freqs is None) == (inv_freq is None):
+        raise ValueError("qk_norm_rope: give either `freqs` or `inv_freq`")
+    heads = groups * (2 * q_per_group + 2 if gated else q_per_group + 2)
+    if qkv.dim() != 2 or heads <= 0 or qkv.shape[1] % heads:
+        raise ValueError(f"qk_norm_rope: {tuple(qkv.shape)} is not [T, {heads} heads * D]")
+    T, D = qkv.shape[0], qkv.shape[1] // heads
+    rot = D if rot_dim is None else rot_dim
+    if rot <= 0 or rot > D or rot % 2:
+        raise ValueError(f"qk_norm_rope: rot_dim {rot} of head dim {D}")
+    if q_weight.shape != (D,) or k_weight.shape != (D,):
+        raise ValueError(f"qk_norm_rope: norm weights must be [{D}]")
+    table = freqs if freqs is not None else inv_freq
+    if table.shape[-1] != rot // 2 or table.dim() != (2 if freqs is not None else 1):
+        raise ValueError(f"qk_norm_rope: {tuple(table.shape)} does not hold {rot // 2} angles per position")
+    if inv_freq is not None:
+        if pos_ids is None or pos_ids.shape[-1] != T or pos_ids.dim() not in (1, 2):
+            raise ValueError("qk_norm_rope: `inv_freq` needs pos_ids [T] or [axes, T]")
+        if axis is not None and axis.shape != (rot // 2,):
+            raise ValueError(f"qk_norm_rope: axis must be [{rot // 2}]")
+        if axis is None and pos_ids.dim() == 2 and pos_ids.shape[0] > 1:
+            raise ValueError("qk_norm_rope: several position axes need `axis`")
+    elif (pos_ids is None and freqs.shape[0] < T) or (pos_ids is not None and pos_ids.shape != (T,)):
+        raise ValueError("qk_norm_rope: freqs / pos_ids do not cover the tokens")
+    if qk_norm_rope_supported(qkv, groups, q_per_group, q_weight, rot_dim, interleaved=interleaved, gated=gated) \
+            and k_weight.dtype == torch.bfloat16:
+        dev = qkv.device
+        x = qkv if qkv.stride(1) == 1 and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0 else qkv.clone(
+            memory_format=torch.contiguous_format)
+
+        def words(t, dt):
+            return None if t is None else t.to(device=dev, dtype=dt).contiguous()
+
+        qw, kw = (w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+                  for w in (q_weight, k_weight))
+        return _QKNormRopeFn.apply(x, qw, kw, groups, q_per_group, gated, words(freqs, torch.float32),
+                                   words(inv_freq, torch.float32), words(pos_ids, torch.int32), words(axis, torch.int32),
+                                   rot, interleaved, float(mscale), float(eps), float(w_offset))
+    return qk_norm_rope_ref(qkv, groups, q_per_group, q_weight, k_weight, freqs=freqs, inv_freq=inv_freq, axis=axis,
+                            pos_ids=pos_ids, rot_dim=rot, interleaved=interleaved, mscale=mscale, eps=eps,
+                            w_offset=w_offset, gated=gated)
+
+
 # ----------------------------------------------------------------------------- SwiGLU
 
 

@@ -84,6 +84,7 @@ class RotaryEmbedding:
         inv, mscale = self._inv_freq(position_ids.device)
         ang = position_ids.float()[:, :, None] * inv[None, None, :]  # [3, T, rot/2]
         sec = cfg.mrope_section or [self.rot_dim // 2]
+        stream = torch.arange(len(sec)).repeat_interleave(torch.tensor(sec)) % 3
         if cfg.mrope_interleaved:
             idx = torch.arange(self.rot_dim // 2, device=ang.device) % 3
             limit = torch.tensor([sec[0] * 3, sec[1] * 3, sec[2] * 3], device=ang.device)
@@ -96,7 +97,13 @@ class RotaryEmbedding:
                 parts.append(ang[i % 3, :, start:start + n])
                 start += n
             mixed = torch.cat(parts, dim=-1)
-        return RotaryInputs(freqs=mixed.contiguous(), mscale=mscale)
+        out = RotaryInputs(freqs=mixed.contiguous(), mscale=mscale)
+        if stream.numel() == inv.numel():
+            out.axis_pos, out.inv_freq = position_ids.to(torch.int32).contiguous(), inv.float().contiguous()
+            if getattr(self, "_axis", None) is None or self._axis.device != inv.device:
+                self._axis = stream.to(device=inv.device, dtype=torch.int32)
+            out.axis = self._axis
+        return out
 
 
 def pipeline_layer_split(num_layers: int, pp: int, custom: Optional[Sequence[int]] = None) -> List[List[int]]:

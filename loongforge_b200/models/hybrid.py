@@ -24,7 +24,7 @@ from ..ops import linear_attn as LA
 from ..parallel import layers as PL
 from ..parallel import state as ps
 from .config import TransformerConfig
-from .transformer import Norm, PackedSeqParams, RotaryInputs, core_attention
+from .transformer import Norm, PackedSeqParams, RotaryInputs, core_attention, fused_qk, fused_qk_applies
 
 
 class GatedAttention(nn.Module):
@@ -55,9 +55,16 @@ class GatedAttention(nn.Module):
         self.rot_dim = int(self.d * cfg.rotary_percent)
 
     def forward(self, x, rotary: Optional[RotaryInputs], packed: Optional[PackedSeqParams], residual=None):
-        T = x.shape[0] * (ps.get_state().dims.tp if self.cfg.sequence_parallel else 1)
-        y = self.linear_qgkv(x).view(-1, self.ng_l, 2 * self.r + 2, self.d)
+        y = self.linear_qgkv(x)
         T = y.shape[0]
+        cu = packed.cu_seqlens if packed is not None else None
+        row_length = packed.row_length if packed is not None else None
+        if fused_qk_applies(self, y, self.ng_l, self.r, rotary, gated=True):
+            q, k, v, gate = fused_qk(self, y, self.ng_l, self.r, rotary, gated=True)
+            o = core_attention(q, k, v, causal=True, scale=self.scale, cu_seqlens=cu, cfg=self.cfg, row_length=row_length)
+            o = o.view(T, self.ng_l, self.r, self.d) * torch.sigmoid(gate.float()).to(o.dtype)
+            return self.linear_proj(o.reshape(T, self.nq_l * self.d), residual)
+        y = y.view(T, self.ng_l, 2 * self.r + 2, self.d)
         q = self.q_layernorm(y[:, :, :self.r].reshape(T, self.nq_l, self.d))
         gate = y[:, :, self.r:2 * self.r].reshape(T, self.nq_l * self.d)
         k = self.k_layernorm(y[:, :, 2 * self.r].contiguous())
@@ -69,9 +76,7 @@ class GatedAttention(nn.Module):
             if f.dim() == 3:
                 f, kw = f[:, 0], {**kw, "pos_ids": None, "interleaved": False}
             q, k = OF.rope(q, f, **kw), OF.rope(k, f, **kw)
-        cu = packed.cu_seqlens if packed is not None else None
-        o = core_attention(q, k, v, causal=True, scale=self.scale, cu_seqlens=cu, cfg=self.cfg,
-                           row_length=packed.row_length if packed is not None else None)
+        o = core_attention(q, k, v, causal=True, scale=self.scale, cu_seqlens=cu, cfg=self.cfg, row_length=row_length)
         o = o.reshape(T, self.nq_l * self.d) * torch.sigmoid(gate.float()).to(o.dtype)
         return self.linear_proj(o, residual)
 
@@ -135,34 +140,86 @@ class GatedDeltaNet(nn.Module):
                                              init_std=cfg.init_method_std / math.sqrt(2.0 * cfg.num_layers),
                                              key=key + ".out_proj", **common)
 
-    def forward(self, x, rotary=None, packed: Optional[PackedSeqParams] = None, residual=None):
+    def _project(self, x):
+        """(q | k | v convolution channels [T, C], z [T, hv, dv], b [T, hv], a [T, hv]) of this rank's heads."""
         hk, r, dk, dv = self.hk_l, self.ratio, self.dk, self.dv
         qkvz = self.in_proj_qkvz(x)
         T = qkvz.shape[0]
-        qkvz = qkvz.view(T, hk, 2 * dk + 2 * r * dv)
-        ba = self.in_proj_ba(x).view(T, hk, 2 * r)
-        q, k, v, z = qkvz.split([dk, dk, r * dv, r * dv], dim=-1)
-        b, a = ba.split([r, r], dim=-1)
-        cu = packed.cu_seqlens if packed is not None else None
+        q, k, v, z = qkvz.view(T, hk, 2 * dk + 2 * r * dv).split([dk, dk, r * dv, r * dv], dim=-1)
+        b, a = self.in_proj_ba(x).view(T, hk, 2 * r).split([r, r], dim=-1)
         # conv over [q | k | v] channels, laid out type-major like the conv weight
         mixed = torch.cat([q.reshape(T, -1), k.reshape(T, -1), v.reshape(T, -1)], dim=-1)
+        return mixed, z.reshape(T, hk * r, dv), b.reshape(T, -1), a.reshape(T, -1)
+
+    def _heads(self, mixed):
+        hk, r, dk, dv = self.hk_l, self.ratio, self.dk, self.dv
+        T = mixed.shape[0]
+        q, k, v = mixed.split([hk * dk, hk * dk, hk * r * dv], dim=-1)
+        return q.view(T, hk, dk), k.view(T, hk, dk), v.view(T, hk * r, dv)
+
+    def _gates(self, b, a):
+        beta = torch.sigmoid(b.float())
+        return -self.A_log.float().exp() * F.softplus(a.float() + self.dt_bias.float()), beta
+
+    def _finish(self, o, z, residual):
+        o = self.out_norm(o, z)
+        return self.out_proj(o.reshape(o.shape[0], -1), residual)
+
+    def forward(self, x, rotary=None, packed: Optional[PackedSeqParams] = None, residual=None):
+        mixed, z, b, a = self._project(x)
+        cu = packed.cu_seqlens if packed is not None else None
         own = None
         if self.cp > 1:
             # The convolution window and the recurrent state cross the chunk boundaries of context parallelism: run
             # both on the gathered sequence (token-wise projections stay local) and keep this rank's outputs.
             from ..parallel.context_parallel import gather_full_sequence
-            (mixed, b, a), own = gather_full_sequence([mixed, b.reshape(T, -1), a.reshape(T, -1)],
-                                                      packed.row_length if packed is not None else None)
-            T_loc, T = T, mixed.shape[0]
+            (mixed, b, a), own = gather_full_sequence([mixed, b, a], packed.row_length if packed is not None else None)
         mixed = LA.causal_conv1d(mixed, self.conv_weight, cu_seqlens=cu, activation="silu")
-        q, k, v = mixed.split([hk * dk, hk * dk, hk * r * dv], dim=-1)
-        q = q.view(T, hk, dk).repeat_interleave(r, dim=1)
-        k = k.view(T, hk, dk).repeat_interleave(r, dim=1)
-        v = v.view(T, hk * r, dv)
-        beta = torch.sigmoid(b.reshape(T, hk * r).float())
-        g = -self.A_log.float().exp() * F.softplus(a.reshape(T, hk * r).float() + self.dt_bias.float())
-        o = LA.gated_delta_rule(q, k, v, g, beta, cu_seqlens=cu, qk_l2norm=True)
+        o = LA.gated_delta_rule(*self._heads(mixed), *self._gates(b, a), cu_seqlens=cu, qk_l2norm=True)
         if own is not None:
-            o, T = o.index_select(0, own), T_loc
-        o = self.out_norm(o, z.reshape(T, hk * r, dv))
-        return self.out_proj(o.reshape(T, hk * r * dv), residual)
+            o = o.index_select(0, own)
+        return self._finish(o, z, residual)
+
+    # ------------------------------------------------------------------ decoding
+    def new_cache(self, slots: int, device=None):
+        """(convolution windows [slots, C, K - 1], states [slots, hv, dk, dv] fp32) for `slots` sequences without tokens."""
+        device = self.conv_weight.device if device is None else device
+        return (torch.zeros(slots, self.conv_weight.shape[0], self.K - 1, dtype=self.conv_weight.dtype, device=device),
+                torch.zeros(slots, self.hv_l, self.dk, self.dv, device=device))
+
+    def _check_decoding(self):
+        if self.cp > 1 or (self.cfg.sequence_parallel and ps.get_state().dims.tp > 1):
+            raise ValueError("decoding runs without context or sequence parallelism: every rank sees all rows")
+
+    @torch.no_grad()
+    def prefill(self, x, cache, slots, *, cu_seqlens=None, residual=None):
+        """`forward` over new sequences, one per entry of `slots` (bounds in `cu_seqlens`; None = one sequence); leaves
+        their windows and states in those slots of `cache`."""
+        self._check_decoding()
+        windows, states = cache
+        mixed, z, b, a = self._project(x)
+        y = LA.causal_conv1d(mixed, self.conv_weight, cu_seqlens=cu_seqlens, activation="silu")
+        o, last = LA.gated_delta_rule(*self._heads(y), *self._gates(b, a), cu_seqlens=cu_seqlens, qk_l2norm=True,
+                                      output_final_state=True)
+        slots = torch.as_tensor(slots, dtype=torch.long, device=x.device)
+        if slots.numel() != last.shape[0]:
+            raise ValueError(f"{last.shape[0]} sequences need as many slots, got {slots.numel()}")
+        cu = torch.tensor([0, mixed.shape[0]]) if cu_seqlens is None else torch.as_tensor(cu_seqlens)
+        cu = cu.to(device=x.device, dtype=torch.long)
+        at = cu[1:, None] - torch.arange(self.K - 1, 0, -1, device=x.device)  # the last K - 1 tokens, oldest first
+        inside = at >= cu[:-1, None]
+        rows = mixed[at.clamp(min=0, max=max(mixed.shape[0] - 1, 0))] if mixed.shape[0] else mixed.new_zeros(*at.shape, mixed.shape[1])
+        windows[slots] = torch.where(inside[..., None], rows, torch.zeros_like(rows)).transpose(1, 2).to(windows.dtype)
+        states[slots] = last
+        return self._finish(o, z, residual)
+
+    @torch.no_grad()
+    def step(self, x, cache, *, slots=None, residual=None):
+        """One token of every row of x [B, hidden]: row b continues the sequence in slot ``slots[b]`` of `cache` (its own
+        number without `slots`; negative = padding row), which is updated in place."""
+        self._check_decoding()
+        windows, states = cache
+        mixed, z, b, a = self._project(x)
+        y = LA.causal_conv1d_step(mixed, windows, self.conv_weight, state_indices=slots, activation="silu")
+        o = LA.gated_delta_rule_step(*self._heads(y), *self._gates(b, a), states, state_indices=slots, qk_l2norm=True)
+        return self._finish(o, z, residual)

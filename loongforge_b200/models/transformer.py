@@ -43,6 +43,10 @@ class RotaryInputs:
     freqs: torch.Tensor  # fp32 [P, rot_dim/2] angle table, or per-token angles [T, rot_dim/2]
     pos_ids: Optional[torch.Tensor] = None  # int32 [T] rows of `freqs`; None = row t
     mscale: float = 1.0
+    # several position axes (M-RoPE): angle i of token t is axis_pos[axis[i], t] * inv_freq[i]; `freqs` holds the same
+    axis_pos: Optional[torch.Tensor] = None  # int32 [axes, T]
+    axis: Optional[torch.Tensor] = None  # int32 [rot_dim/2]
+    inv_freq: Optional[torch.Tensor] = None  # fp32 [rot_dim/2]
 
 
 class Norm(nn.Module):
@@ -174,6 +178,27 @@ class MLP(nn.Module):
         return self.linear_fc2(h, residual)
 
 
+def fused_qk_applies(attn, qkv, groups: int, q_per_group: int, rotary: Optional[RotaryInputs], *, gated: bool = False) -> bool:
+    """Whether `attn`'s per-head query / key norms and its rotation run as one kernel on the packed projection."""
+    return (rotary is not None and isinstance(attn.q_layernorm, Norm) and attn.q_layernorm.kind == "RMSNorm"
+            and OF.qk_norm_rope_supported(qkv, groups, q_per_group, attn.q_layernorm.weight, attn.rot_dim,
+                                          interleaved=attn.cfg.rotary_interleaved and rotary.freqs.dim() == 2, gated=gated))
+
+
+def fused_qk(attn, qkv, groups: int, q_per_group: int, rotary: RotaryInputs, *, gated: bool = False):
+    """(q, k, v[, gate]) of the packed projection with norms and rotation applied (`OF.qk_norm_rope`)."""
+    qn, kn = attn.q_layernorm, attn.k_layernorm
+    kw = dict(rot_dim=attn.rot_dim, interleaved=attn.cfg.rotary_interleaved, mscale=rotary.mscale, eps=qn.eps,
+              w_offset=qn.offset, gated=gated)
+    if rotary.axis_pos is not None and rotary.axis_pos.shape[1] == qkv.shape[0]:
+        kw.update(inv_freq=rotary.inv_freq, axis=rotary.axis, pos_ids=rotary.axis_pos)
+    elif rotary.freqs.dim() == 3:  # per-token angles already mixed from the t/h/w streams
+        kw.update(freqs=rotary.freqs[:, 0], interleaved=False)
+    else:
+        kw.update(freqs=rotary.freqs, pos_ids=rotary.pos_ids)
+    return OF.qk_norm_rope(qkv, groups, q_per_group, qn.weight, kn.weight, **kw)
+
+
 class SelfAttention(nn.Module):
     """GQA self attention with a packed QKV projection, optional per-head QK RMSNorm (Qwen3),
     RoPE / M-RoPE applied in place on the packed buffer, and packed-sequence attention."""
@@ -236,6 +261,8 @@ class SelfAttention(nn.Module):
             q = pk4[:, :, :r].reshape(T, g * r, d)
             k = pk4[:, :, r]
             v = pk4[:, :, r + 1]
+        elif not cfg.qk_layernorm_full and fused_qk_applies(self, qkv, g, r, rotary):
+            q, k, v = fused_qk(self, qkv, g, r, rotary)
         else:
             pk4 = qkv.view(T, g, r + 2, d)
             if cfg.qk_layernorm_full:

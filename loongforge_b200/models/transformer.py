@@ -181,8 +181,7 @@ class MLP(nn.Module):
 def fused_qk_applies(attn, qkv, groups: int, q_per_group: int, rotary: Optional[RotaryInputs], *, gated: bool = False) -> bool:
     """Whether `attn`'s per-head query / key norms and its rotation run as one kernel on the packed projection."""
     return (rotary is not None and isinstance(attn.q_layernorm, Norm) and attn.q_layernorm.kind == "RMSNorm"
-            and OF.qk_norm_rope_supported(qkv, groups, q_per_group, attn.q_layernorm.weight, attn.rot_dim,
-                                          interleaved=attn.cfg.rotary_interleaved and rotary.freqs.dim() == 2, gated=gated))
+            and OF.qk_norm_rope_supported(qkv, groups, q_per_group, attn.q_layernorm.weight, attn.rot_dim, gated=gated))
 
 
 def fused_qk(attn, qkv, groups: int, q_per_group: int, rotary: RotaryInputs, *, gated: bool = False):

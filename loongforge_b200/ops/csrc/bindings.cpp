@@ -1291,7 +1291,7 @@ lf::QkNormRopeArgs qk_args(const at::Tensor& x, int64_t G, int64_t R, bool gated
     TORCH_CHECK(w->numel() == a.D && w->is_contiguous() && w->device() == x.device() &&
                     reinterpret_cast<uintptr_t>(w->data_ptr()) % 16 == 0, "norm weights must be contiguous [D], 16-byte aligned");
   const int64_t half = rot_dim / 2;
-  TORCH_CHECK(rot_dim > 0 && rot_dim <= a.D && (interleaved ? rot_dim % 8 == 0 : rot_dim % 16 == 0),
+  TORCH_CHECK(rot_dim > 0 && rot_dim <= a.D && rot_dim % 8 == 0,
               "qk_norm_rope: rot_dim ", rot_dim, " is not covered");
   TORCH_CHECK(freqs.has_value() != inv_freq.has_value(), "give either freqs or inv_freq");
   a.x = x.data_ptr();

@@ -16,26 +16,11 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 
-template <int V> struct Vec;
-template <> struct Vec<8> { using type = uint4; };
-template <> struct Vec<4> { using type = uint2; };
-
-template <int V>
-__device__ __forceinline__ void unpack(const typename Vec<V>::type& q, float (&f)[V]) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
-#pragma unroll
-  for (int i = 0; i < V / 2; ++i) {
-    const float2 t = __bfloat1622float2(h[i]);
-    f[2 * i] = t.x;
-    f[2 * i + 1] = t.y;
-  }
-}
-template <int V>
-__device__ __forceinline__ typename Vec<V>::type pack(const float (&f)[V]) {
-  typename Vec<V>::type q;
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  uint4 q;
   __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&q);
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
   return q;
 }
 
@@ -55,167 +40,224 @@ __device__ __forceinline__ int earlier_tokens(const int* __restrict__ cu, int N,
 
 __device__ __forceinline__ float sigmoid(float p) { return __fdividef(1.f, 1.f + __expf(-p)); }
 
-// Weights of V channels, taps last-to-first: wr[i] multiplies x[t - i].
-template <int V, int K>
-__device__ __forceinline__ void load_weights(const bf16* __restrict__ w, int c, float (&wr)[K][V]) {
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-#pragma unroll
-    for (int i = 0; i < K; ++i) wr[i][j] = __bfloat162float(w[static_cast<long long>(c + j) * K + (K - 1 - i)]);
+// Two neighbouring channels in one 64-bit register pair: one instruction for both halves.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 make2(float x, float y) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 split(f2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 widen(uint32_t w) { return make2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t narrow(f2 v) {
+  const float2 f = split(v);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ f2 sigmoid2(f2 p) {
+  const float2 f = split(p);
+  return make2(sigmoid(f.x), sigmoid(f.y));
 }
 
-constexpr int FWD_THREADS = 128;
-constexpr int FWD_ROWS = 16;
+constexpr int THREADS = 128;
+constexpr int FV = 2, BV = 1;  // channel pairs of a thread, forward and backward (dw and dx sums: more registers a pair)
+// Rows that are loaded ahead of their use. 16384 x 8192: forward 96 us with 8 (104 with 4), backward 211 us with 4 (245 with 8:
+// fewer blocks fit).
+constexpr int FSTEP = 8, BSTEP = 4;
+constexpr int MAX_SPAN = 128;
 
+// Rows [t, t + STEP) into registers; rows from `end` on are left alone.
+template <typename T, int STEP>
+__device__ __forceinline__ void load_rows(T (&r)[STEP], const bf16* p, long long t, long long stride, long long end) {
+  p += t * stride;
+#pragma unroll
+  for (int i = 0; i < STEP; ++i) {
+    if (t + i < end) r[i] = *reinterpret_cast<const T*>(p);
+    p += stride;
+  }
+}
+
+template <int NV, int K>
+__device__ __forceinline__ void load_pairs(const ConvArgs& a, int c, f2 (&wr)[K][NV], f2 (&bias)[NV]) {
+  const bf16* w = static_cast<const bf16*>(a.w) + static_cast<long long>(c) * K;
+  const bf16* b = static_cast<const bf16*>(a.bias) + c;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+#pragma unroll
+    for (int i = 0; i < K; ++i)  // wr[i] multiplies x[t - i]
+      wr[i][j] = make2(__bfloat162float(w[2 * j * K + (K - 1 - i)]), __bfloat162float(w[(2 * j + 1) * K + (K - 1 - i)]));
+    bias[j] = a.bias ? make2(__bfloat162float(b[2 * j]), __bfloat162float(b[2 * j + 1])) : 0ull;
+  }
+}
+
+// A block owns `span` rows of THREADS * FV channel pairs. front[i]: see earlier_tokens; `plain` steps, those whose rows
+// all have the whole window in their own sequence (nearly all of a long row), skip the tests for it.
 template <int K>
-__global__ void __launch_bounds__(FWD_THREADS)
-conv_fwd_kernel(const ConvArgs a, int cblocks) {
-  constexpr int V = 8;
-  __shared__ int front[FWD_ROWS];
-  const long long t0 = static_cast<long long>(blockIdx.x / cblocks) * FWD_ROWS;
-  const int c = ((blockIdx.x % cblocks) * FWD_THREADS + threadIdx.x) * V;
-  if (threadIdx.x < FWD_ROWS) front[threadIdx.x] = earlier_tokens(a.cu, a.N, a.T, t0 + threadIdx.x, K - 1);
+__global__ void __launch_bounds__(THREADS)
+conv_fwd_kernel(const ConvArgs a, int cblocks, int span) {
+  static_assert(FV == 2, "two pairs a thread");
+  constexpr int STEP = FSTEP;
+  __shared__ int front[MAX_SPAN];
+  const long long t0 = static_cast<long long>(blockIdx.x / cblocks) * span;
+  const long long t1 = t0 + span < a.T ? t0 + span : a.T;
+  const int c = ((blockIdx.x % cblocks) * THREADS + threadIdx.x) * 2 * FV;
+  if (threadIdx.x < span) front[threadIdx.x] = earlier_tokens(a.cu, a.N, a.T, t0 + threadIdx.x, K - 1);
   __syncthreads();
   if (c >= a.C) return;
   const bf16* x = static_cast<const bf16*>(a.x) + c;
   bf16* y = static_cast<bf16*>(a.y) + c;
-  float wr[K][V], bias[V], win[K][V];
-  load_weights<V, K>(static_cast<const bf16*>(a.w), c, wr);
-#pragma unroll
-  for (int j = 0; j < V; ++j) bias[j] = a.bias ? __bfloat162float(static_cast<const bf16*>(a.bias)[c + j]) : 0.f;
-  uint4 rows[FWD_ROWS];
-  const int n = a.T - t0 < FWD_ROWS ? static_cast<int>(a.T - t0) : FWD_ROWS;
-#pragma unroll
-  for (int r = 0; r < FWD_ROWS; ++r)
-    if (r < n) rows[r] = *reinterpret_cast<const uint4*>(x + (t0 + r) * a.x_ts);
+  f2 wr[K][FV], bias[FV], win[K][FV];
+  uint2 next[STEP];
+  load_rows(next, x, t0, a.x_ts, t1);
+  load_pairs<FV, K>(a, c, wr, bias);
 #pragma unroll
   for (int i = 1; i < K; ++i) {  // win[i] = x[t - i]
-    if (t0 - i >= 0) {
-      unpack<V>(*reinterpret_cast<const uint4*>(x + (t0 - i) * a.x_ts), win[i]);
+    uint2 r = make_uint2(0u, 0u);
+    if (t0 - i >= 0) r = *reinterpret_cast<const uint2*>(x + (t0 - i) * a.x_ts);
+#pragma unroll
+    for (int j = 0; j < FV; ++j) win[i][j] = widen(j ? r.y : r.x);
+  }
+  for (long long t = t0; t < t1; t += STEP) {
+    uint2 rows[STEP];
+#pragma unroll
+    for (int r = 0; r < STEP; ++r) rows[r] = next[r];
+    load_rows(next, x, t + STEP, a.x_ts, t1);
+    const int* f = front + (t - t0);
+    bool plain = t + STEP <= t1;
+#pragma unroll
+    for (int r = 0; r < STEP; ++r) plain = plain && f[r] == K - 1;
+    bf16* yt = y + t * a.C;
+    auto row = [&](int r, int fr) {
+      uint32_t out[FV];
+#pragma unroll
+      for (int j = 0; j < FV; ++j) {
+        win[0][j] = widen(j ? rows[r].y : rows[r].x);
+        f2 p = fma2(wr[0][j], win[0][j], bias[j]);
+#pragma unroll
+        for (int i = 1; i < K; ++i)
+          if (i <= fr) p = fma2(wr[i][j], win[i][j], p);
+        if (a.silu) p = mul2(p, sigmoid2(p));
+        out[j] = fr < 0 ? 0u : narrow(p);
+#pragma unroll
+        for (int i = K - 1; i > 0; --i) win[i][j] = win[i - 1][j];
+      }
+      *reinterpret_cast<uint2*>(yt + static_cast<long long>(r) * a.C) = make_uint2(out[0], out[1]);
+    };
+    if (plain) {
+#pragma unroll
+      for (int r = 0; r < STEP; ++r) row(r, K - 1);
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) win[i][j] = 0.f;
+      for (int r = 0; r < STEP; ++r)
+        if (t + r < t1) row(r, f[r]);
     }
-  }
-#pragma unroll
-  for (int r = 0; r < FWD_ROWS; ++r) {
-    if (r >= n) break;
-    const int f = front[r];
-    unpack<V>(rows[r], win[0]);
-    float p[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      p[j] = bias[j] + wr[0][j] * win[0][j];
-#pragma unroll
-      for (int i = 1; i < K; ++i)
-        if (i <= f) p[j] += wr[i][j] * win[i][j];
-      if (a.silu) p[j] *= sigmoid(p[j]);
-      if (f < 0) p[j] = 0.f;
-    }
-    *reinterpret_cast<uint4*>(y + (t0 + r) * a.C) = pack<V>(p);
-#pragma unroll
-    for (int i = K - 1; i > 0; --i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) win[i][j] = win[i - 1][j];
   }
 }
 
-// A block owns the rows [t0, t0 + span) of dx; it also visits the K - 1 rows behind them, whose dp reach back into the
-// block, but adds to dw / db from its own rows only.
-constexpr int BWD_THREADS = 128;
-constexpr int BWD_V = 4;
-
+// The same walk for the gradients. A block owns the rows [t0, t1) of dx; it also visits the K - 1 rows behind them, whose
+// dp reach back into the block, but adds to dw / db from its own rows only. acc[i] collects dx of row t - i.
 template <int K>
-__global__ void __launch_bounds__(BWD_THREADS)
+__global__ void __launch_bounds__(THREADS)
 conv_bwd_kernel(const ConvArgs a, int cblocks, int span) {
-  constexpr int V = BWD_V, STEP = 8;
-  using vec = typename Vec<V>::type;
-  __shared__ int front[STEP];
+  static_assert(BV == 1, "one pair a thread");
+  constexpr int STEP = BSTEP;
+  __shared__ int front[MAX_SPAN + STEP];
   const int tb = blockIdx.x / cblocks;
   const long long t0 = static_cast<long long>(tb) * span;
-  const int c = ((blockIdx.x % cblocks) * BWD_THREADS + threadIdx.x) * V;
-  const bool act = c < a.C;
-  const long long t1 = t0 + span < a.T ? t0 + span : a.T;  // first row behind the block's own
+  const long long t1 = t0 + span < a.T ? t0 + span : a.T, t2 = t1 + K - 1 < a.T ? t1 + K - 1 : a.T;
+  const int c = ((blockIdx.x % cblocks) * THREADS + threadIdx.x) * 2;
+  for (int i = threadIdx.x; i < span + STEP; i += THREADS) front[i] = earlier_tokens(a.cu, a.N, a.T, t0 + i, K - 1);
+  __syncthreads();
+  if (c >= a.C) return;
   const bf16* x = static_cast<const bf16*>(a.x) + c;
   const bf16* dy = static_cast<const bf16*>(a.dy) + c;
   bf16* dx = static_cast<bf16*>(a.dx) + c;
-  float wr[K][V], bias[V], win[K][V], acc[K][V], dw[K][V], db[V];
-  if (act) {
-    load_weights<V, K>(static_cast<const bf16*>(a.w), c, wr);
+  f2 wr[K][1], bias[1], win[K], acc[K], dw[K], db = 0ull;
+  uint32_t nx[STEP], ng[STEP];
+  load_rows(nx, x, t0, a.x_ts, t2);
+  load_rows(ng, dy, t0, a.C, t2);
+  load_pairs<1, K>(a, c, wr, bias);
 #pragma unroll
-    for (int j = 0; j < V; ++j) bias[j] = a.bias ? __bfloat162float(static_cast<const bf16*>(a.bias)[c + j]) : 0.f;
+  for (int i = 0; i < K; ++i) {
+    win[i] = acc[i] = dw[i] = 0ull;
+    if (i > 0 && t0 - i >= 0) win[i] = widen(*reinterpret_cast<const uint32_t*>(x + (t0 - i) * a.x_ts));
   }
-#pragma unroll
-  for (int i = 0; i < K; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) win[i][j] = acc[i][j] = dw[i][j] = 0.f;
-#pragma unroll
-  for (int j = 0; j < V; ++j) db[j] = 0.f;
-  if (act) {
-#pragma unroll
-    for (int i = 1; i < K; ++i)
-      if (t0 - i >= 0) unpack<V>(*reinterpret_cast<const vec*>(x + (t0 - i) * a.x_ts), win[i]);
-  }
-  for (long long tt = t0; tt < t1 + K - 1; tt += STEP) {
-    __syncthreads();
-    if (threadIdx.x < STEP) front[threadIdx.x] = earlier_tokens(a.cu, a.N, a.T, tt + threadIdx.x, K - 1);
-    __syncthreads();
-    if (!act) continue;
-    vec xr[STEP], gr[STEP];
-#pragma unroll
-    for (int r = 0; r < STEP; ++r)
-      if (tt + r < a.T && tt + r < t1 + K - 1) {
-        xr[r] = *reinterpret_cast<const vec*>(x + (tt + r) * a.x_ts);
-        gr[r] = *reinterpret_cast<const vec*>(dy + (tt + r) * a.C);
-      }
+  for (long long t = t0; t < t1 + K - 1; t += STEP) {
+    uint32_t xr[STEP], gr[STEP];
 #pragma unroll
     for (int r = 0; r < STEP; ++r) {
-      const long long t = tt + r;
-      if (t >= t1 + K - 1) break;
-      const int f = front[r];
-      const bool own = t < t1;
+      xr[r] = nx[r];
+      gr[r] = ng[r];
+    }
+    load_rows(nx, x, t + STEP, a.x_ts, t2);
+    load_rows(ng, dy, t + STEP, a.C, t2);
+    const int* f = front + (t - t0);
+    bool plain = t + STEP <= t1 && t > t0;
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[0][j] = 0.f;
-      if (f >= 0) {  // a token of some sequence (so t < T)
-        float g[V];
-        unpack<V>(xr[r], win[0]);
-        unpack<V>(gr[r], g);
+    for (int r = 0; r < STEP; ++r) plain = plain && f[r] == K - 1;
+    bf16* dxt = dx + (t - (K - 1)) * a.C;
+    // `own`: the row is one of the block's; `out`: row t + r - (K - 1), which no later row reaches, is
+    auto row = [&](int r, int fr, bool own, bool out) {
+      acc[0] = 0ull;
+      if (fr >= 0) {  // a token of some sequence
+        win[0] = widen(xr[r]);
+        f2 d = widen(gr[r]);
+        if (a.silu) {
+          f2 p = fma2(wr[0][0], win[0], bias[0]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float d = g[j];
-          if (a.silu) {
-            float p = bias[j] + wr[0][j] * win[0][j];
+          for (int i = 1; i < K; ++i)
+            if (i <= fr) p = fma2(wr[i][0], win[i], p);
+          const f2 s = sigmoid2(p), ps = mul2(p, s);
+          // silu' = s + p s (1 - s) = s + p s - (p s) s
+          d = mul2(d, add2(s, fma2(mul2(ps, s), make2(-1.f, -1.f), ps)));
+        }
 #pragma unroll
-            for (int i = 1; i < K; ++i)
-              if (i <= f) p += wr[i][j] * win[i][j];
-            const float s = sigmoid(p);
-            d *= s * (1.f + p * (1.f - s));
+        for (int i = 0; i < K; ++i)
+          if (i <= fr) {
+            acc[i] = fma2(wr[i][0], d, acc[i]);
+            if (own) dw[i] = fma2(d, win[i], dw[i]);
           }
-#pragma unroll
-          for (int i = 0; i < K; ++i)
-            if (i <= f) {
-              acc[i][j] += wr[i][j] * d;  // acc[i] belongs to row t - i
-              if (own) dw[i][j] += d * win[i][j];
-            }
-          if (own) db[j] += d;
-        }
+        if (own) db = add2(db, d);
       }
-      const long long done = t - (K - 1);  // no later row reaches it
-      if (done >= t0 && done < t1) *reinterpret_cast<vec*>(dx + done * a.C) = pack<V>(acc[K - 1]);
+      if (out) *reinterpret_cast<uint32_t*>(dxt + static_cast<long long>(r) * a.C) = narrow(acc[K - 1]);
 #pragma unroll
-      for (int i = K - 1; i > 0; --i)
+      for (int i = K - 1; i > 0; --i) {
+        win[i] = win[i - 1];
+        acc[i] = acc[i - 1];
+      }
+    };
+    if (plain) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          win[i][j] = win[i - 1][j];
-          acc[i][j] = acc[i - 1][j];
-        }
+      for (int r = 0; r < STEP; ++r) row(r, K - 1, true, true);
+    } else {
+#pragma unroll
+      for (int r = 0; r < STEP; ++r)
+        if (t + r < t1 + K - 1) row(r, f[r], t + r < t1, t + r - (K - 1) >= t0);
     }
   }
-  if (!act) return;
   float* p = a.partial + static_cast<long long>(tb) * (K + 1) * a.C + c;
 #pragma unroll
-  for (int i = 0; i < K; ++i) *reinterpret_cast<float4*>(p + static_cast<long long>(i) * a.C) = make_float4(dw[i][0], dw[i][1], dw[i][2], dw[i][3]);
-  *reinterpret_cast<float4*>(p + static_cast<long long>(K) * a.C) = make_float4(db[0], db[1], db[2], db[3]);
+  for (int i = 0; i < K; ++i) *reinterpret_cast<float2*>(p + static_cast<long long>(i) * a.C) = split(dw[i]);
+  *reinterpret_cast<float2*>(p + static_cast<long long>(K) * a.C) = split(db);
 }
 
 // dw[c, K - 1 - i] = sum over blocks of partial[b, i, c], in block order; db likewise from row K.
@@ -232,10 +274,11 @@ __global__ void conv_dw_kernel(const float* __restrict__ partial, int blocks, in
   else if (db) db[c] = __float2bfloat16(s);
 }
 
-int bwd_span(long long T, int C) {
-  // long enough that the fp32 partial sums stay a few per cent of the traffic, short enough for two blocks per SM
-  const long long cblocks = (C + BWD_V * BWD_THREADS - 1) / (BWD_V * BWD_THREADS);
-  int span = 128;
+// Rows of a block: long, so that halo rows and the fp32 partial sums of dw stay a few per cent of the traffic, but short
+// enough that there are two blocks per SM.
+int row_span(long long T, int C, int v) {
+  const long long cblocks = (C + 2 * v * THREADS - 1) / (2 * v * THREADS);
+  int span = MAX_SPAN;
   while (span > 16 && (T + span - 1) / span * cblocks < 2 * 148) span >>= 1;
   return span;
 }
@@ -245,7 +288,7 @@ constexpr int STEP_THREADS = 128;
 template <int K>
 __global__ void __launch_bounds__(STEP_THREADS)
 conv_step_kernel(const ConvStepArgs a, int cblocks) {
-  constexpr int V = 8;
+  constexpr int V = 8;  // channels of a thread: 16-byte pieces of x, state and weights
   const int b = blockIdx.x / cblocks;
   const int c = ((blockIdx.x % cblocks) * STEP_THREADS + threadIdx.x) * V;
   long long slot = b;
@@ -292,40 +335,39 @@ conv_step_kernel(const ConvStepArgs a, int cblocks) {
 #pragma unroll
     for (int i = 0; i < K - 1; ++i) st[i] = out[i];
   }
-  *reinterpret_cast<uint4*>(static_cast<bf16*>(a.y) + static_cast<long long>(b) * a.C + c) = pack<V>(p);
+  *reinterpret_cast<uint4*>(static_cast<bf16*>(a.y) + static_cast<long long>(b) * a.C + c) = pack8(p);
 }
 
 }  // namespace
 
 int conv_blocks(long long T, int C) {
-  const int span = bwd_span(T, C);
+  const int span = row_span(T, C, BV);
   return static_cast<int>((T + span - 1) / span);
 }
 
 int conv_fwd(const ConvArgs& a, cudaStream_t s) {
   if (a.K < 2 || a.K > 4 || a.C % 8 != 0) return -1;
-  if (a.T == 0) return 0;
-  const int cblocks = (a.C + 8 * FWD_THREADS - 1) / (8 * FWD_THREADS);
-  const long long grid = (a.T + FWD_ROWS - 1) / FWD_ROWS * cblocks;
+  const int cblocks = (a.C + 2 * FV * THREADS - 1) / (2 * FV * THREADS), span = row_span(a.T, a.C, FV);
+  const long long grid = (a.T + span - 1) / span * cblocks;
   if (grid > INT32_MAX) return -2;
+  if (grid == 0) return 0;
   const unsigned gd = static_cast<unsigned>(grid);
-  if (a.K == 2) conv_fwd_kernel<2><<<gd, FWD_THREADS, 0, s>>>(a, cblocks);
-  else if (a.K == 3) conv_fwd_kernel<3><<<gd, FWD_THREADS, 0, s>>>(a, cblocks);
-  else conv_fwd_kernel<4><<<gd, FWD_THREADS, 0, s>>>(a, cblocks);
+  if (a.K == 2) conv_fwd_kernel<2><<<gd, THREADS, 0, s>>>(a, cblocks, span);
+  else if (a.K == 3) conv_fwd_kernel<3><<<gd, THREADS, 0, s>>>(a, cblocks, span);
+  else conv_fwd_kernel<4><<<gd, THREADS, 0, s>>>(a, cblocks, span);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 int conv_bwd(const ConvArgs& a, cudaStream_t s) {
   if (a.K < 2 || a.K > 4 || a.C % 8 != 0) return -1;
-  const int span = bwd_span(a.T, a.C), blocks = conv_blocks(a.T, a.C);
-  const int cblocks = (a.C + BWD_V * BWD_THREADS - 1) / (BWD_V * BWD_THREADS);
+  const int cblocks = (a.C + 2 * BV * THREADS - 1) / (2 * BV * THREADS), span = row_span(a.T, a.C, BV), blocks = conv_blocks(a.T, a.C);
   const long long grid = static_cast<long long>(blocks) * cblocks;
   if (grid > INT32_MAX) return -2;
   if (grid > 0) {
     const unsigned gd = static_cast<unsigned>(grid);
-    if (a.K == 2) conv_bwd_kernel<2><<<gd, BWD_THREADS, 0, s>>>(a, cblocks, span);
-    else if (a.K == 3) conv_bwd_kernel<3><<<gd, BWD_THREADS, 0, s>>>(a, cblocks, span);
-    else conv_bwd_kernel<4><<<gd, BWD_THREADS, 0, s>>>(a, cblocks, span);
+    if (a.K == 2) conv_bwd_kernel<2><<<gd, THREADS, 0, s>>>(a, cblocks, span);
+    else if (a.K == 3) conv_bwd_kernel<3><<<gd, THREADS, 0, s>>>(a, cblocks, span);
+    else conv_bwd_kernel<4><<<gd, THREADS, 0, s>>>(a, cblocks, span);
   }
   const long long n = static_cast<long long>(a.K + 1) * a.C;
   conv_dw_kernel<<<static_cast<unsigned>((n + 127) / 128), 128, 0, s>>>(a.partial, blocks, a.C, a.K,

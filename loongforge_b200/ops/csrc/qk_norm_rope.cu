@@ -8,10 +8,11 @@
 // (time, height, width). They are reduced to turns in 64 bits before sine and cosine: positions far into a long
 // context keep their fraction.
 //
-// Bound by memory. D / 8 lanes hold a head, 16 bytes each; the rotation's partner elements are a shuffle away. The
-// cosines of a few tokens are made once per block and shared by all their heads. The value (and gate) heads of the
-// packed row are not touched forward; backward copies their gradients into the packed gradient, which is so written in
-// one pass.
+// Bound by memory. D / 8 lanes hold a head. A lane holds both elements of its rotated pairs (four of each half, 8 bytes
+// at a time; eight neighbours behind the rotated span), so the rotation stays in the lane. A block takes a few tokens and
+// lays (head, token) out so that a lane keeps one token, hence its cosines, for all its heads. The value (and gate) heads
+// of the packed row are not touched forward; backward copies their gradients into the packed gradient, which is so
+// written in one pass.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -24,6 +25,7 @@ using bf16 = __nv_bfloat16;
 constexpr int THREADS = 256;
 constexpr int TOK = 4;       // tokens of a block's turn
 constexpr int MAX_HALF = 128;
+constexpr int AHEAD = 3, BAHEAD = 1;  // heads of a lane that are loaded before the first is worked on, forward and backward
 
 __device__ __forceinline__ void unpack8(const uint4& q, float (&f)[8]) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
@@ -55,7 +57,10 @@ __device__ __forceinline__ void make_rotation(const QkNormRopeArgs& a, long long
   for (int i = threadIdx.x; i < TOK * half; i += THREADS) {
     const int tk = i / half, f = i - tk * half;
     const long long t = t0 + tk;
-    if (t >= a.T) continue;
+    if (t >= a.T) {  // its lanes work on zeros
+      cs[tk][f] = sn[tk][f] = 0.f;
+      continue;
+    }
     double ang = 0.0;
     if (a.freqs) {
       const long long row = a.pos ? a.pos[t] : t;
@@ -74,147 +79,210 @@ __device__ __forceinline__ void make_rotation(const QkNormRopeArgs& a, long long
   }
 }
 
-// Rotates the thread's eight elements [8 * hl, 8 * hl + 8) of a head by sign * angle; all lanes of the warp call it.
-template <int LANES>
-__device__ __forceinline__ void rotate(float (&f)[8], int hl, const float* cs, const float* sn, int rot_dim, int interleaved, float sign) {
-  const int e0 = hl * 8;
-  if (interleaved) {
-    if (e0 < rot_dim) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float c = cs[e0 / 2 + j], s = sign * sn[e0 / 2 + j], x = f[2 * j], y = f[2 * j + 1];
-        f[2 * j] = x * c - y * s;
-        f[2 * j + 1] = y * c + x * s;
-      }
-    }
-    return;
+// Where the lane's two groups of four elements lie in a head, and whether they rotate.
+struct Place {
+  int e0, e1, f0;  // f0: first of the four angles
+  bool in;
+};
+__device__ __forceinline__ Place place(const QkNormRopeArgs& a, int hl) {
+  Place p;
+  const int half = a.rot_dim >> 1;
+  if (a.interleaved) {
+    p.e0 = 8 * hl;
+    p.e1 = p.e0 + 4;
+    p.in = p.e0 < a.rot_dim;
+    p.f0 = 4 * hl;
+  } else {
+    p.in = 4 * hl < half;
+    p.e0 = p.in ? 4 * hl : 8 * hl;  // behind the span: rot_dim + 8 (hl - half / 4)
+    p.e1 = p.in ? half + 4 * hl : p.e0 + 4;
+    p.f0 = 4 * hl;
   }
-  const int half = rot_dim >> 1, step = half >> 3;
-  const bool in = e0 < rot_dim, upper = e0 >= half;
-  const int partner = in ? (upper ? hl - step : hl + step) : hl;
-  const int src = (threadIdx.x & 31 & ~(LANES - 1)) + partner;
-  const int i0 = in ? (upper ? e0 - half : e0) : 0;
+  if (!p.in) p.f0 = 0;
+  return p;
+}
+
+struct Rotation {
+  float c[4], s[4];
+};
+__device__ __forceinline__ Rotation rotation_of(const Place& p, const float* cs, const float* sn) {
+  Rotation r;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float other = __shfl_sync(0xffffffffu, f[j], src);
-    if (in) {
-      const float c = cs[i0 + j], s = sign * sn[i0 + j];
-      f[j] = upper ? f[j] * c + other * s : f[j] * c - other * s;
-    }
+  for (int j = 0; j < 4; ++j) {
+    r.c[j] = p.in ? cs[p.f0 + j] : 1.f;
+    r.s[j] = p.in ? sn[p.f0 + j] : 0.f;
+  }
+  return r;
+}
+
+// f[0..3] and f[4..7] are the lane's two groups; pairs are (j, j + 4), or (2j, 2j + 1) when interleaved.
+__device__ __forceinline__ void rotate(float (&f)[8], const Rotation& r, int interleaved, float sign) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float s = sign * r.s[j];
+    float& x = interleaved ? f[2 * j] : f[j];
+    float& y = interleaved ? f[2 * j + 1] : f[j + 4];
+    const float a = x * r.c[j] - y * s, b = y * r.c[j] + x * s;
+    x = a;
+    y = b;
   }
 }
 
-template <int LANES>
+__device__ __forceinline__ void widen(const uint2& a, const uint2& b, float (&f)[8]) { unpack8(make_uint4(a.x, a.y, b.x, b.y), f); }
+
+template <int LANES, bool IL>
 __global__ void __launch_bounds__(THREADS)
 qk_fwd_kernel(const QkNormRopeArgs a) {
   constexpr int D = LANES * 8, HEADS = THREADS / LANES;
+  static_assert(HEADS % TOK == 0, "a lane keeps its token");
   __shared__ float cs[TOK][MAX_HALF], sn[TOK][MAX_HALF];
   const long long t0 = static_cast<long long>(blockIdx.x) * TOK;
+  const int hl = threadIdx.x % LANES, slot = threadIdx.x / LANES, tk = slot % TOK;
+  const Place pl = place(a, hl);
+  const long long t = t0 + tk;
+  const bool live = t < a.T;
+  const int per = a.G * (a.R + 1);
+  const bf16* row = static_cast<const bf16*>(a.x) + (live ? t : 0) * a.x_ts;
+  uint2 lo[AHEAD], hi[AHEAD];
+  auto fetch = [&](int hd0) {
+#pragma unroll
+    for (int w = 0; w < AHEAD; ++w) {
+      const int hd = hd0 + w * (HEADS / TOK), grp = hd / (a.R + 1), r = hd - grp * (a.R + 1);
+      const bf16* src = row + (grp * a.P + (r == a.R ? a.P - 2 : r)) * D;
+      const bool ok = live && hd < per;
+      lo[w] = ok ? *reinterpret_cast<const uint2*>(src + pl.e0) : make_uint2(0u, 0u);
+      hi[w] = ok ? *reinterpret_cast<const uint2*>(src + pl.e1) : make_uint2(0u, 0u);
+    }
+  };
+  fetch(slot / TOK);
   make_rotation(a, t0, cs, sn);
-  const int hl = threadIdx.x % LANES, slot = threadIdx.x / LANES;
   float wq[8], wk[8];
-  unpack8(reinterpret_cast<const uint4*>(a.qw)[hl], wq);
-  unpack8(reinterpret_cast<const uint4*>(a.kw)[hl], wk);
+  widen(*reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.qw) + pl.e0), *reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.qw) + pl.e1), wq);
+  widen(*reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.kw) + pl.e0), *reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.kw) + pl.e1), wk);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     wq[j] += a.w_offset;
     wk[j] += a.w_offset;
   }
   __syncthreads();
-  const int per = a.G * (a.R + 1), n = static_cast<int>(a.T - t0 < TOK ? a.T - t0 : TOK) * per;
-  // the loop runs the same number of turns in every lane of a warp: shuffles need them all
-  for (int base = 0; base < n; base += HEADS) {
-    const int idx = base + slot;
-    const bool act = idx < n;
-    const int tk = act ? idx / per : 0, hd = act ? idx - tk * per : 0;
-    const int grp = hd / (a.R + 1), r = hd - grp * (a.R + 1);
-    const bool is_k = r == a.R;
-    const long long t = t0 + tk;
-    const bf16* src = static_cast<const bf16*>(a.x) + t * a.x_ts + (static_cast<long long>(grp) * a.P + (is_k ? a.P - 2 : r)) * D;
-    float f[8];
-    unpack8(act ? reinterpret_cast<const uint4*>(src)[hl] : make_uint4(0u, 0u, 0u, 0u), f);
-    float ss = 0.f;
+  const Rotation rot = rotation_of(pl, cs[tk], sn[tk]);
+  // every lane of a warp makes the same number of turns: the sums over a head need them all
+  const int turns = (per + AHEAD * (HEADS / TOK) - 1) / (AHEAD * (HEADS / TOK));
+  for (int n = 0; n < turns; ++n) {
+    const int hd0 = n * AHEAD * (HEADS / TOK) + slot / TOK;
+    if (n > 0) fetch(hd0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
-    const float rstd = rsqrtf(head_sum<LANES>(ss) / static_cast<float>(D) + a.eps);
+    for (int w = 0; w < AHEAD; ++w) {
+      const int hd = hd0 + w * (HEADS / TOK), grp = hd / (a.R + 1), r = hd - grp * (a.R + 1);
+      const bool is_k = r == a.R;
+      float f[8];
+      widen(lo[w], hi[w], f);
+      float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] *= rstd * (is_k ? wk[j] : wq[j]);
-    rotate<LANES>(f, hl, cs[tk], sn[tk], a.rot_dim, a.interleaved, 1.f);
-    if (act) {
-      bf16* dst = is_k ? static_cast<bf16*>(a.k) + (t * a.G + grp) * D : static_cast<bf16*>(a.q) + (t * a.G * a.R + grp * a.R + r) * D;
-      reinterpret_cast<uint4*>(dst)[hl] = pack8(f);
+      for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+      const float rstd = rsqrtf(head_sum<LANES>(ss) * (1.f / D) + a.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] *= rstd * (is_k ? wk[j] : wq[j]);
+      rotate(f, rot, IL, 1.f);
+      if (live && hd < per) {
+        bf16* dst = is_k ? static_cast<bf16*>(a.k) + (t * a.G + grp) * D : static_cast<bf16*>(a.q) + (t * a.G * a.R + hd - grp) * D;
+        const uint4 o = pack8(f);
+        *reinterpret_cast<uint2*>(dst + pl.e0) = make_uint2(o.x, o.y);
+        *reinterpret_cast<uint2*>(dst + pl.e1) = make_uint2(o.z, o.w);
+      }
     }
   }
 }
 
-template <int LANES>
-__global__ void __launch_bounds__(THREADS)
+template <int LANES, bool IL>
+__global__ void __launch_bounds__(THREADS, 3)
 qk_bwd_kernel(const QkNormRopeArgs a) {
   constexpr int D = LANES * 8, HEADS = THREADS / LANES;
   __shared__ float cs[TOK][MAX_HALF], sn[TOK][MAX_HALF];
   __shared__ float red[HEADS][D];
-  const int hl = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+  const int hl = threadIdx.x % LANES, slot = threadIdx.x / LANES, tk = slot % TOK;
+  const Place pl = place(a, hl);
   float wq[8], wk[8], dwq[8], dwk[8];
-  unpack8(reinterpret_cast<const uint4*>(a.qw)[hl], wq);
-  unpack8(reinterpret_cast<const uint4*>(a.kw)[hl], wk);
+  widen(*reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.qw) + pl.e0), *reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.qw) + pl.e1), wq);
+  widen(*reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.kw) + pl.e0), *reinterpret_cast<const uint2*>(static_cast<const bf16*>(a.kw) + pl.e1), wk);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     wq[j] += a.w_offset;
     wk[j] += a.w_offset;
     dwq[j] = dwk[j] = 0.f;
   }
-  const int per = a.G * a.P;
+  const int per = a.G * a.P, turns = (per + BAHEAD * (HEADS / TOK) - 1) / (BAHEAD * (HEADS / TOK));
   for (long long t0 = static_cast<long long>(blockIdx.x) * TOK; t0 < a.T; t0 += static_cast<long long>(gridDim.x) * TOK) {
+    const long long t = t0 + tk;
+    const bool live = t < a.T;
     __syncthreads();
     make_rotation(a, t0, cs, sn);
     __syncthreads();
-    const int n = static_cast<int>(a.T - t0 < TOK ? a.T - t0 : TOK) * per;
-    for (int base = 0; base < n; base += HEADS) {
-      const int idx = base + slot;
-      const bool act = idx < n;
-      const int tk = act ? idx / per : 0, hd = act ? idx - tk * per : 0;
-      const int grp = hd / a.P, p = hd - grp * a.P;
-      const bool is_q = p < a.R, is_k = p == a.P - 2, is_v = p == a.P - 1;
-      const long long t = t0 + tk;
-      const bf16* g;
-      if (is_q) g = static_cast<const bf16*>(a.dq) + (t * a.G * a.R + grp * a.R + p) * D;
-      else if (is_k) g = static_cast<const bf16*>(a.dk) + (t * a.G + grp) * D;
-      else if (is_v) g = static_cast<const bf16*>(a.dv) + (t * a.G + grp) * D;
-      else g = static_cast<const bf16*>(a.dgate) + (t * a.G * a.R + grp * a.R + p - a.R) * D;
-      const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-      const bool turn = act && (is_q || is_k);
-      const uint4 graw = act ? reinterpret_cast<const uint4*>(g)[hl] : zero;
-      const uint4 xraw = turn ? reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.x) + t * a.x_ts + static_cast<long long>(hd) * D)[hl] : zero;
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<bf16*>(a.dx) + (t * per + hd) * D) + hl;
-      float d[8], x[8];
-      unpack8(graw, d);
-      unpack8(xraw, x);
-      rotate<LANES>(d, hl, cs[tk], sn[tk], a.rot_dim, a.interleaved, -1.f);
-      float ss = 0.f;
+    const Rotation rot = rotation_of(pl, cs[tk], sn[tk]);
+    const long long tl = live ? t : 0;
+    const bf16* xrow = static_cast<const bf16*>(a.x) + tl * a.x_ts;
+    const bf16* dq = static_cast<const bf16*>(a.dq) + tl * a.G * a.R * D;
+    const bf16* dk = static_cast<const bf16*>(a.dk) + tl * a.G * D;
+    const bf16* dv = static_cast<const bf16*>(a.dv) + tl * a.G * D;
+    const bf16* dgate = static_cast<const bf16*>(a.dgate) + tl * a.G * a.R * D;
+    bf16* dxrow = static_cast<bf16*>(a.dx) + tl * per * D;
+    for (int n = 0; n < turns; ++n) {
+      const int hd0 = n * BAHEAD * (HEADS / TOK) + slot / TOK;
+      uint2 glo[BAHEAD], ghi[BAHEAD], xlo[BAHEAD], xhi[BAHEAD];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
-      const float rstd = rsqrtf(head_sum<LANES>(ss) / static_cast<float>(D) + a.eps);
-      float dot = 0.f;
-      if (turn) {
+      for (int w = 0; w < BAHEAD; ++w) {
+        const int hd = hd0 + w * (HEADS / TOK), grp = hd / a.P, p = hd - grp * a.P;
+        const bf16* g = p < a.R ? dq + (grp * a.R + p) * D : p == a.P - 2 ? dk + grp * D : p == a.P - 1 ? dv + grp * D : dgate + (grp * a.R + p - a.R) * D;
+        const bool ok = live && hd < per, turn = ok && (p < a.R || p == a.P - 2);
+        const uint2 zero = make_uint2(0u, 0u);
+        glo[w] = ok ? *reinterpret_cast<const uint2*>(g + pl.e0) : zero;
+        ghi[w] = ok ? *reinterpret_cast<const uint2*>(g + pl.e1) : zero;
+        xlo[w] = turn ? *reinterpret_cast<const uint2*>(xrow + hd * D + pl.e0) : zero;
+        xhi[w] = turn ? *reinterpret_cast<const uint2*>(xrow + hd * D + pl.e1) : zero;
+      }
+#pragma unroll
+      for (int w = 0; w < BAHEAD; ++w) {
+        const int hd = hd0 + w * (HEADS / TOK), grp = hd / a.P, p = hd - grp * a.P;
+        const bool is_k = p == a.P - 2, turn = p < a.R || is_k;
+        float d[8], x[8];
+        const uint2 zero = make_uint2(0u, 0u);
+        widen(turn ? glo[w] : zero, turn ? ghi[w] : zero, d);
+        widen(xlo[w], xhi[w], x);
+        rotate(d, rot, IL, -1.f);
+        // the two sums over the head: x . x and d w . x
+        float ss = 0.f, dot = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float w = d[j] * x[j] * rstd;
-          if (is_k) dwk[j] += w; else dwq[j] += w;
-          d[j] *= is_k ? wk[j] : wq[j];
-          dot += d[j] * x[j];
+          ss += x[j] * x[j];
+          dot += d[j] * (is_k ? wk[j] : wq[j]) * x[j];
+        }
+        ss = head_sum<LANES>(ss);
+        dot = head_sum<LANES>(dot);
+        const float rstd = rsqrtf(ss * (1.f / D) + a.eps), m = dot * rstd * rstd * (1.f / D);
+        const float rq = is_k ? 0.f : rstd, rk = is_k ? rstd : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // both are zero where nothing turns
+          const float v = d[j] * x[j];
+          dwq[j] += v * rq;
+          dwk[j] += v * rk;
+          d[j] = rstd * (d[j] * (is_k ? wk[j] : wq[j]) - x[j] * m);
+        }
+        if (live && hd < per) {
+          const uint4 o = pack8(d);
+          *reinterpret_cast<uint2*>(dxrow + hd * D + pl.e0) = turn ? make_uint2(o.x, o.y) : glo[w];
+          *reinterpret_cast<uint2*>(dxrow + hd * D + pl.e1) = turn ? make_uint2(o.z, o.w) : ghi[w];
         }
       }
-      dot = head_sum<LANES>(dot) * rstd * rstd / static_cast<float>(D);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = rstd * (d[j] - x[j] * dot);
-      if (act) *dst = turn ? pack8(d) : graw;
     }
   }
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 8; ++j) red[slot][hl * 8 + j] = which ? dwk[j] : dwq[j];
+    for (int j = 0; j < 4; ++j) {
+      red[slot][pl.e0 + j] = which ? dwk[j] : dwq[j];
+      red[slot][pl.e1 + j] = which ? dwk[j + 4] : dwq[j + 4];
+    }
     __syncthreads();
     for (int c = threadIdx.x; c < D; c += THREADS) {
       float s = 0.f;
@@ -225,26 +293,38 @@ qk_bwd_kernel(const QkNormRopeArgs a) {
   }
 }
 
-// dw = sum over blocks of partial[b, ., c] in a fixed order: a block per 32 columns, 8 rows of threads.
+// dw = sum over blocks of partial[b, ., c] in a fixed order: a block per 32 columns, 32 rows of threads.
 __global__ void qk_dw_kernel(const float* __restrict__ partial, int blocks, int D, bf16* __restrict__ dqw, bf16* __restrict__ dkw) {
-  __shared__ float red[8][32];
+  __shared__ float red[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float s = 0.f;
-  for (int b = threadIdx.y; b < blocks; b += 8) s += partial[static_cast<long long>(b) * 2 * D + c];
+#pragma unroll 8
+  for (int b = threadIdx.y; b < blocks; b += 32) s += partial[static_cast<long long>(b) * 2 * D + c];
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y == 0) {
+  s = red[threadIdx.x][threadIdx.y];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
-    (c < D ? dqw[c] : dkw[c - D]) = __float2bfloat16(s);
-  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int col = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0) (col < D ? dqw[col] : dkw[col - D]) = __float2bfloat16(s);
+}
+
+template <int LANES>
+void launch_fwd(const QkNormRopeArgs& a, unsigned grid, cudaStream_t s) {
+  if (a.interleaved) qk_fwd_kernel<LANES, true><<<grid, THREADS, 0, s>>>(a);
+  else qk_fwd_kernel<LANES, false><<<grid, THREADS, 0, s>>>(a);
+}
+template <int LANES>
+void launch_bwd(const QkNormRopeArgs& a, int grid, cudaStream_t s) {
+  if (a.interleaved) qk_bwd_kernel<LANES, true><<<grid, THREADS, 0, s>>>(a);
+  else qk_bwd_kernel<LANES, false><<<grid, THREADS, 0, s>>>(a);
 }
 
 }  // namespace
 
 int qk_norm_rope_bwd_grid(long long T) {
   const long long b = (T + TOK - 1) / TOK;
-  return static_cast<int>(b < 148 * 4 ? b : 148 * 4);
+  return static_cast<int>(b < 148 * 3 ? b : 148 * 3);
 }
 
 int qk_norm_rope_fwd(const QkNormRopeArgs& a, cudaStream_t s) {
@@ -253,9 +333,9 @@ int qk_norm_rope_fwd(const QkNormRopeArgs& a, cudaStream_t s) {
   const long long grid = (a.T + TOK - 1) / TOK;
   if (grid > INT32_MAX) return -2;
   const unsigned gd = static_cast<unsigned>(grid);
-  if (a.D == 64) qk_fwd_kernel<8><<<gd, THREADS, 0, s>>>(a);
-  else if (a.D == 128) qk_fwd_kernel<16><<<gd, THREADS, 0, s>>>(a);
-  else if (a.D == 256) qk_fwd_kernel<32><<<gd, THREADS, 0, s>>>(a);
+  if (a.D == 64) launch_fwd<8>(a, gd, s);
+  else if (a.D == 128) launch_fwd<16>(a, gd, s);
+  else if (a.D == 256) launch_fwd<32>(a, gd, s);
   else return -1;
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
@@ -264,11 +344,11 @@ int qk_norm_rope_bwd(const QkNormRopeArgs& a, cudaStream_t s) {
   if (a.rot_dim / 2 > MAX_HALF || (a.D != 64 && a.D != 128 && a.D != 256)) return -1;
   const int grid = qk_norm_rope_bwd_grid(a.T);
   if (grid > 0) {
-    if (a.D == 64) qk_bwd_kernel<8><<<grid, THREADS, 0, s>>>(a);
-    else if (a.D == 128) qk_bwd_kernel<16><<<grid, THREADS, 0, s>>>(a);
-    else qk_bwd_kernel<32><<<grid, THREADS, 0, s>>>(a);
+    if (a.D == 64) launch_bwd<8>(a, grid, s);
+    else if (a.D == 128) launch_bwd<16>(a, grid, s);
+    else launch_bwd<32>(a, grid, s);
   }
-  qk_dw_kernel<<<2 * a.D / 32, dim3(32, 8), 0, s>>>(a.partial, grid, a.D, static_cast<bf16*>(a.dqw), static_cast<bf16*>(a.dkw));
+  qk_dw_kernel<<<2 * a.D / 32, dim3(32, 32), 0, s>>>(a.partial, grid, a.D, static_cast<bf16*>(a.dqw), static_cast<bf16*>(a.dkw));
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 

@@ -355,15 +355,14 @@ class _QKNormRopeFn(torch.autograd.Function):
 
 
 def qk_norm_rope_supported(qkv, groups: int, q_per_group: int, q_weight, rot_dim: Optional[int] = None, *,
-                           interleaved: bool = False, gated: bool = False) -> bool:
-    """Whether the one-pass kernel covers this call: bf16 on a GPU, head dim 64, 128 or 256, rotated span a multiple of 16
-    (8 for interleaved pairs)."""
+                           gated: bool = False) -> bool:
+    """Whether the one-pass kernel covers this call: bf16 on a GPU, head dim 64, 128 or 256, rotated span a multiple of 8."""
     if not (qkv.is_cuda and qkv.dtype == q_weight.dtype == torch.bfloat16 and qkv.dim() == 2):
         return False
     heads = groups * (2 * q_per_group + 2 if gated else q_per_group + 2)
     D = qkv.shape[1] // heads
     r = D if rot_dim is None else rot_dim
-    return (qkv.shape[1] == heads * D and D in (64, 128, 256) and 0 < r <= D and r % (8 if interleaved else 16) == 0)
+    return (qkv.shape[1] == heads * D and D in (64, 128, 256) and 0 < r <= D and r % 8 == 0)
 
 
 def qk_norm_rope(qkv: torch.Tensor, groups: int, q_per_group: int, q_weight: torch.Tensor, k_weight: torch.Tensor, *,
@@ -406,7 +405,7 @@ def qk_norm_rope(qkv: torch.Tensor, groups: int, q_per_group: int, q_weight: tor
             raise ValueError("qk_norm_rope: several position axes need `axis`")
     elif (pos_ids is None and freqs.shape[0] < T) or (pos_ids is not None and pos_ids.shape != (T,)):
         raise ValueError("qk_norm_rope: freqs / pos_ids do not cover the tokens")
-    if qk_norm_rope_supported(qkv, groups, q_per_group, q_weight, rot_dim, interleaved=interleaved, gated=gated) \
+    if qk_norm_rope_supported(qkv, groups, q_per_group, q_weight, rot_dim, gated=gated) \
             and k_weight.dtype == torch.bfloat16:
         dev = qkv.device
         x = qkv if qkv.stride(1) == 1 and qkv.stride(0) % 8 == 0 and qkv.data_ptr() % 16 == 0 else qkv.clone(

@@ -68,7 +68,7 @@ def check(T, G, R, D, rot, *, gated=False, axes=1, table=False, interleaved=Fals
         near(a, b, n)
 
 
-@pytest.mark.parametrize("T,G,R,D,rot", [(1, 1, 1, 64, 64), (3, 2, 4, 128, 128), (4, 1, 8, 256, 64), (5, 3, 3, 64, 32), (130, 2, 5, 128, 16), (9, 1, 2, 256, 256)])
+@pytest.mark.parametrize("T,G,R,D,rot", [(1, 1, 1, 64, 64), (3, 2, 4, 128, 128), (4, 1, 8, 256, 64), (5, 3, 3, 64, 32), (130, 2, 5, 128, 16), (9, 1, 2, 256, 256), (7, 2, 2, 128, 24)])
 @pytest.mark.parametrize("gated", [False, True])
 def test_qk_norm_rope_shapes(T, G, R, D, rot, gated):
     check(T, G, R, D, rot, gated=gated)

@@ -1032,9 +1032,12 @@ lf::DeltaArgs delta_args(const at::Tensor& q, const at::Tensor& k, const at::Ten
 // chunk states, A / P, factors} (see DeltaArgs).
 std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
                                   const at::Tensor& beta, c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first,
-                                  double scale, bool l2norm, c10::optional<at::Tensor> s_in, bool want_state, bool keep) {
+                                  double scale, bool l2norm, c10::optional<at::Tensor> s_in, bool want_state, bool keep,
+                                  const at::Tensor& status) {
   c10::cuda::CUDAGuard guard(q.device());
   lf::DeltaArgs a = delta_args(q, k, v, g, beta, bounds, first, scale, l2norm);
+  check_status(status, q);
+  a.status = status.data_ptr<int>();
   auto bf = v.options(), fl = g.options();
   at::Tensor o = at::empty({a.T, a.Hv, a.dv}, bf);
   at::Tensor s_out = want_state ? at::empty({a.N, a.Hv, a.dk, a.dv}, fl) : at::empty({0}, fl);
@@ -1080,9 +1083,11 @@ std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tens
                                   c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first, double scale, bool l2norm,
                                   bool want_ds, const at::Tensor& past, const at::Tensor& mem, const at::Tensor& mem_lo,
                                   const at::Tensor& u, const at::Tensor& u_lo, const at::Tensor& states, const at::Tensor& ap,
-                                  const at::Tensor& vec) {
+                                  const at::Tensor& vec, const at::Tensor& status) {
   c10::cuda::CUDAGuard guard(q.device());
   lf::DeltaArgs a = delta_args(q, k, v, g, beta, bounds, first, scale, l2norm);
+  check_status(status, q);
+  a.status = status.data_ptr<int>();
   check_heads(dout, "dout", q);
   for (const at::Tensor* t : {&dout, &mem, &mem_lo, &u, &u_lo})
     TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kBFloat16 && t->is_contiguous() &&
@@ -1096,7 +1101,7 @@ std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tens
   at::Tensor dg = at::empty_like(g), dbeta = at::empty_like(beta);
   at::Tensor ds_in = want_ds ? at::empty({a.N, a.Hv, a.dk, a.dv}, fl) : at::empty({0}, fl);
   at::Tensor dstates = at::empty({a.NC, a.Hv, a.dv, a.dk}, bf);
-  at::Tensor rowdots = at::empty({a.NC, a.Hv, a.dv / 16, 3, 64}, fl), sdots = at::empty({a.NC, a.Hv, a.dv / 16}, fl);
+  at::Tensor rowdots = at::empty({a.NC, a.Hv, a.dv / 16, 3, 64}, fl), sdots = at::empty({a.NC, a.Hv, a.dv / 16, 4}, fl);
   a.dout = dout.data_ptr();
   if (ds_out.has_value()) {
     check_state(*ds_out, "the final state's gradient", a.N, q, v);

@@ -26,10 +26,10 @@
 // Kernels:
 //   prepare   one block per (chunk, key head): Q K^T and K K^T once, then A, P and the per-token factors of each of its
 //             value heads.
-//   forward   one warp owns 16 of the dv columns of a head and walks along the sequence; the delta rule acts on every
-//             column by itself, so a warp never waits for another one. It keeps S^T [16, dk] in the accumulators of
-//             mma.sync and works on transposed products throughout: an accumulator tile is then, register by register,
-//             the A operand of the next product, and nothing of the chain S -> K S -> U -> S goes through shared memory.
+//   forward   walks along the sequence. The delta rule acts on every column of dv by itself, so 16 columns of a head make
+//             a unit that never waits for another one. All products are transposed: S^T [16, dk] lies in accumulators of
+//             mma.sync, and an accumulator tile is, register by register, the A operand of the next product. Four warps
+//             share a unit (by dk for the state, by tokens for the rest) and hand their operands to each other.
 //   backward  the same in reverse with dS^T.
 //   dqk       one block per (chunk, key head): dQ and dK, parallel over chunks.
 //   gates     dg and dbeta.
@@ -40,8 +40,9 @@
 // bf16: there S0, dS1, dV and N enter with the high part alone (2^-9 relative each, in terms that decay has made small);
 // U and W, whose products can cancel to little when keys are alike, keep both parts.
 //
-// The chain is bound by the tensor pipe's latency and rate at one warp per scheduler, not by bandwidth; mma.sync runs at
-// a quarter of tcgen05's rate but its operands and results stay in registers.
+// The chain is bound by latency: three dependent products of at most 64 x 128 x 16 per chunk, with a hand-over between
+// them. mma.sync runs at a quarter of tcgen05's rate, but operands and results stay in registers, and 32 heads make 1024
+// warps of such work.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -460,42 +461,81 @@ prepare_kernel(const DeltaArgs a) {
   }
 }
 
-// ---------------------------------------------------------------------------------------------------------- forward
-
-template <int COLS, int THREADS>
-__device__ __forceinline__ void load_square(bf16* dst, const bf16* src) {  // n x [64, 64] contiguous -> pitch APITCH
-  for (int i = threadIdx.x; i < COLS * C * 8; i += THREADS) {
-    const int r = i >> 3, v = i & 7;
-    cp16(dst + r * APITCH + v * 8, src + r * C + v * 8, true);
-  }
-}
-
 template <int THREADS>
 __device__ __forceinline__ void load_vec(float* dst, const float* src, int rows) {
   for (int i = threadIdx.x; i < rows * 16; i += THREADS) cp16(dst + i * 4, src + i * 4, true);
 }
 
-// The warp's [16 columns, 64 tokens] tile of fp32 accumulators, rounded to bf16, to rows of a token-major tensor
-// through `stage` (the warp's own columns of a [64, pitch] tile).
-template <typename F>
-__device__ __forceinline__ void store_tokens(bf16* stage, int pitch, bf16* out, long long stride, int len, F value) {
-#pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    uint32_t r[4];
-    r[0] = pack2(value(j, 0), value(j, 1));
-    r[1] = pack2(value(j, 2), value(j, 3));
-    r[2] = pack2(value(j + 1, 0), value(j + 1, 1));
-    r[3] = pack2(value(j + 1, 2), value(j + 1, 3));
-    stsm_t(const_cast<bf16*>(at_cr(stage, pitch, 8 * j, 0)), r);
-  }
-  __syncwarp();
+// ------------------------------------------------------------------------------------------- along the sequence: parts
+
+// A unit is 16 columns of dv of one head and four warps. Warp w holds columns [w dk/4, (w + 1) dk/4) of the unit's state
+// S^T [16, dk] in fp32, and makes everything that is per token for tokens [16 w, 16 w + 16) of a chunk. What the others
+// need of it (the state, R, U) goes through shared memory as ready A operands, high and low part, 16 bytes a lane.
+struct Operands {  // one k step of 16
+  uint4 hi[32], lo[32];
+};
+__device__ __forceinline__ void put(Operands& x, const uint32_t (&hi)[4], const uint32_t (&lo)[4]) {
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 16 + (lane >> 1), v = (lane & 1) * 8;
-    if (r < len) *reinterpret_cast<uint4*>(out + r * stride + v) = *reinterpret_cast<const uint4*>(stage + r * pitch + v);
-  }
+  x.hi[lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  x.lo[lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+__device__ __forceinline__ void get(const Operands& x, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  const int lane = threadIdx.x & 31;
+  const uint4 h = x.hi[lane], l = x.lo[lane];
+  hi[0] = h.x; hi[1] = h.y; hi[2] = h.z; hi[3] = h.w;
+  lo[0] = l.x; lo[1] = l.y; lo[2] = l.z; lo[3] = l.w;
+}
+
+// Barriers of the four warps of a unit (a warp arrives once) and of a buffer's copies. They complete in every chunk, so a
+// wait ends unless the kernel is wrong; after a limit far above any chunk's time it reports and goes on.
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {  // whole warp; what its lanes wrote is seen behind the wait
   __syncwarp();
+  if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ void bar_wait(uint64_t* b, uint32_t parity, int* status) {
+  uint32_t done = 0;
+  for (int i = 0; i < (1 << 22); ++i) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(smem_addr(b)), "r"(parity) : "memory");
+    if (done) return;
+  }
+  *status = 1;
+}
+// The calling thread's copies so far arrive on the barrier when they have landed.
+__device__ __forceinline__ void bar_arrive_copies(uint64_t* b) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+
+// Copies `rows` x COLS bf16 (rows from `len` on become zeros): a thread takes one 16-byte column of every
+// (THREADS / (COLS / 8))th row.
+template <int COLS, int THREADS>
+__device__ __forceinline__ void copy_tile(bf16* dst, int pitch, const bf16* src, long long stride, int rows, int len) {
+  constexpr int V = COLS / 8, STEP = THREADS / V;
+  const int v = threadIdx.x % V;
+  const bf16* p = src + (threadIdx.x / V) * stride + v * 8;
+  bf16* d = dst + (threadIdx.x / V) * pitch + v * 8;
+  for (int r = threadIdx.x / V; r < rows; r += STEP, p += STEP * stride, d += STEP * pitch) cp16(d, r < len ? p : src, r < len);
+}
+
+// The warp's 16 tokens x 16 columns of fp32 accumulators, rounded to bf16, to rows of a token-major tensor through the
+// warp's own `stage` [16][24].
+constexpr int OUT_PITCH = 24;
+__device__ __forceinline__ void store_tile(bf16* stage, bf16* out, long long stride, int len, const float (&c0)[4], const float (&c1)[4]) {
+  const uint32_t r[4] = {pack2(c0[0], c0[1]), pack2(c0[2], c0[3]), pack2(c1[0], c1[1]), pack2(c1[2], c1[3])};
+  __syncwarp();
+  stsm_t(const_cast<bf16*>(at_cr(stage, OUT_PITCH, 0, 0)), r);
+  __syncwarp();
+  const int lane = threadIdx.x & 31, row = lane >> 1, v = (lane & 1) * 8;
+  if (row < len) *reinterpret_cast<uint4*>(out + row * stride + v) = *reinterpret_cast<const uint4*>(stage + row * OUT_PITCH + v);
+}
+__device__ __forceinline__ float rest(float f) { return f - __bfloat162float(__float2bfloat16(f)); }
+__device__ __forceinline__ void store_rest(bf16* stage, bf16* out, long long stride, int len, const float (&c0)[4], const float (&c1)[4]) {
+  const float a[4] = {rest(c0[0]), rest(c0[1]), rest(c0[2]), rest(c0[3])}, b[4] = {rest(c1[0]), rest(c1[1]), rest(c1[2]), rest(c1[3])};
+  store_tile(stage, out, stride, len, a, b);
 }
 
 // Two neighbouring tokens of one column: m from its parts, U = beta (v - m).
@@ -506,509 +546,602 @@ __device__ __forceinline__ void memory_term(uint32_t v, uint32_t mh, uint32_t ml
   u1 = beta.y * (hi_half(v) - m1);
 }
 
-template <int DK, int NW>
+// Values of a factor row for the lane's four tokens: tile f, element pair.
+__device__ __forceinline__ void factors(const float* row, float2 (&x)[2]) {
+  x[0] = *reinterpret_cast<const float2*>(row);
+  x[1] = *reinterpret_cast<const float2*>(row + 8);
+}
+// c[f][e] *= x for the token of element e
+__device__ __forceinline__ void scale_tokens(float (&c)[2][4], const float2 (&x)[2]) {
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    c[f][0] *= x[f].x;
+    c[f][1] *= x[f].y;
+    c[f][2] *= x[f].x;
+    c[f][3] *= x[f].y;
+  }
+}
+__device__ __forceinline__ void clear(float (&c)[2][4]) {
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[f][e] = 0.f;
+}
+__device__ __forceinline__ void mma_pair(float (&c)[2][4], const uint32_t (&a)[4], const uint32_t (&b)[4]) {
+  mma(c[0], a, b[0], b[1]);
+  mma(c[1], a, b[2], b[3]);
+}
+__device__ __forceinline__ void add_to(float (&c)[2][4], const float (&d)[2][4]) {
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[f][e] += d[f][e];
+}
+
+// ---------------------------------------------------------------------------------------------------------- forward
+
+template <int DK, int NU>
 struct FwdStage {
-  static constexpr int P = DK + 8, VP = NW * 16 + 8;
+  static constexpr int P = DK + 8, VP = NU * 16 + 8;
   bf16 k[C * P], q[C * P], v[C * VP], ap[4 * C * APITCH];
   float vec[SEQ_ROWS * 64];
 };
+template <int DK, int NU>
+struct FwdSmem {
+  FwdStage<DK, NU> stage[2];
+  Operands state[NU][DK / 16], r[NU][4], u[NU][4], su[NU][4];
+  bf16 out[NU * 4][16 * OUT_PITCH];
+  uint64_t full[2], empty[2], state_ready[NU], r_ready[NU], u_ready[NU];
+};
 
 // KEEP: also write what the backward pass needs; the results are the same, bit by bit.
-template <int DK, int NW, bool KEEP>
-__global__ void __launch_bounds__(NW * 32, 1)
+template <int DK, int NU, bool KEEP>
+__global__ void __launch_bounds__(NU * 128, 1)
 forward_kernel(const DeltaArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  using Stage = FwdStage<DK, NW>;
-  constexpr int P = Stage::P, VP = Stage::VP, THREADS = NW * 32, KT = DK / 16;
-  Stage* st = reinterpret_cast<Stage*>(smem);
-  const int splits = a.dv / (NW * 16);
+  using Smem = FwdSmem<DK, NU>;
+  using Stage = FwdStage<DK, NU>;
+  constexpr int P = Stage::P, VP = Stage::VP, THREADS = NU * 128, KT = DK / 16, KW = KT / 4;
+  Smem& sm = *reinterpret_cast<Smem*>(smem);
+  const int splits = a.dv / (NU * 16);
   const int vb = blockIdx.x % splits, h = (blockIdx.x / splits) % a.Hv, n = blockIdx.x / (splits * a.Hv);
   const int hk = h / (a.Hv / a.Hk);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t2 = (lane & 3) * 2;
-  const int col0 = vb * NW * 16 + warp * 16;  // the warp's first column of dv
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, unit = warp >> 2, w = warp & 3, g = lane >> 2, t2 = (lane & 3) * 2;
+  const int col0 = vb * NU * 16 + unit * 16;  // the unit's first column of dv
   const long long start = a.cu ? a.cu[n] : 0, end = a.cu ? a.cu[n + 1] : a.T, c0 = a.cu ? a.cbase[n] : 0;
   const int chunks = static_cast<int>((end - start + C - 1) / C);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sm.full[i], THREADS);
+      bar_init(&sm.empty[i], NU * 4);
+    }
+    for (int i = 0; i < NU; ++i) {
+      bar_init(&sm.state_ready[i], 4);
+      bar_init(&sm.r_ready[i], 4);
+      bar_init(&sm.u_ready[i], 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
 
-  float s[2 * KT][4];  // S^T: rows = columns of dv, columns = dk
+  float s[2 * KW][4];  // rows = columns of dv, columns = dk [16 KW w, 16 KW (w + 1))
   const long long sbase = (static_cast<long long>(n) * a.Hv + h) * DK * a.dv + col0;
+  const int kd0 = 16 * KW * w;
 #pragma unroll
-  for (int j = 0; j < 2 * KT; ++j)
+  for (int j = 0; j < 2 * KW; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      s[j][e] = a.s_in ? a.s_in[sbase + static_cast<long long>(8 * j + t2 + (e & 1)) * a.dv + g + 8 * (e >> 1)] : 0.f;
+      s[j][e] = a.s_in ? a.s_in[sbase + static_cast<long long>(kd0 + 8 * j + t2 + (e & 1)) * a.dv + g + 8 * (e >> 1)] : 0.f;
 
   auto fetch = [&](int c) {
-    Stage& x = st[c & 1];
+    Stage& x = sm.stage[c & 1];
     const long long t0 = start + static_cast<long long>(c) * C;
     const int len = end - t0 < C ? static_cast<int>(end - t0) : C;
     const long long rec = (c0 + c) * a.Hv + h;
-    load_rows<DK, THREADS>(x.k, P, static_cast<const bf16*>(a.k) + t0 * a.k_ts + hk * a.k_hs, a.k_ts, len);
-    load_rows<DK, THREADS>(x.q, P, static_cast<const bf16*>(a.q) + t0 * a.q_ts + hk * a.q_hs, a.q_ts, len);
-    load_rows<NW * 16, THREADS>(x.v, VP, static_cast<const bf16*>(a.v) + t0 * a.v_ts + h * a.v_hs + vb * NW * 16, a.v_ts, len);
-    load_square<4, THREADS>(x.ap, static_cast<const bf16*>(a.ap) + rec * DELTA_AP);
+    copy_tile<DK, THREADS>(x.k, P, static_cast<const bf16*>(a.k) + t0 * a.k_ts + hk * a.k_hs, a.k_ts, C, len);
+    copy_tile<64, THREADS>(x.ap, APITCH, static_cast<const bf16*>(a.ap) + rec * DELTA_AP, C, 4 * C, 4 * C);
+    copy_tile<DK, THREADS>(x.q, P, static_cast<const bf16*>(a.q) + t0 * a.q_ts + hk * a.q_hs, a.q_ts, C, len);
+    copy_tile<NU * 16, THREADS>(x.v, VP, static_cast<const bf16*>(a.v) + t0 * a.v_ts + h * a.v_hs + vb * NU * 16, a.v_ts, C, len);
     load_vec<THREADS>(x.vec, a.vec + rec * DELTA_VEC, SEQ_ROWS);
+    bar_arrive_copies(&sm.full[c & 1]);
   };
-  if (chunks > 0) fetch(0);
-  cp_commit();
+  // The state in front of chunk c: for the unit's other warps, and for the backward pass.
+  auto publish_state = [&](int c) {
+    uint4* sf = KEEP ? reinterpret_cast<uint4*>(a.states) + ((((c0 + c) * a.Hv + h) * (a.dv / 16) + (col0 >> 4)) * 2) * KT * 32 + lane : nullptr;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      uint32_t hi[4], lo[4];
+      split_a(s[2 * k], s[2 * k + 1], hi, lo);
+      put(sm.state[unit][KW * w + k], hi, lo);
+      if (KEEP) {
+        sf[(KW * w + k) * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        sf[(KT + KW * w + k) * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+    bar_arrive(&sm.state_ready[unit]);
+  };
+  if (chunks > 0) {
+    fetch(0);
+    publish_state(0);
+  }
   for (int c = 0; c < chunks; ++c) {
-    if (c + 1 < chunks) fetch(c + 1);
-    cp_commit();
-    cp_wait<1>();
-    __syncthreads();
-    Stage& x = st[c & 1];
+    Stage& x = sm.stage[c & 1];
+    const uint32_t parity = c & 1, turn = (c >> 1) & 1;
     const long long t0 = start + static_cast<long long>(c) * C;
     const int len = end - t0 < C ? static_cast<int>(end - t0) : C;
     const bf16 *ahi = x.ap, *alo = x.ap + C * APITCH, *phi = x.ap + 2 * C * APITCH, *plo = x.ap + 3 * C * APITCH;
-    uint4* sf = KEEP ? reinterpret_cast<uint4*>(a.states) + ((((c0 + c) * a.Hv + h) * (a.dv / 16) + (col0 >> 4)) * 2) * KT * 32 + lane : nullptr;
+    const int tok = 16 * w;  // the warp's first token
+    const float* vec = x.vec + tok + t2;
+    if (c + 1 < chunks) {  // the other buffer is free when all warps are done with chunk c - 1
+      if (c > 0) bar_wait(&sm.empty[(c + 1) & 1], ((c - 1) >> 1) & 1, a.status);
+      fetch(c + 1);
+    }
+    bar_wait(&sm.full[c & 1], turn, a.status);
+    bar_wait(&sm.state_ready[unit], parity, a.status);
 
-    bf16* stage = x.v + warp * 16;
-    const long long out0 = (t0 * a.Hv + h) * a.dv + col0, ostride = static_cast<long long>(a.Hv) * a.dv;
-    auto rest = [](float f) { return f - __bfloat162float(__float2bfloat16(f)); };
-
-    // (K S)^T
-    float u[8][4], y[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[j][e] = 0.f;
+    // (K S)^T of the warp's tokens
+    float y[2][4], z[2][4];
+    clear(y);
+    clear(z);
 #pragma unroll
     for (int kk = 0; kk < KT; ++kk) {
-      uint32_t hi[4], lo[4], b[4][4];
-      split_a(s[2 * kk], s[2 * kk + 1], hi, lo);
-      if (KEEP) {
-        sf[kk * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        sf[(KT + kk) * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b_from_nk(b[j], x.k, P, 16 * j, 16 * kk);
-      mma2<4>(y, hi, lo, b);
+      uint32_t hi[4], lo[4], b[4];
+      get(sm.state[unit][kk], hi, lo);
+      b_from_nk(b, x.k, P, tok, 16 * kk);
+      mma_pair(y, hi, b);
+      mma_pair(z, lo, b);
     }
-    // u <- beta (V - e^G K S)^T
+    add_to(y, z);
+    // r = beta (V - e^G K S)^T
+    uint32_t v[4];
+    float2 be[2], f2[2];
+    a_from_km(v, x.v, VP, tok, unit * 16);
+    factors(vec + V_YK * 64, f2);
+    scale_tokens(y, f2);
+    factors(vec + V_BETA * 64, be);
+    float u[2][4];
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      uint32_t v[4];
-      a_from_km(v, x.v, VP, 8 * j, warp * 16);
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const int tok = 8 * (j + f) + t2;
-        const float2 yk = *reinterpret_cast<const float2*>(x.vec + V_YK * 64 + tok);
-        const float2 be = *reinterpret_cast<const float2*>(x.vec + V_BETA * 64 + tok);
-        float(&z)[4] = y[j + f];
-        z[0] *= yk.x;
-        z[1] *= yk.y;
-        z[2] *= yk.x;
-        z[3] *= yk.y;
-        u[j + f][0] = be.x * (lo_half(v[2 * f]) - z[0]);
-        u[j + f][1] = be.y * (hi_half(v[2 * f]) - z[1]);
-        u[j + f][2] = be.x * (lo_half(v[2 * f + 1]) - z[2]);
-        u[j + f][3] = be.y * (hi_half(v[2 * f + 1]) - z[3]);
-      }
+    for (int f = 0; f < 2; ++f) {
+      u[f][0] = be[f].x * (lo_half(v[2 * f]) - y[f][0]);
+      u[f][1] = be[f].y * (hi_half(v[2 * f]) - y[f][1]);
+      u[f][2] = be[f].x * (lo_half(v[2 * f + 1]) - y[f][2]);
+      u[f][3] = be[f].y * (hi_half(v[2 * f + 1]) - y[f][3]);
     }
-    // U^T = u + u (A - I)^T, from the last tokens to the first: column tile n needs the tiles up to n, so it may replace
-    // its own. y becomes the memory read at each token, m = e^G K S - ((A - I) u) / beta, in 16 bits, and U is
+    {
+      uint32_t hi[4], lo[4];
+      split_a(u[0], u[1], hi, lo);
+      put(sm.r[unit][w], hi, lo);
+    }
+    bar_arrive(&sm.r_ready[unit]);
+    // while the others get there: e^G Q S
+    float o[2][4];
+    clear(o);
+    clear(z);
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) {
+      uint32_t hi[4], lo[4], b[4];
+      get(sm.state[unit][kk], hi, lo);
+      b_from_nk(b, x.q, P, tok, 16 * kk);
+      mma_pair(o, hi, b);
+      mma_pair(z, lo, b);
+    }
+    add_to(o, z);
+    factors(vec + V_OQ * 64, f2);
+    scale_tokens(o, f2);
+    bar_wait(&sm.r_ready[unit], parity, a.status);
+    // (A - I) r; y becomes the memory read at each token, m = e^G K S - ((A - I) r) / beta, in 16 bits, and U is
     // beta (V - m), which the backward pass makes again from the m it reads: the products of dg must see the same U.
+    float m[2][4], m2[2][4], m3[2][4];
+    clear(m);
+    clear(m2);
+    clear(m3);
+    for (int kk = 0; kk <= w; ++kk) {
+      uint32_t hi[4], lo[4], b[4];
+      get(sm.r[unit][kk], hi, lo);
+      b_from_nk(b, ahi, APITCH, tok, 16 * kk);
+      mma_pair(m, hi, b);
+      mma_pair(m2, lo, b);
+      b_from_nk(b, alo, APITCH, tok, 16 * kk);
+      mma_pair(m3, hi, b);
+    }
+    add_to(m2, m3);
+    add_to(m, m2);
+    uint32_t mh[4], ml[4];
 #pragma unroll
-    for (int np = 3; np >= 0; --np) {
-      float w[2][4];
+    for (int f = 0; f < 2; ++f) {
+      m[f][0] = y[f][0] - __fdividef(m[f][0], be[f].x);
+      m[f][1] = y[f][1] - __fdividef(m[f][1], be[f].y);
+      m[f][2] = y[f][2] - __fdividef(m[f][2], be[f].x);
+      m[f][3] = y[f][3] - __fdividef(m[f][3], be[f].y);
+    }
+    split_a(m[0], m[1], mh, ml);
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * f + e;
+        memory_term(v[i], mh[i], ml[i], be[f], m[f][2 * e], m[f][2 * e + 1], u[f][2 * e], u[f][2 * e + 1]);
+      }
+    {
+      uint32_t hi[4], lo[4];
+      split_a(u[0], u[1], hi, lo);
+      put(sm.u[unit][w], hi, lo);
+      float su[2][4];
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[f][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk <= np; ++kk) {
-        uint32_t hi[4], lo[4], b[4], c[4];
-        split_a(u[2 * kk], u[2 * kk + 1], hi, lo);
-        b_from_nk(b, ahi, APITCH, 16 * np, 16 * kk);
-        b_from_nk(c, alo, APITCH, 16 * np, 16 * kk);
-        mma(w[0], hi, b[0], b[1]);
-        mma(w[1], hi, b[2], b[3]);
-        mma(w[0], lo, b[0], b[1]);
-        mma(w[1], lo, b[2], b[3]);
-        mma(w[0], hi, c[0], c[1]);
-        mma(w[1], hi, c[2], c[3]);
-      }
-      uint32_t v[4], mh[4], ml[4];
-      a_from_km(v, x.v, VP, 16 * np, warp * 16);
-      float m[2][4];
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float2 be = *reinterpret_cast<const float2*>(x.vec + V_BETA * 64 + 16 * np + 8 * f + t2);
-        m[f][0] = y[2 * np + f][0] - __fdividef(w[f][0], be.x);
-        m[f][1] = y[2 * np + f][1] - __fdividef(w[f][1], be.y);
-        m[f][2] = y[2 * np + f][2] - __fdividef(w[f][2], be.x);
-        m[f][3] = y[2 * np + f][3] - __fdividef(w[f][3], be.y);
-      }
-      split_a(m[0], m[1], mh, ml);
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float2 be = *reinterpret_cast<const float2*>(x.vec + V_BETA * 64 + 16 * np + 8 * f + t2);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * f + e;
-          memory_term(v[i], mh[i], ml[i], be, y[2 * np + f][2 * e], y[2 * np + f][2 * e + 1], u[2 * np + f][2 * e], u[2 * np + f][2 * e + 1]);
-        }
-      }
+        for (int e = 0; e < 4; ++e) su[f][e] = u[f][e];
+      factors(vec + V_SU * 64, f2);
+      scale_tokens(su, f2);
+      split_a(su[0], su[1], hi, lo);
+      put(sm.su[unit][w], hi, lo);
     }
-    if (KEEP) {
-      __syncwarp();
-      store_tokens(stage, VP, static_cast<bf16*>(a.mem) + out0, ostride, len, [&](int j, int e) { return y[j][e]; });
-      store_tokens(stage, VP, static_cast<bf16*>(a.mem_lo) + out0, ostride, len, [&](int j, int e) { return rest(y[j][e]); });
-      store_tokens(stage, VP, static_cast<bf16*>(a.u) + out0, ostride, len, [&](int j, int e) { return u[j][e]; });
-      store_tokens(stage, VP, static_cast<bf16*>(a.u_lo) + out0, ostride, len, [&](int j, int e) { return rest(u[j][e]); });
-    }
-    // what earlier tokens give to the output: e^G Q S + (P - diag P) U
-    float(&o)[8][4] = y;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < KT; ++kk) {
-      uint32_t hi[4], lo[4], b[4][4];
-      split_a(s[2 * kk], s[2 * kk + 1], hi, lo);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b_from_nk(b[j], x.q, P, 16 * j, 16 * kk);
-      mma2<4>(o, hi, lo, b);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 oq = *reinterpret_cast<const float2*>(x.vec + V_OQ * 64 + 8 * j + t2);
-      o[j][0] *= oq.x;
-      o[j][1] *= oq.y;
-      o[j][2] *= oq.x;
-      o[j][3] *= oq.y;
-    }
-    // with U: its part of the output, and S^T <- e^{G_C} S^T + (e^{G_C - G} U)^T K
+    bar_arrive(&sm.u_ready[unit]);
+    bf16* stage = sm.out[warp];
+    const int left = len - tok;  // of the warp's tokens
+    const long long out0 = ((t0 + tok) * a.Hv + h) * a.dv + col0, ostride = static_cast<long long>(a.Hv) * a.dv;
+    bar_wait(&sm.u_ready[unit], parity, a.status);
+    // S^T <- e^{G_C} S^T + (e^{G_C - G} U)^T K, the warp's columns of dk
     const float ge = x.vec[V_END * 64];
 #pragma unroll
-    for (int j = 0; j < 2 * KT; ++j)
+    for (int j = 0; j < 2 * KW; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[j][e] *= ge;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      uint32_t hi[4], lo[4], b[4], c4[4];
-      split_a(u[2 * kk], u[2 * kk + 1], hi, lo);
+      uint32_t hi[4], lo[4], b[KW][4];
+      get(sm.su[unit][kk], hi, lo);
 #pragma unroll
-      for (int np = kk; np < 4; ++np) {  // all four parts: the backward pass multiplies with this P and this U too
-        b_from_nk(b, phi, APITCH, 16 * np, 16 * kk);
-        b_from_nk(c4, plo, APITCH, 16 * np, 16 * kk);
-        mma(o[2 * np], hi, b[0], b[1]);
-        mma(o[2 * np + 1], hi, b[2], b[3]);
-        mma(o[2 * np], lo, b[0], b[1]);
-        mma(o[2 * np + 1], lo, b[2], b[3]);
-        mma(o[2 * np], hi, c4[0], c4[1]);
-        mma(o[2 * np + 1], hi, c4[2], c4[3]);
-        mma(o[2 * np], lo, c4[0], c4[1]);
-        mma(o[2 * np + 1], lo, c4[2], c4[3]);
-      }
-      float w[2][4];
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float2 su = *reinterpret_cast<const float2*>(x.vec + V_SU * 64 + 16 * kk + 8 * f + t2);
-        w[f][0] = u[2 * kk + f][0] * su.x;
-        w[f][1] = u[2 * kk + f][1] * su.y;
-        w[f][2] = u[2 * kk + f][2] * su.x;
-        w[f][3] = u[2 * kk + f][3] * su.y;
-      }
-      split_a(w[0], w[1], hi, lo);
-#pragma unroll
-      for (int j0 = 0; j0 < KT; j0 += 4) {
-        uint32_t bs[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) b_from_kn(bs[j], x.k, P, 16 * kk, 16 * (j0 + j));
-        mma2<4>(s + 2 * j0, hi, lo, bs);
-      }
+      for (int j = 0; j < KW; ++j) b_from_kn(b[j], x.k, P, 16 * kk, kd0 + 16 * j);
+      mma2<KW>(s, hi, lo, b);
     }
+    if (c + 1 < chunks) publish_state(c + 1);
+    // what earlier tokens give to the output: + (P - diag P) U, with all four parts: the backward pass multiplies with
+    // this P and this U too
+    clear(z);
+    clear(m2);
+    clear(m3);
+    for (int kk = 0; kk <= w; ++kk) {
+      uint32_t hi[4], lo[4], b[4];
+      get(sm.u[unit][kk], hi, lo);
+      b_from_nk(b, phi, APITCH, tok, 16 * kk);
+      mma_pair(o, hi, b);
+      mma_pair(z, lo, b);
+      b_from_nk(b, plo, APITCH, tok, 16 * kk);
+      mma_pair(m2, hi, b);
+      mma_pair(m3, lo, b);
+    }
+    add_to(m2, m3);
+    add_to(z, m2);
+    add_to(o, z);
     if (KEEP) {  // eight neighbouring columns of a token per quarter of the warp: full 32-byte sectors
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int tok = 8 * j + t2 + (e & 1);
-          if (tok < len) a.past[out0 + tok * ostride + g + 8 * (e >> 1)] = o[j][e];
+          const int i = 8 * f + t2 + (e & 1);
+          if (i < left) a.past[out0 + i * ostride + g + 8 * (e >> 1)] = o[f][e];
         }
+      store_tile(stage, static_cast<bf16*>(a.mem) + out0, ostride, left, m[0], m[1]);
+      store_rest(stage, static_cast<bf16*>(a.mem_lo) + out0, ostride, left, m[0], m[1]);
+      store_tile(stage, static_cast<bf16*>(a.u) + out0, ostride, left, u[0], u[1]);
+      store_rest(stage, static_cast<bf16*>(a.u_lo) + out0, ostride, left, u[0], u[1]);
     }
-    __syncwarp();
+    factors(vec + V_PD * 64, f2);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 pd = *reinterpret_cast<const float2*>(x.vec + V_PD * 64 + 8 * j + t2);
-      o[j][0] += pd.x * u[j][0];
-      o[j][1] += pd.y * u[j][1];
-      o[j][2] += pd.x * u[j][2];
-      o[j][3] += pd.y * u[j][3];
+    for (int f = 0; f < 2; ++f) {
+      o[f][0] += f2[f].x * u[f][0];
+      o[f][1] += f2[f].y * u[f][1];
+      o[f][2] += f2[f].x * u[f][2];
+      o[f][3] += f2[f].y * u[f][3];
     }
-    store_tokens(stage, VP, static_cast<bf16*>(a.o) + out0, ostride, len, [&](int j, int e) { return o[j][e]; });
-    __syncthreads();  // the buffer is filled again in the next turn
+    store_tile(stage, static_cast<bf16*>(a.o) + out0, ostride, left, o[0], o[1]);
+    bar_arrive(&sm.empty[c & 1]);
   }
-  cp_wait<0>();
   if (a.s_out) {
 #pragma unroll
-    for (int j = 0; j < 2 * KT; ++j)
+    for (int j = 0; j < 2 * KW; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        a.s_out[sbase + static_cast<long long>(8 * j + t2 + (e & 1)) * a.dv + g + 8 * (e >> 1)] = s[j][e];
+        a.s_out[sbase + static_cast<long long>(kd0 + 8 * j + t2 + (e & 1)) * a.dv + g + 8 * (e >> 1)] = s[j][e];
   }
 }
 
 // --------------------------------------------------------------------------------------------------------- backward
 
-template <int DK, int NW>
+template <int DK, int NU>
 struct BwdStage {
-  static constexpr int P = DK + 8, VP = NW * 16 + 8;
+  static constexpr int P = DK + 8, VP = NU * 16 + 8;
   bf16 k[C * P], q[C * P], dO[C * VP], v[C * VP], m[C * VP], ml[C * VP], ap[4 * C * APITCH];
   float vec[SEQ_ROWS * 64];
 };
+template <int DK, int NU>
+struct BwdSmem {
+  BwdStage<DK, NU> stage[2];
+  Operands state[NU][DK / 16], du[NU][4], dv[NU][4];
+  bf16 out[NU * 4][16 * OUT_PITCH];
+  uint64_t full[2], empty[2], state_ready[NU], du_ready[NU], dv_ready[NU];
+};
 
-template <int DK, int NW>
-__global__ void __launch_bounds__(NW * 32, 1)
+template <int DK, int NU>
+__global__ void __launch_bounds__(NU * 128, 1)
 backward_kernel(const DeltaArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  using Stage = BwdStage<DK, NW>;
-  constexpr int P = Stage::P, VP = Stage::VP, THREADS = NW * 32, KT = DK / 16;
-  Stage* st = reinterpret_cast<Stage*>(smem);
-  const int splits = a.dv / (NW * 16);
+  using Smem = BwdSmem<DK, NU>;
+  using Stage = BwdStage<DK, NU>;
+  constexpr int P = Stage::P, VP = Stage::VP, THREADS = NU * 128, KT = DK / 16, KW = KT / 4;
+  Smem& sm = *reinterpret_cast<Smem*>(smem);
+  const int splits = a.dv / (NU * 16);
   const int vb = blockIdx.x % splits, h = (blockIdx.x / splits) % a.Hv, n = blockIdx.x / (splits * a.Hv);
   const int hk = h / (a.Hv / a.Hk);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t2 = (lane & 3) * 2;
-  const int col0 = vb * NW * 16 + warp * 16, VT = a.dv / 16, vt = col0 >> 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, unit = warp >> 2, w = warp & 3, g = lane >> 2, t2 = (lane & 3) * 2;
+  const int col0 = vb * NU * 16 + unit * 16, VT = a.dv / 16, vt = col0 >> 4;
   const long long start = a.cu ? a.cu[n] : 0, end = a.cu ? a.cu[n + 1] : a.T, c0 = a.cu ? a.cbase[n] : 0;
   const int chunks = static_cast<int>((end - start + C - 1) / C);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&sm.full[i], THREADS);
+      bar_init(&sm.empty[i], NU * 4);
+    }
+    for (int i = 0; i < NU; ++i) {
+      bar_init(&sm.state_ready[i], 4);
+      bar_init(&sm.du_ready[i], 4);
+      bar_init(&sm.dv_ready[i], 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
 
-  float s[2 * KT][4];  // dS^T
+  float s[2 * KW][4];  // dS^T, the warp's columns of dk
   const long long sbase = (static_cast<long long>(n) * a.Hv + h) * DK * a.dv + col0;
+  const int kd0 = 16 * KW * w;
 #pragma unroll
-  for (int j = 0; j < 2 * KT; ++j)
+  for (int j = 0; j < 2 * KW; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      s[j][e] = a.ds_out ? a.ds_out[sbase + static_cast<long long>(8 * j + t2 + (e & 1)) * a.dv + g + 8 * (e >> 1)] : 0.f;
+      s[j][e] = a.ds_out ? a.ds_out[sbase + static_cast<long long>(kd0 + 8 * j + t2 + (e & 1)) * a.dv + g + 8 * (e >> 1)] : 0.f;
 
-  auto fetch = [&](int c) {
-    Stage& x = st[c & 1];
+  // i counts the chunks from the last one
+  auto fetch = [&](int i) {
+    Stage& x = sm.stage[i & 1];
+    const int c = chunks - 1 - i;
     const long long t0 = start + static_cast<long long>(c) * C;
     const int len = end - t0 < C ? static_cast<int>(end - t0) : C;
     const long long rec = (c0 + c) * a.Hv + h;
-    const long long row = (t0 * a.Hv + h) * a.dv + vb * NW * 16, stride = static_cast<long long>(a.Hv) * a.dv;
-    load_rows<DK, THREADS>(x.k, P, static_cast<const bf16*>(a.k) + t0 * a.k_ts + hk * a.k_hs, a.k_ts, len);
-    load_rows<DK, THREADS>(x.q, P, static_cast<const bf16*>(a.q) + t0 * a.q_ts + hk * a.q_hs, a.q_ts, len);
-    load_rows<NW * 16, THREADS>(x.dO, VP, static_cast<const bf16*>(a.dout) + row, stride, len);
-    load_rows<NW * 16, THREADS>(x.v, VP, static_cast<const bf16*>(a.v) + t0 * a.v_ts + h * a.v_hs + vb * NW * 16, a.v_ts, len);
-    load_rows<NW * 16, THREADS>(x.m, VP, static_cast<const bf16*>(a.mem) + row, stride, len);
-    load_rows<NW * 16, THREADS>(x.ml, VP, static_cast<const bf16*>(a.mem_lo) + row, stride, len);
-    load_square<4, THREADS>(x.ap, static_cast<const bf16*>(a.ap) + rec * DELTA_AP);
+    const long long row = (t0 * a.Hv + h) * a.dv + vb * NU * 16, stride = static_cast<long long>(a.Hv) * a.dv;
+    copy_tile<DK, THREADS>(x.k, P, static_cast<const bf16*>(a.k) + t0 * a.k_ts + hk * a.k_hs, a.k_ts, C, len);
+    copy_tile<64, THREADS>(x.ap, APITCH, static_cast<const bf16*>(a.ap) + rec * DELTA_AP, C, 4 * C, 4 * C);
+    copy_tile<NU * 16, THREADS>(x.dO, VP, static_cast<const bf16*>(a.dout) + row, stride, C, len);
+    copy_tile<DK, THREADS>(x.q, P, static_cast<const bf16*>(a.q) + t0 * a.q_ts + hk * a.q_hs, a.q_ts, C, len);
+    copy_tile<NU * 16, THREADS>(x.v, VP, static_cast<const bf16*>(a.v) + t0 * a.v_ts + h * a.v_hs + vb * NU * 16, a.v_ts, C, len);
+    copy_tile<NU * 16, THREADS>(x.m, VP, static_cast<const bf16*>(a.mem) + row, stride, C, len);
+    copy_tile<NU * 16, THREADS>(x.ml, VP, static_cast<const bf16*>(a.mem_lo) + row, stride, C, len);
     load_vec<THREADS>(x.vec, a.vec + rec * DELTA_VEC, SEQ_ROWS);
+    bar_arrive_copies(&sm.full[i & 1]);
   };
-  if (chunks > 0) fetch(chunks - 1);
-  cp_commit();
-  for (int c = chunks - 1; c >= 0; --c) {
-    if (c > 0) fetch(c - 1);
-    cp_commit();
-    cp_wait<1>();
-    __syncthreads();
-    Stage& x = st[c & 1];
+  // The gradient of the state behind chunk c: for the unit's other warps, and (high part) for dqk.
+  auto publish_state = [&](int c) {
+    uint4* df = reinterpret_cast<uint4*>(a.dstates) + (((c0 + c) * a.Hv + h) * VT + vt) * KT * 32 + lane;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      uint32_t hi[4], lo[4];
+      split_a(s[2 * k], s[2 * k + 1], hi, lo);
+      put(sm.state[unit][KW * w + k], hi, lo);
+      df[(KW * w + k) * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    }
+    bar_arrive(&sm.state_ready[unit]);
+  };
+  if (chunks > 0) {
+    fetch(0);
+    publish_state(chunks - 1);
+  }
+  for (int i = 0; i < chunks; ++i) {
+    const int c = chunks - 1 - i;
+    Stage& x = sm.stage[i & 1];
+    const uint32_t parity = i & 1, turn = (i >> 1) & 1;
     const long long t0 = start + static_cast<long long>(c) * C;
     const int len = end - t0 < C ? static_cast<int>(end - t0) : C;
     const long long rec = (c0 + c) * a.Hv + h;
     const bf16 *ahi = x.ap, *alo = x.ap + C * APITCH, *phi = x.ap + 2 * C * APITCH, *plo = x.ap + 3 * C * APITCH;
-    uint4* df = reinterpret_cast<uint4*>(a.dstates) + (rec * VT + vt) * KT * 32 + lane;
+    const int tok = 16 * w;
+    const float* vec = x.vec + tok + t2;
+    // the warp's part of the state in front of the chunk, for <dS1, S0>
     const uint4* nf = reinterpret_cast<const uint4*>(a.states) + ((rec * VT + vt) * 2) * KT * 32 + lane;
+    uint4 sh[KW], sl[KW];
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      sh[k] = nf[(KW * w + k) * 32];
+      sl[k] = nf[(KT + KW * w + k) * 32];
+    }
+    if (i + 1 < chunks) {
+      if (i > 0) bar_wait(&sm.empty[(i + 1) & 1], ((i - 1) >> 1) & 1, a.status);
+      fetch(i + 1);
+    }
+    bar_wait(&sm.full[i & 1], turn, a.status);
 
-    // u = (e^{G_C - G} K dS1)^T; on the way <dS1, S0>
-    float u[8][4], sdot = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) u[j][e] = 0.f;
+    // what does not wait for the state: ((P - diag P)^T dO)^T of the warp's tokens
+    float u[2][4], z[2][4], y[2][4];
+    clear(u);
+    clear(z);
+    uint32_t fo[4];  // dO^T of the warp's tokens
+    a_from_km(fo, x.dO, VP, tok, unit * 16);
+    for (int kk = w; kk < 4; ++kk) {
+      uint32_t f[4], b[4];
+      a_from_km(f, x.dO, VP, 16 * kk, unit * 16);
+      b_from_kn(b, phi, APITCH, 16 * kk, tok);
+      mma_pair(u, f, b);
+      b_from_kn(b, plo, APITCH, 16 * kk, tok);
+      mma_pair(z, f, b);
+    }
+    add_to(u, z);
+    bar_wait(&sm.state_ready[unit], parity, a.status);
+    // y = (e^{G_C - G} K dS1)^T
+    clear(y);
+    clear(z);
 #pragma unroll
     for (int kk = 0; kk < KT; ++kk) {
-      uint32_t hi[4], lo[4], b[4][4];
-      split_a(s[2 * kk], s[2 * kk + 1], hi, lo);
-      df[kk * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      const uint4 qh = nf[kk * 32], ql = nf[(KT + kk) * 32];
-      const uint32_t wh[4] = {qh.x, qh.y, qh.z, qh.w}, wl[4] = {ql.x, ql.y, ql.z, ql.w};
+      uint32_t hi[4], lo[4], b[4];
+      get(sm.state[unit][kk], hi, lo);
+      b_from_nk(b, x.k, P, tok, 16 * kk);
+      mma_pair(y, hi, b);
+      mma_pair(z, lo, b);
+    }
+    add_to(y, z);
+    float2 f2[2], be[2];
+    factors(vec + V_SU * 64, f2);
+    scale_tokens(y, f2);
+    // du = dU^T = y + u + (diag P dO)^T
+    add_to(u, y);
+    float du[2][4];
+    factors(vec + V_PD * 64, f2);
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      du[f][0] = f2[f].x * lo_half(fo[2 * f]);
+      du[f][1] = f2[f].y * hi_half(fo[2 * f]);
+      du[f][2] = f2[f].x * lo_half(fo[2 * f + 1]);
+      du[f][3] = f2[f].y * hi_half(fo[2 * f + 1]);
+    }
+    {
+      float d[2][4];
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[f][e] = u[f][e] + du[f][e];
+      split_a(d[0], d[1], hi, lo);
+      put(sm.du[unit][w], hi, lo);
+    }
+    bar_arrive(&sm.du_ready[unit]);
+    // while the others get there: S0 . dS1, U and m of the warp's tokens, and Q^T diag(e^G) dO into the state
+    const float ge = x.vec[V_END * 64];
+    float sdot = 0.f;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const uint32_t wh[4] = {sh[k].x, sh[k].y, sh[k].z, sh[k].w}, wl[4] = {sl[k].x, sl[k].y, sl[k].z, sl[k].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        sdot += s[2 * kk + (e >> 1)][2 * (e & 1)] * (lo_half(wh[e]) + lo_half(wl[e]));
-        sdot += s[2 * kk + (e >> 1)][2 * (e & 1) + 1] * (hi_half(wh[e]) + hi_half(wl[e]));
+        sdot += s[2 * k + (e >> 1)][2 * (e & 1)] * (lo_half(wh[e]) + lo_half(wl[e]));
+        sdot += s[2 * k + (e >> 1)][2 * (e & 1) + 1] * (hi_half(wh[e]) + hi_half(wl[e]));
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b_from_nk(b[j], x.k, P, 16 * j, 16 * kk);
-      mma2<4>(u, hi, lo, b);
     }
-    const float ge = x.vec[V_END * 64];
     sdot *= ge;
+    uint32_t fv[4], fm[4], fl[4];
+    a_from_km(fv, x.v, VP, tok, unit * 16);
+    a_from_km(fm, x.m, VP, tok, unit * 16);
+    a_from_km(fl, x.ml, VP, tok, unit * 16);
+    factors(vec + V_BETA * 64, be);
+    float mm[2][4], uu[2][4];
 #pragma unroll
-    for (int j = 0; j < 2 * KT; ++j)
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[j][e] *= ge;
-    // Tiles j, j + 1 of the memory term m^T and of U^T = beta (V - m)^T
-    auto load_mu = [&](int j, float(&mm)[2][4], float(&uu)[2][4]) {
-      uint32_t fv[4], fm[4], fl[4];
-      a_from_km(fv, x.v, VP, 8 * j, warp * 16);
-      a_from_km(fm, x.m, VP, 8 * j, warp * 16);
-      a_from_km(fl, x.ml, VP, 8 * j, warp * 16);
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float2 be = *reinterpret_cast<const float2*>(x.vec + V_BETA * 64 + 8 * (j + f) + t2);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * f + e;
-          memory_term(fv[i], fm[i], fl[i], be, mm[f][2 * e], mm[f][2 * e + 1], uu[f][2 * e], uu[f][2 * e + 1]);
-          uint32_t hi, lo;  // the two parts that the forward pass multiplied with P
-          split2(uu[f][2 * e], uu[f][2 * e + 1], hi, lo);
-          uu[f][2 * e] = lo_half(hi) + lo_half(lo);
-          uu[f][2 * e + 1] = hi_half(hi) + hi_half(lo);
-        }
+      for (int e = 0; e < 2; ++e) {
+        const int q = 2 * f + e;
+        memory_term(fv[q], fm[q], fl[q], be[f], mm[f][2 * e], mm[f][2 * e + 1], uu[f][2 * e], uu[f][2 * e + 1]);
+        uint32_t hi, lo;  // the two parts that the forward pass multiplied with P
+        split2(uu[f][2 * e], uu[f][2 * e + 1], hi, lo);
+        uu[f][2 * e] = lo_half(hi) + lo_half(lo);
+        uu[f][2 * e + 1] = hi_half(hi) + hi_half(lo);
       }
-    };
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      float mm[2][4], uu[2][4];
-      load_mu(j, mm, uu);
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float2 su = *reinterpret_cast<const float2*>(x.vec + V_SU * 64 + 8 * (j + f) + t2);
-        u[j + f][0] *= su.x;
-        u[j + f][1] *= su.y;
-        u[j + f][2] *= su.x;
-        u[j + f][3] *= su.y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sdot += u[j + f][e] * uu[f][e];
-      }
-    }
+      for (int e = 0; e < 4; ++e) sdot += y[f][e] * uu[f][e];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sdot += __shfl_xor_sync(0xffffffffu, sdot, o);
-    if (lane == 0) a.sdots[rec * VT + vt] = sdot;
-    // u += ((P - diag P)^T dO)^T, du = u + (diag P dO)^T = dU^T; and Q^T diag(e^G) dO into the state
-    float du[8][4];
+    if (lane == 0) a.sdots[(rec * VT + vt) * 4 + w] = sdot;
+#pragma unroll
+    for (int j = 0; j < 2 * KW; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[j][e] *= ge;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      uint32_t f[4], hi[4], lo[4], b[4];
-      a_from_km(f, x.dO, VP, 16 * kk, warp * 16);
+      uint32_t f[4], hi[4], lo[4], b[KW][4];
+      a_from_km(f, x.dO, VP, 16 * kk, unit * 16);
+      float2 oq[2];
+      factors(x.vec + V_OQ * 64 + 16 * kk + t2, oq);
 #pragma unroll
-      for (int np = 0; np <= kk; ++np) {
-        b_from_kn(b, phi, APITCH, 16 * kk, 16 * np);
-        mma(u[2 * np], f, b[0], b[1]);
-        mma(u[2 * np + 1], f, b[2], b[3]);
-        b_from_kn(b, plo, APITCH, 16 * kk, 16 * np);
-        mma(u[2 * np], f, b[0], b[1]);
-        mma(u[2 * np + 1], f, b[2], b[3]);
-      }
+      for (int e = 0; e < 4; ++e) split2(lo_half(f[e]) * oq[e >> 1].x, hi_half(f[e]) * oq[e >> 1].y, hi[e], lo[e]);
+#pragma unroll
+      for (int j = 0; j < KW; ++j) b_from_kn(b[j], x.q, P, 16 * kk, kd0 + 16 * j);
+      mma2<KW>(s, hi, lo, b);
+    }
+    bar_wait(&sm.du_ready[unit], parity, a.status);
+    // u <- u + dU^T (A - I): X without what the token's own output asks for
+    clear(y);
+    clear(z);
+    for (int kk = w; kk < 4; ++kk) {
+      uint32_t hi[4], lo[4], b[4];
+      get(sm.du[unit][kk], hi, lo);
+      b_from_kn(b, ahi, APITCH, 16 * kk, tok);
+      mma_pair(u, hi, b);
+      mma_pair(y, lo, b);
+      b_from_kn(b, alo, APITCH, 16 * kk, tok);
+      mma_pair(z, hi, b);
+    }
+    add_to(y, z);
+    add_to(u, y);
+    // X = u + (diag P dO)^T, dV = beta X, and the row sums U . u, U . X and m . dV over the unit's 16 columns
+    float d[3][4];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      d[0][2 * f] = uu[f][0] * u[f][0] + uu[f][2] * u[f][2];
+      d[0][2 * f + 1] = uu[f][1] * u[f][1] + uu[f][3] * u[f][3];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[f][e] += du[f][e];
+      d[1][2 * f] = uu[f][0] * u[f][0] + uu[f][2] * u[f][2];
+      d[1][2 * f + 1] = uu[f][1] * u[f][1] + uu[f][3] * u[f][3];
+    }
+    scale_tokens(u, be);
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      d[2][2 * f] = mm[f][0] * u[f][0] + mm[f][2] * u[f][2];
+      d[2][2 * f + 1] = mm[f][1] * u[f][1] + mm[f][3] * u[f][3];
+    }
+    {
+      float b[2][4];
+      uint32_t hi[4], lo[4];
+      factors(vec + V_YK * 64, f2);
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[f][e] = -u[f][e];
+      scale_tokens(b, f2);
+      split_a(b[0], b[1], hi, lo);
+      put(sm.dv[unit][w], hi, lo);
+    }
+    bar_arrive(&sm.dv_ready[unit]);
+    float* rd = a.rowdots + (rec * VT + vt) * 192 + tok + t2;
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 pd = *reinterpret_cast<const float2*>(x.vec + V_PD * 64 + 16 * kk + 8 * (e >> 1) + t2);
-        du[2 * kk + (e >> 1)][2 * (e & 1)] = pd.x * lo_half(f[e]);
-        du[2 * kk + (e >> 1)][2 * (e & 1) + 1] = pd.y * hi_half(f[e]);
+        float r = d[q][e];
+        r += __shfl_xor_sync(0xffffffffu, r, 4);
+        r += __shfl_xor_sync(0xffffffffu, r, 8);
+        r += __shfl_xor_sync(0xffffffffu, r, 16);
+        if (g == 0) rd[q * 64 + 8 * (e >> 1) + (e & 1)] = r;
       }
-      const float2 q0 = *reinterpret_cast<const float2*>(x.vec + V_OQ * 64 + 16 * kk + t2);
-      const float2 q1 = *reinterpret_cast<const float2*>(x.vec + V_OQ * 64 + 16 * kk + 8 + t2);
-      split2(lo_half(f[0]) * q0.x, hi_half(f[0]) * q0.y, hi[0], lo[0]);
-      split2(lo_half(f[1]) * q0.x, hi_half(f[1]) * q0.y, hi[1], lo[1]);
-      split2(lo_half(f[2]) * q1.x, hi_half(f[2]) * q1.y, hi[2], lo[2]);
-      split2(lo_half(f[3]) * q1.x, hi_half(f[3]) * q1.y, hi[3], lo[3]);
-#pragma unroll
-      for (int j0 = 0; j0 < KT; j0 += 4) {
-        uint32_t bs[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) b_from_kn(bs[j], x.q, P, 16 * kk, 16 * (j0 + j));
-        mma2<4>(s + 2 * j0, hi, lo, bs);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) du[j][e] += u[j][e];
-    // u <- u + dU^T (A - I): X without what the token's own output asks for
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint32_t hi[4], lo[4], b[4];
-      split_a(du[2 * kk], du[2 * kk + 1], hi, lo);
-#pragma unroll
-      for (int np = 0; np <= kk; ++np) {
-        b_from_kn(b, ahi, APITCH, 16 * kk, 16 * np);
-        mma(u[2 * np], hi, b[0], b[1]);
-        mma(u[2 * np + 1], hi, b[2], b[3]);
-        mma(u[2 * np], lo, b[0], b[1]);
-        mma(u[2 * np + 1], lo, b[2], b[3]);
-        b_from_kn(b, alo, APITCH, 16 * kk, 16 * np);
-        mma(u[2 * np], hi, b[0], b[1]);
-        mma(u[2 * np + 1], hi, b[2], b[3]);
-      }
-    }
-    // X = u + (diag P dO)^T, and the row sums U . u, U . X and beta m . X over the warp's 16 columns
-    float d[3][16];
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      float mm[2][4], uu[2][4];
-      uint32_t fo[4];
-      load_mu(j, mm, uu);
-      a_from_km(fo, x.dO, VP, 8 * j, warp * 16);
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float2 pd = *reinterpret_cast<const float2*>(x.vec + V_PD * 64 + 8 * (j + f) + t2);
-        const float2 be = *reinterpret_cast<const float2*>(x.vec + V_BETA * 64 + 8 * (j + f) + t2);
-        float(&z)[4] = u[j + f];
-        const int c0 = 2 * (j + f);
-        d[0][c0] = uu[f][0] * z[0] + uu[f][2] * z[2];
-        d[0][c0 + 1] = uu[f][1] * z[1] + uu[f][3] * z[3];
-        z[0] += pd.x * lo_half(fo[2 * f]);
-        z[1] += pd.y * hi_half(fo[2 * f]);
-        z[2] += pd.x * lo_half(fo[2 * f + 1]);
-        z[3] += pd.y * hi_half(fo[2 * f + 1]);
-        d[1][c0] = uu[f][0] * z[0] + uu[f][2] * z[2];
-        d[1][c0 + 1] = uu[f][1] * z[1] + uu[f][3] * z[3];
-        z[0] *= be.x;  // dV = beta X
-        z[1] *= be.y;
-        z[2] *= be.x;
-        z[3] *= be.y;
-        d[2][c0] = mm[f][0] * z[0] + mm[f][2] * z[2];
-        d[2][c0 + 1] = mm[f][1] * z[1] + mm[f][3] * z[3];
-      }
-    }
-    float* rd = a.rowdots + (rec * VT + vt) * 192;
-#pragma unroll
-    for (int m = 0; m < 3; ++m)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float v = d[m][i];
-        v += __shfl_xor_sync(0xffffffffu, v, 4);
-        v += __shfl_xor_sync(0xffffffffu, v, 8);
-        v += __shfl_xor_sync(0xffffffffu, v, 16);
-        if (g == 0) rd[m * 64 + 8 * (i >> 1) + t2 + (i & 1)] = v;
-      }
+    store_tile(sm.out[warp], static_cast<bf16*>(a.dv_) + ((t0 + tok) * a.Hv + h) * a.dv + col0,
+               static_cast<long long>(a.Hv) * a.dv, len - tok, u[0], u[1]);
+    bar_wait(&sm.dv_ready[unit], parity, a.status);
     // dS0 -= K^T diag(e^G) dV
-    __syncwarp();
-    store_tokens(x.v + warp * 16, VP, static_cast<bf16*>(a.dv_) + (t0 * a.Hv + h) * a.dv + col0,
-                 static_cast<long long>(a.Hv) * a.dv, len, [&](int j, int e) { return u[j][e]; });
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      uint32_t hi[4], lo[4], b[4];
-      float w[2][4];
+      uint32_t hi[4], lo[4], b[KW][4];
+      get(sm.dv[unit][kk], hi, lo);
 #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float2 yk = *reinterpret_cast<const float2*>(x.vec + V_YK * 64 + 16 * kk + 8 * f + t2);
-        w[f][0] = -u[2 * kk + f][0] * yk.x;
-        w[f][1] = -u[2 * kk + f][1] * yk.y;
-        w[f][2] = -u[2 * kk + f][2] * yk.x;
-        w[f][3] = -u[2 * kk + f][3] * yk.y;
-      }
-      split_a(w[0], w[1], hi, lo);
-#pragma unroll
-      for (int j0 = 0; j0 < KT; j0 += 4) {
-        uint32_t bs[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) b_from_kn(bs[j], x.k, P, 16 * kk, 16 * (j0 + j));
-        mma2<4>(s + 2 * j0, hi, lo, bs);
-      }
+      for (int j = 0; j < KW; ++j) b_from_kn(b[j], x.k, P, 16 * kk, kd0 + 16 * j);
+      mma2<KW>(s, hi, lo, b);
     }
-    __syncthreads();
+    if (c > 0) publish_state(c - 1);
+    bar_arrive(&sm.empty[i & 1]);
   }
-  cp_wait<0>();
   if (a.ds_in) {
 #pragma unroll
-    for (int j = 0; j < 2 * KT; ++j)
+    for (int j = 0; j < 2 * KW; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        a.ds_in[sbase + static_cast<long long>(8 * j + t2 + (e & 1)) * a.dv + g + 8 * (e >> 1)] = s[j][e];
+        a.ds_in[sbase + static_cast<long long>(kd0 + 8 * j + t2 + (e & 1)) * a.dv + g + 8 * (e >> 1)] = s[j][e];
   }
 }
 
@@ -1266,7 +1399,7 @@ gates_kernel(const DeltaArgs a) {
   if (warp != 0) return;
   const float* rd = a.rowdots + rec * VT * 192;
   double carry = 0.0;
-  for (int v = 0; v < VT; ++v) carry += a.sdots[rec * VT + v];
+  for (int v = 0; v < 4 * VT; ++v) carry += a.sdots[rec * 4 * VT + v];
 #pragma unroll
   for (int half = 1; half >= 0; --half) {
     const int i = half * 32 + lane;
@@ -1299,23 +1432,23 @@ bool allow_smem(K kernel, size_t bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess;
 }
 
-template <int DK, int NW, bool KEEP>
+template <int DK, int NU, bool KEEP>
 int launch_forward(const DeltaArgs& a, cudaStream_t s) {
-  const long long grid = static_cast<long long>(a.N) * a.Hv * (a.dv / (NW * 16));
+  const long long grid = static_cast<long long>(a.N) * a.Hv * (a.dv / (NU * 16));
   if (grid > INT32_MAX) return -2;
-  const size_t bytes = 2 * sizeof(FwdStage<DK, NW>);
-  if (!allow_smem(forward_kernel<DK, NW, KEEP>, bytes)) return -3;
-  forward_kernel<DK, NW, KEEP><<<static_cast<unsigned>(grid), NW * 32, bytes, s>>>(a);
+  const size_t bytes = sizeof(FwdSmem<DK, NU>);
+  if (!allow_smem(forward_kernel<DK, NU, KEEP>, bytes)) return -3;
+  forward_kernel<DK, NU, KEEP><<<static_cast<unsigned>(grid), NU * 128, bytes, s>>>(a);
   return 0;
 }
 
-template <int DK, int NW>
+template <int DK, int NU>
 int launch_backward(const DeltaArgs& a, cudaStream_t s) {
-  const long long grid = static_cast<long long>(a.N) * a.Hv * (a.dv / (NW * 16));
+  const long long grid = static_cast<long long>(a.N) * a.Hv * (a.dv / (NU * 16));
   if (grid > INT32_MAX) return -2;
-  const size_t bytes = 2 * sizeof(BwdStage<DK, NW>);
-  if (!allow_smem(backward_kernel<DK, NW>, bytes)) return -3;
-  backward_kernel<DK, NW><<<static_cast<unsigned>(grid), NW * 32, bytes, s>>>(a);
+  const size_t bytes = sizeof(BwdSmem<DK, NU>);
+  if (!allow_smem(backward_kernel<DK, NU>, bytes)) return -3;
+  backward_kernel<DK, NU><<<static_cast<unsigned>(grid), NU * 128, bytes, s>>>(a);
   return 0;
 }
 
@@ -1334,14 +1467,14 @@ int forward_dk(const DeltaArgs& a, cudaStream_t s) {
     if (!allow_smem(prepare_kernel<DK>, bytes)) return -3;
     prepare_kernel<DK><<<static_cast<unsigned>(a.NC * a.Hk), PREP_THREADS, bytes, s>>>(a);
   }
-  const int rc = a.states ? launch_forward<DK, 4, true>(a, s) : launch_forward<DK, 4, false>(a, s);
+  const int rc = a.states ? launch_forward<DK, 2, true>(a, s) : launch_forward<DK, 2, false>(a, s);
   if (rc) return rc;
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 
 template <int DK>
 int backward_dk(const DeltaArgs& a, cudaStream_t s) {
-  int rc = launch_backward<DK, 4>(a, s);
+  int rc = launch_backward<DK, 2>(a, s);
   if (rc) return rc;
   if (a.NC > 0) {
     rc = a.dv == 64 ? launch_dqk<DK, 64>(a, s) : launch_dqk<DK, 128>(a, s);

@@ -34,10 +34,10 @@ struct DeltaArgs {
   float* ds_in = nullptr;         // gradient of s_in or null
   void* dstates = nullptr;      // bf16 fragments of the state gradients, half the size of `states`
   float* rowdots = nullptr;     // fp32 [NC, Hv, dv / 16, 3, 64]
-  float* sdots = nullptr;       // fp32 [NC, Hv, dv / 16]
+  float* sdots = nullptr;       // fp32 [NC, Hv, dv / 16, 4]
   void *dq = nullptr, *dkey = nullptr, *dv_ = nullptr;  // bf16, contiguous
   float *dg = nullptr, *dbeta = nullptr;                // fp32 [T, Hv]
-  int* status = nullptr;
+  int* status = nullptr;  // set when a wait runs out
 };
 
 // 0 on success; negative when the shape is not covered (dk, dv in {64, 128}).

@@ -107,7 +107,8 @@ class _GatedDeltaFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, s_in, bounds, first, scale, l2norm, want_state, keep):
         ctx.set_materialize_grads(False)
-        o, s_out, *kept = _ext.require().delta_fwd(q, k, v, g, beta, bounds, first, scale, l2norm, s_in, want_state, keep)
+        o, s_out, *kept = _ext.require().delta_fwd(q, k, v, g, beta, bounds, first, scale, l2norm, s_in, want_state, keep,
+                                                       _ext.status_tensor(v.device))
         if keep:
             ctx.save_for_backward(q, k, v, g, beta, bounds, first, *kept)
         ctx.cfg = (scale, l2norm)
@@ -122,7 +123,8 @@ class _GatedDeltaFn(torch.autograd.Function):
         want_ds = ctx.needs_input_grad[5]
         do = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if do is None else _dense16(do)
         dq, dk, dv, dg, dbeta, ds_in = _ext.require().delta_bwd(
-            do, None if ds_out is None else _dense16(ds_out), q, k, v, g, beta, bounds, first, scale, l2norm, want_ds, *kept)
+            do, None if ds_out is None else _dense16(ds_out), q, k, v, g, beta, bounds, first, scale, l2norm, want_ds, *kept,
+            _ext.status_tensor(v.device))
         return (dq, dk, dv, dg, dbeta, ds_in if want_ds else None) + (None,) * 6
 
 

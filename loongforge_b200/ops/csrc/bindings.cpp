@@ -1028,8 +1028,8 @@ lf::DeltaArgs delta_args(const at::Tensor& q, const at::Tensor& k, const at::Ten
   return a;
 }
 
-// {o, final state or empty}, and with `keep` what the backward pass reads: {past, memory, its remainder, U, its remainder,
-// chunk states, A / P, factors} (see DeltaArgs).
+// {o, final state or empty}, and with `keep` what the backward pass reads: {past, memory, U, chunk states, A / P,
+// factors} (see DeltaArgs).
 std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
                                   const at::Tensor& beta, c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first,
                                   double scale, bool l2norm, c10::optional<at::Tensor> s_in, bool want_state, bool keep,
@@ -1052,16 +1052,14 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, cons
   if (want_state) a.s_out = s_out.data_ptr<float>();
   std::vector<at::Tensor> out = {o, s_out};
   if (keep) {
-    at::Tensor past = at::empty({a.T, a.Hv, a.dv}, fl);
-    at::Tensor mem = at::empty_like(o), mem_lo = at::empty_like(o), u = at::empty_like(o), u_lo = at::empty_like(o);
+    const int64_t rows = a.NC * a.Hv * lf::DELTA_CHUNK;
+    at::Tensor past = at::empty({rows, a.dv}, fl), mem = at::empty({2, rows, a.dv}, bf), u = at::empty({2, rows, a.dv}, bf);
     at::Tensor states = at::empty({a.NC, a.Hv, 2, a.dv, a.dk}, bf);
-    a.past = past.data_ptr<float>();
+    a.past = past.data_ptr();
     a.mem = mem.data_ptr();
-    a.mem_lo = mem_lo.data_ptr();
     a.u = u.data_ptr();
-    a.u_lo = u_lo.data_ptr();
     a.states = states.data_ptr();
-    out.insert(out.end(), {past, mem, mem_lo, u, u_lo, states, ap, vec});
+    out.insert(out.end(), {past, mem, u, states, ap, vec});
   }
   const int rc = lf::delta_forward(a, cur_stream());
   TORCH_CHECK(rc == 0, "lf::delta_forward failed with code ", rc, " (dk = ", a.dk, ", dv = ", a.dv, ")");
@@ -1081,18 +1079,19 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, cons
 std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tensor> ds_out, const at::Tensor& q, const at::Tensor& k,
                                   const at::Tensor& v, const at::Tensor& g, const at::Tensor& beta,
                                   c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first, double scale, bool l2norm,
-                                  bool want_ds, const at::Tensor& past, const at::Tensor& mem, const at::Tensor& mem_lo,
-                                  const at::Tensor& u, const at::Tensor& u_lo, const at::Tensor& states, const at::Tensor& ap,
+                                  bool want_ds, const at::Tensor& past, const at::Tensor& mem, const at::Tensor& u,
+                                  const at::Tensor& states, const at::Tensor& ap,
                                   const at::Tensor& vec, const at::Tensor& status) {
   c10::cuda::CUDAGuard guard(q.device());
   lf::DeltaArgs a = delta_args(q, k, v, g, beta, bounds, first, scale, l2norm);
   check_status(status, q);
   a.status = status.data_ptr<int>();
   check_heads(dout, "dout", q);
-  for (const at::Tensor* t : {&dout, &mem, &mem_lo, &u, &u_lo})
-    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kBFloat16 && t->is_contiguous() &&
-                    t->numel() == a.T * a.Hv * a.dv, "the outputs' gradient must be contiguous bf16 [T, value heads, dv]");
-  TORCH_CHECK(past.device() == q.device() && past.scalar_type() == at::kFloat && past.is_contiguous() && past.numel() == a.T * a.Hv * a.dv);
+  TORCH_CHECK(dout.is_contiguous() && dout.numel() == a.T * a.Hv * a.dv, "the outputs' gradient must be contiguous bf16 [T, value heads, dv]");
+  const int64_t kept = a.NC * a.Hv * lf::DELTA_CHUNK * a.dv;
+  TORCH_CHECK(past.device() == q.device() && past.scalar_type() == at::kFloat && past.numel() == kept && mem.scalar_type() == at::kBFloat16 &&
+              mem.numel() == 2 * kept && u.scalar_type() == at::kBFloat16 && u.numel() == 2 * kept,
+              "what the forward pass kept does not fit these inputs");
   TORCH_CHECK(states.device() == q.device() && states.scalar_type() == at::kBFloat16 && states.numel() == a.NC * a.Hv * 2 * a.dk * a.dv &&
               ap.scalar_type() == at::kBFloat16 && ap.numel() == a.NC * a.Hv * lf::DELTA_AP && vec.scalar_type() == at::kFloat &&
               vec.numel() == a.NC * a.Hv * lf::DELTA_VEC, "what the forward pass kept does not fit these inputs");
@@ -1101,18 +1100,16 @@ std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tens
   at::Tensor dg = at::empty_like(g), dbeta = at::empty_like(beta);
   at::Tensor ds_in = want_ds ? at::empty({a.N, a.Hv, a.dk, a.dv}, fl) : at::empty({0}, fl);
   at::Tensor dstates = at::empty({a.NC, a.Hv, a.dv, a.dk}, bf);
-  at::Tensor rowdots = at::empty({a.NC, a.Hv, a.dv / 16, 3, 64}, fl), sdots = at::empty({a.NC, a.Hv, a.dv / 16, 4}, fl);
+  at::Tensor rowdots = at::empty({a.NC, a.Hv, a.dv / 16, 2, 64}, fl), sdots = at::empty({a.NC, a.Hv, a.dv / 16, 4}, fl);
   a.dout = dout.data_ptr();
   if (ds_out.has_value()) {
     check_state(*ds_out, "the final state's gradient", a.N, q, v);
     a.ds_out = ds_out->data_ptr<float>();
   }
   if (want_ds) a.ds_in = ds_in.data_ptr<float>();
-  a.past = past.data_ptr<float>();
+  a.past = past.data_ptr();
   a.mem = mem.data_ptr();
-  a.mem_lo = mem_lo.data_ptr();
   a.u = u.data_ptr();
-  a.u_lo = u_lo.data_ptr();
   a.states = states.data_ptr();
   a.ap = ap.data_ptr();
   a.vec = vec.data_ptr<float>();

@@ -532,18 +532,20 @@ __device__ __forceinline__ void store_tile(bf16* stage, bf16* out, long long str
   const int lane = threadIdx.x & 31, row = lane >> 1, v = (lane & 1) * 8;
   if (row < len) *reinterpret_cast<uint4*>(out + row * stride + v) = *reinterpret_cast<const uint4*>(stage + row * OUT_PITCH + v);
 }
-__device__ __forceinline__ float rest(float f) { return f - __bfloat162float(__float2bfloat16(f)); }
-__device__ __forceinline__ void store_rest(bf16* stage, bf16* out, long long stride, int len, const float (&c0)[4], const float (&c1)[4]) {
-  const float a[4] = {rest(c0[0]), rest(c0[1]), rest(c0[2]), rest(c0[3])}, b[4] = {rest(c1[0]), rest(c1[1]), rest(c1[2]), rest(c1[3])};
-  store_tile(stage, out, stride, len, a, b);
+// U = beta (v - m) of two neighbouring tokens of one column, m from its parts.
+__device__ __forceinline__ void memory_term(uint32_t v, uint32_t mh, uint32_t ml, float2 beta, float& u0, float& u1) {
+  u0 = beta.x * (lo_half(v) - (lo_half(mh) + lo_half(ml)));
+  u1 = beta.y * (hi_half(v) - (hi_half(mh) + hi_half(ml)));
 }
 
-// Two neighbouring tokens of one column: m from its parts, U = beta (v - m).
-__device__ __forceinline__ void memory_term(uint32_t v, uint32_t mh, uint32_t ml, float2 beta, float& m0, float& m1, float& u0, float& u1) {
-  m0 = lo_half(mh) + lo_half(ml);
-  m1 = hi_half(mh) + hi_half(ml);
-  u0 = beta.x * (lo_half(v) - m0);
-  u1 = beta.y * (hi_half(v) - m1);
+// The fp32 values of a fragment's two parts.
+__device__ __forceinline__ void join(const uint4& hi, const uint4& lo, float (&c)[2][4]) {
+  const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    c[i >> 1][2 * (i & 1)] = lo_half(h[i]) + lo_half(l[i]);
+    c[i >> 1][2 * (i & 1) + 1] = hi_half(h[i]) + hi_half(l[i]);
+  }
 }
 
 // Values of a factor row for the lane's four tokens: tile f, element pair.
@@ -677,28 +679,31 @@ forward_kernel(const DeltaArgs a) {
       fetch(c + 1);
     }
     bar_wait(&sm.full[c & 1], turn, a.status);
+    // everything that does not wait for the state is in registers before it comes
+    uint32_t bk[KT][4], v[4];
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) b_from_nk(bk[kk], x.k, P, tok, 16 * kk);
+    a_from_km(v, x.v, VP, tok, unit * 16);
+    float2 yk[2], be[2];
+    factors(vec + V_YK * 64, yk);
+    factors(vec + V_BETA * 64, be);
     bar_wait(&sm.state_ready[unit], parity, a.status);
 
     // (K S)^T of the warp's tokens
     float y[2][4], z[2][4];
+    uint32_t sh[KT][4], sl[KT][4];
     clear(y);
     clear(z);
 #pragma unroll
+    for (int kk = 0; kk < KT; ++kk) get(sm.state[unit][kk], sh[kk], sl[kk]);
+#pragma unroll
     for (int kk = 0; kk < KT; ++kk) {
-      uint32_t hi[4], lo[4], b[4];
-      get(sm.state[unit][kk], hi, lo);
-      b_from_nk(b, x.k, P, tok, 16 * kk);
-      mma_pair(y, hi, b);
-      mma_pair(z, lo, b);
+      mma_pair(y, sh[kk], bk[kk]);
+      mma_pair(z, sl[kk], bk[kk]);
     }
     add_to(y, z);
     // r = beta (V - e^G K S)^T
-    uint32_t v[4];
-    float2 be[2], f2[2];
-    a_from_km(v, x.v, VP, tok, unit * 16);
-    factors(vec + V_YK * 64, f2);
-    scale_tokens(y, f2);
-    factors(vec + V_BETA * 64, be);
+    scale_tokens(y, yk);
     float u[2][4];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
@@ -707,93 +712,104 @@ forward_kernel(const DeltaArgs a) {
       u[f][2] = be[f].x * (lo_half(v[2 * f + 1]) - y[f][2]);
       u[f][3] = be[f].y * (hi_half(v[2 * f + 1]) - y[f][3]);
     }
-    {
-      uint32_t hi[4], lo[4];
-      split_a(u[0], u[1], hi, lo);
-      put(sm.r[unit][w], hi, lo);
-    }
+    uint32_t rh[4], rl[4];  // the warp's own part of r
+    split_a(u[0], u[1], rh, rl);
+    put(sm.r[unit][w], rh, rl);
     bar_arrive(&sm.r_ready[unit]);
-    // while the others get there: e^G Q S
+    // while the others get there: e^G Q S, and (A - I) r with the warp's own part
     float o[2][4];
     clear(o);
     clear(z);
 #pragma unroll
     for (int kk = 0; kk < KT; ++kk) {
-      uint32_t hi[4], lo[4], b[4];
-      get(sm.state[unit][kk], hi, lo);
+      uint32_t b[4];
       b_from_nk(b, x.q, P, tok, 16 * kk);
-      mma_pair(o, hi, b);
-      mma_pair(z, lo, b);
+      mma_pair(o, sh[kk], b);
+      mma_pair(z, sl[kk], b);
     }
-    add_to(o, z);
-    factors(vec + V_OQ * 64, f2);
-    scale_tokens(o, f2);
-    bar_wait(&sm.r_ready[unit], parity, a.status);
-    // (A - I) r; y becomes the memory read at each token, m = e^G K S - ((A - I) r) / beta, in 16 bits, and U is
-    // beta (V - m), which the backward pass makes again from the m it reads: the products of dg must see the same U.
     float m[2][4], m2[2][4], m3[2][4];
     clear(m);
     clear(m2);
     clear(m3);
-    for (int kk = 0; kk <= w; ++kk) {
-      uint32_t hi[4], lo[4], b[4];
-      get(sm.r[unit][kk], hi, lo);
+    {
+      uint32_t b[4], bl[4];
+      b_from_nk(b, ahi, APITCH, tok, tok);
+      b_from_nk(bl, alo, APITCH, tok, tok);
+      mma_pair(m, rh, b);
+      mma_pair(m2, rl, b);
+      mma_pair(m3, rh, bl);
+    }
+    add_to(o, z);
+    float2 f2[2], ib[2];
+    factors(vec + V_OQ * 64, f2);
+    scale_tokens(o, f2);
+#pragma unroll
+    for (int f = 0; f < 2; ++f) ib[f] = make_float2(__fdividef(1.f, be[f].x), __fdividef(1.f, be[f].y));
+    factors(vec + V_SU * 64, f2);
+    bar_wait(&sm.r_ready[unit], parity, a.status);
+    // (A - I) r; y becomes the memory read at each token, m = e^G K S - ((A - I) r) / beta, in 16 bits, and U is
+    // beta (V - m), made of the rounded m and used in two parts everywhere: the products of dg must see the same U.
+    for (int kk = 0; kk < w; ++kk) {
+      uint32_t hi[4], lo[4], b[4], bl[4];
       b_from_nk(b, ahi, APITCH, tok, 16 * kk);
+      b_from_nk(bl, alo, APITCH, tok, 16 * kk);
+      get(sm.r[unit][kk], hi, lo);
       mma_pair(m, hi, b);
       mma_pair(m2, lo, b);
-      b_from_nk(b, alo, APITCH, tok, 16 * kk);
-      mma_pair(m3, hi, b);
+      mma_pair(m3, hi, bl);
     }
-    add_to(m2, m3);
-    add_to(m, m2);
-    uint32_t mh[4], ml[4];
+    uint32_t mh[4], ml[4], uh[4], ul[4];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
-      m[f][0] = y[f][0] - __fdividef(m[f][0], be[f].x);
-      m[f][1] = y[f][1] - __fdividef(m[f][1], be[f].y);
-      m[f][2] = y[f][2] - __fdividef(m[f][2], be[f].x);
-      m[f][3] = y[f][3] - __fdividef(m[f][3], be[f].y);
+      m[f][0] = y[f][0] - (m[f][0] + (m2[f][0] + m3[f][0])) * ib[f].x;
+      m[f][1] = y[f][1] - (m[f][1] + (m2[f][1] + m3[f][1])) * ib[f].y;
+      m[f][2] = y[f][2] - (m[f][2] + (m2[f][2] + m3[f][2])) * ib[f].x;
+      m[f][3] = y[f][3] - (m[f][3] + (m2[f][3] + m3[f][3])) * ib[f].y;
     }
     split_a(m[0], m[1], mh, ml);
 #pragma unroll
-    for (int f = 0; f < 2; ++f)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * f + e;
-        memory_term(v[i], mh[i], ml[i], be[f], m[f][2 * e], m[f][2 * e + 1], u[f][2 * e], u[f][2 * e + 1]);
-      }
+    for (int i = 0; i < 4; ++i) memory_term(v[i], mh[i], ml[i], be[i >> 1], u[i >> 1][2 * (i & 1)], u[i >> 1][2 * (i & 1) + 1]);
+    split_a(u[0], u[1], uh, ul);
     {
-      uint32_t hi[4], lo[4];
-      split_a(u[0], u[1], hi, lo);
-      put(sm.u[unit][w], hi, lo);
       float su[2][4];
+      uint32_t hi[4], lo[4];
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) su[f][e] = u[f][e];
-      factors(vec + V_SU * 64, f2);
       scale_tokens(su, f2);
       split_a(su[0], su[1], hi, lo);
       put(sm.su[unit][w], hi, lo);
     }
+    put(sm.u[unit][w], uh, ul);
     bar_arrive(&sm.u_ready[unit]);
-    bf16* stage = sm.out[warp];
-    const int left = len - tok;  // of the warp's tokens
-    const long long out0 = ((t0 + tok) * a.Hv + h) * a.dv + col0, ostride = static_cast<long long>(a.Hv) * a.dv;
-    bar_wait(&sm.u_ready[unit], parity, a.status);
-    // S^T <- e^{G_C} S^T + (e^{G_C - G} U)^T K, the warp's columns of dk
+    // meanwhile: what is kept, and K for the state
+    const long long piece = (((c0 + c) * a.Hv + h) * (a.dv / 16) + (col0 >> 4)) * 4 + w;
+    if (KEEP) {
+      uint4* mf = reinterpret_cast<uint4*>(a.mem) + piece * 64 + lane;
+      mf[0] = make_uint4(mh[0], mh[1], mh[2], mh[3]);
+      mf[32] = make_uint4(ml[0], ml[1], ml[2], ml[3]);
+      uint4* uf = reinterpret_cast<uint4*>(a.u) + piece * 64 + lane;
+      uf[0] = make_uint4(uh[0], uh[1], uh[2], uh[3]);
+      uf[32] = make_uint4(ul[0], ul[1], ul[2], ul[3]);
+    }
     const float ge = x.vec[V_END * 64];
 #pragma unroll
     for (int j = 0; j < 2 * KW; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[j][e] *= ge;
+    uint32_t bt[4][KW][4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int j = 0; j < KW; ++j) b_from_kn(bt[kk][j], x.k, P, 16 * kk, kd0 + 16 * j);
+    bar_wait(&sm.u_ready[unit], parity, a.status);
+    // S^T <- e^{G_C} S^T + (e^{G_C - G} U)^T K, the warp's columns of dk
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      uint32_t hi[4], lo[4], b[KW][4];
+      uint32_t hi[4], lo[4];
       get(sm.su[unit][kk], hi, lo);
-#pragma unroll
-      for (int j = 0; j < KW; ++j) b_from_kn(b[j], x.k, P, 16 * kk, kd0 + 16 * j);
-      mma2<KW>(s, hi, lo, b);
+      mma2<KW>(s, hi, lo, bt[kk]);
     }
     if (c + 1 < chunks) publish_state(c + 1);
     // what earlier tokens give to the output: + (P - diag P) U, with all four parts: the backward pass multiplies with
@@ -802,30 +818,22 @@ forward_kernel(const DeltaArgs a) {
     clear(m2);
     clear(m3);
     for (int kk = 0; kk <= w; ++kk) {
-      uint32_t hi[4], lo[4], b[4];
-      get(sm.u[unit][kk], hi, lo);
+      uint32_t hi[4], lo[4], b[4], bl[4];
       b_from_nk(b, phi, APITCH, tok, 16 * kk);
+      b_from_nk(bl, plo, APITCH, tok, 16 * kk);
+      get(sm.u[unit][kk], hi, lo);
       mma_pair(o, hi, b);
       mma_pair(z, lo, b);
-      b_from_nk(b, plo, APITCH, tok, 16 * kk);
-      mma_pair(m2, hi, b);
-      mma_pair(m3, lo, b);
+      mma_pair(m2, hi, bl);
+      mma_pair(m3, lo, bl);
     }
     add_to(m2, m3);
     add_to(z, m2);
     add_to(o, z);
-    if (KEEP) {  // eight neighbouring columns of a token per quarter of the warp: full 32-byte sectors
-#pragma unroll
-      for (int f = 0; f < 2; ++f)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 8 * f + t2 + (e & 1);
-          if (i < left) a.past[out0 + i * ostride + g + 8 * (e >> 1)] = o[f][e];
-        }
-      store_tile(stage, static_cast<bf16*>(a.mem) + out0, ostride, left, m[0], m[1]);
-      store_rest(stage, static_cast<bf16*>(a.mem_lo) + out0, ostride, left, m[0], m[1]);
-      store_tile(stage, static_cast<bf16*>(a.u) + out0, ostride, left, u[0], u[1]);
-      store_rest(stage, static_cast<bf16*>(a.u_lo) + out0, ostride, left, u[0], u[1]);
+    if (KEEP) {
+      float4* pf = reinterpret_cast<float4*>(a.past) + piece * 64 + lane;
+      pf[0] = make_float4(o[0][0], o[0][1], o[0][2], o[0][3]);
+      pf[32] = make_float4(o[1][0], o[1][1], o[1][2], o[1][3]);
     }
     factors(vec + V_PD * 64, f2);
 #pragma unroll
@@ -835,8 +843,9 @@ forward_kernel(const DeltaArgs a) {
       o[f][2] += f2[f].x * u[f][2];
       o[f][3] += f2[f].y * u[f][3];
     }
-    store_tile(stage, static_cast<bf16*>(a.o) + out0, ostride, left, o[0], o[1]);
     bar_arrive(&sm.empty[c & 1]);
+    store_tile(sm.out[warp], static_cast<bf16*>(a.o) + ((t0 + tok) * a.Hv + h) * a.dv + col0, static_cast<long long>(a.Hv) * a.dv,
+               len - tok, o[0], o[1]);
   }
   if (a.s_out) {
 #pragma unroll
@@ -852,7 +861,7 @@ forward_kernel(const DeltaArgs a) {
 template <int DK, int NU>
 struct BwdStage {
   static constexpr int P = DK + 8, VP = NU * 16 + 8;
-  bf16 k[C * P], q[C * P], dO[C * VP], v[C * VP], m[C * VP], ml[C * VP], ap[4 * C * APITCH];
+  bf16 k[C * P], q[C * P], dO[C * VP], ap[4 * C * APITCH];
   float vec[SEQ_ROWS * 64];
 };
 template <int DK, int NU>
@@ -913,9 +922,6 @@ backward_kernel(const DeltaArgs a) {
     copy_tile<64, THREADS>(x.ap, APITCH, static_cast<const bf16*>(a.ap) + rec * DELTA_AP, C, 4 * C, 4 * C);
     copy_tile<NU * 16, THREADS>(x.dO, VP, static_cast<const bf16*>(a.dout) + row, stride, C, len);
     copy_tile<DK, THREADS>(x.q, P, static_cast<const bf16*>(a.q) + t0 * a.q_ts + hk * a.q_hs, a.q_ts, C, len);
-    copy_tile<NU * 16, THREADS>(x.v, VP, static_cast<const bf16*>(a.v) + t0 * a.v_ts + h * a.v_hs + vb * NU * 16, a.v_ts, C, len);
-    copy_tile<NU * 16, THREADS>(x.m, VP, static_cast<const bf16*>(a.mem) + row, stride, C, len);
-    copy_tile<NU * 16, THREADS>(x.ml, VP, static_cast<const bf16*>(a.mem_lo) + row, stride, C, len);
     load_vec<THREADS>(x.vec, a.vec + rec * DELTA_VEC, SEQ_ROWS);
     bar_arrive_copies(&sm.full[i & 1]);
   };
@@ -931,8 +937,28 @@ backward_kernel(const DeltaArgs a) {
     }
     bar_arrive(&sm.state_ready[unit]);
   };
+  // What a chunk's warp reads of the forward pass: its part of the state in front, and m, U, past of its tokens.
+  struct Kept {
+    uint4 sh[KW], sl[KW], m[2], u[2], past[2];
+  } now, next;
+  auto load_kept = [&](int c, Kept& x) {
+    const long long piece = ((c0 + c) * a.Hv + h) * VT + vt;
+    const uint4* nf = reinterpret_cast<const uint4*>(a.states) + piece * 2 * KT * 32 + lane;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      x.sh[k] = nf[(KW * w + k) * 32];
+      x.sl[k] = nf[(KT + KW * w + k) * 32];
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      x.m[k] = (reinterpret_cast<const uint4*>(a.mem) + (piece * 4 + w) * 64 + lane)[32 * k];
+      x.u[k] = (reinterpret_cast<const uint4*>(a.u) + (piece * 4 + w) * 64 + lane)[32 * k];
+      x.past[k] = (reinterpret_cast<const uint4*>(a.past) + (piece * 4 + w) * 64 + lane)[32 * k];
+    }
+  };
   if (chunks > 0) {
     fetch(0);
+    load_kept(chunks - 1, next);
     publish_state(chunks - 1);
   }
   for (int i = 0; i < chunks; ++i) {
@@ -945,79 +971,74 @@ backward_kernel(const DeltaArgs a) {
     const bf16 *ahi = x.ap, *alo = x.ap + C * APITCH, *phi = x.ap + 2 * C * APITCH, *plo = x.ap + 3 * C * APITCH;
     const int tok = 16 * w;
     const float* vec = x.vec + tok + t2;
-    // the warp's part of the state in front of the chunk, for <dS1, S0>
-    const uint4* nf = reinterpret_cast<const uint4*>(a.states) + ((rec * VT + vt) * 2) * KT * 32 + lane;
-    uint4 sh[KW], sl[KW];
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-      sh[k] = nf[(KW * w + k) * 32];
-      sl[k] = nf[(KT + KW * w + k) * 32];
-    }
+    now = next;
     if (i + 1 < chunks) {
+      load_kept(c - 1, next);
       if (i > 0) bar_wait(&sm.empty[(i + 1) & 1], ((i - 1) >> 1) & 1, a.status);
       fetch(i + 1);
     }
     bar_wait(&sm.full[i & 1], turn, a.status);
 
-    // what does not wait for the state: ((P - diag P)^T dO)^T of the warp's tokens
-    float u[2][4], z[2][4], y[2][4];
+    // what does not wait for the state: ((P - diag P)^T dO)^T of the warp's tokens, K and factors
+    float u[2][4], z[2][4], y[2][4], du[2][4];
     clear(u);
     clear(z);
     uint32_t fo[4];  // dO^T of the warp's tokens
     a_from_km(fo, x.dO, VP, tok, unit * 16);
     for (int kk = w; kk < 4; ++kk) {
-      uint32_t f[4], b[4];
+      uint32_t f[4], b[4], bl[4];
       a_from_km(f, x.dO, VP, 16 * kk, unit * 16);
       b_from_kn(b, phi, APITCH, 16 * kk, tok);
+      b_from_kn(bl, plo, APITCH, 16 * kk, tok);
       mma_pair(u, f, b);
-      b_from_kn(b, plo, APITCH, 16 * kk, tok);
-      mma_pair(z, f, b);
+      mma_pair(z, f, bl);
     }
     add_to(u, z);
+    float2 f2[2], su[2], be[2];
+    factors(vec + V_PD * 64, f2);
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {  // diag P dO
+      du[f][0] = f2[f].x * lo_half(fo[2 * f]);
+      du[f][1] = f2[f].y * hi_half(fo[2 * f]);
+      du[f][2] = f2[f].x * lo_half(fo[2 * f + 1]);
+      du[f][3] = f2[f].y * hi_half(fo[2 * f + 1]);
+    }
+    factors(vec + V_SU * 64, su);
+    uint32_t bk[KT][4];
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) b_from_nk(bk[kk], x.k, P, tok, 16 * kk);
     bar_wait(&sm.state_ready[unit], parity, a.status);
     // y = (e^{G_C - G} K dS1)^T
     clear(y);
     clear(z);
 #pragma unroll
     for (int kk = 0; kk < KT; ++kk) {
-      uint32_t hi[4], lo[4], b[4];
+      uint32_t hi[4], lo[4];
       get(sm.state[unit][kk], hi, lo);
-      b_from_nk(b, x.k, P, tok, 16 * kk);
-      mma_pair(y, hi, b);
-      mma_pair(z, lo, b);
+      mma_pair(y, hi, bk[kk]);
+      mma_pair(z, lo, bk[kk]);
     }
     add_to(y, z);
-    float2 f2[2], be[2];
-    factors(vec + V_SU * 64, f2);
-    scale_tokens(y, f2);
-    // du = dU^T = y + u + (diag P dO)^T
+    scale_tokens(y, su);
+    // dU^T = y + u + (diag P dO)^T
     add_to(u, y);
-    float du[2][4];
-    factors(vec + V_PD * 64, f2);
-#pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      du[f][0] = f2[f].x * lo_half(fo[2 * f]);
-      du[f][1] = f2[f].y * hi_half(fo[2 * f]);
-      du[f][2] = f2[f].x * lo_half(fo[2 * f + 1]);
-      du[f][3] = f2[f].y * hi_half(fo[2 * f + 1]);
-    }
+    uint32_t dh[4], dl[4];
     {
       float d[2][4];
-      uint32_t hi[4], lo[4];
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[f][e] = u[f][e] + du[f][e];
-      split_a(d[0], d[1], hi, lo);
-      put(sm.du[unit][w], hi, lo);
+      split_a(d[0], d[1], dh, dl);
+      put(sm.du[unit][w], dh, dl);
     }
     bar_arrive(&sm.du_ready[unit]);
-    // while the others get there: S0 . dS1, U and m of the warp's tokens, and Q^T diag(e^G) dO into the state
+    // while the others get there: <dS1, S0>, U and m of the warp's tokens, and Q^T diag(e^G) dO into the state
     const float ge = x.vec[V_END * 64];
     float sdot = 0.f;
 #pragma unroll
     for (int k = 0; k < KW; ++k) {
-      const uint32_t wh[4] = {sh[k].x, sh[k].y, sh[k].z, sh[k].w}, wl[4] = {sl[k].x, sl[k].y, sl[k].z, sl[k].w};
+      const uint32_t wh[4] = {now.sh[k].x, now.sh[k].y, now.sh[k].z, now.sh[k].w}, wl[4] = {now.sl[k].x, now.sl[k].y, now.sl[k].z, now.sl[k].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         sdot += s[2 * k + (e >> 1)][2 * (e & 1)] * (lo_half(wh[e]) + lo_half(wl[e]));
@@ -1025,30 +1046,13 @@ backward_kernel(const DeltaArgs a) {
       }
     }
     sdot *= ge;
-    uint32_t fv[4], fm[4], fl[4];
-    a_from_km(fv, x.v, VP, tok, unit * 16);
-    a_from_km(fm, x.m, VP, tok, unit * 16);
-    a_from_km(fl, x.ml, VP, tok, unit * 16);
-    factors(vec + V_BETA * 64, be);
     float mm[2][4], uu[2][4];
-#pragma unroll
-    for (int f = 0; f < 2; ++f)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int q = 2 * f + e;
-        memory_term(fv[q], fm[q], fl[q], be[f], mm[f][2 * e], mm[f][2 * e + 1], uu[f][2 * e], uu[f][2 * e + 1]);
-        uint32_t hi, lo;  // the two parts that the forward pass multiplied with P
-        split2(uu[f][2 * e], uu[f][2 * e + 1], hi, lo);
-        uu[f][2 * e] = lo_half(hi) + lo_half(lo);
-        uu[f][2 * e + 1] = hi_half(hi) + hi_half(lo);
-      }
+    join(now.m[0], now.m[1], mm);
+    join(now.u[0], now.u[1], uu);
 #pragma unroll
     for (int f = 0; f < 2; ++f)
 #pragma unroll
       for (int e = 0; e < 4; ++e) sdot += y[f][e] * uu[f][e];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sdot += __shfl_xor_sync(0xffffffffu, sdot, o);
-    if (lane == 0) a.sdots[(rec * VT + vt) * 4 + w] = sdot;
 #pragma unroll
     for (int j = 0; j < 2 * KW; ++j)
 #pragma unroll
@@ -1065,42 +1069,46 @@ backward_kernel(const DeltaArgs a) {
       for (int j = 0; j < KW; ++j) b_from_kn(b[j], x.q, P, 16 * kk, kd0 + 16 * j);
       mma2<KW>(s, hi, lo, b);
     }
-    bar_wait(&sm.du_ready[unit], parity, a.status);
-    // u <- u + dU^T (A - I): X without what the token's own output asks for
+    factors(vec + V_BETA * 64, be);
+    factors(vec + V_YK * 64, f2);
+    // u <- u + dU^T (A - I): X without what the token's own output asks for; first with the warp's own part
     clear(y);
     clear(z);
-    for (int kk = w; kk < 4; ++kk) {
-      uint32_t hi[4], lo[4], b[4];
-      get(sm.du[unit][kk], hi, lo);
+    {
+      uint32_t b[4], bl[4];
+      b_from_kn(b, ahi, APITCH, tok, tok);
+      b_from_kn(bl, alo, APITCH, tok, tok);
+      mma_pair(u, dh, b);
+      mma_pair(y, dl, b);
+      mma_pair(z, dh, bl);
+    }
+    bar_wait(&sm.du_ready[unit], parity, a.status);
+    for (int kk = w + 1; kk < 4; ++kk) {
+      uint32_t hi[4], lo[4], b[4], bl[4];
       b_from_kn(b, ahi, APITCH, 16 * kk, tok);
+      b_from_kn(bl, alo, APITCH, 16 * kk, tok);
+      get(sm.du[unit][kk], hi, lo);
       mma_pair(u, hi, b);
       mma_pair(y, lo, b);
-      b_from_kn(b, alo, APITCH, 16 * kk, tok);
-      mma_pair(z, hi, b);
+      mma_pair(z, hi, bl);
     }
     add_to(y, z);
     add_to(u, y);
-    // X = u + (diag P dO)^T, dV = beta X, and the row sums U . u, U . X and m . dV over the unit's 16 columns
-    float d[3][4];
+    // X = u + (diag P dO)^T, dV = beta X; row sums over the unit's 16 columns: past . dO - m . dV - U . u, and U . X
+    float d[2][4];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
-      d[0][2 * f] = uu[f][0] * u[f][0] + uu[f][2] * u[f][2];
-      d[0][2 * f + 1] = uu[f][1] * u[f][1] + uu[f][3] * u[f][3];
+      d[0][2 * f] = -(uu[f][0] * u[f][0] + uu[f][2] * u[f][2]);
+      d[0][2 * f + 1] = -(uu[f][1] * u[f][1] + uu[f][3] * u[f][3]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) u[f][e] += du[f][e];
       d[1][2 * f] = uu[f][0] * u[f][0] + uu[f][2] * u[f][2];
       d[1][2 * f + 1] = uu[f][1] * u[f][1] + uu[f][3] * u[f][3];
     }
     scale_tokens(u, be);
-#pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      d[2][2 * f] = mm[f][0] * u[f][0] + mm[f][2] * u[f][2];
-      d[2][2 * f + 1] = mm[f][1] * u[f][1] + mm[f][3] * u[f][3];
-    }
     {
       float b[2][4];
       uint32_t hi[4], lo[4];
-      factors(vec + V_YK * 64, f2);
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
@@ -1110,9 +1118,32 @@ backward_kernel(const DeltaArgs a) {
       put(sm.dv[unit][w], hi, lo);
     }
     bar_arrive(&sm.dv_ready[unit]);
-    float* rd = a.rowdots + (rec * VT + vt) * 192 + tok + t2;
 #pragma unroll
-    for (int q = 0; q < 3; ++q)
+    for (int f = 0; f < 2; ++f) {
+      const float* past = reinterpret_cast<const float*>(&now.past[f]);
+      d[0][2 * f] += past[0] * lo_half(fo[2 * f]) + past[2] * lo_half(fo[2 * f + 1]) - (mm[f][0] * u[f][0] + mm[f][2] * u[f][2]);
+      d[0][2 * f + 1] += past[1] * hi_half(fo[2 * f]) + past[3] * hi_half(fo[2 * f + 1]) - (mm[f][1] * u[f][1] + mm[f][3] * u[f][3]);
+    }
+    uint32_t bt[4][KW][4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int j = 0; j < KW; ++j) b_from_kn(bt[kk][j], x.k, P, 16 * kk, kd0 + 16 * j);
+    bar_wait(&sm.dv_ready[unit], parity, a.status);
+    // dS0 -= K^T diag(e^G) dV
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      uint32_t hi[4], lo[4];
+      get(sm.dv[unit][kk], hi, lo);
+      mma2<KW>(s, hi, lo, bt[kk]);
+    }
+    if (c > 0) publish_state(c - 1);
+    bar_arrive(&sm.empty[i & 1]);
+    store_tile(sm.out[warp], static_cast<bf16*>(a.dv_) + ((t0 + tok) * a.Hv + h) * a.dv + col0,
+               static_cast<long long>(a.Hv) * a.dv, len - tok, u[0], u[1]);
+    float* rd = a.rowdots + (rec * VT + vt) * 128 + tok + t2;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float r = d[q][e];
@@ -1121,20 +1152,9 @@ backward_kernel(const DeltaArgs a) {
         r += __shfl_xor_sync(0xffffffffu, r, 16);
         if (g == 0) rd[q * 64 + 8 * (e >> 1) + (e & 1)] = r;
       }
-    store_tile(sm.out[warp], static_cast<bf16*>(a.dv_) + ((t0 + tok) * a.Hv + h) * a.dv + col0,
-               static_cast<long long>(a.Hv) * a.dv, len - tok, u[0], u[1]);
-    bar_wait(&sm.dv_ready[unit], parity, a.status);
-    // dS0 -= K^T diag(e^G) dV
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint32_t hi[4], lo[4], b[KW][4];
-      get(sm.dv[unit][kk], hi, lo);
-#pragma unroll
-      for (int j = 0; j < KW; ++j) b_from_kn(b[j], x.k, P, 16 * kk, kd0 + 16 * j);
-      mma2<KW>(s, hi, lo, b);
-    }
-    if (c > 0) publish_state(c - 1);
-    bar_arrive(&sm.empty[i & 1]);
+    for (int o = 16; o > 0; o >>= 1) sdot += __shfl_xor_sync(0xffffffffu, sdot, o);
+    if (lane == 0) a.sdots[(rec * VT + vt) * 4 + w] = sdot;
   }
   if (a.ds_in) {
 #pragma unroll
@@ -1150,7 +1170,7 @@ backward_kernel(const DeltaArgs a) {
 template <int DK, int DV>
 struct DqkSmem {
   static constexpr int P = DK + 8, VP = DV + 8;
-  bf16 q[C * P], k[C * P], dO[C * VP], dV[C * VP], u[C * VP], ul[C * VP], s0[DV * P], ds[DV * P];
+  bf16 q[C * P], k[C * P], dO[C * VP], dV[C * VP], u[DV * APITCH], ul[DV * APITCH], s0[DV * P], ds[DV * P];
   bf16 w1[C * APITCH], w1l[C * APITCH], w2[C * APITCH];
   float vec[8 * 64];
   float dots[2][2][C];
@@ -1170,6 +1190,20 @@ __device__ __forceinline__ void load_fragments(bf16* dst, const uint4* src, int 
     *reinterpret_cast<uint32_t*>(p + 8 * P) = f.y;
     *reinterpret_cast<uint32_t*>(p + 8) = f.z;
     *reinterpret_cast<uint32_t*>(p + 8 * P + 8) = f.w;
+  }
+}
+
+// U^T and its remainder -> [DV][64 tokens] rows of pitch APITCH.
+template <int DV>
+__device__ __forceinline__ void load_u(bf16* hi, bf16* lo, const uint4* src) {
+  for (int i = threadIdx.x; i < DV / 16 * 256; i += DQK_THREADS) {
+    const int lane = i & 31, part = (i >> 5) & 1, w = (i >> 6) & 3, vt = i >> 8, g = lane >> 2, t2 = (lane & 3) * 2;
+    const uint4 f = src[i];
+    bf16* p = (part ? lo : hi) + (vt * 16 + g) * APITCH + w * 16 + t2;
+    *reinterpret_cast<uint32_t*>(p) = f.x;
+    *reinterpret_cast<uint32_t*>(p + 8 * APITCH) = f.y;
+    *reinterpret_cast<uint32_t*>(p + 8) = f.z;
+    *reinterpret_cast<uint32_t*>(p + 8 * APITCH + 8) = f.w;
   }
 }
 
@@ -1200,10 +1234,9 @@ dqk_kernel(const DeltaArgs a) {
     __syncthreads();
     load_rows<DV, DQK_THREADS>(x.dO, VP, static_cast<const bf16*>(a.dout) + row, stride, sp.len);
     load_rows<DV, DQK_THREADS>(x.dV, VP, static_cast<const bf16*>(a.dv_) + row, stride, sp.len);
-    load_rows<DV, DQK_THREADS>(x.u, VP, static_cast<const bf16*>(a.u) + row, stride, sp.len);
-    load_rows<DV, DQK_THREADS>(x.ul, VP, static_cast<const bf16*>(a.u_lo) + row, stride, sp.len);
     load_vec<DQK_THREADS>(x.vec, a.vec + rec * DELTA_VEC, 8);
     cp_commit();
+    load_u<DV>(x.u, x.ul, reinterpret_cast<const uint4*>(a.u) + rec * (DV / 16) * 256);
     load_fragments<DK, DV>(x.s0, reinterpret_cast<const uint4*>(a.states) + rec * (DV / 16) * 2 * KT * 32, 2 * KT * 32);
     load_fragments<DK, DV>(x.ds, reinterpret_cast<const uint4*>(a.dstates) + rec * (DV / 16) * KT * 32, KT * 32);
     cp_wait<0>();
@@ -1222,12 +1255,12 @@ dqk_kernel(const DeltaArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (wn * 2 + j > wm) continue;
-        b_from_nk(b, x.u, VP, wn * 32 + j * 16, kk * 16);
+        b_from_kn(b, x.u, APITCH, kk * 16, wn * 32 + j * 16);
         mma(p[2 * j], fo, b[0], b[1]);
         mma(p[2 * j + 1], fo, b[2], b[3]);
         mma(nn[2 * j], fv, b[0], b[1]);
         mma(nn[2 * j + 1], fv, b[2], b[3]);
-        b_from_nk(bl, x.ul, VP, wn * 32 + j * 16, kk * 16);
+        b_from_kn(bl, x.ul, APITCH, kk * 16, wn * 32 + j * 16);
         mma(p[2 * j], fo, bl[0], bl[1]);
         mma(p[2 * j + 1], fo, bl[2], bl[3]);
       }
@@ -1261,12 +1294,12 @@ dqk_kernel(const DeltaArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[j][e] = 0.f;
     };
-    auto product = [&](const bf16* rows, const bf16* state) {
+    auto product = [&](const bf16* rows, const bf16* state, bool transposed) {
       clear();
 #pragma unroll
       for (int kk = 0; kk < DV / 16; ++kk) {
         uint32_t f[4], b[4];
-        a_from_mk(f, rows, VP, wm * 16, kk * 16);
+        if (transposed) a_from_km(f, rows, APITCH, kk * 16, wm * 16); else a_from_mk(f, rows, VP, wm * 16, kk * 16);
 #pragma unroll
         for (int j = 0; j < NT / 2; ++j) {
           b_from_kn(b, state, P, kk * 16, n0 + j * 16);
@@ -1284,11 +1317,11 @@ dqk_kernel(const DeltaArgs a) {
         acc[j][3] += f1 * t[j][3];
       }
     };
-    product(x.dO, x.s0);
+    product(x.dO, x.s0, false);
     add(dq, x.vec[V_OQ * 64 + r0], x.vec[V_OQ * 64 + r0 + 8]);
-    product(x.dV, x.s0);
+    product(x.dV, x.s0, false);
     add(dk, -x.vec[V_YK * 64 + r0], -x.vec[V_YK * 64 + r0 + 8]);
-    product(x.u, x.ds);
+    product(x.u, x.ds, true);
     add(dk, x.vec[V_SU * 64 + r0], x.vec[V_SU * 64 + r0 + 8]);
     __syncthreads();  // w1, w2
 #pragma unroll
@@ -1371,45 +1404,29 @@ dqk_kernel(const DeltaArgs a) {
 
 // ------------------------------------------------------------------------------------------------------------ gates
 
-// One block per (chunk, value head): o~ . do per token, then dbeta and the suffix sums of dg in 64 bits.
-__global__ void __launch_bounds__(128)
+// One warp per (chunk, value head): sums over the units, then dbeta and the suffix sums of dg in 64 bits.
+constexpr int GATE_WARPS = 4;
+__global__ void __launch_bounds__(GATE_WARPS * 32)
 gates_kernel(const DeltaArgs a) {
-  __shared__ double od[C];
-  const long long c = blockIdx.x / a.Hv;
-  const int h = blockIdx.x % a.Hv;
+  const long long rec = static_cast<long long>(blockIdx.x) * GATE_WARPS + (threadIdx.x >> 5);
+  const long long c = rec / a.Hv;
+  const int h = static_cast<int>(rec - c * a.Hv);
+  if (c >= a.NC) return;
   const Span sp = chunk_span(a, c);
   if (sp.len == 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, VT = a.dv / 16;
-  const long long rec = c * a.Hv + h;
-  for (int i = warp; i < C; i += 4) {
-    float s = 0.f;
-    if (i < sp.len) {
-      const long long row = ((sp.start + i) * a.Hv + h) * a.dv;
-      for (int v = lane * 2; v < a.dv; v += 64) {
-        const float2 p = *reinterpret_cast<const float2*>(a.past + row + v);
-        const uint32_t d = *reinterpret_cast<const uint32_t*>(static_cast<const bf16*>(a.dout) + row + v);
-        s += p.x * lo_half(d) + p.y * hi_half(d);
-      }
-    }
+  const int lane = threadIdx.x & 31, VT = a.dv / 16;
+  const float* rd = a.rowdots + rec * VT * 128;
+  double carry = lane < 4 * VT ? a.sdots[rec * 4 * VT + lane] : 0.f;  // dv / 4 <= 32 of them
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) od[i] = s;
-  }
-  __syncthreads();
-  if (warp != 0) return;
-  const float* rd = a.rowdots + rec * VT * 192;
-  double carry = 0.0;
-  for (int v = 0; v < 4 * VT; ++v) carry += a.sdots[rec * 4 * VT + v];
+  for (int o = 16; o > 0; o >>= 1) carry += __shfl_xor_sync(0xffffffffu, carry, o);
 #pragma unroll
   for (int half = 1; half >= 0; --half) {
     const int i = half * 32 + lane;
-    double later = 0.0, xu = 0.0, read = 0.0;
+    double s = 0.0, xu = 0.0;
     for (int v = 0; v < VT; ++v) {
-      later += rd[v * 192 + i];
-      xu += rd[v * 192 + 64 + i];
-      read += rd[v * 192 + 128 + i];
+      s += rd[v * 128 + i];
+      xu += rd[v * 128 + 64 + i];
     }
-    double s = od[i] - read - later;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double y = __shfl_down_sync(0xffffffffu, s, o);
@@ -1479,7 +1496,7 @@ int backward_dk(const DeltaArgs& a, cudaStream_t s) {
   if (a.NC > 0) {
     rc = a.dv == 64 ? launch_dqk<DK, 64>(a, s) : launch_dqk<DK, 128>(a, s);
     if (rc) return rc;
-    gates_kernel<<<static_cast<unsigned>(a.NC * a.Hv), 128, 0, s>>>(a);
+    gates_kernel<<<static_cast<unsigned>((a.NC * a.Hv + GATE_WARPS - 1) / GATE_WARPS), GATE_WARPS * 32, 0, s>>>(a);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }

@@ -22,10 +22,10 @@ struct DeltaArgs {
   const float* s_in = nullptr;  // [N, Hv, dk, dv] or null (zero)
   float* s_out = nullptr;       // [N, Hv, dk, dv] or null
   void *o = nullptr;            // bf16 [T, Hv, dv]
-  // Kept for the backward pass (all or none), [T, Hv, dv]: what o owes to earlier tokens (fp32), the memory read at each
-  // token and U (bf16 with the remainder of the rounding); and the state in front of every chunk.
-  float* past = nullptr;
-  void *mem = nullptr, *mem_lo = nullptr, *u = nullptr, *u_lo = nullptr, *states = nullptr;
+  // Kept for the backward pass (all or none), as the fragments that one warp's lanes hold, [NC, Hv, dv / 16, 4, ..., 32]:
+  // what o owes to earlier tokens (fp32), the memory read at each token and U (bf16 and the remainder of the rounding);
+  // and the state in front of every chunk.
+  void *past = nullptr, *mem = nullptr, *u = nullptr, *states = nullptr;
   void* ap = nullptr;    // bf16 [NC, Hv, DELTA_AP]
   float* vec = nullptr;  // fp32 [NC, Hv, DELTA_VEC]
   // backward
@@ -33,7 +33,7 @@ struct DeltaArgs {
   const float* ds_out = nullptr;  // gradient of s_out or null
   float* ds_in = nullptr;         // gradient of s_in or null
   void* dstates = nullptr;      // bf16 fragments of the state gradients, half the size of `states`
-  float* rowdots = nullptr;     // fp32 [NC, Hv, dv / 16, 3, 64]
+  float* rowdots = nullptr;     // fp32 [NC, Hv, dv / 16, 2, 64]
   float* sdots = nullptr;       // fp32 [NC, Hv, dv / 16, 4]
   void *dq = nullptr, *dkey = nullptr, *dv_ = nullptr;  // bf16, contiguous
   float *dg = nullptr, *dbeta = nullptr;                // fp32 [T, Hv]

@@ -1028,8 +1028,8 @@ lf::DeltaArgs delta_args(const at::Tensor& q, const at::Tensor& k, const at::Ten
   return a;
 }
 
-// {o, final state or empty}, and with `keep` what the backward pass reads: {past, memory, U, chunk states, A / P,
-// factors} (see DeltaArgs).
+// {o, final state or empty}, and with `keep` what the backward pass reads: {past, memory, U, chunk states, q and k
+// tiles, A / P, factors} (see DeltaArgs).
 std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
                                   const at::Tensor& beta, c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first,
                                   double scale, bool l2norm, c10::optional<at::Tensor> s_in, bool want_state, bool keep,
@@ -1042,6 +1042,8 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, cons
   at::Tensor o = at::empty({a.T, a.Hv, a.dv}, bf);
   at::Tensor s_out = want_state ? at::empty({a.N, a.Hv, a.dk, a.dv}, fl) : at::empty({0}, fl);
   at::Tensor ap = at::empty({a.NC, a.Hv, lf::DELTA_AP}, bf), vec = at::empty({a.NC, a.Hv, lf::DELTA_VEC}, fl);
+  at::Tensor qk = at::empty({a.NC, a.Hk, 2, lf::DELTA_CHUNK, a.dk + lf::DELTA_ROW_PAD}, bf);
+  a.qk = qk.data_ptr();
   a.o = o.data_ptr();
   a.ap = ap.data_ptr();
   a.vec = vec.data_ptr<float>();
@@ -1059,7 +1061,7 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, cons
     a.mem = mem.data_ptr();
     a.u = u.data_ptr();
     a.states = states.data_ptr();
-    out.insert(out.end(), {past, mem, u, states, ap, vec});
+    out.insert(out.end(), {past, mem, u, states, qk, ap, vec});
   }
   const int rc = lf::delta_forward(a, cur_stream());
   TORCH_CHECK(rc == 0, "lf::delta_forward failed with code ", rc, " (dk = ", a.dk, ", dv = ", a.dv, ")");
@@ -1080,7 +1082,7 @@ std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tens
                                   const at::Tensor& v, const at::Tensor& g, const at::Tensor& beta,
                                   c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first, double scale, bool l2norm,
                                   bool want_ds, const at::Tensor& past, const at::Tensor& mem, const at::Tensor& u,
-                                  const at::Tensor& states, const at::Tensor& ap,
+                                  const at::Tensor& states, const at::Tensor& qk, const at::Tensor& ap,
                                   const at::Tensor& vec, const at::Tensor& status) {
   c10::cuda::CUDAGuard guard(q.device());
   lf::DeltaArgs a = delta_args(q, k, v, g, beta, bounds, first, scale, l2norm);
@@ -1093,6 +1095,7 @@ std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tens
               mem.numel() == 2 * kept && u.scalar_type() == at::kBFloat16 && u.numel() == 2 * kept,
               "what the forward pass kept does not fit these inputs");
   TORCH_CHECK(states.device() == q.device() && states.scalar_type() == at::kBFloat16 && states.numel() == a.NC * a.Hv * 2 * a.dk * a.dv &&
+              qk.scalar_type() == at::kBFloat16 && qk.numel() == a.NC * a.Hk * 2 * lf::DELTA_CHUNK * (a.dk + lf::DELTA_ROW_PAD) &&
               ap.scalar_type() == at::kBFloat16 && ap.numel() == a.NC * a.Hv * lf::DELTA_AP && vec.scalar_type() == at::kFloat &&
               vec.numel() == a.NC * a.Hv * lf::DELTA_VEC, "what the forward pass kept does not fit these inputs");
   auto bf = v.options(), fl = g.options();
@@ -1111,6 +1114,7 @@ std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tens
   a.mem = mem.data_ptr();
   a.u = u.data_ptr();
   a.states = states.data_ptr();
+  a.qk = qk.data_ptr();
   a.ap = ap.data_ptr();
   a.vec = vec.data_ptr<float>();
   a.dstates = dstates.data_ptr();

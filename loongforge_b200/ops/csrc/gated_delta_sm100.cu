@@ -283,6 +283,13 @@ prepare_kernel(const DeltaArgs a) {
   cp_commit();
   cp_wait<0>();
   __syncthreads();
+  // the padded tiles as they are, for the kernels along the sequence: one bulk copy each there
+  {
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<bf16*>(a.qk) + (c * a.Hk + hk) * 2 * C * P);
+    const uint4* src = reinterpret_cast<const uint4*>(qs);  // k lies behind q
+    for (int i = tid; i < 2 * C * P / 8; i += PREP_THREADS)
+      if (i % (P / 8) < DK / 8) dst[i] = src[i];
+  }
   {
     const bf16* row = (tid < C ? qs : ks) + (tid & 63) * P;
     float ss = 0.f;
@@ -385,8 +392,8 @@ prepare_kernel(const DeltaArgs a) {
         *reinterpret_cast<float2*>(M + i * MP + j0) = make_float2(m[0], m[1]);
         uint32_t hi, lo;
         split2(p[0], p[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(ap + 2 * C * C + i * C + j0) = hi;
-        *reinterpret_cast<uint32_t*>(ap + 3 * C * C + i * C + j0) = lo;
+        *reinterpret_cast<uint32_t*>(ap + 2 * C * APITCH + i * APITCH + j0) = hi;
+        *reinterpret_cast<uint32_t*>(ap + 3 * C * APITCH + i * APITCH + j0) = lo;
       }
     }
     __syncthreads();
@@ -455,8 +462,8 @@ prepare_kernel(const DeltaArgs a) {
         if (r == c8 + 2 * x + 1) v.y = 0.f;
         split2(v.x, v.y, hi[x], lo[x]);
       }
-      *reinterpret_cast<uint4*>(ap + r * C + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(ap + C * C + r * C + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      *reinterpret_cast<uint4*>(ap + r * APITCH + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(ap + C * APITCH + r * APITCH + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   }
 }
@@ -505,20 +512,26 @@ __device__ __forceinline__ void bar_wait(uint64_t* b, uint32_t parity, int* stat
   }
   *status = 1;
 }
-// The calling thread's copies so far arrive on the barrier when they have landed.
+// The calling thread's cp.async copies so far arrive on the barrier when they have landed.
 __device__ __forceinline__ void bar_arrive_copies(uint64_t* b) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
 }
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
+}
+// One thread copies a contiguous piece (16-byte aligned, a multiple of 16 bytes); it arrives on the barrier by its bytes.
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* b) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_addr(dst)),
+               "l"(src), "r"(bytes), "r"(smem_addr(b)) : "memory");
+}
 
-// Copies `rows` x COLS bf16 (rows from `len` on become zeros): a thread takes one 16-byte column of every
-// (THREADS / (COLS / 8))th row.
+// Copies 64 rows x COLS bf16 (rows from `len` on become zeros), a 16-byte piece per thread.
 template <int COLS, int THREADS>
-__device__ __forceinline__ void copy_tile(bf16* dst, int pitch, const bf16* src, long long stride, int rows, int len) {
-  constexpr int V = COLS / 8, STEP = THREADS / V;
-  const int v = threadIdx.x % V;
-  const bf16* p = src + (threadIdx.x / V) * stride + v * 8;
-  bf16* d = dst + (threadIdx.x / V) * pitch + v * 8;
-  for (int r = threadIdx.x / V; r < rows; r += STEP, p += STEP * stride, d += STEP * pitch) cp16(d, r < len ? p : src, r < len);
+__device__ __forceinline__ void copy_rows(bf16* dst, int pitch, const bf16* src, long long stride, int len) {
+  constexpr int V = COLS / 8;
+  static_assert(THREADS == C * V, "one piece a thread");
+  const int r = threadIdx.x / V, v = (threadIdx.x % V) * 8;
+  cp16(dst + r * pitch + v, src + (r < len ? r * stride : 0) + v, r < len);
 }
 
 // The warp's 16 tokens x 16 columns of fp32 accumulators, rounded to bf16, to rows of a token-major tensor through the
@@ -584,9 +597,10 @@ __device__ __forceinline__ void add_to(float (&c)[2][4], const float (&d)[2][4])
 
 template <int DK, int NU>
 struct FwdStage {
-  static constexpr int P = DK + 8, VP = NU * 16 + 8;
-  bf16 k[C * P], q[C * P], v[C * VP], ap[4 * C * APITCH];
+  static constexpr int P = DK + DELTA_ROW_PAD, VP = NU * 16 + 8;
+  bf16 qk[2 * C * P], ap[DELTA_AP], v[C * VP];
   float vec[SEQ_ROWS * 64];
+  static constexpr uint32_t BULK = (2 * C * P + DELTA_AP) * sizeof(bf16) + SEQ_ROWS * 64 * sizeof(float);
 };
 template <int DK, int NU>
 struct FwdSmem {
@@ -614,7 +628,7 @@ forward_kernel(const DeltaArgs a) {
   const int chunks = static_cast<int>((end - start + C - 1) / C);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      bar_init(&sm.full[i], THREADS);
+      bar_init(&sm.full[i], THREADS + 1);
       bar_init(&sm.empty[i], NU * 4);
     }
     for (int i = 0; i < NU; ++i) {
@@ -640,38 +654,44 @@ forward_kernel(const DeltaArgs a) {
     const long long t0 = start + static_cast<long long>(c) * C;
     const int len = end - t0 < C ? static_cast<int>(end - t0) : C;
     const long long rec = (c0 + c) * a.Hv + h;
-    copy_tile<DK, THREADS>(x.k, P, static_cast<const bf16*>(a.k) + t0 * a.k_ts + hk * a.k_hs, a.k_ts, C, len);
-    copy_tile<64, THREADS>(x.ap, APITCH, static_cast<const bf16*>(a.ap) + rec * DELTA_AP, C, 4 * C, 4 * C);
-    copy_tile<DK, THREADS>(x.q, P, static_cast<const bf16*>(a.q) + t0 * a.q_ts + hk * a.q_hs, a.q_ts, C, len);
-    copy_tile<NU * 16, THREADS>(x.v, VP, static_cast<const bf16*>(a.v) + t0 * a.v_ts + h * a.v_hs + vb * NU * 16, a.v_ts, C, len);
-    load_vec<THREADS>(x.vec, a.vec + rec * DELTA_VEC, SEQ_ROWS);
+    copy_rows<NU * 16, THREADS>(x.v, VP, static_cast<const bf16*>(a.v) + t0 * a.v_ts + h * a.v_hs + vb * NU * 16, a.v_ts, len);
     bar_arrive_copies(&sm.full[c & 1]);
+    if (threadIdx.x == 0) {
+      bar_expect(&sm.full[c & 1], Stage::BULK);
+      bulk_copy(x.qk, static_cast<const bf16*>(a.qk) + ((c0 + c) * a.Hk + hk) * 2 * C * P, sizeof(x.qk), &sm.full[c & 1]);
+      bulk_copy(x.ap, static_cast<const bf16*>(a.ap) + rec * DELTA_AP, sizeof(x.ap), &sm.full[c & 1]);
+      bulk_copy(x.vec, a.vec + rec * DELTA_VEC, sizeof(x.vec), &sm.full[c & 1]);
+    }
   };
-  // The state in front of chunk c: for the unit's other warps, and for the backward pass.
-  auto publish_state = [&](int c) {
-    uint4* sf = KEEP ? reinterpret_cast<uint4*>(a.states) + ((((c0 + c) * a.Hv + h) * (a.dv / 16) + (col0 >> 4)) * 2) * KT * 32 + lane : nullptr;
+  // The state in front of the next chunk: for the unit's other warps, and (keep_state) for the backward pass.
+  uint32_t ph[KW][4], pl[KW][4];
+  auto publish_state = [&]() {
 #pragma unroll
     for (int k = 0; k < KW; ++k) {
-      uint32_t hi[4], lo[4];
-      split_a(s[2 * k], s[2 * k + 1], hi, lo);
-      put(sm.state[unit][KW * w + k], hi, lo);
-      if (KEEP) {
-        sf[(KW * w + k) * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        sf[(KT + KW * w + k) * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
+      split_a(s[2 * k], s[2 * k + 1], ph[k], pl[k]);
+      put(sm.state[unit][KW * w + k], ph[k], pl[k]);
     }
     bar_arrive(&sm.state_ready[unit]);
   };
+  auto keep_state = [&](int c) {
+    uint4* sf = reinterpret_cast<uint4*>(a.states) + ((((c0 + c) * a.Hv + h) * (a.dv / 16) + (col0 >> 4)) * 2) * KT * 32 + lane;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      sf[(KW * w + k) * 32] = make_uint4(ph[k][0], ph[k][1], ph[k][2], ph[k][3]);
+      sf[(KT + KW * w + k) * 32] = make_uint4(pl[k][0], pl[k][1], pl[k][2], pl[k][3]);
+    }
+  };
   if (chunks > 0) {
     fetch(0);
-    publish_state(0);
+    publish_state();
+    if (KEEP) keep_state(0);
   }
   for (int c = 0; c < chunks; ++c) {
     Stage& x = sm.stage[c & 1];
     const uint32_t parity = c & 1, turn = (c >> 1) & 1;
     const long long t0 = start + static_cast<long long>(c) * C;
     const int len = end - t0 < C ? static_cast<int>(end - t0) : C;
-    const bf16 *ahi = x.ap, *alo = x.ap + C * APITCH, *phi = x.ap + 2 * C * APITCH, *plo = x.ap + 3 * C * APITCH;
+    const bf16 *xq = x.qk, *xk = x.qk + C * P, *ahi = x.ap, *alo = x.ap + C * APITCH, *phi = x.ap + 2 * C * APITCH, *plo = x.ap + 3 * C * APITCH;
     const int tok = 16 * w;  // the warp's first token
     const float* vec = x.vec + tok + t2;
     if (c + 1 < chunks) {  // the other buffer is free when all warps are done with chunk c - 1
@@ -682,7 +702,7 @@ forward_kernel(const DeltaArgs a) {
     // everything that does not wait for the state is in registers before it comes
     uint32_t bk[KT][4], v[4];
 #pragma unroll
-    for (int kk = 0; kk < KT; ++kk) b_from_nk(bk[kk], x.k, P, tok, 16 * kk);
+    for (int kk = 0; kk < KT; ++kk) b_from_nk(bk[kk], xk, P, tok, 16 * kk);
     a_from_km(v, x.v, VP, tok, unit * 16);
     float2 yk[2], be[2];
     factors(vec + V_YK * 64, yk);
@@ -716,17 +736,17 @@ forward_kernel(const DeltaArgs a) {
     split_a(u[0], u[1], rh, rl);
     put(sm.r[unit][w], rh, rl);
     bar_arrive(&sm.r_ready[unit]);
-    // while the others get there: e^G Q S, and (A - I) r with the warp's own part
-    float o[2][4];
-    clear(o);
-    clear(z);
+    // while the others get there: (A - I) r with the warp's own part, the rest of A, and e^G Q S. The output is made for
+    // tokens [tok2, tok2 + 16), mirrored: the warp with the most of A has the least of P.
+    const int tok2 = 48 - tok;
+    const float* vec2 = x.vec + tok2 + t2;
+    uint32_t ab[3][2][4];
 #pragma unroll
-    for (int kk = 0; kk < KT; ++kk) {
-      uint32_t b[4];
-      b_from_nk(b, x.q, P, tok, 16 * kk);
-      mma_pair(o, sh[kk], b);
-      mma_pair(z, sl[kk], b);
-    }
+    for (int kk = 0; kk < 3; ++kk)
+      if (kk < w) {
+        b_from_nk(ab[kk][0], ahi, APITCH, tok, 16 * kk);
+        b_from_nk(ab[kk][1], alo, APITCH, tok, 16 * kk);
+      }
     float m[2][4], m2[2][4], m3[2][4];
     clear(m);
     clear(m2);
@@ -739,25 +759,22 @@ forward_kernel(const DeltaArgs a) {
       mma_pair(m2, rl, b);
       mma_pair(m3, rh, bl);
     }
-    add_to(o, z);
     float2 f2[2], ib[2];
-    factors(vec + V_OQ * 64, f2);
-    scale_tokens(o, f2);
 #pragma unroll
     for (int f = 0; f < 2; ++f) ib[f] = make_float2(__fdividef(1.f, be[f].x), __fdividef(1.f, be[f].y));
     factors(vec + V_SU * 64, f2);
     bar_wait(&sm.r_ready[unit], parity, a.status);
     // (A - I) r; y becomes the memory read at each token, m = e^G K S - ((A - I) r) / beta, in 16 bits, and U is
     // beta (V - m), made of the rounded m and used in two parts everywhere: the products of dg must see the same U.
-    for (int kk = 0; kk < w; ++kk) {
-      uint32_t hi[4], lo[4], b[4], bl[4];
-      b_from_nk(b, ahi, APITCH, tok, 16 * kk);
-      b_from_nk(bl, alo, APITCH, tok, 16 * kk);
-      get(sm.r[unit][kk], hi, lo);
-      mma_pair(m, hi, b);
-      mma_pair(m2, lo, b);
-      mma_pair(m3, hi, bl);
-    }
+#pragma unroll
+    for (int kk = 0; kk < 3; ++kk)
+      if (kk < w) {
+        uint32_t hi[4], lo[4];
+        get(sm.r[unit][kk], hi, lo);
+        mma_pair(m, hi, ab[kk][0]);
+        mma_pair(m2, lo, ab[kk][0]);
+        mma_pair(m3, hi, ab[kk][1]);
+      }
     uint32_t mh[4], ml[4], uh[4], ul[4];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
@@ -769,7 +786,6 @@ forward_kernel(const DeltaArgs a) {
     split_a(m[0], m[1], mh, ml);
 #pragma unroll
     for (int i = 0; i < 4; ++i) memory_term(v[i], mh[i], ml[i], be[i >> 1], u[i >> 1][2 * (i & 1)], u[i >> 1][2 * (i & 1) + 1]);
-    split_a(u[0], u[1], uh, ul);
     {
       float su[2][4];
       uint32_t hi[4], lo[4];
@@ -781,18 +797,10 @@ forward_kernel(const DeltaArgs a) {
       split_a(su[0], su[1], hi, lo);
       put(sm.su[unit][w], hi, lo);
     }
+    split_a(u[0], u[1], uh, ul);
     put(sm.u[unit][w], uh, ul);
     bar_arrive(&sm.u_ready[unit]);
-    // meanwhile: what is kept, and K for the state
-    const long long piece = (((c0 + c) * a.Hv + h) * (a.dv / 16) + (col0 >> 4)) * 4 + w;
-    if (KEEP) {
-      uint4* mf = reinterpret_cast<uint4*>(a.mem) + piece * 64 + lane;
-      mf[0] = make_uint4(mh[0], mh[1], mh[2], mh[3]);
-      mf[32] = make_uint4(ml[0], ml[1], ml[2], ml[3]);
-      uint4* uf = reinterpret_cast<uint4*>(a.u) + piece * 64 + lane;
-      uf[0] = make_uint4(uh[0], uh[1], uh[2], uh[3]);
-      uf[32] = make_uint4(ul[0], ul[1], ul[2], ul[3]);
-    }
+    // meanwhile: K for the state, e^G Q S, and what is kept
     const float ge = x.vec[V_END * 64];
 #pragma unroll
     for (int j = 0; j < 2 * KW; ++j)
@@ -802,7 +810,17 @@ forward_kernel(const DeltaArgs a) {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-      for (int j = 0; j < KW; ++j) b_from_kn(bt[kk][j], x.k, P, 16 * kk, kd0 + 16 * j);
+      for (int j = 0; j < KW; ++j) b_from_kn(bt[kk][j], xk, P, 16 * kk, kd0 + 16 * j);
+    float o[2][4];
+    clear(o);
+    clear(z);
+#pragma unroll
+    for (int kk = 0; kk < KT; ++kk) {
+      uint32_t b[4];
+      b_from_nk(b, xq, P, tok2, 16 * kk);
+      mma_pair(o, sh[kk], b);
+      mma_pair(z, sl[kk], b);
+    }
     bar_wait(&sm.u_ready[unit], parity, a.status);
     // S^T <- e^{G_C} S^T + (e^{G_C - G} U)^T K, the warp's columns of dk
 #pragma unroll
@@ -811,31 +829,49 @@ forward_kernel(const DeltaArgs a) {
       get(sm.su[unit][kk], hi, lo);
       mma2<KW>(s, hi, lo, bt[kk]);
     }
-    if (c + 1 < chunks) publish_state(c + 1);
+    if (c + 1 < chunks) publish_state();
     // what earlier tokens give to the output: + (P - diag P) U, with all four parts: the backward pass multiplies with
     // this P and this U too
+    add_to(o, z);
+    factors(vec2 + V_OQ * 64, f2);
+    scale_tokens(o, f2);
     clear(z);
     clear(m2);
     clear(m3);
-    for (int kk = 0; kk <= w; ++kk) {
-      uint32_t hi[4], lo[4], b[4], bl[4];
-      b_from_nk(b, phi, APITCH, tok, 16 * kk);
-      b_from_nk(bl, plo, APITCH, tok, 16 * kk);
-      get(sm.u[unit][kk], hi, lo);
-      mma_pair(o, hi, b);
-      mma_pair(z, lo, b);
-      mma_pair(m2, hi, bl);
-      mma_pair(m3, lo, bl);
-    }
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      if (kk <= 3 - w) {
+        uint32_t hi[4], lo[4], b[4], bl[4];
+        b_from_nk(b, phi, APITCH, tok2, 16 * kk);
+        b_from_nk(bl, plo, APITCH, tok2, 16 * kk);
+        get(sm.u[unit][kk], hi, lo);
+        mma_pair(o, hi, b);
+        mma_pair(z, lo, b);
+        mma_pair(m2, hi, bl);
+        mma_pair(m3, lo, bl);
+      }
     add_to(m2, m3);
     add_to(z, m2);
     add_to(o, z);
     if (KEEP) {
-      float4* pf = reinterpret_cast<float4*>(a.past) + piece * 64 + lane;
-      pf[0] = make_float4(o[0][0], o[0][1], o[0][2], o[0][3]);
-      pf[32] = make_float4(o[1][0], o[1][1], o[1][2], o[1][3]);
+      const long long piece = (((c0 + c) * a.Hv + h) * (a.dv / 16) + (col0 >> 4)) * 4;
+      uint4* mf = reinterpret_cast<uint4*>(a.mem) + (piece + w) * 64 + lane;
+      mf[0] = make_uint4(mh[0], mh[1], mh[2], mh[3]);
+      mf[32] = make_uint4(ml[0], ml[1], ml[2], ml[3]);
+      uint4* uf = reinterpret_cast<uint4*>(a.u) + (piece + w) * 64 + lane;
+      uf[0] = make_uint4(uh[0], uh[1], uh[2], uh[3]);
+      uf[32] = make_uint4(ul[0], ul[1], ul[2], ul[3]);
+      uint4* pf = reinterpret_cast<uint4*>(a.past) + (piece + 3 - w) * 64 + lane;
+      pf[0] = make_uint4(__float_as_uint(o[0][0]), __float_as_uint(o[0][1]), __float_as_uint(o[0][2]), __float_as_uint(o[0][3]));
+      pf[32] = make_uint4(__float_as_uint(o[1][0]), __float_as_uint(o[1][1]), __float_as_uint(o[1][2]), __float_as_uint(o[1][3]));
+      if (c + 1 < chunks) keep_state(c + 1);
     }
-    factors(vec + V_PD * 64, f2);
+    {
+      uint32_t hi[4], lo[4];
+      get(sm.u[unit][3 - w], hi, lo);
+      join(make_uint4(hi[0], hi[1], hi[2], hi[3]), make_uint4(lo[0], lo[1], lo[2], lo[3]), u);
+    }
+    factors(vec2 + V_PD * 64, f2);
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
       o[f][0] += f2[f].x * u[f][0];
@@ -844,8 +880,8 @@ forward_kernel(const DeltaArgs a) {
       o[f][3] += f2[f].y * u[f][3];
     }
     bar_arrive(&sm.empty[c & 1]);
-    store_tile(sm.out[warp], static_cast<bf16*>(a.o) + ((t0 + tok) * a.Hv + h) * a.dv + col0, static_cast<long long>(a.Hv) * a.dv,
-               len - tok, o[0], o[1]);
+    store_tile(sm.out[warp], static_cast<bf16*>(a.o) + ((t0 + tok2) * a.Hv + h) * a.dv + col0, static_cast<long long>(a.Hv) * a.dv,
+               len - tok2, o[0], o[1]);
   }
   if (a.s_out) {
 #pragma unroll
@@ -860,14 +896,15 @@ forward_kernel(const DeltaArgs a) {
 
 template <int DK, int NU>
 struct BwdStage {
-  static constexpr int P = DK + 8, VP = NU * 16 + 8;
-  bf16 k[C * P], q[C * P], dO[C * VP], ap[4 * C * APITCH];
+  static constexpr int P = DK + DELTA_ROW_PAD, VP = NU * 16 + 8;
+  bf16 qk[2 * C * P], ap[DELTA_AP], dO[C * VP];
   float vec[SEQ_ROWS * 64];
+  static constexpr uint32_t BULK = (2 * C * P + DELTA_AP) * sizeof(bf16) + SEQ_ROWS * 64 * sizeof(float);
 };
 template <int DK, int NU>
 struct BwdSmem {
   BwdStage<DK, NU> stage[2];
-  Operands state[NU][DK / 16], du[NU][4], dv[NU][4];
+  Operands state[NU][DK / 16], du[NU][4], dv[NU][4], go[NU][4];
   bf16 out[NU * 4][16 * OUT_PITCH];
   uint64_t full[2], empty[2], state_ready[NU], du_ready[NU], dv_ready[NU];
 };
@@ -889,7 +926,7 @@ backward_kernel(const DeltaArgs a) {
   const int chunks = static_cast<int>((end - start + C - 1) / C);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      bar_init(&sm.full[i], THREADS);
+      bar_init(&sm.full[i], THREADS + 1);
       bar_init(&sm.empty[i], NU * 4);
     }
     for (int i = 0; i < NU; ++i) {
@@ -918,24 +955,30 @@ backward_kernel(const DeltaArgs a) {
     const int len = end - t0 < C ? static_cast<int>(end - t0) : C;
     const long long rec = (c0 + c) * a.Hv + h;
     const long long row = (t0 * a.Hv + h) * a.dv + vb * NU * 16, stride = static_cast<long long>(a.Hv) * a.dv;
-    copy_tile<DK, THREADS>(x.k, P, static_cast<const bf16*>(a.k) + t0 * a.k_ts + hk * a.k_hs, a.k_ts, C, len);
-    copy_tile<64, THREADS>(x.ap, APITCH, static_cast<const bf16*>(a.ap) + rec * DELTA_AP, C, 4 * C, 4 * C);
-    copy_tile<NU * 16, THREADS>(x.dO, VP, static_cast<const bf16*>(a.dout) + row, stride, C, len);
-    copy_tile<DK, THREADS>(x.q, P, static_cast<const bf16*>(a.q) + t0 * a.q_ts + hk * a.q_hs, a.q_ts, C, len);
-    load_vec<THREADS>(x.vec, a.vec + rec * DELTA_VEC, SEQ_ROWS);
+    copy_rows<NU * 16, THREADS>(x.dO, VP, static_cast<const bf16*>(a.dout) + row, stride, len);
     bar_arrive_copies(&sm.full[i & 1]);
+    if (threadIdx.x == 0) {
+      bar_expect(&sm.full[i & 1], Stage::BULK);
+      bulk_copy(x.qk, static_cast<const bf16*>(a.qk) + ((c0 + c) * a.Hk + hk) * 2 * C * P, sizeof(x.qk), &sm.full[i & 1]);
+      bulk_copy(x.ap, static_cast<const bf16*>(a.ap) + rec * DELTA_AP, sizeof(x.ap), &sm.full[i & 1]);
+      bulk_copy(x.vec, a.vec + rec * DELTA_VEC, sizeof(x.vec), &sm.full[i & 1]);
+    }
   };
-  // The gradient of the state behind chunk c: for the unit's other warps, and (high part) for dqk.
-  auto publish_state = [&](int c) {
-    uint4* df = reinterpret_cast<uint4*>(a.dstates) + (((c0 + c) * a.Hv + h) * VT + vt) * KT * 32 + lane;
+  // The gradient of the state behind a chunk: for the unit's other warps, and (keep_state, high part) for dqk.
+  uint32_t ph[KW][4];
+  auto publish_state = [&]() {
 #pragma unroll
     for (int k = 0; k < KW; ++k) {
-      uint32_t hi[4], lo[4];
-      split_a(s[2 * k], s[2 * k + 1], hi, lo);
-      put(sm.state[unit][KW * w + k], hi, lo);
-      df[(KW * w + k) * 32] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      uint32_t lo[4];
+      split_a(s[2 * k], s[2 * k + 1], ph[k], lo);
+      put(sm.state[unit][KW * w + k], ph[k], lo);
     }
     bar_arrive(&sm.state_ready[unit]);
+  };
+  auto keep_state = [&](int c) {
+    uint4* df = reinterpret_cast<uint4*>(a.dstates) + (((c0 + c) * a.Hv + h) * VT + vt) * KT * 32 + lane;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) df[(KW * w + k) * 32] = make_uint4(ph[k][0], ph[k][1], ph[k][2], ph[k][3]);
   };
   // What a chunk's warp reads of the forward pass: its part of the state in front, and m, U, past of its tokens.
   struct Kept {
@@ -959,7 +1002,8 @@ backward_kernel(const DeltaArgs a) {
   if (chunks > 0) {
     fetch(0);
     load_kept(chunks - 1, next);
-    publish_state(chunks - 1);
+    publish_state();
+    keep_state(chunks - 1);
   }
   for (int i = 0; i < chunks; ++i) {
     const int c = chunks - 1 - i;
@@ -968,7 +1012,7 @@ backward_kernel(const DeltaArgs a) {
     const long long t0 = start + static_cast<long long>(c) * C;
     const int len = end - t0 < C ? static_cast<int>(end - t0) : C;
     const long long rec = (c0 + c) * a.Hv + h;
-    const bf16 *ahi = x.ap, *alo = x.ap + C * APITCH, *phi = x.ap + 2 * C * APITCH, *plo = x.ap + 3 * C * APITCH;
+    const bf16 *xq = x.qk, *xk = x.qk + C * P, *ahi = x.ap, *alo = x.ap + C * APITCH, *phi = x.ap + 2 * C * APITCH, *plo = x.ap + 3 * C * APITCH;
     const int tok = 16 * w;
     const float* vec = x.vec + tok + t2;
     now = next;
@@ -984,17 +1028,23 @@ backward_kernel(const DeltaArgs a) {
     clear(u);
     clear(z);
     uint32_t fo[4];  // dO^T of the warp's tokens
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      if (kk >= w) {
+        uint32_t f[4], b[4], bl[4];
+        a_from_km(f, x.dO, VP, 16 * kk, unit * 16);
+        b_from_kn(b, phi, APITCH, 16 * kk, tok);
+        b_from_kn(bl, plo, APITCH, 16 * kk, tok);
+        mma_pair(u, f, b);
+        mma_pair(z, f, bl);
+      }
     a_from_km(fo, x.dO, VP, tok, unit * 16);
-    for (int kk = w; kk < 4; ++kk) {
-      uint32_t f[4], b[4], bl[4];
-      a_from_km(f, x.dO, VP, 16 * kk, unit * 16);
-      b_from_kn(b, phi, APITCH, 16 * kk, tok);
-      b_from_kn(bl, plo, APITCH, 16 * kk, tok);
-      mma_pair(u, f, b);
-      mma_pair(z, f, bl);
-    }
-    add_to(u, z);
     float2 f2[2], su[2], be[2];
+    factors(vec + V_OQ * 64, f2);
+    uint32_t gh[4], gl[4];  // e^G dO, for the state
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split2(lo_half(fo[e]) * f2[e >> 1].x, hi_half(fo[e]) * f2[e >> 1].y, gh[e], gl[e]);
+    add_to(u, z);
     factors(vec + V_PD * 64, f2);
 #pragma unroll
     for (int f = 0; f < 2; ++f) {  // diag P dO
@@ -1006,8 +1056,9 @@ backward_kernel(const DeltaArgs a) {
     factors(vec + V_SU * 64, su);
     uint32_t bk[KT][4];
 #pragma unroll
-    for (int kk = 0; kk < KT; ++kk) b_from_nk(bk[kk], x.k, P, tok, 16 * kk);
+    for (int kk = 0; kk < KT; ++kk) b_from_nk(bk[kk], xk, P, tok, 16 * kk);
     bar_wait(&sm.state_ready[unit], parity, a.status);
+    put(sm.go[unit][w], gh, gl);  // not before: the last chunk's is read until the state is published
     // y = (e^{G_C - G} K dS1)^T
     clear(y);
     clear(z);
@@ -1033,45 +1084,23 @@ backward_kernel(const DeltaArgs a) {
       put(sm.du[unit][w], dh, dl);
     }
     bar_arrive(&sm.du_ready[unit]);
-    // while the others get there: <dS1, S0>, U and m of the warp's tokens, and Q^T diag(e^G) dO into the state
+    // while the others get there: U + dU^T (A - I) begins with the warp's own part
     const float ge = x.vec[V_END * 64];
-    float sdot = 0.f;
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-      const uint32_t wh[4] = {now.sh[k].x, now.sh[k].y, now.sh[k].z, now.sh[k].w}, wl[4] = {now.sl[k].x, now.sl[k].y, now.sl[k].z, now.sl[k].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sdot += s[2 * k + (e >> 1)][2 * (e & 1)] * (lo_half(wh[e]) + lo_half(wl[e]));
-        sdot += s[2 * k + (e >> 1)][2 * (e & 1) + 1] * (hi_half(wh[e]) + hi_half(wl[e]));
-      }
-    }
-    sdot *= ge;
     float mm[2][4], uu[2][4];
     join(now.m[0], now.m[1], mm);
     join(now.u[0], now.u[1], uu);
+    float sdot = 0.f, bdot = 0.f;
 #pragma unroll
     for (int f = 0; f < 2; ++f)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sdot += y[f][e] * uu[f][e];
+      for (int e = 0; e < 4; ++e) bdot += y[f][e] * uu[f][e];
+    uint32_t ab[3][2][4];
 #pragma unroll
-    for (int j = 0; j < 2 * KW; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[j][e] *= ge;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      uint32_t f[4], hi[4], lo[4], b[KW][4];
-      a_from_km(f, x.dO, VP, 16 * kk, unit * 16);
-      float2 oq[2];
-      factors(x.vec + V_OQ * 64 + 16 * kk + t2, oq);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) split2(lo_half(f[e]) * oq[e >> 1].x, hi_half(f[e]) * oq[e >> 1].y, hi[e], lo[e]);
-#pragma unroll
-      for (int j = 0; j < KW; ++j) b_from_kn(b[j], x.q, P, 16 * kk, kd0 + 16 * j);
-      mma2<KW>(s, hi, lo, b);
-    }
-    factors(vec + V_BETA * 64, be);
-    factors(vec + V_YK * 64, f2);
-    // u <- u + dU^T (A - I): X without what the token's own output asks for; first with the warp's own part
+    for (int kk = 1; kk < 4; ++kk)
+      if (kk > w) {
+        b_from_kn(ab[kk - 1][0], ahi, APITCH, 16 * kk, tok);
+        b_from_kn(ab[kk - 1][1], alo, APITCH, 16 * kk, tok);
+      }
     clear(y);
     clear(z);
     {
@@ -1082,16 +1111,19 @@ backward_kernel(const DeltaArgs a) {
       mma_pair(y, dl, b);
       mma_pair(z, dh, bl);
     }
+    factors(vec + V_BETA * 64, be);
+    factors(vec + V_YK * 64, f2);
     bar_wait(&sm.du_ready[unit], parity, a.status);
-    for (int kk = w + 1; kk < 4; ++kk) {
-      uint32_t hi[4], lo[4], b[4], bl[4];
-      b_from_kn(b, ahi, APITCH, 16 * kk, tok);
-      b_from_kn(bl, alo, APITCH, 16 * kk, tok);
-      get(sm.du[unit][kk], hi, lo);
-      mma_pair(u, hi, b);
-      mma_pair(y, lo, b);
-      mma_pair(z, hi, bl);
-    }
+    // u <- u + dU^T (A - I): X without what the token's own output asks for
+#pragma unroll
+    for (int kk = 1; kk < 4; ++kk)
+      if (kk > w) {
+        uint32_t hi[4], lo[4];
+        get(sm.du[unit][kk], hi, lo);
+        mma_pair(u, hi, ab[kk - 1][0]);
+        mma_pair(y, lo, ab[kk - 1][0]);
+        mma_pair(z, hi, ab[kk - 1][1]);
+      }
     add_to(y, z);
     add_to(u, y);
     // X = u + (diag P dO)^T, dV = beta X; row sums over the unit's 16 columns: past . dO - m . dV - U . u, and U . X
@@ -1124,11 +1156,34 @@ backward_kernel(const DeltaArgs a) {
       d[0][2 * f] += past[0] * lo_half(fo[2 * f]) + past[2] * lo_half(fo[2 * f + 1]) - (mm[f][0] * u[f][0] + mm[f][2] * u[f][2]);
       d[0][2 * f + 1] += past[1] * hi_half(fo[2 * f]) + past[3] * hi_half(fo[2 * f + 1]) - (mm[f][1] * u[f][1] + mm[f][3] * u[f][3]);
     }
+    // while the others get there: <dS1, S0>, and Q^T diag(e^G) dO into the state
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const uint32_t wh[4] = {now.sh[k].x, now.sh[k].y, now.sh[k].z, now.sh[k].w}, wl[4] = {now.sl[k].x, now.sl[k].y, now.sl[k].z, now.sl[k].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sdot += s[2 * k + (e >> 1)][2 * (e & 1)] * (lo_half(wh[e]) + lo_half(wl[e]));
+        sdot += s[2 * k + (e >> 1)][2 * (e & 1) + 1] * (hi_half(wh[e]) + hi_half(wl[e]));
+      }
+    }
+    sdot = sdot * ge + bdot;
+#pragma unroll
+    for (int j = 0; j < 2 * KW; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[j][e] *= ge;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      uint32_t hi[4], lo[4], b[KW][4];
+#pragma unroll
+      for (int j = 0; j < KW; ++j) b_from_kn(b[j], xq, P, 16 * kk, kd0 + 16 * j);
+      get(sm.go[unit][kk], hi, lo);
+      mma2<KW>(s, hi, lo, b);
+    }
     uint32_t bt[4][KW][4];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-      for (int j = 0; j < KW; ++j) b_from_kn(bt[kk][j], x.k, P, 16 * kk, kd0 + 16 * j);
+      for (int j = 0; j < KW; ++j) b_from_kn(bt[kk][j], xk, P, 16 * kk, kd0 + 16 * j);
     bar_wait(&sm.dv_ready[unit], parity, a.status);
     // dS0 -= K^T diag(e^G) dV
 #pragma unroll
@@ -1137,8 +1192,9 @@ backward_kernel(const DeltaArgs a) {
       get(sm.dv[unit][kk], hi, lo);
       mma2<KW>(s, hi, lo, bt[kk]);
     }
-    if (c > 0) publish_state(c - 1);
+    if (c > 0) publish_state();
     bar_arrive(&sm.empty[i & 1]);
+    if (c > 0) keep_state(c - 1);
     store_tile(sm.out[warp], static_cast<bf16*>(a.dv_) + ((t0 + tok) * a.Hv + h) * a.dv + col0,
                static_cast<long long>(a.Hv) * a.dv, len - tok, u[0], u[1]);
     float* rd = a.rowdots + (rec * VT + vt) * 128 + tok + t2;

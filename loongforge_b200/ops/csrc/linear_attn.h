@@ -7,7 +7,8 @@ namespace lf {
 
 constexpr int DELTA_CHUNK = 64;      // tokens of one chunk
 constexpr int DELTA_VEC = 11 * 64;   // fp32 words of one chunk's per-token factors (see the prepare kernel)
-constexpr int DELTA_AP = 4 * 64 * 64;  // bf16 words of one chunk's inverse and score matrix (high and low parts)
+constexpr int DELTA_AP = 4 * 64 * 72;  // bf16 words of one chunk's inverse and score matrix (high and low parts, rows of 72)
+constexpr int DELTA_ROW_PAD = 8;       // bf16 behind every row of a chunk's q and k tiles
 
 struct DeltaArgs {
   const void *q = nullptr, *k = nullptr, *v = nullptr;  // bf16 [T, Hk, dk], [T, Hk, dk], [T, Hv, dv]
@@ -26,6 +27,7 @@ struct DeltaArgs {
   // what o owes to earlier tokens (fp32), the memory read at each token and U (bf16 and the remainder of the rounding);
   // and the state in front of every chunk.
   void *past = nullptr, *mem = nullptr, *u = nullptr, *states = nullptr;
+  void* qk = nullptr;    // bf16 [NC, Hk, 2, 64, dk + DELTA_ROW_PAD]: q and k of every chunk, rows behind its end zero
   void* ap = nullptr;    // bf16 [NC, Hv, DELTA_AP]
   float* vec = nullptr;  // fp32 [NC, Hv, DELTA_VEC]
   // backward

@@ -46,6 +46,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <atomic>
 #include "linear_attn.h"
 
 namespace lf {
@@ -1500,9 +1501,16 @@ gates_kernel(const DeltaArgs a) {
 
 // --------------------------------------------------------------------------------------------------------- launches
 
+// Once per kernel and device: the call costs as much as a launch.
 template <typename K>
-bool allow_smem(K kernel, size_t bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess;
+bool allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess) return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 template <int DK, int NU, bool KEEP>
@@ -1510,7 +1518,8 @@ int launch_forward(const DeltaArgs& a, cudaStream_t s) {
   const long long grid = static_cast<long long>(a.N) * a.Hv * (a.dv / (NU * 16));
   if (grid > INT32_MAX) return -2;
   const size_t bytes = sizeof(FwdSmem<DK, NU>);
-  if (!allow_smem(forward_kernel<DK, NU, KEEP>, bytes)) return -3;
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(forward_kernel<DK, NU, KEEP>, bytes, allowed)) return -3;
   forward_kernel<DK, NU, KEEP><<<static_cast<unsigned>(grid), NU * 128, bytes, s>>>(a);
   return 0;
 }
@@ -1520,7 +1529,8 @@ int launch_backward(const DeltaArgs& a, cudaStream_t s) {
   const long long grid = static_cast<long long>(a.N) * a.Hv * (a.dv / (NU * 16));
   if (grid > INT32_MAX) return -2;
   const size_t bytes = sizeof(BwdSmem<DK, NU>);
-  if (!allow_smem(backward_kernel<DK, NU>, bytes)) return -3;
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(backward_kernel<DK, NU>, bytes, allowed)) return -3;
   backward_kernel<DK, NU><<<static_cast<unsigned>(grid), NU * 128, bytes, s>>>(a);
   return 0;
 }
@@ -1528,7 +1538,8 @@ int launch_backward(const DeltaArgs& a, cudaStream_t s) {
 template <int DK, int DV>
 int launch_dqk(const DeltaArgs& a, cudaStream_t s) {
   const size_t bytes = sizeof(DqkSmem<DK, DV>);
-  if (!allow_smem(dqk_kernel<DK, DV>, bytes)) return -3;
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(dqk_kernel<DK, DV>, bytes, allowed)) return -3;
   dqk_kernel<DK, DV><<<static_cast<unsigned>(a.NC * a.Hk), DQK_THREADS, bytes, s>>>(a);
   return 0;
 }
@@ -1537,7 +1548,8 @@ template <int DK>
 int forward_dk(const DeltaArgs& a, cudaStream_t s) {
   if (a.NC > 0) {
     const size_t bytes = (2 * C * (DK + 8)) * sizeof(bf16) + (2 * C * MP + 5 * C) * sizeof(float);
-    if (!allow_smem(prepare_kernel<DK>, bytes)) return -3;
+    static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(prepare_kernel<DK>, bytes, allowed)) return -3;
     prepare_kernel<DK><<<static_cast<unsigned>(a.NC * a.Hk), PREP_THREADS, bytes, s>>>(a);
   }
   const int rc = a.states ? launch_forward<DK, 2, true>(a, s) : launch_forward<DK, 2, false>(a, s);

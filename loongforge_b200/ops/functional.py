@@ -341,7 +341,7 @@ class _QKNormRopeFn(torch.autograd.Function):
         ctx.save_for_backward(qkv, qw, kw, freqs, inv_freq, pos, axis)
         q, k = _C().qk_norm_rope_fwd(qkv, G, R, gated, qw, kw, freqs, inv_freq, pos, axis, *ctx.cfg[1],
                                      _ext.status_tensor(qkv.device))
-        x = qkv.unflatten(1, (G, 2 * R + 2 if gated else R + 2, -1))
+        x = qkv.view(qkv.shape[0], G, 2 * R + 2 if gated else R + 2, q.shape[-1])
         return (q, k, x[:, :, -1]) + ((x[:, :, R:2 * R],) if gated else ())
 
     @staticmethod

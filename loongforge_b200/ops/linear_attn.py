@@ -102,36 +102,52 @@ def _chunk_one(q, k, v, g, beta, chunk: int, state=None):
 class _GatedDeltaFn(torch.autograd.Function):
     """The chunked kernels. Kept for the backward pass: U and the memory read at each token (both with the remainder of
     their bf16 rounding), the part of o that earlier tokens wrote, the state in front of every chunk and the chunk's
-    64 x 64 matrices."""
+    tiles and 64 x 64 matrices."""
 
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, s_in, bounds, first, scale, l2norm, want_state, keep):
+    def forward(ctx, q, k, v, g, beta, s_in, cu, scale, l2norm, want_state, keep):
         ctx.set_materialize_grads(False)
-        o, s_out, *kept = _ext.require().delta_fwd(q, k, v, g, beta, bounds, first, scale, l2norm, s_in, want_state, keep,
-                                                       _ext.status_tensor(v.device))
+        C, status = _ext.require(), _status(v)
+        q, k, v, gf, bf = _rows16(q), _rows16(k), _rows16(v), _fp32(g), _fp32(beta)
+        bounds, first = (None, None) if cu is None else C.delta_plan(cu, q.shape[0], status)
+        o, s_out, *kept = C.delta_fwd(q, k, v, gf, bf, bounds, first, scale, l2norm, s_in, want_state, keep, status)
         if keep:
-            ctx.save_for_backward(q, k, v, g, beta, bounds, first, *kept)
-        ctx.cfg = (scale, l2norm)
+            ctx.save_for_backward(q, k, v, gf, bf, bounds, first, *kept)
+            ctx.cfg = (scale, l2norm, g.dtype, beta.dtype)
         if not want_state:
             ctx.mark_non_differentiable(s_out)
         return o, s_out
 
     @staticmethod
     def backward(ctx, do, ds_out):
-        scale, l2norm = ctx.cfg
+        scale, l2norm, g_dtype, beta_dtype = ctx.cfg
         q, k, v, g, beta, bounds, first, *kept = ctx.saved_tensors
         want_ds = ctx.needs_input_grad[5]
         do = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if do is None else _dense16(do)
         dq, dk, dv, dg, dbeta, ds_in = _ext.require().delta_bwd(
             do, None if ds_out is None else _dense16(ds_out), q, k, v, g, beta, bounds, first, scale, l2norm, want_ds, *kept,
-            _ext.status_tensor(v.device))
-        return (dq, dk, dv, dg, dbeta, ds_in if want_ds else None) + (None,) * 6
+            _status(v))
+        return (dq, dk, dv, dg.to(g_dtype), dbeta.to(beta_dtype), ds_in if want_ds else None) + (None,) * 5
+
+
+def _status(t: torch.Tensor) -> torch.Tensor:
+    s = _ext._status.get(t.get_device())
+    return s if s is not None else _ext.status_tensor(t.device)
+
+
+def _fp32(t: torch.Tensor) -> torch.Tensor:
+    return t.detach().float().contiguous()
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
     """The tensor itself when its rows are unit-stride and 16-byte aligned (what the kernels read), else a copy."""
-    ok = t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        s = t.stride()
+        if s[-1] == 1 and all(x % 8 == 0 for x in s[:-1]):
+            return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _dense16(t: torch.Tensor) -> torch.Tensor:
@@ -147,14 +163,16 @@ def gated_delta_rule_native(q, k, v) -> bool:
 
 
 def _check_delta(q, k, v, g, beta, rows: str):
-    if q.dim() != 3 or k.shape != q.shape or v.dim() != 3 or v.shape[0] != q.shape[0]:
-        raise ValueError(f"q, k [{rows}, key heads, dk] and v [{rows}, value heads, dv] expected, got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
-    if g.shape != v.shape[:2] or beta.shape != v.shape[:2]:
+    qs, vs = q.shape, v.shape
+    if len(qs) != 3 or k.shape != qs or len(vs) != 3 or vs[0] != qs[0]:
+        raise ValueError(f"q, k [{rows}, key heads, dk] and v [{rows}, value heads, dv] expected, got {tuple(qs)}, "
+                         f"{tuple(k.shape)}, {tuple(vs)}")
+    if g.shape != vs[:2] or beta.shape != vs[:2]:
         raise ValueError(f"g and beta [{rows}, value heads] expected, got {tuple(g.shape)}, {tuple(beta.shape)}")
-    if q.shape[1] == 0 or v.shape[1] % q.shape[1]:
-        raise ValueError(f"{v.shape[1]} value heads are not a multiple of {q.shape[1]} key heads")
-    if any(t.device != v.device for t in (q, k, g, beta)):
+    if qs[1] == 0 or vs[1] % qs[1]:
+        raise ValueError(f"{vs[1]} value heads are not a multiple of {qs[1]} key heads")
+    dev = v.device
+    if q.device != dev or k.device != dev or g.device != dev or beta.device != dev:
         raise ValueError("q, k, v, g and beta must be on one device")
 
 
@@ -177,6 +195,8 @@ def _device_bounds(cu_seqlens, T: int, device) -> Optional[torch.Tensor]:
         return torch.tensor(_host_bounds(cu_seqlens, T), dtype=torch.int32, device=device)
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
         raise ValueError("cu_seqlens must hold at least two offsets")
+    if cu_seqlens.dtype == torch.int32 and cu_seqlens.device == device and cu_seqlens.is_contiguous():
+        return cu_seqlens
     return cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
 
 
@@ -199,16 +219,13 @@ def gated_delta_rule(q, k, v, g, beta, *, cu_seqlens=None, scale: Optional[float
     H, dv = v.shape[1:]
     scale = float(scale) if scale is not None else dk ** -0.5
     if gated_delta_rule_native(q, k, v):
-        bounds = _device_bounds(cu_seqlens, T, v.device)
-        n = 1 if bounds is None else bounds.numel() - 1
+        cu = _device_bounds(cu_seqlens, T, v.device)
         if initial_state is not None:
-            _check_state(initial_state, (n, H, dk, dv), v.device, "initial_state")
+            _check_state(initial_state, (1 if cu is None else cu.numel() - 1, H, dk, dv), v.device, "initial_state")
             initial_state = _dense16(initial_state)
-        C = _ext.require()
-        bounds, first = C.delta_plan(bounds, T, _ext.status_tensor(v.device)) if bounds is not None else (None, None)
-        ins = (_rows16(q), _rows16(k), _rows16(v), g.float().contiguous(), beta.float().contiguous(), initial_state)
-        keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ins)
-        o, last = _GatedDeltaFn.apply(*ins, bounds, first, scale, qk_l2norm, output_final_state, keep)
+        keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+                                            or beta.requires_grad or (initial_state is not None and initial_state.requires_grad))
+        o, last = _GatedDeltaFn.apply(q, k, v, g, beta, initial_state, cu, scale, qk_l2norm, output_final_state, keep)
         return (o, last) if output_final_state else o
     dt = v.dtype
     bounds = _host_bounds(cu_seqlens, T)
@@ -233,7 +250,7 @@ def gated_delta_rule(q, k, v, g, beta, *, cu_seqlens=None, scale: Optional[float
 
 
 def _check_state(state, shape, device, name: str):
-    if tuple(state.shape) != tuple(shape) or state.dtype != torch.float32 or state.device != device:
+    if state.shape != shape or state.dtype != torch.float32 or state.device != device:
         raise ValueError(f"{name} must be fp32 {list(shape)} on {device}, got {state.dtype} {list(state.shape)} on "
                          f"{state.device}")
 
@@ -252,13 +269,19 @@ def _step_index(state_indices, rows: int, slots: int, device) -> Optional[torch.
         if len(idx) != rows or any(i >= slots for i in used) or len(set(used)) < len(used):
             raise ValueError(f"state_indices must name {rows} different slots below {slots} (negative: no row)")
         return torch.tensor(idx, dtype=torch.int32, device=device)
-    if state_indices.numel() != rows or state_indices.dim() != 1:
+    if state_indices.shape != (rows,):
         raise ValueError(f"state_indices must hold one slot for each of the {rows} rows")
+    if state_indices.dtype == torch.int32 and state_indices.device == device and state_indices.is_contiguous():
+        return state_indices
     return state_indices.to(device=device, dtype=torch.int32).contiguous()
 
 
 def _no_gradient(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is None or not t.requires_grad:
+            continue
         raise RuntimeError("the single-token form updates its state in place and has no gradient: call it under "
                            "torch.no_grad()")
 
@@ -283,8 +306,9 @@ def gated_delta_rule_step(q, k, v, g, beta, state: torch.Tensor, *, state_indice
     scale = float(scale) if scale is not None else dk ** -0.5
     idx = _step_index(state_indices, B, state.shape[0], v.device)
     if gated_delta_rule_native(q, k, v):
-        return _ext.require().delta_step(_rows16(q), _rows16(k), _rows16(v), g.float().contiguous(), beta.float().contiguous(),
-                                         state, idx, scale, qk_l2norm, _ext.status_tensor(v.device))
+        return _ext.require().delta_step(_rows16(q), _rows16(k), _rows16(v), g if g.dtype == torch.float32 and g.is_contiguous() else _fp32(g),
+                                         beta if beta.dtype == torch.float32 and beta.is_contiguous() else _fp32(beta), state, idx,
+                                         scale, qk_l2norm, _status(v))
     out = v.new_zeros(B, H, dv)
     for b, slot in enumerate(range(B) if idx is None else idx.tolist()):
         if slot < 0:
@@ -339,7 +363,9 @@ def _conv_native(x, weight) -> bool:
 
 def _plain16(t):
     """Contiguous bf16 parameter with a 16-byte aligned base."""
-    return None if t is None else _dense16(t.to(torch.bfloat16))
+    if t is None or (t.dtype == torch.bfloat16 and t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return _dense16(t.to(torch.bfloat16))
 
 
 def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, cu_seqlens=None,
@@ -379,7 +405,7 @@ def causal_conv1d_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     idx = _step_index(state_indices, B, state.shape[0], x.device)
     if _conv_native(x, weight):
         return _ext.require().conv1d_step(_rows16(x), state, _plain16(weight), _plain16(bias), idx, _ACTIVATIONS[activation],
-                                          _ext.status_tensor(x.device))
+                                          _status(x))
     out = torch.zeros_like(x)
     for b, slot in enumerate(range(B) if idx is None else idx.tolist()):
         if slot < 0:

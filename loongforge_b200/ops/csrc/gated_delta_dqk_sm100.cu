@@ -1,0 +1,345 @@
+// dQ and dK of the gated delta rule for head dims dk = dv = 128, on tcgen05 (gated_delta_sm100.cu has the formulas).
+//
+// One (chunk, value head) is five products with 128 rows and 128 columns in TMEM. Tokens are rows, 0-63 for dq and
+// 64-127 for dk (or for what leads there):
+//
+//   D3 = [dO; dV] [U_hi; U_lo]^T                    -> W = lower(dO U^T) D and N = -strict_lower(dV U^T) D, in two parts each
+//   D1 = [dO; dV] S0^T                              -> dq += e^G (.), dk -= e^G (.)
+//   D2 = [  ; U_hi] dS1^T + [  ; U_lo] dS1^T        -> dk += e^{G_C - G} (.)
+//   D4 = [W; N] K + [0; W^T] Q + [0; N^T] K         -> dq += , dk +=
+//
+// Rows are scaled when the accumulators are read, so that every operand is a bf16 tile as it lies in memory. An operand
+// tile whose first 64 rows are not wanted starts 64 rows early: what lies there ends in rows of D2 that nobody reads; for
+// D4 a tile of zeros lies there.
+//
+// Bound by memory: 112 KB a (chunk, value head), of which 64 KB are the two states. One block per SM goes through its share
+// of (chunk, key head) pairs; eight warps bring tiles (they hold register fragments, turned by stmatrix on the way), one
+// thread issues the products, eight warps make W and N, and add up rows over the value heads of a key head.
+#include <atomic>
+#include "gated_delta.cuh"
+#include "sm100_ptx.cuh"
+
+namespace lf {
+namespace {
+
+using namespace delta;
+
+// Warps 0-7 compute, 8-14 load, 15 issues: sixteen warps leave 128 registers a thread, seventeen 96.
+constexpr int D = 128, LOAD_WARPS = 7, LOADERS = 32 * LOAD_WARPS, THREADS = 512;
+constexpr int TILES = 64, MINE = (TILES + LOAD_WARPS - 1) / LOAD_WARPS;  // 16 x 16 fragments of one 128 x 128 operand, and a warp's share
+constexpr uint32_t BIG = 128 * 128, BOX = 64 * 128;                    // bytes of a 128 x 64 and a 64 x 64 box
+
+struct Smem {
+  unsigned char xo[2 * BIG], xu[2 * BIG], s0[2 * BIG], ds[2 * BIG];  // [dO; dV], [U_hi; U_lo]; [v][dk] of both states
+  unsigned char q[2 * BOX], k[2 * BOX], zero[BOX], w[4 * BOX];       // w: W_hi, N_hi, W_lo, N_lo
+  float vec[2][DELTA_VEC];
+  float dots[2][128];
+  uint64_t xou_full, s0_full, ds_full, qk_full, tiles_free, qk_free, d3_done, w_ready, d4_done, acc_free;
+  uint32_t tmem;
+};
+enum { T_D1 = 0, T_D2 = 128, T_D3 = 256, T_D4 = 384 };
+
+// Byte offset of the 16-byte piece c of row r in a swizzled box.
+__device__ __forceinline__ uint32_t piece_at(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+// A [128 rows][K] K-major in boxes of `abox` bytes, B [128 rows][K] K-major / [K][128 columns] in boxes of `bbox`.
+template <int KS>
+__device__ __forceinline__ void mma_kk(uint32_t d, uint32_t a, uint32_t abox, uint32_t b, uint32_t bbox, bool more) {
+  constexpr uint32_t idesc = make_idesc(1, 1, false, false, 128, 128);
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    tc_mma_f16_ss(d, make_smem_desc_sw128(a + (s >> 2) * abox + (s & 3) * 32, 16, 1024), make_smem_desc_sw128(b + (s >> 2) * bbox + (s & 3) * 32, 16, 1024), idesc, more || s > 0);
+}
+template <int KS>
+__device__ __forceinline__ void mma_km(uint32_t d, uint32_t a, uint32_t abox, uint32_t b, uint32_t bbox, bool more) {
+  constexpr uint32_t idesc = make_idesc(1, 1, false, true, 128, 128);
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    tc_mma_f16_ss(d, make_smem_desc_sw128(a + (s >> 2) * abox + (s & 3) * 32, 16, 1024), make_smem_desc_sw128(b + s * 2048, bbox, 1024), idesc, more || s > 0);
+}
+// A^T with A [64 rows of K][64 columns] behind 64 columns of zeros.
+__device__ __forceinline__ void mma_tm(uint32_t d, uint32_t zero, uint32_t a, uint32_t b, uint32_t bbox) {
+  constexpr uint32_t idesc = make_idesc(1, 1, true, true, 128, 128);
+#pragma unroll
+  for (int s = 0; s < 4; ++s) tc_mma_f16_ss(d, make_smem_desc_sw128(zero + s * 2048, a - zero, 1024), make_smem_desc_sw128(b + s * 2048, bbox, 1024), idesc, 1u);
+}
+
+__device__ __forceinline__ void stsm(uint32_t addr, const uint4& r) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
+}
+__device__ __forceinline__ void stsm_t(uint32_t addr, const uint4& r) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+tc_dqk_kernel(const DeltaArgs a) {
+  extern __shared__ unsigned char raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(raw + (1024 - (smem_addr(raw) & 1023)) % 1024);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rep = a.Hv / a.Hk;
+  const long long items = a.NC * a.Hk;
+  if (threadIdx.x == 0) {
+    bar_init(&sm.xou_full, LOAD_WARPS);
+    bar_init(&sm.s0_full, LOAD_WARPS);
+    bar_init(&sm.ds_full, LOAD_WARPS);
+    bar_init(&sm.qk_full, LOAD_WARPS);
+    bar_init(&sm.tiles_free, 1);
+    bar_init(&sm.qk_free, 8);
+    bar_init(&sm.d3_done, 1);
+    bar_init(&sm.w_ready, 8);
+    bar_init(&sm.d4_done, 1);
+    bar_init(&sm.acc_free, 8);
+    fence_mbar_init();
+  }
+  for (int i = threadIdx.x; i < static_cast<int>(sizeof(sm.zero) / 16); i += THREADS) reinterpret_cast<uint4*>(sm.zero)[i] = make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
+  if (warp == 15) tmem_alloc(&sm.tmem, 512);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tm = sm.tmem;
+  // u counts the (chunk, value head) pairs of the block, i the (chunk, key head) pairs; every role goes the same way
+  int u = 0, i = 0;
+
+  if (warp < 8) {
+    const int quarter = warp & 3, half = warp >> 2, r = 32 * quarter + lane, tok = r & 63;
+    const bool key = r >= 64;
+    const uint32_t lanes = tm + (static_cast<uint32_t>(32 * quarter) << 16);
+    const uint32_t wt = smem_addr(sm.w);
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+      const long long c = item / a.Hk;
+      const int hk = static_cast<int>(item - c * a.Hk);
+      const Span sp = chunk_span(a, c);
+      if (sp.len == 0) continue;
+      float acc[64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+      for (int hr = 0; hr < rep; ++hr, ++u) {
+        const float* vec = sm.vec[u & 1];
+        // W_ij = qs_i rk_j D_ij (dO U^T)_ij for i >= j, N_ij = -rk_i rk_j D_ij (dV U^T)_ij for i > j
+        bar_wait(&sm.d3_done, u & 1, a.status);
+        tc_fence_after_sync();
+        const float gh = vec[V_GHI * 64 + tok], gl = vec[V_GLO * 64 + tok];
+        const float f = key ? -vec[V_RK * 64 + tok] : vec[V_QS * 64 + tok];
+        const int last = key ? tok - 1 : tok;  // the last column that counts
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          uint32_t hi[16], lo[16];
+          tmem_ld_32x32b_x16(lanes + T_D3 + 32 * half + 16 * b, hi);
+          tmem_ld_32x32b_x16(lanes + T_D3 + 64 + 32 * half + 16 * b, lo);
+          tmem_ld_wait();
+          uint32_t ph[8], pl[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int j0 = 32 * half + 16 * b + 2 * j;
+            const float2 ch = *reinterpret_cast<const float2*>(vec + V_GHI * 64 + j0), cl = *reinterpret_cast<const float2*>(vec + V_GLO * 64 + j0);
+            const float2 rk = *reinterpret_cast<const float2*>(vec + V_RK * 64 + j0);
+            const float w0 = j0 <= last ? f * rk.x * __expf((gh - ch.x) + (gl - cl.x)) * (__uint_as_float(hi[2 * j]) + __uint_as_float(lo[2 * j])) : 0.f;
+            const float w1 = j0 + 1 <= last ? f * rk.y * __expf((gh - ch.y) + (gl - cl.y)) * (__uint_as_float(hi[2 * j + 1]) + __uint_as_float(lo[2 * j + 1])) : 0.f;
+            split2(w0, w1, ph[j], pl[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t at = piece_at(r, 4 * half + 2 * b + j);
+            *reinterpret_cast<uint4*>(sm.w + at) = make_uint4(ph[4 * j], ph[4 * j + 1], ph[4 * j + 2], ph[4 * j + 3]);
+            *reinterpret_cast<uint4*>(sm.w + 2 * BOX + at) = make_uint4(pl[4 * j], pl[4 * j + 1], pl[4 * j + 2], pl[4 * j + 3]);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
+        bar_arrive(&sm.w_ready);
+        // the rows, scaled
+        const float f1 = key ? -vec[V_YK * 64 + tok] : vec[V_OQ * 64 + tok], f2 = vec[V_SU * 64 + tok];
+        bar_wait(&sm.d4_done, u & 1, a.status);
+        tc_fence_after_sync();
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t x[16], y[16];
+          tmem_ld_32x32b_x16(lanes + T_D1 + 64 * half + 16 * b, x);
+          tmem_ld_32x32b_x16(lanes + T_D4 + 64 * half + 16 * b, y);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[16 * b + j] += f1 * __uint_as_float(x[j]) + __uint_as_float(y[j]);
+          if (key) {  // a whole warp or none of it
+            tmem_ld_32x32b_x16(lanes + T_D2 + 64 * half + 16 * b, x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[16 * b + j] += f2 * __uint_as_float(x[j]);
+          }
+        }
+        tc_fence_before_sync();
+        if (hr + 1 < rep) bar_arrive(&sm.acc_free);
+      }
+      // The rows are r dq^ and r dk^ with r = 1 / norm, so that dq = r dq^ - q r^2 (q . r dq^), the same for k.
+      const unsigned char* tile = key ? sm.k : sm.q;
+      bar_wait(&sm.qk_full, i & 1, a.status);
+      uint4 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const uint4*>(tile + half * BOX + piece_at(tok, j));
+      float f = 0.f;
+      if (a.l2norm) {
+        float d = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d += acc[8 * j + 2 * e] * lo_half(w[e]) + acc[8 * j + 2 * e + 1] * hi_half(w[e]);
+        }
+        sm.dots[half][r] = d;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float norm = sm.vec[(u - 1) & 1][(key ? V_RK : V_RQ) * 64 + tok];
+        f = (sm.dots[0][r] + sm.dots[1][r]) * norm * norm;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      // now the next head's vec may replace this one's, and the next products these
+      bar_arrive(&sm.acc_free);
+      if (tok < sp.len) {
+        uint4* out = reinterpret_cast<uint4*>(static_cast<bf16*>(key ? a.dkey : a.dq) + ((sp.start + tok) * a.Hk + hk) * D + 64 * half);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = pack2(acc[8 * j + 2 * e] - f * lo_half(w[e]), acc[8 * j + 2 * e + 1] - f * hi_half(w[e]));
+          out[j] = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+      bar_arrive(&sm.qk_free);
+      ++i;
+    }
+  } else if (warp < 15) {
+    const int lw = warp - 8, tid = threadIdx.x - 256;
+    const int m = lane >> 3, l8 = lane & 7;
+    const uint32_t xu = smem_addr(sm.xu), s0 = smem_addr(sm.s0), ds = smem_addr(sm.ds);
+    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+      const long long c = item / a.Hk;
+      const int hk = static_cast<int>(item - c * a.Hk);
+      const Span sp = chunk_span(a, c);
+      if (sp.len == 0) continue;
+      for (int hr = 0; hr < rep; ++hr, ++u) {
+        const int h = hk * rep + hr;
+        const long long rec = c * a.Hv + h;
+        // U: 8 tiles of columns x 4 of tokens x 2 parts; the states: 8 tiles of columns x 8 of dk, high part
+        uint4 fu[MINE], fs[MINE];
+        const uint4* us = reinterpret_cast<const uint4*>(a.u) + rec * 8 * 256 + lane;
+        const uint4* ss = reinterpret_cast<const uint4*>(a.states) + rec * 8 * 512 + lane;
+        const uint4* dd = reinterpret_cast<const uint4*>(a.dstates) + rec * 8 * 256 + lane;
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+          const int f = lw + LOAD_WARPS * j;
+          if (f < TILES) {
+            fu[j] = us[32 * f];
+            fs[j] = ss[(f >> 3) * 512 + (f & 7) * 32];
+          }
+        }
+        // the last head's products have read the tiles; D1 of it waited until the vec of two heads ago was read
+        if (u > 0) bar_wait(&sm.tiles_free, (u - 1) & 1, a.status);
+        const long long row = (sp.start * a.Hv + h) * D, stride = static_cast<long long>(a.Hv) * D;
+        for (int idx = tid; idx < 128 * 16; idx += LOADERS) {  // [dO; dV]: 128 rows x 16 pieces
+          const int r = idx >> 4, p = idx & 15, t = r & 63;
+          const bool ok = t < sp.len;
+          cp16(sm.xo + (p >> 3) * BIG + piece_at(r, p & 7), static_cast<const bf16*>(r < 64 ? a.dout : a.dv_) + row + (ok ? t * stride : 0) + p * 8, ok);
+        }
+        if (tid < DELTA_VEC / 4) cp16(&sm.vec[u & 1][tid * 4], a.vec + rec * DELTA_VEC + tid * 4, true);
+        cp_commit();
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+          const int f = lw + LOAD_WARPS * j;
+          const int t = 64 * (f & 1) + 16 * ((f >> 1) & 3) + (m >> 1) * 8 + l8, v = 16 * (f >> 3) + (m & 1) * 8;
+          if (f < TILES) {
+            stsm_t(xu + (v >> 6) * BIG + piece_at(t, (v >> 3) & 7), fu[j]);
+            fu[j] = dd[32 * f];
+          }
+        }
+        cp_wait<0>();
+        fence_proxy_async_smem();
+        bar_arrive(&sm.xou_full);
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+          const int f = lw + LOAD_WARPS * j, v = 16 * (f >> 3) + (m & 1) * 8 + l8, k = 16 * (f & 7) + (m >> 1) * 8;
+          if (f < TILES) stsm(s0 + (k >> 6) * BIG + piece_at(v, (k >> 3) & 7), fs[j]);
+        }
+        fence_proxy_async_smem();
+        bar_arrive(&sm.s0_full);
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+          const int f = lw + LOAD_WARPS * j, v = 16 * (f >> 3) + (m & 1) * 8 + l8, k = 16 * (f & 7) + (m >> 1) * 8;
+          if (f < TILES) stsm(ds + (k >> 6) * BIG + piece_at(v, (k >> 3) & 7), fu[j]);
+        }
+        fence_proxy_async_smem();
+        bar_arrive(&sm.ds_full);
+        if (hr == 0) {
+          if (i > 0) bar_wait(&sm.qk_free, (i - 1) & 1, a.status);
+          const bf16* qp = static_cast<const bf16*>(a.q) + sp.start * a.q_ts + hk * a.q_hs;
+          const bf16* kp = static_cast<const bf16*>(a.k) + sp.start * a.k_ts + hk * a.k_hs;
+          for (int idx = tid; idx < 64 * 16; idx += LOADERS) {
+            const int r = idx >> 4, p = idx & 15;
+            const bool ok = r < sp.len;
+            const uint32_t at = (p >> 3) * BOX + piece_at(r, p & 7);
+            cp16(sm.q + at, qp + (ok ? r * a.q_ts : 0) + p * 8, ok);
+            cp16(sm.k + at, kp + (ok ? r * a.k_ts : 0) + p * 8, ok);
+          }
+          cp_commit();
+          cp_wait<0>();
+          fence_proxy_async_smem();
+          bar_arrive(&sm.qk_full);
+        }
+      }
+      ++i;
+    }
+  } else {
+    if (lane == 0) {
+      const uint32_t xo = smem_addr(sm.xo), xu = smem_addr(sm.xu), s0 = smem_addr(sm.s0), ds = smem_addr(sm.ds);
+      const uint32_t q = smem_addr(sm.q), k = smem_addr(sm.k), zero = smem_addr(sm.zero), w = smem_addr(sm.w);
+      for (long long item = blockIdx.x; item < items; item += gridDim.x) {
+        if (chunk_span(a, item / a.Hk).len == 0) continue;
+        for (int hr = 0; hr < rep; ++hr, ++u) {
+          const uint32_t parity = u & 1;
+          bar_wait(&sm.xou_full, parity, a.status);
+          tc_fence_after_sync();
+          mma_kk<8>(tm + T_D3, xo, BIG, xu, BIG, false);  // W of the last head was made before its D4 was issued
+          tc_commit(&sm.d3_done);
+          if (u > 0) bar_wait(&sm.acc_free, (u - 1) & 1, a.status);
+          bar_wait(&sm.s0_full, parity, a.status);
+          tc_fence_after_sync();
+          mma_km<8>(tm + T_D1, xo, BIG, s0, BIG, false);
+          bar_wait(&sm.ds_full, parity, a.status);
+          tc_fence_after_sync();
+          mma_km<8>(tm + T_D2, xu - BOX, BIG, ds, BIG, false);
+          mma_km<8>(tm + T_D2, xu, BIG, ds, BIG, true);
+          tc_commit(&sm.tiles_free);
+          if (hr == 0) bar_wait(&sm.qk_full, i & 1, a.status);
+          bar_wait(&sm.w_ready, parity, a.status);
+          tc_fence_after_sync();
+          mma_km<4>(tm + T_D4, w, 0, k, BOX, false);
+          mma_km<4>(tm + T_D4, w + 2 * BOX, 0, k, BOX, true);
+          mma_tm(tm + T_D4, zero, w, q, BOX);
+          mma_tm(tm + T_D4, zero, w + 2 * BOX, q, BOX);
+          mma_tm(tm + T_D4, zero, w + BOX, k, BOX);
+          mma_tm(tm + T_D4, zero, w + 3 * BOX, k, BOX);
+          tc_commit(&sm.d4_done);
+        }
+        ++i;
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 15) {
+    tc_fence_after_sync();
+    tmem_dealloc(tm, 512);
+  }
+}
+
+}  // namespace
+
+int delta_tc_dqk(const DeltaArgs& a, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed{0};
+  const size_t bytes = sizeof(Smem) + 1024;
+  if (!allow_smem(tc_dqk_kernel, bytes, allowed)) return -3;
+  const long long items = a.NC * a.Hk;
+  tc_dqk_kernel<<<static_cast<unsigned>(items < 148 ? items : 148), THREADS, bytes, s>>>(a);
+  return 0;
+}
+
+}  // namespace lf

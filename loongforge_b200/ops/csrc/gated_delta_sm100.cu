@@ -43,22 +43,15 @@
 // The chain is bound by latency: three dependent products of at most 64 x 128 x 16 per chunk, with a hand-over between
 // them. mma.sync runs at a quarter of tcgen05's rate, but operands and results stay in registers, and 32 heads make 1024
 // warps of such work.
-#include <cuda_bf16.h>
-#include <cuda_runtime.h>
-#include <stdint.h>
-#include <atomic>
-#include "linear_attn.h"
+#include "gated_delta.cuh"
 
 namespace lf {
 namespace {
 
-using bf16 = __nv_bfloat16;
-constexpr int C = DELTA_CHUNK;
+using namespace delta;
 constexpr int APITCH = 72;  // bf16 per row of a 64-wide tile: odd multiple of 16 bytes, no bank conflicts in ldmatrix
 
 // ------------------------------------------------------------------------------------------------------- primitives
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -78,13 +71,6 @@ __device__ __forceinline__ void stsm_t(bf16* p, const uint32_t (&r)[4]) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(smem_addr(p)), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
-__device__ __forceinline__ void cp16(void* dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // Addresses of the lane for the four 8x8 tiles of one x4 load, p = row-major base, `ld` its pitch. With m = lane / 8:
 // tile m covers rows r0 + 8 * (m & 1), columns c0 + 8 * (m >> 1)
 __device__ __forceinline__ const bf16* at_rc(const bf16* p, int ld, int r0, int c0) {
@@ -103,18 +89,6 @@ __device__ __forceinline__ void b_from_kn(uint32_t (&r)[4], const bf16* p, int l
 __device__ __forceinline__ void a_from_mk(uint32_t (&r)[4], const bf16* p, int ld, int m0, int k0) { ldsm(r, at_rc(p, ld, m0, k0)); }
 __device__ __forceinline__ void a_from_km(uint32_t (&r)[4], const bf16* p, int ld, int k0, int m0) { ldsm_t(r, at_cr(p, ld, k0, m0)); }
 
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float lo_half(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float hi_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-// x, y -> bf16 pair and the bf16 pair of what the rounding left. Volatile, so that the parts of a whole state are made
-// again where they are used again instead of being held in registers in between.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
-  lo = pack2(x - lo_half(hi), y - hi_half(hi));
-}
 // Two accumulator tiles (columns 16 kk .. 16 kk + 15) as the high and low A operand of k step kk.
 __device__ __forceinline__ void split_a(const float (&c0)[4], const float (&c1)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
   split2(c0[0], c0[1], hi[0], lo[0]);
@@ -140,39 +114,6 @@ __device__ __forceinline__ void mma2(float (*acc)[4], const uint32_t (&hi)[4], c
 }
 
 // ---------------------------------------------------------------------------------------------------- sequence plan
-
-struct Span {
-  int n;            // sequence
-  long long start;  // first token of the chunk
-  int len;          // its tokens, 1 .. 64; 0 = no such chunk
-};
-
-__device__ __forceinline__ Span chunk_span(const DeltaArgs& a, long long c) {
-  Span s;
-  if (a.cu == nullptr) {
-    s.n = 0;
-    s.start = c * C;
-    const long long left = a.T - s.start;
-    s.len = left <= 0 ? 0 : (left < C ? static_cast<int>(left) : C);
-    return s;
-  }
-  if (c >= a.cbase[a.N]) {
-    s.n = 0;
-    s.start = 0;
-    s.len = 0;
-    return s;
-  }
-  int lo = 0, hi = a.N;  // last n with cbase[n] <= c; sequences without tokens have no chunk and are passed over
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cbase[mid] <= c) lo = mid; else hi = mid;
-  }
-  s.n = lo;
-  s.start = a.cu[lo] + (c - a.cbase[lo]) * C;
-  const long long left = a.cu[lo + 1] - s.start;
-  s.len = left < C ? static_cast<int>(left) : C;
-  return s;
-}
 
 // cu <- running maximum of the given boundaries clamped to [0, T] (the boundaries themselves when they are valid, else
 // the status word is set), cbase <- first chunk of every sequence. One block.
@@ -252,10 +193,6 @@ __device__ __forceinline__ void load_rows(bf16* dst, int pitch, const bf16* src,
 }
 
 // ---------------------------------------------------------------------------------------------------------- prepare
-
-// Rows of a chunk's factor block, 64 floats each.
-enum { V_YK = 0, V_BETA, V_OQ, V_SU, V_GHI, V_GLO, V_QS, V_RK, V_END, V_PD, V_RQ };  // V_PD: diagonal of P
-constexpr int SEQ_ROWS = V_PD + 1;  // rows that the kernels along the sequence read
 
 constexpr int PREP_THREADS = 128;
 constexpr int MP = 68;  // fp32 pitch of the 64 x 64 matrices: rows 16-byte aligned, neighbours four banks apart
@@ -494,25 +431,6 @@ __device__ __forceinline__ void get(const Operands& x, uint32_t (&hi)[4], uint32
   lo[0] = l.x; lo[1] = l.y; lo[2] = l.z; lo[3] = l.w;
 }
 
-// Barriers of the four warps of a unit (a warp arrives once) and of a buffer's copies. They complete in every chunk, so a
-// wait ends unless the kernel is wrong; after a limit far above any chunk's time it reports and goes on.
-__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint64_t* b) {  // whole warp; what its lanes wrote is seen behind the wait
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
-}
-__device__ __forceinline__ void bar_wait(uint64_t* b, uint32_t parity, int* status) {
-  uint32_t done = 0;
-  for (int i = 0; i < (1 << 22); ++i) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done) : "r"(smem_addr(b)), "r"(parity) : "memory");
-    if (done) return;
-  }
-  *status = 1;
-}
 // The calling thread's cp.async copies so far arrive on the barrier when they have landed.
 __device__ __forceinline__ void bar_arrive_copies(uint64_t* b) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
@@ -1501,18 +1419,6 @@ gates_kernel(const DeltaArgs a) {
 
 // --------------------------------------------------------------------------------------------------------- launches
 
-// Once per kernel and device: the call costs as much as a launch.
-template <typename K>
-bool allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return true;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess) return false;
-  done.fetch_or(bit, std::memory_order_relaxed);
-  return true;
-}
-
 template <int DK, int NU, bool KEEP>
 int launch_forward(const DeltaArgs& a, cudaStream_t s) {
   const long long grid = static_cast<long long>(a.N) * a.Hv * (a.dv / (NU * 16));
@@ -1562,7 +1468,8 @@ int backward_dk(const DeltaArgs& a, cudaStream_t s) {
   int rc = launch_backward<DK, 2>(a, s);
   if (rc) return rc;
   if (a.NC > 0) {
-    rc = a.dv == 64 ? launch_dqk<DK, 64>(a, s) : launch_dqk<DK, 128>(a, s);
+    if (a.dk == 128 && a.dv == 128) rc = delta_tc_dqk(a, s);
+    else rc = a.dv == 64 ? launch_dqk<DK, 64>(a, s) : launch_dqk<DK, 128>(a, s);
     if (rc) return rc;
     gates_kernel<<<static_cast<unsigned>((a.NC * a.Hv + GATE_WARPS - 1) / GATE_WARPS), GATE_WARPS * 32, 0, s>>>(a);
   }

@@ -46,6 +46,7 @@ struct DeltaArgs {
 int delta_plan(const int* cu_in, int N, long long T, int* cu, int* cbase, int* status, cudaStream_t s);
 int delta_forward(const DeltaArgs& a, cudaStream_t s);
 int delta_backward(const DeltaArgs& a, cudaStream_t s);
+int delta_tc_dqk(const DeltaArgs& a, cudaStream_t s);  // its dq / dk for dk = dv = 128 (gated_delta_dqk_sm100.cu)
 // Zeroes the rows [0, cu[0]) and [cu[N], T) of up to six row-major buffers.
 struct ZeroRows {
   void* p[6] = {};

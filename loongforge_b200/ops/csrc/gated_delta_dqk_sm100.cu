@@ -34,7 +34,7 @@ struct Smem {
   unsigned char q[2 * BOX], k[2 * BOX], zero[BOX], w[4 * BOX];       // w: W_hi, N_hi, W_lo, N_lo
   float vec[2][DELTA_VEC];
   float dots[2][128];
-  uint64_t xou_full, s0_full, ds_full, qk_full, tiles_free, qk_free, d3_done, w_ready, d4_done, acc_free;
+  uint64_t xos_full, ds_full, qk_full, tiles_free, qk_free, d3_done, w_ready, d4_done, acc_free;
   uint32_t tmem;
 };
 enum { T_D1 = 0, T_D2 = 128, T_D3 = 256, T_D4 = 384 };
@@ -71,15 +71,41 @@ __device__ __forceinline__ void stsm_t(uint32_t addr, const uint4& r) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
 }
 
+// The block's (chunk, key head) pairs, every gridDim.x-th, without a division each.
+struct Item {
+  int c, hk, dc, dh;
+  __device__ __forceinline__ explicit Item(const DeltaArgs& a) {
+    c = static_cast<int>(blockIdx.x) / a.Hk;
+    hk = static_cast<int>(blockIdx.x) - c * a.Hk;
+    dc = static_cast<int>(gridDim.x) / a.Hk;
+    dh = static_cast<int>(gridDim.x) - dc * a.Hk;
+  }
+  __device__ __forceinline__ void next(const DeltaArgs& a) {
+    c += dc;
+    hk += dh;
+    if (hk >= a.Hk) {
+      hk -= a.Hk;
+      ++c;
+    }
+  }
+};
+
+// Sixteen neighbouring values of a factor row.
+__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 f = reinterpret_cast<const float4*>(p)[i];
+    x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
+  }
+}
+
 __global__ void __launch_bounds__(THREADS, 1)
 tc_dqk_kernel(const DeltaArgs a) {
   extern __shared__ unsigned char raw[];
   Smem& sm = *reinterpret_cast<Smem*>(raw + (1024 - (smem_addr(raw) & 1023)) % 1024);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rep = a.Hv / a.Hk;
-  const long long items = a.NC * a.Hk;
   if (threadIdx.x == 0) {
-    bar_init(&sm.xou_full, LOAD_WARPS);
-    bar_init(&sm.s0_full, LOAD_WARPS);
+    bar_init(&sm.xos_full, LOAD_WARPS);
     bar_init(&sm.ds_full, LOAD_WARPS);
     bar_init(&sm.qk_full, LOAD_WARPS);
     bar_init(&sm.tiles_free, 1);
@@ -105,9 +131,8 @@ tc_dqk_kernel(const DeltaArgs a) {
     const bool key = r >= 64;
     const uint32_t lanes = tm + (static_cast<uint32_t>(32 * quarter) << 16);
     const uint32_t wt = smem_addr(sm.w);
-    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-      const long long c = item / a.Hk;
-      const int hk = static_cast<int>(item - c * a.Hk);
+    for (Item it(a); it.c < a.NC; it.next(a)) {
+      const int c = it.c, hk = it.hk;
       const Span sp = chunk_span(a, c);
       if (sp.len == 0) continue;
       float acc[64];
@@ -123,20 +148,30 @@ tc_dqk_kernel(const DeltaArgs a) {
         const int last = key ? tok - 1 : tok;  // the last column that counts
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          uint32_t hi[16], lo[16];
-          tmem_ld_32x32b_x16(lanes + T_D3 + 32 * half + 16 * b, hi);
-          tmem_ld_32x32b_x16(lanes + T_D3 + 64 + 32 * half + 16 * b, lo);
-          tmem_ld_wait();
-          uint32_t ph[8], pl[8];
+          // element by element the chain of latencies is long: sixteen at a time, made everywhere and selected at the end
+          const int j0 = 32 * half + 16 * b;
+          float e[16], x[16];
+          load16(vec + V_GHI * 64 + j0, e);
+          load16(vec + V_GLO * 64 + j0, x);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int j0 = 32 * half + 16 * b + 2 * j;
-            const float2 ch = *reinterpret_cast<const float2*>(vec + V_GHI * 64 + j0), cl = *reinterpret_cast<const float2*>(vec + V_GLO * 64 + j0);
-            const float2 rk = *reinterpret_cast<const float2*>(vec + V_RK * 64 + j0);
-            const float w0 = j0 <= last ? f * rk.x * __expf((gh - ch.x) + (gl - cl.x)) * (__uint_as_float(hi[2 * j]) + __uint_as_float(lo[2 * j])) : 0.f;
-            const float w1 = j0 + 1 <= last ? f * rk.y * __expf((gh - ch.y) + (gl - cl.y)) * (__uint_as_float(hi[2 * j + 1]) + __uint_as_float(lo[2 * j + 1])) : 0.f;
-            split2(w0, w1, ph[j], pl[j]);
+          for (int j = 0; j < 16; ++j) e[j] = __expf((gh - e[j]) + (gl - x[j]));
+          load16(vec + V_RK * 64 + j0, x);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) e[j] *= f * x[j];
+          uint32_t y[16], ph[8], pl[8];
+          tmem_ld_32x32b_x16(lanes + T_D3 + j0, y);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] = __uint_as_float(y[j]);
+          tmem_ld_32x32b_x16(lanes + T_D3 + 64 + j0, y);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            e[j] *= x[j] + __uint_as_float(y[j]);
+            e[j] = j0 + j <= last ? e[j] : 0.f;
           }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) split2(e[2 * j], e[2 * j + 1], ph[j], pl[j]);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const uint32_t at = piece_at(r, 4 * half + 2 * b + j);
@@ -192,32 +227,38 @@ tc_dqk_kernel(const DeltaArgs a) {
       }
       // now the next head's vec may replace this one's, and the next products these
       bar_arrive(&sm.acc_free);
-      if (tok < sp.len) {
-        uint4* out = reinterpret_cast<uint4*>(static_cast<bf16*>(key ? a.dkey : a.dq) + ((sp.start + tok) * a.Hk + hk) * D + 64 * half);
+      // through w's place, which only these warps write, to whole rows
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-          uint32_t o[4];
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+        uint32_t o[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = pack2(acc[8 * j + 2 * e] - f * lo_half(w[e]), acc[8 * j + 2 * e + 1] - f * hi_half(w[e]));
-          out[j] = make_uint4(o[0], o[1], o[2], o[3]);
-        }
+        for (int e = 0; e < 4; ++e) o[e] = pack2(acc[8 * j + 2 * e] - f * lo_half(w[e]), acc[8 * j + 2 * e + 1] - f * hi_half(w[e]));
+        *reinterpret_cast<uint4*>(sm.w + half * BIG + piece_at(r, j)) = make_uint4(o[0], o[1], o[2], o[3]);
       }
       bar_arrive(&sm.qk_free);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = 16 * warp + 2 * j + (lane >> 4), p = lane & 15, t = row & 63;
+        if (t < sp.len)
+          *reinterpret_cast<uint4*>(static_cast<bf16*>(row < 64 ? a.dq : a.dkey) + ((sp.start + t) * a.Hk + hk) * D + p * 8) =
+              *reinterpret_cast<const uint4*>(sm.w + (p >> 3) * BIG + piece_at(row, p & 7));
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       ++i;
     }
   } else if (warp < 15) {
     const int lw = warp - 8, tid = threadIdx.x - 256;
     const int m = lane >> 3, l8 = lane & 7;
     const uint32_t xu = smem_addr(sm.xu), s0 = smem_addr(sm.s0), ds = smem_addr(sm.ds);
-    for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-      const long long c = item / a.Hk;
-      const int hk = static_cast<int>(item - c * a.Hk);
+    for (Item it(a); it.c < a.NC; it.next(a)) {
+      const int c = it.c, hk = it.hk;
       const Span sp = chunk_span(a, c);
       if (sp.len == 0) continue;
       for (int hr = 0; hr < rep; ++hr, ++u) {
         const int h = hk * rep + hr;
-        const long long rec = c * a.Hv + h;
+        const long long rec = static_cast<long long>(c) * a.Hv + h;
         // U: 8 tiles of columns x 4 of tokens x 2 parts; the states: 8 tiles of columns x 8 of dk, high part
         uint4 fu[MINE], fs[MINE];
         const uint4* us = reinterpret_cast<const uint4*>(a.u) + rec * 8 * 256 + lane;
@@ -234,10 +275,15 @@ tc_dqk_kernel(const DeltaArgs a) {
         // the last head's products have read the tiles; D1 of it waited until the vec of two heads ago was read
         if (u > 0) bar_wait(&sm.tiles_free, (u - 1) & 1, a.status);
         const long long row = (sp.start * a.Hv + h) * D, stride = static_cast<long long>(a.Hv) * D;
-        for (int idx = tid; idx < 128 * 16; idx += LOADERS) {  // [dO; dV]: 128 rows x 16 pieces
-          const int r = idx >> 4, p = idx & 15, t = r & 63;
-          const bool ok = t < sp.len;
-          cp16(sm.xo + (p >> 3) * BIG + piece_at(r, p & 7), static_cast<const bf16*>(r < 64 ? a.dout : a.dv_) + row + (ok ? t * stride : 0) + p * 8, ok);
+        {  // [dO; dV]: a thread takes one 16-byte column of every 14th row
+          const int p = tid & 15;
+          unsigned char* dst = sm.xo + (p >> 3) * BIG;
+#pragma unroll 1
+          for (int part = 0; part < 2; ++part) {
+            const bf16* src = static_cast<const bf16*>(part ? a.dv_ : a.dout) + row + p * 8;
+#pragma unroll 1
+            for (int t = tid >> 4; t < 64; t += LOADERS / 16) cp16(dst + piece_at(64 * part + t, p & 7), src + (t < sp.len ? t * stride : 0), t < sp.len);
+          }
         }
         if (tid < DELTA_VEC / 4) cp16(&sm.vec[u & 1][tid * 4], a.vec + rec * DELTA_VEC + tid * 4, true);
         cp_commit();
@@ -245,21 +291,21 @@ tc_dqk_kernel(const DeltaArgs a) {
         for (int j = 0; j < MINE; ++j) {
           const int f = lw + LOAD_WARPS * j;
           const int t = 64 * (f & 1) + 16 * ((f >> 1) & 3) + (m >> 1) * 8 + l8, v = 16 * (f >> 3) + (m & 1) * 8;
-          if (f < TILES) {
-            stsm_t(xu + (v >> 6) * BIG + piece_at(t, (v >> 3) & 7), fu[j]);
-            fu[j] = dd[32 * f];
-          }
+          if (f < TILES) stsm_t(xu + (v >> 6) * BIG + piece_at(t, (v >> 3) & 7), fu[j]);
         }
-        cp_wait<0>();
-        fence_proxy_async_smem();
-        bar_arrive(&sm.xou_full);
 #pragma unroll
         for (int j = 0; j < MINE; ++j) {
           const int f = lw + LOAD_WARPS * j, v = 16 * (f >> 3) + (m & 1) * 8 + l8, k = 16 * (f & 7) + (m >> 1) * 8;
           if (f < TILES) stsm(s0 + (k >> 6) * BIG + piece_at(v, (k >> 3) & 7), fs[j]);
         }
-        fence_proxy_async_smem();
-        bar_arrive(&sm.s0_full);
+        cp_wait<0>();
+        fence_proxy_async_smem();  // before the loads below: it waits for loads in flight too
+        bar_arrive(&sm.xos_full);
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+          const int f = lw + LOAD_WARPS * j;
+          if (f < TILES) fu[j] = dd[32 * f];
+        }
 #pragma unroll
         for (int j = 0; j < MINE; ++j) {
           const int f = lw + LOAD_WARPS * j, v = 16 * (f >> 3) + (m & 1) * 8 + l8, k = 16 * (f & 7) + (m >> 1) * 8;
@@ -271,8 +317,9 @@ tc_dqk_kernel(const DeltaArgs a) {
           if (i > 0) bar_wait(&sm.qk_free, (i - 1) & 1, a.status);
           const bf16* qp = static_cast<const bf16*>(a.q) + sp.start * a.q_ts + hk * a.q_hs;
           const bf16* kp = static_cast<const bf16*>(a.k) + sp.start * a.k_ts + hk * a.k_hs;
-          for (int idx = tid; idx < 64 * 16; idx += LOADERS) {
-            const int r = idx >> 4, p = idx & 15;
+          const int p = tid & 15;
+#pragma unroll 1
+          for (int r = tid >> 4; r < 64; r += LOADERS / 16) {
             const bool ok = r < sp.len;
             const uint32_t at = (p >> 3) * BOX + piece_at(r, p & 7);
             cp16(sm.q + at, qp + (ok ? r * a.q_ts : 0) + p * 8, ok);
@@ -290,16 +337,15 @@ tc_dqk_kernel(const DeltaArgs a) {
     if (lane == 0) {
       const uint32_t xo = smem_addr(sm.xo), xu = smem_addr(sm.xu), s0 = smem_addr(sm.s0), ds = smem_addr(sm.ds);
       const uint32_t q = smem_addr(sm.q), k = smem_addr(sm.k), zero = smem_addr(sm.zero), w = smem_addr(sm.w);
-      for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-        if (chunk_span(a, item / a.Hk).len == 0) continue;
+      for (Item it(a); it.c < a.NC; it.next(a)) {
+        if (chunk_span(a, it.c).len == 0) continue;
         for (int hr = 0; hr < rep; ++hr, ++u) {
           const uint32_t parity = u & 1;
-          bar_wait(&sm.xou_full, parity, a.status);
+          bar_wait(&sm.xos_full, parity, a.status);
           tc_fence_after_sync();
           mma_kk<8>(tm + T_D3, xo, BIG, xu, BIG, false);  // W of the last head was made before its D4 was issued
           tc_commit(&sm.d3_done);
           if (u > 0) bar_wait(&sm.acc_free, (u - 1) & 1, a.status);
-          bar_wait(&sm.s0_full, parity, a.status);
           tc_fence_after_sync();
           mma_km<8>(tm + T_D1, xo, BIG, s0, BIG, false);
           bar_wait(&sm.ds_full, parity, a.status);

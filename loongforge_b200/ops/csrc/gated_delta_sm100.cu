@@ -312,20 +312,18 @@ prepare_kernel(const DeltaArgs a) {
       for (int e = 0; e < 2; ++e) {
         const int i = warp * 16 + g + 8 * e, j0 = 8 * j + t2;
         float m[2], p[2];
+        const float2 gh = *reinterpret_cast<const float2*>(ghi + j0), gl = *reinterpret_cast<const float2*>(glo + j0);
+        const float2 rkj = *reinterpret_cast<const float2*>(rk + j0);
+        const float gih = ghi[i], gil = glo[i], fq = a.scale * rq[i], fk = bt[i] * rk[i];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
+          // made everywhere and then selected: a branch per element costs its latency each time
           const int jj = j0 + f;
-          m[f] = p[f] = 0.f;
-          if (i >= jj) {
-            const float d = rk[jj] * __expf((ghi[i] - ghi[jj]) + (glo[i] - glo[jj]));
-            p[f] = a.scale * rq[i] * d * qk[j][2 * e + f];
-            if (i > jj) {
-              m[f] = bt[i] * rk[i] * d * kk[j][2 * e + f];
-            } else {
-              vec[V_PD * 64 + i] = p[f];
-              p[f] = 0.f;
-            }
-          }
+          const float d = (f ? rkj.y : rkj.x) * __expf((gih - (f ? gh.y : gh.x)) + (gil - (f ? gl.y : gl.x)));
+          const float pv = fq * d * qk[j][2 * e + f], mv = fk * d * kk[j][2 * e + f];
+          m[f] = i > jj ? mv : 0.f;
+          p[f] = i > jj ? pv : 0.f;
+          if (i == jj) vec[V_PD * 64 + i] = pv;
         }
         *reinterpret_cast<float2*>(M + i * MP + j0) = make_float2(m[0], m[1]);
         uint32_t hi, lo;
@@ -1383,9 +1381,9 @@ dqk_kernel(const DeltaArgs a) {
 constexpr int GATE_WARPS = 4;
 __global__ void __launch_bounds__(GATE_WARPS * 32)
 gates_kernel(const DeltaArgs a) {
-  const long long rec = static_cast<long long>(blockIdx.x) * GATE_WARPS + (threadIdx.x >> 5);
-  const long long c = rec / a.Hv;
-  const int h = static_cast<int>(rec - c * a.Hv);
+  const unsigned pair = blockIdx.x * GATE_WARPS + (threadIdx.x >> 5);  // at most 2^31 of them
+  const int c = static_cast<int>(pair / static_cast<unsigned>(a.Hv)), h = static_cast<int>(pair - c * static_cast<unsigned>(a.Hv));
+  const long long rec = pair;
   if (c >= a.NC) return;
   const Span sp = chunk_span(a, c);
   if (sp.len == 0) return;

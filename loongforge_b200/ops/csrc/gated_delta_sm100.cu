@@ -197,16 +197,47 @@ __device__ __forceinline__ void load_rows(bf16* dst, int pitch, const bf16* src,
 constexpr int PREP_THREADS = 128;
 constexpr int MP = 68;  // fp32 pitch of the 64 x 64 matrices: rows 16-byte aligned, neighbours four banks apart
 
+// s += row [K] times K rows of four neighbouring columns.
+template <int K>
+__device__ __forceinline__ void mul4(float4& s, const float* row, const float* cols) {
+#pragma unroll 4
+  for (int k = 0; k < K; k += 4) {
+    const float4 m = *reinterpret_cast<const float4*>(row + k);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float mv = x == 0 ? m.x : x == 1 ? m.y : x == 2 ? m.z : m.w;
+      const float4 v = *reinterpret_cast<const float4*>(cols + (k + x) * MP);
+      s.x += mv * v.x; s.y += mv * v.y; s.z += mv * v.z; s.w += mv * v.w;
+    }
+  }
+}
+
+constexpr size_t PREP_PART = 2 * C * APITCH * sizeof(bf16);  // high and low of A, or of P, as they lie in the record
+constexpr size_t PREP_TILES = 2 * PREP_PART + C * MP * sizeof(float);
+
+// A contiguous piece of shared memory to device memory, behind a fence and a barrier of those who wrote it.
+__device__ __forceinline__ void bulk_out(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_addr(src)), "r"(bytes)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// What this thread wrote to shared memory is seen by bulk copies that begin behind the next barrier.
+__device__ __forceinline__ void fence_bulk() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bulk_out_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
 template <int DK>
-__global__ void __launch_bounds__(PREP_THREADS)
+__global__ void __launch_bounds__(PREP_THREADS, 4)
 prepare_kernel(const DeltaArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   constexpr int P = DK + 8;
   bf16* qs = reinterpret_cast<bf16*>(smem);
   bf16* ks = qs + C * P;
-  float* M = reinterpret_cast<float*>(ks + C * P);
-  float* A = M + C * MP;
-  float* rq = A + C * MP;
+  // q and k are in registers when these are written; M is done with when A is split into its place
+  float* M = reinterpret_cast<float*>(smem);
+  bf16* As = reinterpret_cast<bf16*>(smem);
+  bf16* Ps = As + 2 * C * APITCH;
+  float* A = reinterpret_cast<float*>(Ps + 2 * C * APITCH);
+  float* rq = reinterpret_cast<float*>(smem + PREP_TILES);
   float* rk = rq + C;
   float* ghi = rk + C;
   float* glo = ghi + C;
@@ -218,23 +249,24 @@ prepare_kernel(const DeltaArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t2 = (lane & 3) * 2;
   load_rows<DK, PREP_THREADS>(qs, P, static_cast<const bf16*>(a.q) + sp.start * a.q_ts + hk * a.q_hs, a.q_ts, sp.len);
   load_rows<DK, PREP_THREADS>(ks, P, static_cast<const bf16*>(a.k) + sp.start * a.k_ts + hk * a.k_hs, a.k_ts, sp.len);
+  // the padding travels too, as zeros
+  *reinterpret_cast<uint4*>(qs + tid * P + DK) = make_uint4(0, 0, 0, 0);
   cp_commit();
   cp_wait<0>();
+  fence_bulk();
   __syncthreads();
-  // the padded tiles as they are, for the kernels along the sequence: one bulk copy each there
-  {
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<bf16*>(a.qk) + (c * a.Hk + hk) * 2 * C * P);
-    const uint4* src = reinterpret_cast<const uint4*>(qs);  // k lies behind q
-    for (int i = tid; i < 2 * C * P / 8; i += PREP_THREADS)
-      if (i % (P / 8) < DK / 8) dst[i] = src[i];
-  }
+  // the padded tiles as they are, for the kernels along the sequence: one bulk copy each there. k lies behind q.
+  if (tid == 0) bulk_out(static_cast<bf16*>(a.qk) + (c * a.Hk + hk) * 2 * C * P, qs, 2 * C * P * sizeof(bf16));
   {
     const bf16* row = (tid < C ? qs : ks) + (tid & 63) * P;
     float ss = 0.f;
 #pragma unroll 4
-    for (int i = 0; i < DK / 2; ++i) {
-      const uint32_t w = reinterpret_cast<const uint32_t*>(row)[i];
-      ss += lo_half(w) * lo_half(w) + hi_half(w) * hi_half(w);
+    for (int i = 0; i < DK / 8; ++i) {
+      const uint4 w = reinterpret_cast<const uint4*>(row)[i];
+      ss += lo_half(w.x) * lo_half(w.x) + hi_half(w.x) * hi_half(w.x);
+      ss += lo_half(w.y) * lo_half(w.y) + hi_half(w.y) * hi_half(w.y);
+      ss += lo_half(w.z) * lo_half(w.z) + hi_half(w.z) * hi_half(w.z);
+      ss += lo_half(w.w) * lo_half(w.w) + hi_half(w.w) * hi_half(w.w);
     }
     (tid < C ? rq : rk)[tid & 63] = a.l2norm ? rsqrtf(ss + 1e-6f) : 1.f;
   }
@@ -264,6 +296,7 @@ prepare_kernel(const DeltaArgs a) {
     const long long rec = c * a.Hv + h;
     float* vec = a.vec + rec * DELTA_VEC;
     bf16* ap = static_cast<bf16*>(a.ap) + rec * DELTA_AP;
+    if (tid == 0) bulk_out_read();  // what left from here is read
     __syncthreads();
     if (warp == 0) {
       // Running sum of g in 64 bits, kept as two floats: differences of neighbours stay exact next to strong decays.
@@ -306,21 +339,28 @@ prepare_kernel(const DeltaArgs a) {
       vec[V_END * 64 + tid] = __expf(ghi[63]) * (1.f + glo[63]);
       vec[V_RQ * 64 + tid] = rq[tid];
     }
+    float gih[2], gil[2], fq[2], fk[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = warp * 16 + g + 8 * e;
+      gih[e] = ghi[i]; gil[e] = glo[i];
+      fq[e] = a.scale * rq[i]; fk[e] = bt[i] * rk[i];
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
+      const int j0 = 8 * j + t2;
+      const float2 gh = *reinterpret_cast<const float2*>(ghi + j0), gl = *reinterpret_cast<const float2*>(glo + j0);
+      const float2 rkj = *reinterpret_cast<const float2*>(rk + j0);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int i = warp * 16 + g + 8 * e, j0 = 8 * j + t2;
+        const int i = warp * 16 + g + 8 * e;
         float m[2], p[2];
-        const float2 gh = *reinterpret_cast<const float2*>(ghi + j0), gl = *reinterpret_cast<const float2*>(glo + j0);
-        const float2 rkj = *reinterpret_cast<const float2*>(rk + j0);
-        const float gih = ghi[i], gil = glo[i], fq = a.scale * rq[i], fk = bt[i] * rk[i];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           // made everywhere and then selected: a branch per element costs its latency each time
           const int jj = j0 + f;
-          const float d = (f ? rkj.y : rkj.x) * __expf((gih - (f ? gh.y : gh.x)) + (gil - (f ? gl.y : gl.x)));
-          const float pv = fq * d * qk[j][2 * e + f], mv = fk * d * kk[j][2 * e + f];
+          const float d = (f ? rkj.y : rkj.x) * __expf((gih[e] - (f ? gh.y : gh.x)) + (gil[e] - (f ? gl.y : gl.x)));
+          const float pv = fq[e] * d * qk[j][2 * e + f], mv = fk[e] * d * kk[j][2 * e + f];
           m[f] = i > jj ? mv : 0.f;
           p[f] = i > jj ? pv : 0.f;
           if (i == jj) vec[V_PD * 64 + i] = pv;
@@ -328,11 +368,14 @@ prepare_kernel(const DeltaArgs a) {
         *reinterpret_cast<float2*>(M + i * MP + j0) = make_float2(m[0], m[1]);
         uint32_t hi, lo;
         split2(p[0], p[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(ap + 2 * C * APITCH + i * APITCH + j0) = hi;
-        *reinterpret_cast<uint32_t*>(ap + 3 * C * APITCH + i * APITCH + j0) = lo;
+        *reinterpret_cast<uint32_t*>(Ps + i * APITCH + j0) = hi;
+        *reinterpret_cast<uint32_t*>(Ps + C * APITCH + i * APITCH + j0) = lo;
       }
     }
+    *reinterpret_cast<uint4*>(Ps + tid * APITCH + C) = make_uint4(0, 0, 0, 0);
+    fence_bulk();
     __syncthreads();
+    if (tid == 0) bulk_out(ap + 2 * C * APITCH, Ps, PREP_PART);
     // Inverse of I + M in fp32: the four 16 x 16 diagonal blocks by forward substitution, a thread per column ...
     if (tid < 64) {
       const int b0 = tid & 48, col = tid & 15;
@@ -341,52 +384,49 @@ prepare_kernel(const DeltaArgs a) {
       for (int i = 0; i < 16; ++i) {
         float s = i == col ? 1.f : 0.f;
 #pragma unroll
-        for (int j = 0; j < i; ++j) s -= M[(b0 + i) * MP + b0 + j] * x[j];
+        for (int j = 0; j < i; j += 4) {
+          const float4 m = *reinterpret_cast<const float4*>(M + (b0 + i) * MP + b0 + j);
+          s -= m.x * x[j];
+          if (j + 1 < i) s -= m.y * x[j + 1];
+          if (j + 2 < i) s -= m.z * x[j + 2];
+          if (j + 3 < i) s -= m.w * x[j + 3];
+        }
         x[i] = s;
         A[(b0 + i) * MP + b0 + col] = s;
       }
     }
     __syncthreads();
-    // ... then the blocks below, a diagonal at a time: A_IJ = -A_II sum_{J <= K < I} M_IK A_KJ. A thread makes four
-    // neighbouring columns of one row.
-    for (int d = 1; d < 4; ++d) {
-      for (int w = tid; w < (4 - d) * 64; w += PREP_THREADS) {
-        const int J = w >> 6, I = J + d, r = (w >> 2) & 15, cc = (w & 3) * 4;
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int K = J * 16; K < I * 16; K += 4) {
-          const float4 m = *reinterpret_cast<const float4*>(M + (I * 16 + r) * MP + K);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float mv = x == 0 ? m.x : x == 1 ? m.y : x == 2 ? m.z : m.w;
-            const float4 v = *reinterpret_cast<const float4*>(A + (K + x) * MP + J * 16 + cc);
-            s.x += mv * v.x; s.y += mv * v.y; s.z += mv * v.z; s.w += mv * v.w;
-          }
-        }
-        // the sum goes where the result will lie; A_IJ is not read before the next diagonal
-        *reinterpret_cast<float4*>(A + (I * 16 + r) * MP + J * 16 + cc) = s;
-      }
+    // ... then [[X, 0], [M, Y]]^-1 has -Y^-1 M X^-1 below, for the two pairs of 16 and for the pair of 32. M X^-1 waits
+    // in the upper part of A, which is zero and read by nobody.
+    {
+      const int b0 = (tid >> 6) * 32, r = (tid >> 2) & 15, cc = (tid & 3) * 4;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      mul4<16>(s, M + (b0 + 16 + r) * MP + b0, A + b0 * MP + b0 + cc);
+      *reinterpret_cast<float4*>(A + (b0 + r) * MP + b0 + 16 + cc) = s;
       __syncthreads();
-      float4 res[2];
-      int n = 0;
-      for (int w = tid; w < (4 - d) * 64; w += PREP_THREADS, ++n) {
-        const int J = w >> 6, I = J + d, r = (w >> 2) & 15, cc = (w & 3) * 4;
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const float mv = A[(I * 16 + r) * MP + I * 16 + x];
-          const float4 v = *reinterpret_cast<const float4*>(A + (I * 16 + x) * MP + J * 16 + cc);
-          s.x -= mv * v.x; s.y -= mv * v.y; s.z -= mv * v.z; s.w -= mv * v.w;
-        }
-        if (n == 0) res[0] = s; else res[1] = s;
-      }
-      __syncthreads();
-      n = 0;
-      for (int w = tid; w < (4 - d) * 64; w += PREP_THREADS, ++n) {
-        const int J = w >> 6, I = J + d, r = (w >> 2) & 15, cc = (w & 3) * 4;
-        *reinterpret_cast<float4*>(A + (I * 16 + r) * MP + J * 16 + cc) = n == 0 ? res[0] : res[1];
-      }
-      __syncthreads();
+      s = make_float4(0.f, 0.f, 0.f, 0.f);
+      mul4<16>(s, A + (b0 + 16 + r) * MP + b0 + 16, A + b0 * MP + b0 + 16 + cc);
+      *reinterpret_cast<float4*>(A + (b0 + 16 + r) * MP + b0 + cc) = make_float4(-s.x, -s.y, -s.z, -s.w);
     }
+    __syncthreads();
+    {
+      const int r = tid >> 2, cc = (tid & 3) * 4;  // X^-1 is lower triangular: columns 16 .. 31 begin at its row 16
+      float4 s0 = make_float4(0.f, 0.f, 0.f, 0.f), s1 = s0;
+      mul4<32>(s0, M + (32 + r) * MP, A + cc);
+      mul4<16>(s1, M + (32 + r) * MP + 16, A + 16 * MP + 16 + cc);
+      *reinterpret_cast<float4*>(A + r * MP + 32 + cc) = s0;
+      *reinterpret_cast<float4*>(A + r * MP + 48 + cc) = s1;
+    }
+    __syncthreads();
+    {
+      const int r = tid >> 3, cc = (tid & 7) * 4;  // Y^-1 too: its rows 0 .. 15 end at column 16
+      float4 s0 = make_float4(0.f, 0.f, 0.f, 0.f), s1 = s0;
+      mul4<16>(s0, A + (32 + r) * MP + 32, A + 32 + cc);
+      mul4<32>(s1, A + (48 + r) * MP + 32, A + 32 + cc);
+      *reinterpret_cast<float4*>(A + (32 + r) * MP + cc) = make_float4(-s0.x, -s0.y, -s0.z, -s0.w);
+      *reinterpret_cast<float4*>(A + (48 + r) * MP + cc) = make_float4(-s1.x, -s1.y, -s1.z, -s1.w);
+    }
+    __syncthreads();
     for (int w = tid; w < C * 8; w += PREP_THREADS) {
       const int r = w >> 3, c8 = (w & 7) * 8;
       uint32_t hi[4], lo[4];
@@ -398,10 +438,15 @@ prepare_kernel(const DeltaArgs a) {
         if (r == c8 + 2 * x + 1) v.y = 0.f;
         split2(v.x, v.y, hi[x], lo[x]);
       }
-      *reinterpret_cast<uint4*>(ap + r * APITCH + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(ap + C * APITCH + r * APITCH + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      *reinterpret_cast<uint4*>(As + r * APITCH + c8) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(As + C * APITCH + r * APITCH + c8) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
+    *reinterpret_cast<uint4*>(As + tid * APITCH + C) = make_uint4(0, 0, 0, 0);
+    fence_bulk();
+    __syncthreads();
+    if (tid == 0) bulk_out(ap, As, PREP_PART);
   }
+  if (tid == 0) bulk_out_read();
 }
 
 template <int THREADS>
@@ -1451,7 +1496,7 @@ int launch_dqk(const DeltaArgs& a, cudaStream_t s) {
 template <int DK>
 int forward_dk(const DeltaArgs& a, cudaStream_t s) {
   if (a.NC > 0) {
-    const size_t bytes = (2 * C * (DK + 8)) * sizeof(bf16) + (2 * C * MP + 5 * C) * sizeof(float);
+    const size_t bytes = PREP_TILES + 5 * C * sizeof(float);
     static std::atomic<uint64_t> allowed{0};
   if (!allow_smem(prepare_kernel<DK>, bytes, allowed)) return -3;
     prepare_kernel<DK><<<static_cast<unsigned>(a.NC * a.Hk), PREP_THREADS, bytes, s>>>(a);

@@ -195,21 +195,81 @@ __device__ __forceinline__ void load_rows(bf16* dst, int pitch, const bf16* src,
 // ---------------------------------------------------------------------------------------------------------- prepare
 
 constexpr int PREP_THREADS = 128;
-constexpr int MP = 68;  // fp32 pitch of the 64 x 64 matrices: rows 16-byte aligned, neighbours four banks apart
+// fp32 pitches of the 64 x 64 matrices: A's is read down its columns as well (two rows 8 banks apart), M's along rows
+constexpr int MP = 68, MMP = 72;
 
-// s += row [K] times K rows of four neighbouring columns.
-template <int K>
-__device__ __forceinline__ void mul4(float4& s, const float* row, const float* cols) {
-#pragma unroll 4
-  for (int k = 0; k < K; k += 4) {
-    const float4 m = *reinterpret_cast<const float4*>(row + k);
+// Operands of fp32 matrices in shared memory, each value as a high and a low bf16 (16 bits of it), and the product of
+// two such: what is left out is the low times the low.
+struct Split2 { uint32_t hi[4], lo[4]; };
+__device__ __forceinline__ void operand_a(Split2& o, const float* x, int pitch, int lane) {  // x [16 m, 16 k]
+  const float* p = x + (lane >> 2) * pitch + (lane & 3) * 2;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float mv = x == 0 ? m.x : x == 1 ? m.y : x == 2 ? m.z : m.w;
-      const float4 v = *reinterpret_cast<const float4*>(cols + (k + x) * MP);
-      s.x += mv * v.x; s.y += mv * v.y; s.z += mv * v.z; s.w += mv * v.w;
+  for (int e = 0; e < 4; ++e) {
+    const float2 v = *reinterpret_cast<const float2*>(p + (e & 1) * 8 * pitch + (e >> 1) * 8);
+    split2(v.x, v.y, o.hi[e], o.lo[e]);
+  }
+}
+__device__ __forceinline__ void operand_at(Split2& o, const float* x, int pitch, int lane) {  // x [16 k, 16 m]
+  const float* p = x + (lane & 3) * 2 * pitch + (lane >> 2);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float* y = p + (e & 1) * 8 + (e >> 1) * 8 * pitch;
+    split2(y[0], y[pitch], o.hi[e], o.lo[e]);
+  }
+}
+__device__ __forceinline__ void mma_split(float (&d)[4], const Split2& x, const uint32_t (&hi)[2], const uint32_t (&lo)[2]) {
+  mma(d, x.hi, hi[0], hi[1]);
+  mma(d, x.hi, lo[0], lo[1]);
+  mma(d, x.lo, hi[0], hi[1]);
+}
+
+// out = -Y (M X) for 16 columns of X and 16 rows of Y, KX and KY steps of 16 along the inner sides. (M X)^T comes out of
+// the matrix unit as Y's second operand has to lie.
+template <int KX, int KY>
+__device__ __forceinline__ void join(float* out, const float* Y, const float* M, const float* X, int lane) {
+  float m[2 * KY][4];
+#pragma unroll
+  for (int j = 0; j < 2 * KY; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[j][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < KX; ++k) {
+    Split2 x;
+    operand_at(x, X + 16 * k * MP, MP, lane);
+#pragma unroll
+    for (int j = 0; j < 2 * KY; ++j) {
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float2 v = *reinterpret_cast<const float2*>(M + (8 * j + (lane >> 2)) * MMP + 16 * k + 8 * e + (lane & 3) * 2);
+        split2(v.x, v.y, hi[e], lo[e]);
+      }
+      mma_split(m[j], x, hi, lo);
     }
   }
+  float s[2][4];
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < KY; ++k) {
+    Split2 y;
+    operand_a(y, Y + 16 * k, MP, lane);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) split2(m[2 * k + e][2 * n], m[2 * k + e][2 * n + 1], hi[e], lo[e]);
+      mma_split(s[n], y, hi, lo);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<float2*>(out + ((lane >> 2) + 8 * e) * MP + 8 * n + (lane & 3) * 2) =
+          make_float2(-s[n][2 * e], -s[n][2 * e + 1]);
 }
 
 constexpr size_t PREP_PART = 2 * C * APITCH * sizeof(bf16);  // high and low of A, or of P, as they lie in the record
@@ -365,7 +425,7 @@ prepare_kernel(const DeltaArgs a) {
           p[f] = i > jj ? pv : 0.f;
           if (i == jj) vec[V_PD * 64 + i] = pv;
         }
-        *reinterpret_cast<float2*>(M + i * MP + j0) = make_float2(m[0], m[1]);
+        *reinterpret_cast<float2*>(M + i * MMP + j0) = make_float2(m[0], m[1]);
         uint32_t hi, lo;
         split2(p[0], p[1], hi, lo);
         *reinterpret_cast<uint32_t*>(Ps + i * APITCH + j0) = hi;
@@ -385,7 +445,7 @@ prepare_kernel(const DeltaArgs a) {
         float s = i == col ? 1.f : 0.f;
 #pragma unroll
         for (int j = 0; j < i; j += 4) {
-          const float4 m = *reinterpret_cast<const float4*>(M + (b0 + i) * MP + b0 + j);
+          const float4 m = *reinterpret_cast<const float4*>(M + (b0 + i) * MMP + b0 + j);
           s -= m.x * x[j];
           if (j + 1 < i) s -= m.y * x[j + 1];
           if (j + 2 < i) s -= m.z * x[j + 2];
@@ -396,36 +456,17 @@ prepare_kernel(const DeltaArgs a) {
       }
     }
     __syncthreads();
-    // ... then [[X, 0], [M, Y]]^-1 has -Y^-1 M X^-1 below, for the two pairs of 16 and for the pair of 32. M X^-1 waits
-    // in the upper part of A, which is zero and read by nobody.
-    {
-      const int b0 = (tid >> 6) * 32, r = (tid >> 2) & 15, cc = (tid & 3) * 4;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      mul4<16>(s, M + (b0 + 16 + r) * MP + b0, A + b0 * MP + b0 + cc);
-      *reinterpret_cast<float4*>(A + (b0 + r) * MP + b0 + 16 + cc) = s;
-      __syncthreads();
-      s = make_float4(0.f, 0.f, 0.f, 0.f);
-      mul4<16>(s, A + (b0 + 16 + r) * MP + b0 + 16, A + b0 * MP + b0 + 16 + cc);
-      *reinterpret_cast<float4*>(A + (b0 + 16 + r) * MP + b0 + cc) = make_float4(-s.x, -s.y, -s.z, -s.w);
+    // ... then [[X, 0], [M, Y]]^-1 has -Y^-1 M X^-1 below, for the two pairs of 16 and for the pair of 32, whose X^-1
+    // and Y^-1 are lower triangular.
+    if (warp < 2) {
+      const int b0 = warp * 32;
+      join<1, 1>(A + (b0 + 16) * MP + b0, A + (b0 + 16) * MP + b0 + 16, M + (b0 + 16) * MMP + b0, A + b0 * MP + b0, lane);
     }
     __syncthreads();
-    {
-      const int r = tid >> 2, cc = (tid & 3) * 4;  // X^-1 is lower triangular: columns 16 .. 31 begin at its row 16
-      float4 s0 = make_float4(0.f, 0.f, 0.f, 0.f), s1 = s0;
-      mul4<32>(s0, M + (32 + r) * MP, A + cc);
-      mul4<16>(s1, M + (32 + r) * MP + 16, A + 16 * MP + 16 + cc);
-      *reinterpret_cast<float4*>(A + r * MP + 32 + cc) = s0;
-      *reinterpret_cast<float4*>(A + r * MP + 48 + cc) = s1;
-    }
-    __syncthreads();
-    {
-      const int r = tid >> 3, cc = (tid & 7) * 4;  // Y^-1 too: its rows 0 .. 15 end at column 16
-      float4 s0 = make_float4(0.f, 0.f, 0.f, 0.f), s1 = s0;
-      mul4<16>(s0, A + (32 + r) * MP + 32, A + 32 + cc);
-      mul4<32>(s1, A + (48 + r) * MP + 32, A + 32 + cc);
-      *reinterpret_cast<float4*>(A + (32 + r) * MP + cc) = make_float4(-s0.x, -s0.y, -s0.z, -s0.w);
-      *reinterpret_cast<float4*>(A + (48 + r) * MP + cc) = make_float4(-s1.x, -s1.y, -s1.z, -s1.w);
-    }
+    if (warp == 0) join<2, 1>(A + 32 * MP, A + 32 * MP + 32, M + 32 * MMP, A, lane);
+    if (warp == 1) join<2, 2>(A + 48 * MP, A + 48 * MP + 32, M + 32 * MMP, A, lane);
+    if (warp == 2) join<1, 1>(A + 32 * MP + 16, A + 32 * MP + 32, M + 32 * MMP + 16, A + 16 * MP + 16, lane);
+    if (warp == 3) join<1, 2>(A + 48 * MP + 16, A + 48 * MP + 32, M + 32 * MMP + 16, A + 16 * MP + 16, lane);
     __syncthreads();
     for (int w = tid; w < C * 8; w += PREP_THREADS) {
       const int r = w >> 3, c8 = (w & 7) * 8;

@@ -1375,7 +1375,7 @@ std::vector<at::Tensor> qk_norm_rope_bwd(const at::Tensor& dq, const at::Tensor&
   a.dv = grad(dv, a.T * G * a.D, "dv");
   if (gated) a.dgate = grad(*dgate, a.T * G * R * a.D, "dgate");
   at::Tensor dx = at::empty({a.T, x.size(1)}, x.options()), dqw = at::empty_like(qw), dkw = at::empty_like(kw);
-  at::Tensor partial = at::empty({lf::qk_norm_rope_bwd_grid(a.T), 2, a.D}, x.options().dtype(at::kFloat));
+  at::Tensor partial = at::empty({lf::qk_norm_rope_bwd_grid(a), a.D}, x.options().dtype(at::kFloat));
   a.dx = dx.data_ptr();
   a.partial = partial.data_ptr<float>();
   a.dqw = dqw.data_ptr();

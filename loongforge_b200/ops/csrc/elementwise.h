@@ -49,13 +49,14 @@ struct QkNormRopeArgs {
   void *q = nullptr, *k = nullptr;  // bf16 [T, G * R, D], [T, G, D]
   const void *dq = nullptr, *dk = nullptr, *dv = nullptr, *dgate = nullptr;
   void* dx = nullptr;          // bf16 [T, G * P * D]
-  float* partial = nullptr;    // fp32 [qk_norm_rope_bwd_grid(T), 2, D]
+  float* partial = nullptr;    // fp32 [qk_norm_rope_bwd_grid(a), D]
   void *dqw = nullptr, *dkw = nullptr;  // bf16 [D]
   int* status = nullptr;
+  int q_blocks = 0;  // of the grid, the blocks that take query heads; the rest take key heads (set by the launch)
 };
-int qk_norm_rope_bwd_grid(long long T);
-int qk_norm_rope_fwd(const QkNormRopeArgs& a, cudaStream_t s);  // 0, or negative for shapes that are not covered
-int qk_norm_rope_bwd(const QkNormRopeArgs& a, cudaStream_t s);
+int qk_norm_rope_bwd_grid(QkNormRopeArgs& a);  // blocks of the backward pass
+int qk_norm_rope_fwd(QkNormRopeArgs& a, cudaStream_t s);  // 0, or negative for shapes that are not covered
+int qk_norm_rope_bwd(QkNormRopeArgs& a, cudaStream_t s);
 
 // MoE router (router.cu). score: 0 softmax over the selected k, 1 softmax over all experts then top-k, 2 sigmoid.
 struct RouterArgs {

@@ -52,7 +52,8 @@ struct QkNormRopeArgs {
   float* partial = nullptr;    // fp32 [qk_norm_rope_bwd_grid(a), D]
   void *dqw = nullptr, *dkw = nullptr;  // bf16 [D]
   int* status = nullptr;
-  int q_blocks = 0;  // of the grid, the blocks that take query heads; the rest take key heads (set by the launch)
+  // set by the launch: the blocks that take query heads (the rest take key heads), log2 of a token's heads at once
+  int q_blocks = 0, q_lg = 0, k_lg = 0;
 };
 int qk_norm_rope_bwd_grid(QkNormRopeArgs& a);  // blocks of the backward pass
 int qk_norm_rope_fwd(QkNormRopeArgs& a, cudaStream_t s);  // 0, or negative for shapes that are not covered

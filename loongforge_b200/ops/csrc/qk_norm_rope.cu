@@ -11,7 +11,7 @@
 // Bound by memory. D / 16 lanes hold a head. A lane holds both elements of its rotated pairs (eight neighbours of each
 // half, 16 bytes at a time; 16 neighbours behind the rotated span), so the rotation stays in the lane. A block takes
 // either query heads or key heads, so that norm weight, their gradient and the pairs' factors stay in registers, and lays
-// (token, head) out so that a lane keeps one token, hence its cosines, for about four heads. What a lane will work on is
+// (token, head) out so that a lane keeps one token, hence its cosines, for up to eight heads. What a lane will work on is
 // copied ahead, over the end of its turn too, into its own places in shared memory, so that nobody waits for anybody. The value (and gate) heads of the packed row are not touched forward; backward copies their
 // gradients into the packed gradient, which is so written in one pass.
 #include <cuda_bf16.h>
@@ -277,14 +277,6 @@ __device__ __forceinline__ void weights(const bf16* p, const Place<MODE>& pl, fl
   }
 }
 
-// log2 of the heads of a token that a block works on at once, of `count`, with room for `room`: a lane keeps about four
-// heads of its token, but a block no more than eight tokens if it can, whose angles it works out for each turn.
-__device__ __host__ __forceinline__ int heads_at_once(int count, int room) {
-  int lg = 0;
-  while ((8 << lg <= count || (room >> lg > 8 && 1 << lg < count)) && 2 << lg <= room) ++lg;
-  return lg;
-}
-
 // The heads of one kind: `per` of a group from head `base` of its `P`, `count` of a token. A block's turn is `tokens`
 // tokens with 2^lg lanes' worth of heads of each at a time.
 struct Part {
@@ -299,7 +291,7 @@ struct Part {
     p.base = q ? 0 : a.P - 2;
     p.count = a.G * p.per;
     p.w = static_cast<const bf16*>(q ? a.qw : a.kw);
-    p.lg = heads_at_once(p.count, HEADS);
+    p.lg = q ? a.q_lg : a.k_lg;
     p.tokens = HEADS >> p.lg;
     p.block = q ? blockIdx.x : blockIdx.x - a.q_blocks;
     p.blocks = q ? a.q_blocks : gridDim.x - a.q_blocks;
@@ -550,20 +542,29 @@ __global__ void qk_dw_kernel(const float* __restrict__ partial, int q_blocks, in
   if (threadIdx.x == 0) (q ? dqw : dkw)[c0 + threadIdx.y] = __float2bfloat16(s);
 }
 
-// Blocks for the query heads and all blocks: two kinds share `room` in proportion to their work (a head's elements, and
-// twice as much for an angle), and none has more than the tokens ask for.
-void share(QkNormRopeArgs& a, int room, int* blocks) {
+// How a launch is laid out; returns its blocks. A lane keeps up to eight heads of its token, which makes the angles cheap
+// (8192 tokens of 4 x 8 heads of 128, forward + backward: 116 us with two, 125 with four, 115 with eight), and fewer while the
+// tokens do not give every block two turns. The two kinds share the blocks in proportion to their work (a head's elements,
+// and twice as much for an angle), and none has more than the tokens ask for.
+int lay_out(QkNormRopeArgs& a, int room) {
   const int heads = THREADS / (a.D / 16);
-  auto turns = [&](int count) {
-    const int tokens = heads >> heads_at_once(count, heads);
-    return (a.T + tokens - 1) / tokens;
+  auto at_once = [&](int count, int keep) {  // log2 of a token's heads that a block works on at once
+    int lg = 0;
+    while (((2 * keep) << lg <= count || (heads >> lg > 2 * keep && 1 << lg < count)) && 2 << lg <= heads) ++lg;
+    return lg;
   };
-  const long long q = turns(a.G * a.R), k = turns(a.G);
+  auto turns = [&](int lg) { return (a.T + (heads >> lg) - 1) / (heads >> lg); };
+  for (int keep = 8; keep > 0; keep >>= 1) {
+    a.q_lg = at_once(a.G * a.R, keep);
+    a.k_lg = at_once(a.G, keep);
+    if (turns(a.q_lg) + turns(a.k_lg) >= 2 * room) break;
+  }
+  const long long q = turns(a.q_lg), k = turns(a.k_lg);
   const double wq = static_cast<double>(a.G) * a.R * a.D + 2.0 * a.rot_dim, wk = static_cast<double>(a.G) * a.D + 2.0 * a.rot_dim;
   int ks = static_cast<int>(room * (wk / (wq + wk)) + 0.5);
   ks = static_cast<int>(k < ks ? k : ks > 1 ? ks : 1);
   a.q_blocks = static_cast<int>(q < room - ks ? q : room - ks);
-  *blocks = a.q_blocks + ks;
+  return a.q_blocks + ks;
 }
 
 using Kernel = void (*)(QkNormRopeArgs);
@@ -589,17 +590,14 @@ bool covered(const QkNormRopeArgs& a) { return (a.D == 64 || a.D == 128 || a.D =
 }  // namespace
 
 int qk_norm_rope_bwd_grid(QkNormRopeArgs& a) {
-  int blocks = 0;
-  share(a, 148 * 2, &blocks);
-  return blocks;
+  return a.T == 0 ? 0 : lay_out(a, 148 * 2);
 }
 
 int qk_norm_rope_fwd(QkNormRopeArgs& a, cudaStream_t s) {
   if (!covered(a)) return -1;
   if (a.T > INT32_MAX / 2) return -2;
   if (a.T == 0) return 0;
-  int blocks = 0;
-  share(a, 148 * 3, &blocks);
+  const int blocks = lay_out(a, 148 * 3);
   const int rc = a.D == 64 ? launch_fwd<4>(a, blocks, s) : a.D == 128 ? launch_fwd<8>(a, blocks, s) : launch_fwd<16>(a, blocks, s);
   if (rc != 0) return rc;
   return cudaGetLastError() == cudaSuccess ? 0 : -3;

@@ -73,25 +73,33 @@ __device__ __forceinline__ uint32_t narrow(f2 v) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// 1 / (1 + 2^(-p log2 e)), without the steps that keep subnormal values: they vanish next to 1, and a quotient below
+// 2^-126 is nothing beside bf16's steps.
 __device__ __forceinline__ f2 sigmoid2(f2 p) {
-  const float2 f = split(p);
-  return make2(sigmoid(f.x), sigmoid(f.y));
+  float2 f = split(mul2(p, make2(-1.4426950408889634f, -1.4426950408889634f)));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(f.x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(f.y));
+  f = split(add2(make2(f.x, f.y), make2(1.f, 1.f)));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(f.x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(f.y));
+  return make2(f.x, f.y);
 }
 
 constexpr int THREADS = 128;
-constexpr int FV = 2, BV = 1;  // channel pairs of a thread, forward and backward (dw and dx sums: more registers a pair)
-// Rows that are loaded ahead of their use. 16384 x 8192: forward 96 us with 8 (104 with 4), backward 211 us with 4 (245 with 8:
-// fewer blocks fit).
+// Channel pairs of a thread: the walk's addresses and tests are paid once for both (16384 x 8192 backward: 187 us with one,
+// 175 with two).
+constexpr int FV = 2, BV = 2;
+// Rows that are loaded ahead of their use. 16384 x 8192: forward 96 us with 8 (104 with 4); backward holds two inputs, three
+// windows and the sums of dw, so 4.
 constexpr int FSTEP = 8, BSTEP = 4;
 constexpr int MAX_SPAN = 128;
 
-// Rows [t, t + STEP) into registers; rows from `end` on are left alone.
+// The next STEP rows from p on into registers, of which there are `left`; p moves on.
 template <typename T, int STEP>
-__device__ __forceinline__ void load_rows(T (&r)[STEP], const bf16* p, long long t, long long stride, long long end) {
-  p += t * stride;
+__device__ __forceinline__ void load_rows(T (&r)[STEP], const bf16*& p, long long stride, int left) {
 #pragma unroll
   for (int i = 0; i < STEP; ++i) {
-    if (t + i < end) r[i] = *reinterpret_cast<const T*>(p);
+    if (i < left) r[i] = *reinterpret_cast<const T*>(p);
     p += stride;
   }
 }
@@ -126,8 +134,10 @@ conv_fwd_kernel(const ConvArgs a, int cblocks, int span) {
   const bf16* x = static_cast<const bf16*>(a.x) + c;
   bf16* y = static_cast<bf16*>(a.y) + c;
   f2 wr[K][FV], bias[FV], win[K][FV];
-  uint2 next[STEP];
-  load_rows(next, x, t0, a.x_ts, t1);
+  uint2 rows0[STEP], rows1[STEP];
+  const bf16* xt = x + t0 * a.x_ts;
+  const int n = static_cast<int>(t1 - t0);
+  load_rows(rows0, xt, a.x_ts, n);
   load_pairs<FV, K>(a, c, wr, bias);
 #pragma unroll
   for (int i = 1; i < K; ++i) {  // win[i] = x[t - i]
@@ -136,16 +146,13 @@ conv_fwd_kernel(const ConvArgs a, int cblocks, int span) {
 #pragma unroll
     for (int j = 0; j < FV; ++j) win[i][j] = widen(j ? r.y : r.x);
   }
-  for (long long t = t0; t < t1; t += STEP) {
-    uint2 rows[STEP];
-#pragma unroll
-    for (int r = 0; r < STEP; ++r) rows[r] = next[r];
-    load_rows(next, x, t + STEP, a.x_ts, t1);
-    const int* f = front + (t - t0);
-    bool plain = t + STEP <= t1;
+  y += t0 * a.C;
+  auto step = [&](int t, uint2 (&rows)[STEP], uint2 (&next)[STEP]) {
+    load_rows(next, xt, a.x_ts, n - t - STEP);
+    const int* f = front + t;
+    bool plain = t + STEP <= n;
 #pragma unroll
     for (int r = 0; r < STEP; ++r) plain = plain && f[r] == K - 1;
-    bf16* yt = y + t * a.C;
     auto row = [&](int r, int fr) {
       uint32_t out[FV];
 #pragma unroll
@@ -160,7 +167,8 @@ conv_fwd_kernel(const ConvArgs a, int cblocks, int span) {
 #pragma unroll
         for (int i = K - 1; i > 0; --i) win[i][j] = win[i - 1][j];
       }
-      *reinterpret_cast<uint2*>(yt + static_cast<long long>(r) * a.C) = make_uint2(out[0], out[1]);
+      *reinterpret_cast<uint2*>(y) = make_uint2(out[0], out[1]);
+      y += a.C;
     };
     if (plain) {
 #pragma unroll
@@ -168,8 +176,12 @@ conv_fwd_kernel(const ConvArgs a, int cblocks, int span) {
     } else {
 #pragma unroll
       for (int r = 0; r < STEP; ++r)
-        if (t + r < t1) row(r, f[r]);
+        if (t + r < n) row(r, f[r]);
     }
+  };
+  for (int t = 0; t < n; t += 2 * STEP) {  // two steps, so that the rows that came ahead need not move
+    step(t, rows0, rows1);
+    if (t + STEP < n) step(t + STEP, rows1, rows0);
   }
 }
 
@@ -178,72 +190,81 @@ conv_fwd_kernel(const ConvArgs a, int cblocks, int span) {
 template <int K>
 __global__ void __launch_bounds__(THREADS)
 conv_bwd_kernel(const ConvArgs a, int cblocks, int span) {
-  static_assert(BV == 1, "one pair a thread");
+  static_assert(BV == 2, "two pairs a thread");
   constexpr int STEP = BSTEP;
   __shared__ int front[MAX_SPAN + STEP];
   const int tb = blockIdx.x / cblocks;
   const long long t0 = static_cast<long long>(tb) * span;
   const long long t1 = t0 + span < a.T ? t0 + span : a.T, t2 = t1 + K - 1 < a.T ? t1 + K - 1 : a.T;
-  const int c = ((blockIdx.x % cblocks) * THREADS + threadIdx.x) * 2;
+  const int c = ((blockIdx.x % cblocks) * THREADS + threadIdx.x) * 2 * BV;
   for (int i = threadIdx.x; i < span + STEP; i += THREADS) front[i] = earlier_tokens(a.cu, a.N, a.T, t0 + i, K - 1);
   __syncthreads();
   if (c >= a.C) return;
   const bf16* x = static_cast<const bf16*>(a.x) + c;
   const bf16* dy = static_cast<const bf16*>(a.dy) + c;
   bf16* dx = static_cast<bf16*>(a.dx) + c;
-  f2 wr[K][1], bias[1], win[K], acc[K], dw[K], db = 0ull;
-  uint32_t nx[STEP], ng[STEP];
-  load_rows(nx, x, t0, a.x_ts, t2);
-  load_rows(ng, dy, t0, a.C, t2);
-  load_pairs<1, K>(a, c, wr, bias);
+  f2 wr[K][BV], bias[BV], win[K][BV], acc[K][BV], dw[K][BV], db[BV];
+  uint2 xr[STEP], gr[STEP];
+  const bf16 *xt = x + t0 * a.x_ts, *gt = dy + t0 * a.C;
+  const int n = static_cast<int>(t1 - t0), n2 = static_cast<int>(t2 - t0);  // the block's rows, and with those behind
+  load_rows(xr, xt, a.x_ts, n2);
+  load_rows(gr, gt, a.C, n2);
+  load_pairs<BV, K>(a, c, wr, bias);
 #pragma unroll
   for (int i = 0; i < K; ++i) {
-    win[i] = acc[i] = dw[i] = 0ull;
-    if (i > 0 && t0 - i >= 0) win[i] = widen(*reinterpret_cast<const uint32_t*>(x + (t0 - i) * a.x_ts));
-  }
-  for (long long t = t0; t < t1 + K - 1; t += STEP) {
-    uint32_t xr[STEP], gr[STEP];
+    uint2 r = make_uint2(0u, 0u);
+    if (i > 0 && t0 - i >= 0) r = *reinterpret_cast<const uint2*>(x + (t0 - i) * a.x_ts);
 #pragma unroll
-    for (int r = 0; r < STEP; ++r) {
-      xr[r] = nx[r];
-      gr[r] = ng[r];
+    for (int j = 0; j < BV; ++j) {
+      win[i][j] = widen(j ? r.y : r.x);
+      acc[i][j] = dw[i][j] = db[j] = 0ull;
     }
-    load_rows(nx, x, t + STEP, a.x_ts, t2);
-    load_rows(ng, dy, t + STEP, a.C, t2);
-    const int* f = front + (t - t0);
-    bool plain = t + STEP <= t1 && t > t0;
+  }
+  dx += (t0 - (K - 1)) * a.C;
+#pragma unroll 1
+  for (int t = 0; t < n + K - 1; t += STEP) {
+    uint2 nx[STEP], ng[STEP];
+    load_rows(nx, xt, a.x_ts, n2 - t - STEP);
+    load_rows(ng, gt, a.C, n2 - t - STEP);
+    const int* f = front + t;
+    bool plain = t + STEP <= n && t > 0;
 #pragma unroll
     for (int r = 0; r < STEP; ++r) plain = plain && f[r] == K - 1;
-    bf16* dxt = dx + (t - (K - 1)) * a.C;
     // `own`: the row is one of the block's; `out`: row t + r - (K - 1), which no later row reaches, is
     auto row = [&](int r, int fr, bool own, bool out) {
-      acc[0] = 0ull;
-      if (fr >= 0) {  // a token of some sequence
-        win[0] = widen(xr[r]);
-        f2 d = widen(gr[r]);
-        if (a.silu) {
-          f2 p = fma2(wr[0][0], win[0], bias[0]);
 #pragma unroll
-          for (int i = 1; i < K; ++i)
-            if (i <= fr) p = fma2(wr[i][0], win[i], p);
-          const f2 s = sigmoid2(p), ps = mul2(p, s);
-          // silu' = s + p s (1 - s) = s + p s - (p s) s
-          d = mul2(d, add2(s, fma2(mul2(ps, s), make2(-1.f, -1.f), ps)));
-        }
+      for (int j = 0; j < BV; ++j) {
+        acc[0][j] = 0ull;
+        if (fr >= 0) {  // a token of some sequence
+          win[0][j] = widen(j ? xr[r].y : xr[r].x);
+          f2 d = widen(j ? gr[r].y : gr[r].x);
+          if (a.silu) {
+            f2 p = fma2(wr[0][j], win[0][j], bias[j]);
 #pragma unroll
-        for (int i = 0; i < K; ++i)
-          if (i <= fr) {
-            acc[i] = fma2(wr[i][0], d, acc[i]);
-            if (own) dw[i] = fma2(d, win[i], dw[i]);
+            for (int i = 1; i < K; ++i)
+              if (i <= fr) p = fma2(wr[i][j], win[i][j], p);
+            const f2 s = sigmoid2(p), ps = mul2(p, s);
+            // silu' = s + p s (1 - s) = s + p s - (p s) s
+            d = mul2(d, add2(s, fma2(mul2(ps, s), make2(-1.f, -1.f), ps)));
           }
-        if (own) db = add2(db, d);
-      }
-      if (out) *reinterpret_cast<uint32_t*>(dxt + static_cast<long long>(r) * a.C) = narrow(acc[K - 1]);
 #pragma unroll
-      for (int i = K - 1; i > 0; --i) {
-        win[i] = win[i - 1];
-        acc[i] = acc[i - 1];
+          for (int i = 0; i < K; ++i)
+            if (i <= fr) {
+              acc[i][j] = fma2(wr[i][j], d, acc[i][j]);
+              if (own) dw[i][j] = fma2(d, win[i][j], dw[i][j]);
+            }
+          if (own) db[j] = add2(db[j], d);
+        }
       }
+      if (out) *reinterpret_cast<uint2*>(dx) = make_uint2(narrow(acc[K - 1][0]), narrow(acc[K - 1][1]));
+      dx += a.C;
+#pragma unroll
+      for (int i = K - 1; i > 0; --i)
+#pragma unroll
+        for (int j = 0; j < BV; ++j) {
+          win[i][j] = win[i - 1][j];
+          acc[i][j] = acc[i - 1][j];
+        }
     };
     if (plain) {
 #pragma unroll
@@ -251,24 +272,41 @@ conv_bwd_kernel(const ConvArgs a, int cblocks, int span) {
     } else {
 #pragma unroll
       for (int r = 0; r < STEP; ++r)
-        if (t + r < t1 + K - 1) row(r, f[r], t + r < t1, t + r - (K - 1) >= t0);
+        if (t + r < n + K - 1) row(r, f[r], t + r < n, t + r >= K - 1);
+    }
+#pragma unroll
+    for (int r = 0; r < STEP; ++r) {
+      xr[r] = nx[r];
+      gr[r] = ng[r];
     }
   }
   float* p = a.partial + static_cast<long long>(tb) * (K + 1) * a.C + c;
 #pragma unroll
-  for (int i = 0; i < K; ++i) *reinterpret_cast<float2*>(p + static_cast<long long>(i) * a.C) = split(dw[i]);
-  *reinterpret_cast<float2*>(p + static_cast<long long>(K) * a.C) = split(db);
+  for (int i = 0; i <= K; ++i) {
+    const float2 u = split(i < K ? dw[i][0] : db[0]), v = split(i < K ? dw[i][1] : db[1]);
+    *reinterpret_cast<float4*>(p + static_cast<long long>(i) * a.C) = make_float4(u.x, u.y, v.x, v.y);
+  }
 }
 
-// dw[c, K - 1 - i] = sum over blocks of partial[b, i, c], in block order; db likewise from row K.
-__global__ void conv_dw_kernel(const float* __restrict__ partial, int blocks, int C, int K, bf16* __restrict__ dw,
-                               bf16* __restrict__ db) {
-  const long long idx = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+// dw[c, K - 1 - i] = sum over blocks of partial[b, i, c], in a fixed order; db likewise from row K. Eight threads share a
+// column, which is a matter of latency: 4 us instead of 18 for 128 blocks of 8192 channels.
+constexpr int DW_COLS = 32, DW_ROWS = 8;
+
+__global__ void __launch_bounds__(DW_COLS * DW_ROWS)
+conv_dw_kernel(const float* __restrict__ partial, int blocks, int C, int K, bf16* __restrict__ dw, bf16* __restrict__ db) {
+  __shared__ float red[DW_ROWS][DW_COLS];
+  const long long idx = static_cast<long long>(blockIdx.x) * DW_COLS + threadIdx.x;
   const long long n = static_cast<long long>(K + 1) * C;
-  if (idx >= n) return;
   float s = 0.f;
+  if (idx < n) {
 #pragma unroll 8
-  for (int b = 0; b < blocks; ++b) s += partial[b * n + idx];
+    for (int b = threadIdx.y; b < blocks; b += DW_ROWS) s += partial[b * n + idx];
+  }
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y != 0 || idx >= n) return;
+#pragma unroll
+  for (int r = 1; r < DW_ROWS; ++r) s += red[r][threadIdx.x];
   const int i = static_cast<int>(idx / C), c = static_cast<int>(idx % C);
   if (i < K) dw[static_cast<long long>(c) * K + (K - 1 - i)] = __float2bfloat16(s);
   else if (db) db[c] = __float2bfloat16(s);
@@ -370,8 +408,8 @@ int conv_bwd(const ConvArgs& a, cudaStream_t s) {
     else conv_bwd_kernel<4><<<gd, THREADS, 0, s>>>(a, cblocks, span);
   }
   const long long n = static_cast<long long>(a.K + 1) * a.C;
-  conv_dw_kernel<<<static_cast<unsigned>((n + 127) / 128), 128, 0, s>>>(a.partial, blocks, a.C, a.K,
-                                                                        static_cast<bf16*>(a.dw), static_cast<bf16*>(a.db));
+  conv_dw_kernel<<<static_cast<unsigned>((n + DW_COLS - 1) / DW_COLS), dim3(DW_COLS, DW_ROWS), 0, s>>>(
+      a.partial, blocks, a.C, a.K, static_cast<bf16*>(a.dw), static_cast<bf16*>(a.db));
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
 }
 

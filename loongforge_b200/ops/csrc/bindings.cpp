@@ -1028,8 +1028,29 @@ lf::DeltaArgs delta_args(const at::Tensor& q, const at::Tensor& k, const at::Ten
   return a;
 }
 
-// {o, final state or empty}, and with `keep` what the backward pass reads: {past, memory, U, chunk states, q and k
-// tiles, A / P, factors} (see DeltaArgs).
+// What the kernels write and the backward pass reads (see DeltaArgs), behind one another in one buffer; `keep`: with the
+// parts that only the backward pass reads. Returns its bytes; base may be null.
+int64_t delta_carve(lf::DeltaArgs& a, bool keep, char* base) {
+  const int64_t heads = a.NC * a.Hv, rows = heads * lf::DELTA_CHUNK;
+  int64_t at = 0;
+  auto part = [&](int64_t bytes) {
+    char* p = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  };
+  a.ap = part(heads * lf::DELTA_AP * 2);
+  a.vec = reinterpret_cast<float*>(part(heads * lf::DELTA_VEC * 4));
+  a.qk = part(a.NC * a.Hk * 2 * lf::DELTA_CHUNK * (a.dk + lf::DELTA_ROW_PAD) * 2);
+  if (keep) {
+    a.past = part(rows * a.dv * 4);
+    a.mem = part(2 * rows * a.dv * 2);
+    a.u = part(2 * rows * a.dv * 2);
+    a.states = part(heads * 2 * a.dv * a.dk * 2);
+  }
+  return at;
+}
+
+// {o, final state or empty, the buffer above}
 std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
                                   const at::Tensor& beta, c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first,
                                   double scale, bool l2norm, c10::optional<at::Tensor> s_in, bool want_state, bool keep,
@@ -1041,28 +1062,14 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, cons
   auto bf = v.options(), fl = g.options();
   at::Tensor o = at::empty({a.T, a.Hv, a.dv}, bf);
   at::Tensor s_out = want_state ? at::empty({a.N, a.Hv, a.dk, a.dv}, fl) : at::empty({0}, fl);
-  at::Tensor ap = at::empty({a.NC, a.Hv, lf::DELTA_AP}, bf), vec = at::empty({a.NC, a.Hv, lf::DELTA_VEC}, fl);
-  at::Tensor qk = at::empty({a.NC, a.Hk, 2, lf::DELTA_CHUNK, a.dk + lf::DELTA_ROW_PAD}, bf);
-  a.qk = qk.data_ptr();
+  at::Tensor work = at::empty({delta_carve(a, keep, nullptr)}, bf.dtype(at::kByte));
+  delta_carve(a, keep, static_cast<char*>(work.data_ptr()));
   a.o = o.data_ptr();
-  a.ap = ap.data_ptr();
-  a.vec = vec.data_ptr<float>();
   if (s_in.has_value()) {
     check_state(*s_in, "initial_state", a.N, q, v);
     a.s_in = s_in->data_ptr<float>();
   }
   if (want_state) a.s_out = s_out.data_ptr<float>();
-  std::vector<at::Tensor> out = {o, s_out};
-  if (keep) {
-    const int64_t rows = a.NC * a.Hv * lf::DELTA_CHUNK;
-    at::Tensor past = at::empty({rows, a.dv}, fl), mem = at::empty({2, rows, a.dv}, bf), u = at::empty({2, rows, a.dv}, bf);
-    at::Tensor states = at::empty({a.NC, a.Hv, 2, a.dv, a.dk}, bf);
-    a.past = past.data_ptr();
-    a.mem = mem.data_ptr();
-    a.u = u.data_ptr();
-    a.states = states.data_ptr();
-    out.insert(out.end(), {past, mem, u, states, qk, ap, vec});
-  }
   const int rc = lf::delta_forward(a, cur_stream());
   TORCH_CHECK(rc == 0, "lf::delta_forward failed with code ", rc, " (dk = ", a.dk, ", dv = ", a.dv, ")");
   g_launches += a.NC > 0 ? 2 : 1;
@@ -1074,52 +1081,40 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, cons
     lf::delta_zero_uncovered(z, a.cu, a.N, a.T, cur_stream());
     ++g_launches;
   }
-  return out;
+  return {o, s_out, work};
 }
 
 // {dq, dk, dv, dg, dbeta, gradient of the initial state or empty}
 std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tensor> ds_out, const at::Tensor& q, const at::Tensor& k,
                                   const at::Tensor& v, const at::Tensor& g, const at::Tensor& beta,
                                   c10::optional<at::Tensor> bounds, c10::optional<at::Tensor> first, double scale, bool l2norm,
-                                  bool want_ds, const at::Tensor& past, const at::Tensor& mem, const at::Tensor& u,
-                                  const at::Tensor& states, const at::Tensor& qk, const at::Tensor& ap,
-                                  const at::Tensor& vec, const at::Tensor& status) {
+                                  bool want_ds, const at::Tensor& kept, const at::Tensor& status) {
   c10::cuda::CUDAGuard guard(q.device());
   lf::DeltaArgs a = delta_args(q, k, v, g, beta, bounds, first, scale, l2norm);
   check_status(status, q);
   a.status = status.data_ptr<int>();
   check_heads(dout, "dout", q);
   TORCH_CHECK(dout.is_contiguous() && dout.numel() == a.T * a.Hv * a.dv, "the outputs' gradient must be contiguous bf16 [T, value heads, dv]");
-  const int64_t kept = a.NC * a.Hv * lf::DELTA_CHUNK * a.dv;
-  TORCH_CHECK(past.device() == q.device() && past.scalar_type() == at::kFloat && past.numel() == kept && mem.scalar_type() == at::kBFloat16 &&
-              mem.numel() == 2 * kept && u.scalar_type() == at::kBFloat16 && u.numel() == 2 * kept,
-              "what the forward pass kept does not fit these inputs");
-  TORCH_CHECK(states.device() == q.device() && states.scalar_type() == at::kBFloat16 && states.numel() == a.NC * a.Hv * 2 * a.dk * a.dv &&
-              qk.scalar_type() == at::kBFloat16 && qk.numel() == a.NC * a.Hk * 2 * lf::DELTA_CHUNK * (a.dk + lf::DELTA_ROW_PAD) &&
-              ap.scalar_type() == at::kBFloat16 && ap.numel() == a.NC * a.Hv * lf::DELTA_AP && vec.scalar_type() == at::kFloat &&
-              vec.numel() == a.NC * a.Hv * lf::DELTA_VEC, "what the forward pass kept does not fit these inputs");
+  TORCH_CHECK(kept.device() == q.device() && kept.scalar_type() == at::kByte && kept.is_contiguous() &&
+                  kept.numel() == delta_carve(a, true, nullptr), "what the forward pass kept does not fit these inputs");
+  delta_carve(a, true, static_cast<char*>(kept.data_ptr()));
   auto bf = v.options(), fl = g.options();
   at::Tensor dq = at::empty(q.sizes(), bf), dk = at::empty(k.sizes(), bf), dv = at::empty(v.sizes(), bf);
   at::Tensor dg = at::empty_like(g), dbeta = at::empty_like(beta);
   at::Tensor ds_in = want_ds ? at::empty({a.N, a.Hv, a.dk, a.dv}, fl) : at::empty({0}, fl);
-  at::Tensor dstates = at::empty({a.NC, a.Hv, a.dv, a.dk}, bf);
-  at::Tensor rowdots = at::empty({a.NC, a.Hv, a.dv / 16, 2, 64}, fl), sdots = at::empty({a.NC, a.Hv, a.dv / 16, 4}, fl);
+  // [NC, Hv] x: dstates bf16 [dv, dk], rowdots fp32 [dv / 16, 2, 64], sdots fp32 [dv / 16, 4], all multiples of 64 bytes
+  const int64_t heads = a.NC * a.Hv, sbytes = heads * a.dv * a.dk * 2, rbytes = heads * (a.dv / 16) * 2 * 64 * 4;
+  at::Tensor work = at::empty({sbytes + rbytes + heads * (a.dv / 16) * 4 * 4}, bf.dtype(at::kByte));
+  char* base = static_cast<char*>(work.data_ptr());
   a.dout = dout.data_ptr();
   if (ds_out.has_value()) {
     check_state(*ds_out, "the final state's gradient", a.N, q, v);
     a.ds_out = ds_out->data_ptr<float>();
   }
   if (want_ds) a.ds_in = ds_in.data_ptr<float>();
-  a.past = past.data_ptr();
-  a.mem = mem.data_ptr();
-  a.u = u.data_ptr();
-  a.states = states.data_ptr();
-  a.qk = qk.data_ptr();
-  a.ap = ap.data_ptr();
-  a.vec = vec.data_ptr<float>();
-  a.dstates = dstates.data_ptr();
-  a.rowdots = rowdots.data_ptr<float>();
-  a.sdots = sdots.data_ptr<float>();
+  a.dstates = base;
+  a.rowdots = reinterpret_cast<float*>(base + sbytes);
+  a.sdots = reinterpret_cast<float*>(base + sbytes + rbytes);
   a.dq = dq.data_ptr();
   a.dkey = dk.data_ptr();
   a.dv_ = dv.data_ptr();
@@ -1352,7 +1347,10 @@ std::vector<at::Tensor> qk_norm_rope_fwd(const at::Tensor& x, int64_t G, int64_t
   const int rc = lf::qk_norm_rope_fwd(a, cur_stream());
   TORCH_CHECK(rc == 0, "lf::qk_norm_rope_fwd failed with code ", rc);
   ++g_launches;
-  return {q, k};
+  const int64_t row = x.stride(0), grp = static_cast<int64_t>(a.P) * a.D, at = x.storage_offset();
+  std::vector<at::Tensor> out = {q, k, x.as_strided({a.T, G, a.D}, {row, grp, 1}, at + (a.P - 1) * static_cast<int64_t>(a.D))};
+  if (gated) out.push_back(x.as_strided({a.T, G, R, a.D}, {row, grp, a.D, 1}, at + R * a.D));
+  return out;
 }
 
 // {gradient of the packed row, of q_weight, of k_weight}

@@ -339,10 +339,9 @@ class _QKNormRopeFn(torch.autograd.Function):
     def forward(ctx, qkv, qw, kw, G, R, gated, freqs, inv_freq, pos, axis, rot_dim, interleaved, mscale, eps, w_offset):
         ctx.cfg = (G, R, gated), (rot_dim, interleaved, mscale, eps, w_offset)
         ctx.save_for_backward(qkv, qw, kw, freqs, inv_freq, pos, axis)
-        q, k = _C().qk_norm_rope_fwd(qkv, G, R, gated, qw, kw, freqs, inv_freq, pos, axis, *ctx.cfg[1],
-                                     _ext.status_tensor(qkv.device))
-        x = qkv.view(qkv.shape[0], G, 2 * R + 2 if gated else R + 2, q.shape[-1])
-        return (q, k, x[:, :, -1]) + ((x[:, :, R:2 * R],) if gated else ())
+        # q, k and views of the packed rows: v (and the gates)
+        return tuple(_C().qk_norm_rope_fwd(qkv, G, R, gated, qw, kw, freqs, inv_freq, pos, axis, *ctx.cfg[1],
+                                           _ext.status_tensor(qkv.device)))
 
     @staticmethod
     def backward(ctx, *grads):
@@ -412,7 +411,9 @@ def qk_norm_rope(qkv: torch.Tensor, groups: int, q_per_group: int, q_weight: tor
             memory_format=torch.contiguous_format)
 
         def words(t, dt):
-            return None if t is None else t.to(device=dev, dtype=dt).contiguous()
+            if t is None or (t.dtype == dt and t.device == dev and t.is_contiguous()):
+                return t
+            return t.to(device=dev, dtype=dt).contiguous()
 
         qw, kw = (w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
                   for w in (q_weight, k_weight))

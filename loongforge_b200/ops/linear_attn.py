@@ -110,9 +110,9 @@ class _GatedDeltaFn(torch.autograd.Function):
         C, status = _ext.require(), _status(v)
         q, k, v, gf, bf = _rows16(q), _rows16(k), _rows16(v), _fp32(g), _fp32(beta)
         bounds, first = (None, None) if cu is None else C.delta_plan(cu, q.shape[0], status)
-        o, s_out, *kept = C.delta_fwd(q, k, v, gf, bf, bounds, first, scale, l2norm, s_in, want_state, keep, status)
+        o, s_out, kept = C.delta_fwd(q, k, v, gf, bf, bounds, first, scale, l2norm, s_in, want_state, keep, status)
         if keep:
-            ctx.save_for_backward(q, k, v, gf, bf, bounds, first, *kept)
+            ctx.save_for_backward(q, k, v, gf, bf, bounds, first, kept)
             ctx.cfg = (scale, l2norm, g.dtype, beta.dtype)
         if not want_state:
             ctx.mark_non_differentiable(s_out)
@@ -121,11 +121,11 @@ class _GatedDeltaFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do, ds_out):
         scale, l2norm, g_dtype, beta_dtype = ctx.cfg
-        q, k, v, g, beta, bounds, first, *kept = ctx.saved_tensors
+        q, k, v, g, beta, bounds, first, kept = ctx.saved_tensors
         want_ds = ctx.needs_input_grad[5]
         do = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if do is None else _dense16(do)
         dq, dk, dv, dg, dbeta, ds_in = _ext.require().delta_bwd(
-            do, None if ds_out is None else _dense16(ds_out), q, k, v, g, beta, bounds, first, scale, l2norm, want_ds, *kept,
+            do, None if ds_out is None else _dense16(ds_out), q, k, v, g, beta, bounds, first, scale, l2norm, want_ds, kept,
             _status(v))
         return (dq, dk, dv, dg.to(g_dtype), dbeta.to(beta_dtype), ds_in if want_ds else None) + (None,) * 5
 
@@ -212,7 +212,8 @@ def gated_delta_rule(q, k, v, g, beta, *, cu_seqlens=None, scale: Optional[float
 
     On a GPU (bf16, head dims 64 or 128) the chunk is 64 tokens whatever ``chunk`` says. A decay below ``exp(-120)`` counts
     as zero there. With gradients enabled the forward pass keeps, per token and value head, ``12 dv`` bytes of partial
-    results, ``dk dv / 16`` bytes of states and 556 bytes of chunk matrices and factors until the backward pass.
+    results, ``dk dv / 16`` bytes of states and 620 bytes of chunk matrices and factors, and per token and key head
+    ``4 dk + 32`` bytes of tiles, until the backward pass.
     """
     _check_delta(q, k, v, g, beta, "T")
     T, _, dk = q.shape

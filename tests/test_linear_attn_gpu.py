@@ -463,3 +463,87 @@ def test_causal_conv1d_step(B, C, K, bias):
     assert not y[-1].any()
     with pytest.raises(RuntimeError, match="out of range"):
         _ext.check_status()
+
+
+def test_causal_conv1d_far_ends_of_silu():
+    """Sums of tens of thousands either way: silu and its derivative are the sum and one, or zero and zero."""
+    x = torch.tensor([[3e4, -3e4, 90.0, -90.0, 0.0, 1e-30, -1e38, 1e38]], device="cuda").to(BF16).requires_grad_()
+    w = torch.zeros(8, 4, device="cuda", dtype=BF16)
+    w[:, -1] = 1
+    y = LA.causal_conv1d(x, w)
+    d = torch.autograd.grad(y, x, torch.ones_like(y))[0]
+    r = x.detach().double()
+    s = torch.sigmoid(r)
+    for a, b in ((y, r * s), (d, s + r * s * (1 - s))):
+        assert ((a.double() - b).abs() <= b.abs() * 2.0 ** -8 + 2.0 ** -40).all(), (a, b)
+
+
+def test_single_tokens_captured_and_on_a_side_stream():
+    """Convolution and memory of one token as a decoder captures them: slots and inputs change between replays."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    B, hk, hv, dk, dv, S, K = 3, 1, 2, 128, 128, 6, 4
+    C = 2 * hk * dk + hv * dv
+    x, w = randn(gen, B, C, dtype=BF16), randn(gen, C, K, dtype=BF16)
+    g, beta = -torch.rand(B, hv, generator=gen, device="cuda"), torch.rand(B, hv, generator=gen, device="cuda")
+    win0, mem0 = randn(gen, S, C, K - 1, dtype=BF16), randn(gen, S, hv, dk, dv)
+    slots = torch.tensor([4, 0, 2], device="cuda", dtype=torch.int32)
+
+    def token(win, mem):
+        y = LA.causal_conv1d_step(x, win, w, state_indices=slots)
+        q, k, v = y.split([hk * dk, hk * dk, hv * dv], -1)
+        return LA.gated_delta_rule_step(q.view(B, hk, dk), k.view(B, hk, dk), v.view(B, hv, dv), g, beta, mem, state_indices=slots)
+
+    with torch.no_grad():
+        win, mem = win0.clone(), mem0.clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            token(win, mem)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o = token(win, mem)
+        win.copy_(win0)
+        mem.copy_(mem0)
+        rwin, rmem = win0.clone(), mem0.clone()
+        for step in range(3):
+            x.copy_(randn(gen, B, C, dtype=BF16))
+            slots.copy_(torch.tensor([[4, 0, 2], [1, -1, 5], [4, 3, 0]][step], dtype=torch.int32))
+            graph.replay()
+            torch.cuda.synchronize()
+            want = token(rwin, rmem)
+            assert torch.equal(o, want) and torch.equal(win, rwin) and torch.equal(mem, rmem)
+    _ext.check_status()
+
+
+def test_no_rows_of_single_tokens():
+    mem, win = torch.randn(2, 2, 64, 64, device="cuda"), torch.randn(2, 64, 3, device="cuda").to(BF16)
+    m0, w0 = mem.clone(), win.clone()
+    e = torch.empty(0, 2, 64, device="cuda", dtype=BF16)
+    gates = torch.empty(0, 2, device="cuda")
+    with torch.no_grad():
+        assert LA.gated_delta_rule_step(e, e, e, gates, gates, mem).shape == (0, 2, 64)
+        assert LA.causal_conv1d_step(e.view(0, 128)[:, :64], win, torch.zeros(64, 4, device="cuda", dtype=BF16)).shape == (0, 64)
+    assert torch.equal(mem, m0) and torch.equal(win, w0)
+
+
+def test_two_training_calls_at_once_on_two_streams():
+    """Neither call's workspace is the other's."""
+    sets = [make([700, 33], 2, 4, 128, 128, seed) for seed in (1, 2)]
+
+    def run(s):
+        q, k, v, g, beta, do, cu = s
+        ins = [t.detach().requires_grad_() for t in (q, k, v, g, beta)]
+        o = LA.gated_delta_rule(*ins, cu_seqlens=cu)
+        return [o.detach(), *torch.autograd.grad(o, ins, do)]
+
+    want = [run(s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for st, s in zip(streams, sets):
+        with torch.cuda.stream(st):
+            got.append(run(s))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -138,3 +138,70 @@ def test_qk_norm_rope_matches_the_separate_passes_on_attention():
     assert (q.float() - q2.float()).abs().max() <= 3 * 2.0 ** -8 * q.float().abs().max()
     a, b = OF.attention(q, k, v), OF.attention(q2, k2, x[:, :, R + 1])
     assert (a.float() - b.float()).norm() / b.float().norm() < 0.03
+
+
+@pytest.mark.parametrize("T,G,R,D,rot,kw", [(1500, 1, 1, 64, 64, {}), (2100, 4, 4, 64, 16, dict(gated=True)), (701, 2, 16, 64, 24, {}),
+                                            (1201, 1, 8, 256, 8, dict(interleaved=True)), (3, 8, 3, 128, 40, dict(interleaved=True)),
+                                            (2500, 3, 2, 128, 128, dict(interleaved=True, axes=2))])
+def test_qk_norm_rope_layouts(T, G, R, D, rot, kw):
+    """Many tokens and few, one head of a kind and many: a lane keeps from one to eight heads of its token."""
+    check(T, G, R, D, rot, **kw)
+
+
+def test_qk_norm_rope_values_and_gates_keep_to_themselves():
+    """NaN in the value and gate heads, and in one query head, reaches no other head; their gradients go straight through."""
+    torch.manual_seed(3)
+    T, G, R, D = 9, 2, 3, 128
+    w = torch.randn(D, device="cuda").to(BF16)
+    freqs = torch.rand(T, D // 2, device="cuda")
+    clean = torch.randn(T, G, 2 * R + 2, D, device="cuda").to(BF16)
+    sick = clean.clone()
+    sick[:, :, R:2 * R] = sick[:, :, -1] = float("nan")
+    sick[4, 1, 0, 5] = float("inf")
+    xs = [t.view(T, -1).requires_grad_() for t in (clean, sick)]
+    a, b = (OF.qk_norm_rope(x, G, R, w, w, freqs=freqs, gated=True) for x in xs)
+    ups = [torch.randn_like(t) for t in a]
+    da, db = (torch.autograd.grad(o, x, ups)[0].view(T, G, 2 * R + 2, D) for o, x in zip((a, b), xs))
+    there = torch.ones(T, G * R, dtype=torch.bool, device="cuda")
+    there[4, R] = False
+    assert torch.equal(a[0][there], b[0][there]) and torch.equal(a[1], b[1])
+    keep = torch.ones(T, G, 2 * R + 2, dtype=torch.bool, device="cuda")
+    keep[4, 1, 0] = False
+    assert torch.equal(da[keep], db[keep]) and torch.equal(db[:, :, R:2 * R], ups[3]) and torch.equal(db[:, :, -1], ups[2])
+
+
+def test_qk_norm_rope_upstream_layouts_streams_and_replay():
+    torch.manual_seed(4)
+    T, G, R, D = 300, 2, 4, 128
+    qkv = torch.randn(T, G * (R + 2) * D, device="cuda").to(BF16)
+    w = torch.randn(D, device="cuda").to(BF16)
+    inv, pos = torch.rand(D // 2, device="cuda"), torch.arange(T, device="cuda", dtype=torch.int32)
+    ups = [torch.randn(G * R, T, D, device="cuda").to(BF16).transpose(0, 1), torch.randn(1, 1, D, device="cuda").to(BF16).expand(T, G, D),
+           torch.randn(T, G, 2 * D, device="cuda").to(BF16)[..., :D]]
+
+    def run(x, qw, kw, up):
+        out = OF.qk_norm_rope(x, G, R, qw, kw, inv_freq=inv, pos_ids=pos)
+        return [*(t.detach().clone() for t in out), *torch.autograd.grad(out, (x, qw, kw), up)]
+
+    def leaves():
+        return [t.detach().clone().requires_grad_() for t in (qkv, w, w)]
+
+    want = run(*leaves(), [u.contiguous() for u in ups])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run(*leaves(), ups)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ins = leaves()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = run(*ins, ups)
+    with torch.no_grad():
+        qkv.copy_(qkv.flip(0))
+        ins[0].copy_(qkv)
+        pos.add_(17)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = run(*leaves(), ups)
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))

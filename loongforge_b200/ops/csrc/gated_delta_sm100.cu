@@ -198,10 +198,10 @@ __device__ __forceinline__ void load_rows(bf16* dst, int pitch, const bf16* src,
 
 // ---------------------------------------------------------------------------------------------------------- prepare
 
-// 128 KB leave and come for each (chunk, key head) of 128 with two value heads: 70 us at 16384 tokens and 16 key heads,
-// where the kernel takes 132 (2.4 TB/s). What is left is latency between its eight barriers a head; four blocks of four
-// warps share an SM (three took 177, with fp32 joins of the inverse's halves in place of the matrix unit; five spill).
-// Everything leaves by bulk copies: 16 bytes a row from the accumulators' owners cost 60 us more.
+// 147 KB come and leave for each (chunk, key head) of 128 with two value heads: 92 us at 16384 tokens and 16 key heads,
+// where the kernel takes 132 (4.6 TB/s). What is left is latency between the eight barriers of a head; four blocks of four
+// warps share an SM (a fifth spills). The joins of the inverse on the matrix unit: 177 -> 132 us; records that leave by bulk
+// copies instead of from the accumulators' owners, 16 bytes a row: 237 -> 177.
 
 constexpr int PREP_THREADS = 128;
 // fp32 pitches of the 64 x 64 matrices: A's is read down its columns as well (two rows 8 banks apart), M's along rows

@@ -6,7 +6,7 @@
 // registers across one reduction over dk, and written once. Bound by memory: 8 dk dv bytes per row and head.
 // A block takes COLS of the dv columns of one (row, head): the columns are independent, so few rows are cut into more
 // blocks until the SMs are full.
-// 192 rows of 32 heads of 128 x 128: 210 us, 5.8 TB/s; one row of 32 heads: 4.5 us, which is launch and one trip to memory.
+// 192 rows of 48 heads of 128 x 128: 210 us, 5.8 TB/s; one row of 32 heads: 4.5 us, which is launch and one trip to memory.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -12,11 +12,12 @@
 // half, 16 bytes at a time; 16 neighbours behind the rotated span), so the rotation stays in the lane. A block takes
 // either query heads or key heads, so that norm weight, their gradient and the pairs' factors stay in registers, and lays
 // (token, head) out so that a lane keeps one token, hence its cosines, for up to eight heads. What a lane will work on is
-// copied ahead, over the end of its turn too, into its own places in shared memory, so that nobody waits for anybody. The value (and gate) heads of the packed row are not touched forward; backward copies their
-// gradients into the packed gradient, which is so written in one pass.
+// copied ahead, over the end of its turn too, into its own places in shared memory, so that nobody waits for anybody. The
+// value (and gate) heads of the packed row are not touched forward; backward copies their gradients into the packed
+// gradient, which is so written in one pass.
 // 8192 tokens, 4 x 8 heads of 128: forward 41 us (3.7 TB/s), backward 74 us (3.3 TB/s); 4099 tokens, gated 2 x 16 heads of
-// 256: 36 us (4.0 TB/s), backward 78 us (4.6 TB/s). Both issue every second cycle; what is left is the two barriers' worth of
-// waiting for the angles at each turn and the uneven last turn.
+// 256: 36 us (4.0 TB/s), backward 78 us (4.6 TB/s). Both issue every second cycle; what is left is the wait for the
+// angles at each turn and the uneven last turn.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -98,7 +98,7 @@ class RotaryEmbedding:
                 start += n
             mixed = torch.cat(parts, dim=-1)
         out = RotaryInputs(freqs=mixed.contiguous(), mscale=mscale)
-        if stream.numel() == inv.numel():
+        if stream.numel() == inv.numel() and not position_ids.is_floating_point():
             out.axis_pos, out.inv_freq = position_ids.to(torch.int32).contiguous(), inv.float().contiguous()
             if getattr(self, "_axis", None) is None or self._axis.device != inv.device:
                 self._axis = stream.to(device=inv.device, dtype=torch.int32)

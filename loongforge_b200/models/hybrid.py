@@ -194,16 +194,20 @@ class GatedDeltaNet(nn.Module):
     @torch.no_grad()
     def prefill(self, x, cache, slots, *, cu_seqlens=None, residual=None):
         """`forward` over new sequences, one per entry of `slots` (bounds in `cu_seqlens`; None = one sequence); leaves
-        their windows and states in those slots of `cache`."""
+        their windows and states in those slots of `cache`. The slots are read on the host: they must differ and exist."""
         self._check_decoding()
         windows, states = cache
+        slots = [int(i) for i in (slots.tolist() if torch.is_tensor(slots) else slots)]
+        n = 1 if cu_seqlens is None else len(cu_seqlens) - 1
+        if len(slots) != n:
+            raise ValueError(f"{n} sequences need as many slots, got {len(slots)}")
+        if len(set(slots)) < n or any(i < 0 or i >= states.shape[0] for i in slots):
+            raise ValueError(f"slots must be {n} different ones of the cache's {states.shape[0]}, got {slots[:8]}")
         mixed, z, b, a = self._project(x)
         y = LA.causal_conv1d(mixed, self.conv_weight, cu_seqlens=cu_seqlens, activation="silu")
         o, last = LA.gated_delta_rule(*self._heads(y), *self._gates(b, a), cu_seqlens=cu_seqlens, qk_l2norm=True,
                                       output_final_state=True)
-        slots = torch.as_tensor(slots, dtype=torch.long, device=x.device)
-        if slots.numel() != last.shape[0]:
-            raise ValueError(f"{last.shape[0]} sequences need as many slots, got {slots.numel()}")
+        slots = torch.tensor(slots, dtype=torch.long, device=x.device)
         cu = torch.tensor([0, mixed.shape[0]]) if cu_seqlens is None else torch.as_tensor(cu_seqlens)
         cu = cu.to(device=x.device, dtype=torch.long)
         at = cu[1:, None] - torch.arange(self.K - 1, 0, -1, device=x.device)  # the last K - 1 tokens, oldest first

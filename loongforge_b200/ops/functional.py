@@ -392,6 +392,8 @@ def qk_norm_rope(qkv: torch.Tensor, groups: int, q_per_group: int, q_weight: tor
         raise ValueError(f"qk_norm_rope: rot_dim {rot} of head dim {D}")
     if q_weight.shape != (D,) or k_weight.shape != (D,):
         raise ValueError(f"qk_norm_rope: norm weights must be [{D}]")
+    if any(t is not None and t.is_floating_point() for t in (pos_ids, axis)):
+        raise ValueError("qk_norm_rope: pos_ids and axis hold whole numbers")
     table = freqs if freqs is not None else inv_freq
     if table.shape[-1] != rot // 2 or table.dim() != (2 if freqs is not None else 1):
         raise ValueError(f"qk_norm_rope: {tuple(table.shape)} does not hold {rot // 2} angles per position")
@@ -413,6 +415,8 @@ def qk_norm_rope(qkv: torch.Tensor, groups: int, q_per_group: int, q_weight: tor
         def words(t, dt):
             if t is None or (t.dtype == dt and t.device == dev and t.is_contiguous()):
                 return t
+            if t.dtype == torch.int64:  # a row that does not fit stays out of range instead of wrapping into it
+                t = t.clamp(-2 ** 31, 2 ** 31 - 1)
             return t.to(device=dev, dtype=dt).contiguous()
 
         qw, kw = (w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)

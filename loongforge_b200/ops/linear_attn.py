@@ -186,9 +186,16 @@ def _host_bounds(cu_seqlens, T: int) -> list:
     return b
 
 
+def _int32(t: torch.Tensor, device) -> torch.Tensor:
+    """Numbers as int32 on `device`; one that does not fit stays out of range instead of wrapping into it."""
+    if t.dtype == torch.int64:
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
 def _device_bounds(cu_seqlens, T: int, device) -> Optional[torch.Tensor]:
     """Sequence boundaries as int32 on `device`. Boundaries that are on the host are checked here; those on the device
-    are clamped by the kernels, which report a bad one through the status word."""
+    are clamped by the kernels (the delta rule also reports a bad one through the status word)."""
     if cu_seqlens is None:
         return None
     if not torch.is_tensor(cu_seqlens) or not cu_seqlens.is_cuda:
@@ -197,7 +204,7 @@ def _device_bounds(cu_seqlens, T: int, device) -> Optional[torch.Tensor]:
         raise ValueError("cu_seqlens must hold at least two offsets")
     if cu_seqlens.dtype == torch.int32 and cu_seqlens.device == device and cu_seqlens.is_contiguous():
         return cu_seqlens
-    return cu_seqlens.to(device=device, dtype=torch.int32).contiguous()
+    return _int32(cu_seqlens, device)
 
 
 def gated_delta_rule(q, k, v, g, beta, *, cu_seqlens=None, scale: Optional[float] = None, qk_l2norm: bool = True,
@@ -274,7 +281,7 @@ def _step_index(state_indices, rows: int, slots: int, device) -> Optional[torch.
         raise ValueError(f"state_indices must hold one slot for each of the {rows} rows")
     if state_indices.dtype == torch.int32 and state_indices.device == device and state_indices.is_contiguous():
         return state_indices
-    return state_indices.to(device=device, dtype=torch.int32).contiguous()
+    return _int32(state_indices, device)
 
 
 def _no_gradient(*tensors):

@@ -53,6 +53,24 @@ def test_prefill_refuses_a_wrong_number_of_slots():
         net.prefill(torch.randn(8, cfg.hidden_size), net.new_cache(4), [0], cu_seqlens=[0, 3, 8])
 
 
+@pytest.mark.parametrize("slots", [[0, 0], [0, 4], [-1, 2], torch.tensor([1, 7])])
+def test_prefill_refuses_slots_that_are_taken_twice_or_not_there(slots):
+    cfg, net = layer()
+    cache = net.new_cache(4)
+    with pytest.raises(ValueError, match="slots"):
+        net.prefill(torch.randn(8, cfg.hidden_size), cache, slots, cu_seqlens=[0, 3, 8])
+    assert not cache[0].any() and not cache[1].any()
+
+
+def test_positions_that_are_not_whole_numbers_keep_to_the_angle_table():
+    from loongforge_b200.models.gpt import RotaryEmbedding
+    from loongforge_b200.models.registry import get_model_config
+
+    cfg = get_model_config("tiny-qwen3-next", position_embedding_type="mrope", mrope_section=[3, 3, 2], mrope_interleaved=True)
+    r = RotaryEmbedding(cfg, 16).mrope(torch.rand(3, 20) * 9)
+    assert r.axis_pos is None and r.freqs.shape == (20, 8)
+
+
 def test_gated_attention_and_mrope_inputs_agree_on_the_angles():
     """The several-axis form of the rotary inputs names the same angles as the table beside it."""
     from loongforge_b200.models.gpt import RotaryEmbedding

@@ -547,3 +547,26 @@ def test_two_training_calls_at_once_on_two_streams():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_wide_indices_do_not_wrap_into_range():
+    """2^32 is no slot, no boundary and no row of a table, although its low 32 bits are zero."""
+    from loongforge_b200.ops import functional as OF
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    mem = randn(gen, 2, 1, 64, 64)
+    m0 = mem.clone()
+    x = randn(gen, 1, 1, 64, dtype=BF16)
+    gate = torch.zeros(1, 1, device="cuda")
+    far = torch.tensor([2 ** 32], device="cuda")
+    with torch.no_grad():
+        o = LA.gated_delta_rule_step(x, x, x, gate, gate + 1, mem, state_indices=far)
+    assert not o.any() and torch.equal(mem, m0)
+    with pytest.raises(RuntimeError, match="out of range"):
+        _ext.check_status()
+    xs = randn(gen, 10, 64, dtype=BF16)
+    y = LA.causal_conv1d(xs, randn(gen, 64, 4, dtype=BF16), cu_seqlens=torch.tensor([0, 2 ** 32 + 4], device="cuda"))
+    assert y[4:].any()  # clamped to the ten rows
+    OF.qk_norm_rope(randn(gen, 1, 192, dtype=BF16), 1, 1, *(torch.ones(64, device="cuda", dtype=BF16),) * 2,
+                    freqs=torch.rand(4, 32, device="cuda"), pos_ids=far)
+    with pytest.raises(RuntimeError, match="out of range"):
+        _ext.check_status()

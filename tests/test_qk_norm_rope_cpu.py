@@ -95,6 +95,7 @@ def test_refusals():
         (dict(inv_freq=inv, pos_ids=pos[:3]), "pos_ids"), (dict(inv_freq=inv, pos_ids=pos.expand(2, T)), "axis"),
         (dict(inv_freq=inv, pos_ids=pos, axis=torch.zeros(3, dtype=torch.int32)), "axis"),
         (dict(freqs=f[:3]), "cover"), (dict(freqs=f, pos_ids=pos[:3]), "cover"), (dict(freqs=f[:, :4]), "angles"),
+        (dict(inv_freq=inv, pos_ids=pos + 0.5), "whole"), (dict(inv_freq=inv, pos_ids=pos, axis=torch.zeros(D // 2)), "whole"),
         (dict(freqs=f, rot_dim=7), "rot_dim"), (dict(freqs=f, rot_dim=32), "rot_dim"), (dict(freqs=f, gated=True), "heads"),
     ]
     for kw, what in bad:

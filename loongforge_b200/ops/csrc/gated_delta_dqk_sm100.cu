@@ -142,6 +142,7 @@ tc_dqk_kernel(const DeltaArgs a) {
       float acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+      float norm = 1.f;
       for (int hr = 0; hr < rep; ++hr, ++u) {
         const float* vec = sm.vec[u & 1];
         // W_ij = qs_i rk_j D_ij (dO U^T)_ij for i >= j, N_ij = -rk_i rk_j D_ij (dV U^T)_ij for i > j
@@ -186,18 +187,18 @@ tc_dqk_kernel(const DeltaArgs a) {
         fence_proxy_async_smem();
         tc_fence_before_sync();
         bar_arrive(&sm.w_ready);
-        // the rows, scaled
+        // the rows, scaled; D1 and D2 while D4 is under way
         const float f1 = key ? -vec[V_YK * 64 + tok] : vec[V_OQ * 64 + tok], f2 = vec[V_SU * 64 + tok];
-        bar_wait(&sm.d4_done, u & 1, a.status);
+        norm = vec[(key ? V_RK : V_RQ) * 64 + tok];
+        bar_wait(&sm.tiles_free, u & 1, a.status);
         tc_fence_after_sync();
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          uint32_t x[16], y[16];
+          uint32_t x[16];
           tmem_ld_32x32b_x16(lanes + T_D1 + 64 * half + 16 * b, x);
-          tmem_ld_32x32b_x16(lanes + T_D4 + 64 * half + 16 * b, y);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) acc[16 * b + j] += f1 * __uint_as_float(x[j]) + __uint_as_float(y[j]);
+          for (int j = 0; j < 16; ++j) acc[16 * b + j] += f1 * __uint_as_float(x[j]);
           if (key) {  // a whole warp or none of it
             tmem_ld_32x32b_x16(lanes + T_D2 + 64 * half + 16 * b, x);
             tmem_ld_wait();
@@ -206,7 +207,17 @@ tc_dqk_kernel(const DeltaArgs a) {
           }
         }
         tc_fence_before_sync();
-        if (hr + 1 < rep) bar_arrive(&sm.acc_free);
+        bar_arrive(&sm.acc_free);  // now the next head's vec may replace this one's, and the next products these
+        bar_wait(&sm.d4_done, u & 1, a.status);
+        tc_fence_after_sync();
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          uint32_t x[16];
+          tmem_ld_32x32b_x16(lanes + T_D4 + 64 * half + 16 * b, x);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[16 * b + j] += __uint_as_float(x[j]);
+        }
       }
       // The rows are r dq^ and r dk^ with r = 1 / norm, so that dq = r dq^ - q r^2 (q . r dq^), the same for k.
       const unsigned char* tile = key ? sm.k : sm.q;
@@ -225,12 +236,9 @@ tc_dqk_kernel(const DeltaArgs a) {
         }
         sm.dots[half][r] = d;
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const float norm = sm.vec[(u - 1) & 1][(key ? V_RK : V_RQ) * 64 + tok];
         f = (sm.dots[0][r] + sm.dots[1][r]) * norm * norm;
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
-      // now the next head's vec may replace this one's, and the next products these
-      bar_arrive(&sm.acc_free);
       // through w's place, which only these warps write, to whole rows
 #pragma unroll
       for (int j = 0; j < 8; ++j) {

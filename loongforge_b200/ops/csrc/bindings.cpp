@@ -1073,14 +1073,6 @@ std::vector<at::Tensor> delta_fwd(const at::Tensor& q, const at::Tensor& k, cons
   const int rc = lf::delta_forward(a, cur_stream());
   TORCH_CHECK(rc == 0, "lf::delta_forward failed with code ", rc, " (dk = ", a.dk, ", dv = ", a.dv, ")");
   g_launches += a.NC > 0 ? 2 : 1;
-  if (a.cu) {
-    lf::ZeroRows z;
-    z.n = 1;
-    z.p[0] = a.o;
-    z.row_bytes[0] = 2LL * a.Hv * a.dv;
-    lf::delta_zero_uncovered(z, a.cu, a.N, a.T, cur_stream());
-    ++g_launches;
-  }
   return {o, s_out, work};
 }
 
@@ -1123,18 +1115,6 @@ std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tens
   const int rc = lf::delta_backward(a, cur_stream());
   TORCH_CHECK(rc == 0, "lf::delta_backward failed with code ", rc, " (dk = ", a.dk, ", dv = ", a.dv, ")");
   g_launches += a.NC > 0 ? 3 : 1;
-  if (a.cu) {
-    lf::ZeroRows z;
-    z.n = 5;
-    void* p[5] = {a.dq, a.dkey, a.dv_, a.dg, a.dbeta};
-    const long long b[5] = {2LL * a.Hk * a.dk, 2LL * a.Hk * a.dk, 2LL * a.Hv * a.dv, 4LL * a.Hv, 4LL * a.Hv};
-    for (int i = 0; i < 5; ++i) {
-      z.p[i] = p[i];
-      z.row_bytes[i] = b[i];
-    }
-    lf::delta_zero_uncovered(z, a.cu, a.N, a.T, cur_stream());
-    ++g_launches;
-  }
   return {dq, dk, dv, dg, dbeta, ds_in};
 }
 

@@ -172,16 +172,14 @@ __global__ void plan_kernel(const int* __restrict__ in, int N, long long T, int*
   }
 }
 
-__global__ void zero_rows_kernel(const ZeroRows z, const int* __restrict__ cu, int N, long long T) {
-  const long long first = cu[0], last = cu[N], rows = first + T - last;
-  if (rows <= 0) return;
-  for (int i = 0; i < z.n; ++i) {
-    const long long words = z.row_bytes[i] / 4;
-    uint32_t* p = static_cast<uint32_t*>(z.p[i]);
-    for (long long w = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; w < rows * words; w += static_cast<long long>(gridDim.x) * blockDim.x) {
-      const long long r = w / words;
-      p[(r < first ? r : last + (r - first)) * words + w % words] = 0u;
-    }
+// Zeroes the rows that no sequence covers, [0, cu[0]) and [cu[N], T), of a row-major buffer. The kernels that run anyway do
+// it with their first blocks: a launch of its own costs a small call as much as its largest kernel.
+constexpr int ZERO_BLOCKS = 148;
+__device__ __forceinline__ void zero_rows(const DeltaArgs& a, long long first, long long last, void* buffer, long long words) {
+  const long long n = (first + a.T - last) * words, step = static_cast<long long>(gridDim.x < ZERO_BLOCKS ? gridDim.x : ZERO_BLOCKS) * blockDim.x;
+  for (long long w = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; w < n; w += step) {
+    const long long r = w / words;
+    static_cast<uint32_t*>(buffer)[(r < first ? r : last + (r - first)) * words + w % words] = 0u;
   }
 }
 
@@ -314,6 +312,7 @@ prepare_kernel(const DeltaArgs a) {
   const long long c = blockIdx.x / a.Hk;
   const int hk = blockIdx.x % a.Hk;
   const Span sp = chunk_span(a, c);
+  if (a.cu && blockIdx.x < ZERO_BLOCKS) zero_rows(a, a.cu[0], a.cu[a.N], a.o, a.Hv * a.dv / 2);
   if (sp.len == 0) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t2 = (lane & 3) * 2;
   load_rows<DK, PREP_THREADS>(qs, P, static_cast<const bf16*>(a.q) + sp.start * a.q_ts + hk * a.q_hs, a.q_ts, sp.len);
@@ -1476,6 +1475,14 @@ dqk_kernel(const DeltaArgs a) {
 constexpr int GATE_WARPS = 4;
 __global__ void __launch_bounds__(GATE_WARPS * 32)
 gates_kernel(const DeltaArgs a) {
+  if (a.cu && blockIdx.x < ZERO_BLOCKS) {
+    const long long first = a.cu[0], last = a.cu[a.N];
+    zero_rows(a, first, last, a.dq, a.Hk * a.dk / 2);
+    zero_rows(a, first, last, a.dkey, a.Hk * a.dk / 2);
+    zero_rows(a, first, last, a.dv_, a.Hv * a.dv / 2);
+    zero_rows(a, first, last, a.dg, a.Hv);
+    zero_rows(a, first, last, a.dbeta, a.Hv);
+  }
   const unsigned pair = blockIdx.x * GATE_WARPS + (threadIdx.x >> 5);  // at most 2^31 of them
   const int c = static_cast<int>(pair / static_cast<unsigned>(a.Hv)), h = static_cast<int>(pair - c * static_cast<unsigned>(a.Hv));
   const long long rec = pair;
@@ -1578,10 +1585,6 @@ bool covered(const DeltaArgs& a) {
 int delta_plan(const int* cu_in, int N, long long T, int* cu, int* cbase, int* status, cudaStream_t s) {
   plan_kernel<<<1, 1024, 0, s>>>(cu_in, N, T, cu, cbase, status);
   return cudaGetLastError() == cudaSuccess ? 0 : -3;
-}
-
-void delta_zero_uncovered(const ZeroRows& z, const int* cu, int N, long long T, cudaStream_t s) {
-  zero_rows_kernel<<<148, 256, 0, s>>>(z, cu, N, T);
 }
 
 int delta_forward(const DeltaArgs& a, cudaStream_t s) {

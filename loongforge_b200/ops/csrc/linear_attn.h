@@ -47,14 +47,6 @@ int delta_plan(const int* cu_in, int N, long long T, int* cu, int* cbase, int* s
 int delta_forward(const DeltaArgs& a, cudaStream_t s);
 int delta_backward(const DeltaArgs& a, cudaStream_t s);
 int delta_tc_dqk(const DeltaArgs& a, cudaStream_t s);  // its dq / dk for dk = dv = 128 (gated_delta_dqk_sm100.cu)
-// Zeroes the rows [0, cu[0]) and [cu[N], T) of up to six row-major buffers.
-struct ZeroRows {
-  void* p[6] = {};
-  long long row_bytes[6] = {};
-  int n = 0;
-};
-void delta_zero_uncovered(const ZeroRows& z, const int* cu, int N, long long T, cudaStream_t s);
-
 struct DeltaStepArgs {
   const void *q = nullptr, *k = nullptr, *v = nullptr;  // bf16 [B, Hk, dk], [B, Hk, dk], [B, Hv, dv]
   long long q_ts = 0, q_hs = 0, k_ts = 0, k_hs = 0, v_ts = 0, v_hs = 0;

@@ -13,12 +13,12 @@
 // D4 a tile of zeros lies there.
 //
 // 112 KB a (chunk, value head) come in, of which 64 KB are the two states: 141 us at 16384 tokens and 32 heads, where the
-// kernel takes 386 (101 at 4096; the mma.sync kernel of the smaller head dims took 697 and 175). One block per SM goes
+// kernel takes 364 (97 at 4096; the mma.sync kernel of the smaller head dims took 697 and 175). One block per SM goes
 // through its share of (chunk, key head) pairs; seven warps bring tiles (fragments of registers, turned by stmatrix on the
 // way), one thread issues the products, eight warps make W and N, and add up rows over the value heads of a key head. The
-// tiles fill shared memory, so a unit's loads begin when its predecessor's products are done: what bounds it is that round,
-// 3K cycles of loads, 1.5K of products, 2.5K for W and N and 1.8K for the last product, of which the last two overlap the
-// next unit's loads.
+// tiles fill shared memory, so a unit's loads begin when its predecessor's products are done: what bounds it are that
+// round (4K cycles of loads, 3.5K until the state products are done) and the eight warps' (2.6K for W and N, 3.5K to read the
+// products, 6K to put out two heads' rows), which run against each other at 12K cycles a unit.
 #include <atomic>
 #include "gated_delta.cuh"
 #include "sm100_ptx.cuh"

@@ -43,7 +43,7 @@
 // The chain is bound by latency: three dependent products of at most 64 x 128 x 16 per chunk, with a hand-over between
 // them, 5.8K cycles a chunk forward and 7K backward. mma.sync runs at a quarter of tcgen05's rate, but operands and results
 // stay in registers, and 32 heads make 1024 warps of such work. One sequence of 4096 tokens with 32 heads of 128 x 128 (five
-// sequences of 16384): prepare 39 us (132), forward 190 (660), backward 238 (826), dqk 101 (386), gates 8 (16). Measured
+// sequences of 16384): prepare 38 us (131), forward 190 (660), backward 238 (826), dqk 97 (364), gates 8 (16). Measured
 // against it: a whole unit in one warp 471 (959) forward and 620 (1278) backward; eight warps along the chain and eight
 // beside it 208 (713) and 257 (874), bound by shared memory; a head as one 128-column product on tcgen05 11.7K cycles a
 // chunk, 5K of them the work on elements between the products, on an eighth as many blocks.

@@ -10,7 +10,7 @@ Per head, with state ``S [dk, dv]``, decay ``a_t = exp(g_t)`` and write strength
 ``gated_delta_rule_recurrent`` is that recurrence literally (the oracle); ``gated_delta_rule`` is the
 chunk-parallel form (WY representation inside a chunk, one state update per chunk), forward and backward, and
 ``gated_delta_rule_step`` advances a pool of states by one token per row (decoding). ``causal_conv1d`` /
-``causal_conv1d_step`` are the same pair for the convolution. The reference calls the ``fla`` Triton kernels for this
+``causal_conv1d_step`` are the same pair for the convolution. The reference calls library kernels here
 (loongforge/models/foundation/qwen3_next/gated_deltanet.py:49-52,354).
 
 On a GPU bf16 inputs run on the kernels of ``csrc/gated_delta_sm100.cu``, ``csrc/gated_delta_step.cu`` and

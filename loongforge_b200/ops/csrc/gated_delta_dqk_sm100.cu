@@ -3,22 +3,25 @@
 // One (chunk, value head) is five products with 128 rows and 128 columns in TMEM. Tokens are rows, 0-63 for dq and
 // 64-127 for dk (or for what leads there):
 //
-//   D3 = [dO; dV] [U_hi; U_lo]^T                    -> W = lower(dO U^T) D and N = -strict_lower(dV U^T) D, in two parts each
-//   D1 = [dO; dV] S0^T                              -> dq += e^G (.), dk -= e^G (.)
-//   D2 = [  ; U_hi] dS1^T + [  ; U_lo] dS1^T        -> dk += e^{G_C - G} (.)
+//   D3 = [dO; dV] [U; u]^T + [0; v] [U; u]^T        -> W = lower(dO U^T) D and N = -strict_lower(dV U^T) D, in two parts each
+//   D1 = [dO; dV] (S0 + s0)^T + [0; v] S0^T         -> dq += e^G (.), dk -= e^G (.)
+//   D2 = [  ; U] (dS1 + ds1)^T + [  ; u] dS1^T      -> dk += e^{G_C - G} (.)
 //   D4 = [W; N] K + [0; W^T] Q + [0; N^T] K         -> dq += , dk +=
 //
-// Rows are scaled when the accumulators are read, so that every operand is a bf16 tile as it lies in memory. An operand
-// tile whose first 64 rows are not wanted starts 64 rows early: what lies there ends in rows of D2 that nobody reads; for
-// D4 a tile of zeros lies there.
+// with capitals for the bf16 high parts and v, u, s0, ds1 for what they leave of dV, U and the states; products of two such
+// remainders are left out (2^-18 of the term). Rows are scaled when the accumulators are read, so that every operand is a
+// bf16 tile as it lies in memory. An operand tile whose first 64 rows are not wanted starts 64 rows early: what lies there
+// ends in rows of D2 that nobody reads; where they have to be zeros, v, W and N lie columns first, so that their first 64
+// rows can come from a tile of zeros elsewhere.
 //
-// 112 KB a (chunk, value head) come in, of which 64 KB are the two states: 141 us at 16384 tokens and 32 heads, where the
-// kernel takes 364 (97 at 4096; the mma.sync kernel of the smaller head dims took 697 and 175). One block per SM goes
-// through its share of (chunk, key head) pairs; seven warps bring tiles (fragments of registers, turned by stmatrix on the
-// way), one thread issues the products, eight warps make W and N, and add up rows over the value heads of a key head. The
-// tiles fill shared memory, so a unit's loads begin when its predecessor's products are done: what bounds it are that
-// round (4K cycles of loads, 3.5K until the state products are done) and the eight warps' (2.6K for W and N, 3.5K to read the
-// products, 6K to put out two heads' rows), which run against each other at 12K cycles a unit.
+// 208 KB a (chunk, value head) come in, 128 of them the two states in two parts each, and 48 a (chunk, key head): about
+// 290 us at 16384 tokens, 16 key and 32 value heads, where the kernel takes 520 (138 at 4096). With the high parts of S0, dS1
+// and dV alone it took 358 (97), and dq and dk were off by 2.4e-3 where decays are near one, instead of the 1.66e-3 of their
+// rounding. One block per SM goes through its share of (chunk, key head) pairs; seven warps bring tiles (fragments of
+// registers, turned by stmatrix on the way), one thread issues the products, eight warps make W and N, and add up rows over
+// the value heads of a key head. The tiles fill shared memory: a state's low part takes the place of its high part when the
+// products have read that, and a unit's loads begin when its predecessor's products are done. What bounds it are these two
+// rounds of loads, which alternate with the products: 18K cycles a unit.
 #include <atomic>
 #include "gated_delta.cuh"
 #include "sm100_ptx.cuh"
@@ -30,15 +33,16 @@ using namespace delta;
 
 // Warps 0-7 compute, 8-14 load, 15 issues: sixteen warps leave 128 registers a thread, seventeen 96.
 constexpr int D = 128, LOAD_WARPS = 7, LOADERS = 32 * LOAD_WARPS, THREADS = 512;
-constexpr int TILES = 64, MINE = (TILES + LOAD_WARPS - 1) / LOAD_WARPS;  // 16 x 16 fragments of one 128 x 128 operand, and a warp's share
+// 16 x 16 fragments of one 128 x 128 operand, of one 128 x 64, and a warp's shares
+constexpr int TILES = 64, MINE = (TILES + LOAD_WARPS - 1) / LOAD_WARPS, VTILES = 32, VMINE = (VTILES + LOAD_WARPS - 1) / LOAD_WARPS;
 constexpr uint32_t BIG = 128 * 128, BOX = 64 * 128;                    // bytes of a 128 x 64 and a 64 x 64 box
 
 struct Smem {
   unsigned char xo[2 * BIG], xu[2 * BIG], s0[2 * BIG], ds[2 * BIG];  // [dO; dV], [U_hi; U_lo]; [v][dk] of both states
-  unsigned char q[2 * BOX], k[2 * BOX], zero[BOX], w[4 * BOX];       // w: W_hi, N_hi, W_lo, N_lo
+  unsigned char q[2 * BOX], k[2 * BOX], zero[BOX], w[4 * BOX], v[2 * BOX];  // w: W_hi, N_hi, W_lo, N_lo; v: [v][token]
   float vec[2][DELTA_VEC];
   float dots[2][128];
-  uint64_t xos_full, ds_full, qk_full, tiles_free, qk_free, d3_done, w_ready, d4_done, acc_free;
+  uint64_t xos_full, ds_full, s0_free, ds_free, s0_low, ds_low, qk_full, tiles_free, qk_free, d3_done, w_ready, d4_done, acc_free;
   uint32_t tmem;
 };
 enum { T_D1 = 0, T_D2 = 128, T_D3 = 256, T_D4 = 384 };
@@ -61,11 +65,24 @@ __device__ __forceinline__ void mma_km(uint32_t d, uint32_t a, uint32_t abox, ui
   for (int s = 0; s < KS; ++s)
     tc_mma_f16_ss(d, make_smem_desc_sw128(a + (s >> 2) * abox + (s & 3) * 32, 16, 1024), make_smem_desc_sw128(b + s * 2048, bbox, 1024), idesc, more || s > 0);
 }
-// A^T with A [64 rows of K][64 columns] behind 64 columns of zeros.
+// A^T with A [16 KS rows of K][64 columns] behind 64 columns of zeros, of which 64 rows serve for all; added to D.
+template <int KS>
 __device__ __forceinline__ void mma_tm(uint32_t d, uint32_t zero, uint32_t a, uint32_t b, uint32_t bbox) {
   constexpr uint32_t idesc = make_idesc(1, 1, true, true, 128, 128);
 #pragma unroll
-  for (int s = 0; s < 4; ++s) tc_mma_f16_ss(d, make_smem_desc_sw128(zero + s * 2048, a - zero, 1024), make_smem_desc_sw128(b + s * 2048, bbox, 1024), idesc, 1u);
+  for (int s = 0; s < KS; ++s) {
+    const uint32_t z = zero + (s & 3) * 2048;
+    tc_mma_f16_ss(d, make_smem_desc_sw128(z, a + s * 2048 - z, 1024), make_smem_desc_sw128(b + s * 2048, bbox, 1024), idesc, 1u);
+  }
+}
+template <int KS>
+__device__ __forceinline__ void mma_tk(uint32_t d, uint32_t zero, uint32_t a, uint32_t b, uint32_t bbox) {
+  constexpr uint32_t idesc = make_idesc(1, 1, true, false, 128, 128);
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const uint32_t z = zero + (s & 3) * 2048;
+    tc_mma_f16_ss(d, make_smem_desc_sw128(z, a + s * 2048 - z, 1024), make_smem_desc_sw128(b + (s >> 2) * bbox + (s & 3) * 32, 16, 1024), idesc, 1u);
+  }
 }
 
 __device__ __forceinline__ void stsm(uint32_t addr, const uint4& r) {
@@ -111,6 +128,10 @@ tc_dqk_kernel(const DeltaArgs a) {
   if (threadIdx.x == 0) {
     bar_init(&sm.xos_full, LOAD_WARPS);
     bar_init(&sm.ds_full, LOAD_WARPS);
+    bar_init(&sm.s0_free, 1);
+    bar_init(&sm.ds_free, 1);
+    bar_init(&sm.s0_low, LOAD_WARPS);
+    bar_init(&sm.ds_low, LOAD_WARPS);
     bar_init(&sm.qk_full, LOAD_WARPS);
     bar_init(&sm.tiles_free, 1);
     bar_init(&sm.qk_free, 8);
@@ -263,7 +284,7 @@ tc_dqk_kernel(const DeltaArgs a) {
   } else if (warp < 15) {
     const int lw = warp - 8, tid = threadIdx.x - 256;
     const int m = lane >> 3, l8 = lane & 7;
-    const uint32_t xu = smem_addr(sm.xu), s0 = smem_addr(sm.s0), ds = smem_addr(sm.ds);
+    const uint32_t xu = smem_addr(sm.xu), s0 = smem_addr(sm.s0), ds = smem_addr(sm.ds), vl = smem_addr(sm.v);
     for (Item it(a); it.c < a.NC; it.next(a)) {
       const int c = it.c, hk = it.hk;
       const Span sp = chunk_span(a, c);
@@ -271,19 +292,32 @@ tc_dqk_kernel(const DeltaArgs a) {
       for (int hr = 0; hr < rep; ++hr, ++u) {
         const int h = hk * rep + hr;
         const long long rec = static_cast<long long>(c) * a.Hv + h;
-        // U: 8 tiles of columns x 4 of tokens x 2 parts; the states: 8 tiles of columns x 8 of dk, high part
+        // U: 8 tiles of columns x 4 of tokens x 2 parts; v the same of one part; the states: 8 tiles of columns x 2 parts x 8 of dk
         uint4 fu[MINE], fs[MINE];
         const uint4* us = reinterpret_cast<const uint4*>(a.u) + rec * 8 * 256 + lane;
+        const uint4* vs = reinterpret_cast<const uint4*>(a.dv_lo) + rec * 8 * 128 + lane;
         const uint4* ss = reinterpret_cast<const uint4*>(a.states) + rec * 8 * 512 + lane;
-        const uint4* dd = reinterpret_cast<const uint4*>(a.dstates) + rec * 8 * 256 + lane;
+        const uint4* dd = reinterpret_cast<const uint4*>(a.dstates) + rec * 8 * 512 + lane;
+        auto take_state = [&](uint4 (&f)[MINE], const uint4* src, int part) {
+#pragma unroll
+          for (int j = 0; j < MINE; ++j) {
+            const int t = lw + LOAD_WARPS * j;
+            if (t < TILES) f[j] = src[(t >> 3) * 512 + part * 256 + (t & 7) * 32];
+          }
+        };
+        auto put_state = [&](uint32_t dst, const uint4 (&f)[MINE]) {
+#pragma unroll
+          for (int j = 0; j < MINE; ++j) {
+            const int t = lw + LOAD_WARPS * j, v = 16 * (t >> 3) + (m & 1) * 8 + l8, k = 16 * (t & 7) + (m >> 1) * 8;
+            if (t < TILES) stsm(dst + (k >> 6) * BIG + piece_at(v, (k >> 3) & 7), f[j]);
+          }
+        };
 #pragma unroll
         for (int j = 0; j < MINE; ++j) {
-          const int f = lw + LOAD_WARPS * j;
-          if (f < TILES) {
-            fu[j] = us[32 * f];
-            fs[j] = ss[(f >> 3) * 512 + (f & 7) * 32];
-          }
+          const int t = lw + LOAD_WARPS * j;
+          if (t < TILES) fu[j] = us[32 * t];
         }
+        take_state(fs, ss, 0);
         // the last head's products have read the tiles; D1 of it waited until the vec of two heads ago was read
         if (u > 0) bar_wait(&sm.tiles_free, (u - 1) & 1, a.status);
         const long long row = (sp.start * a.Hv + h) * D, stride = static_cast<long long>(a.Hv) * D;
@@ -306,25 +340,25 @@ tc_dqk_kernel(const DeltaArgs a) {
           if (f < TILES) stsm_t(xu + (v >> 6) * BIG + piece_at(t, (v >> 3) & 7), fu[j]);
         }
 #pragma unroll
-        for (int j = 0; j < MINE; ++j) {
-          const int f = lw + LOAD_WARPS * j, v = 16 * (f >> 3) + (m & 1) * 8 + l8, k = 16 * (f & 7) + (m >> 1) * 8;
-          if (f < TILES) stsm(s0 + (k >> 6) * BIG + piece_at(v, (k >> 3) & 7), fs[j]);
+        for (int j = 0; j < VMINE; ++j) {
+          const int t = lw + LOAD_WARPS * j;
+          if (t < VTILES) fu[j] = vs[32 * t];
+        }
+        put_state(s0, fs);
+#pragma unroll
+        for (int j = 0; j < VMINE; ++j) {
+          const int f = lw + LOAD_WARPS * j, v = 16 * (f >> 2) + (m & 1) * 8 + l8;
+          if (f < VTILES) stsm(vl + piece_at(v, 2 * (f & 3) + (m >> 1)), fu[j]);
         }
         cp_wait<0>();
         fence_proxy_async_smem();  // before the loads below: it waits for loads in flight too
         bar_arrive(&sm.xos_full);
-#pragma unroll
-        for (int j = 0; j < MINE; ++j) {
-          const int f = lw + LOAD_WARPS * j;
-          if (f < TILES) fu[j] = dd[32 * f];
-        }
-#pragma unroll
-        for (int j = 0; j < MINE; ++j) {
-          const int f = lw + LOAD_WARPS * j, v = 16 * (f >> 3) + (m & 1) * 8 + l8, k = 16 * (f & 7) + (m >> 1) * 8;
-          if (f < TILES) stsm(ds + (k >> 6) * BIG + piece_at(v, (k >> 3) & 7), fu[j]);
-        }
+        take_state(fu, dd, 0);
+        take_state(fs, ss, 1);
+        put_state(ds, fu);
         fence_proxy_async_smem();
         bar_arrive(&sm.ds_full);
+        take_state(fu, dd, 1);
         if (hr == 0) {
           if (i > 0) bar_wait(&sm.qk_free, (i - 1) & 1, a.status);
           const bf16* qp = static_cast<const bf16*>(a.q) + sp.start * a.q_ts + hk * a.q_hs;
@@ -342,13 +376,22 @@ tc_dqk_kernel(const DeltaArgs a) {
           fence_proxy_async_smem();
           bar_arrive(&sm.qk_full);
         }
+        // the states' low parts, where the high ones have been read
+        bar_wait(&sm.s0_free, u & 1, a.status);
+        put_state(s0, fs);
+        fence_proxy_async_smem();
+        bar_arrive(&sm.s0_low);
+        bar_wait(&sm.ds_free, u & 1, a.status);
+        put_state(ds, fu);
+        fence_proxy_async_smem();
+        bar_arrive(&sm.ds_low);
       }
       ++i;
     }
   } else {
     if (lane == 0) {
       const uint32_t xo = smem_addr(sm.xo), xu = smem_addr(sm.xu), s0 = smem_addr(sm.s0), ds = smem_addr(sm.ds);
-      const uint32_t q = smem_addr(sm.q), k = smem_addr(sm.k), zero = smem_addr(sm.zero), w = smem_addr(sm.w);
+      const uint32_t q = smem_addr(sm.q), k = smem_addr(sm.k), zero = smem_addr(sm.zero), w = smem_addr(sm.w), v = smem_addr(sm.v);
       for (Item it(a); it.c < a.NC; it.next(a)) {
         if (chunk_span(a, it.c).len == 0) continue;
         for (int hr = 0; hr < rep; ++hr, ++u) {
@@ -356,24 +399,34 @@ tc_dqk_kernel(const DeltaArgs a) {
           bar_wait(&sm.xos_full, parity, a.status);
           tc_fence_after_sync();
           mma_kk<8>(tm + T_D3, xo, BIG, xu, BIG, false);  // W of the last head was made before its D4 was issued
+          mma_tk<8>(tm + T_D3, zero, v, xu, BIG);
           tc_commit(&sm.d3_done);
           if (u > 0) bar_wait(&sm.acc_free, (u - 1) & 1, a.status);
           tc_fence_after_sync();
           mma_km<8>(tm + T_D1, xo, BIG, s0, BIG, false);
+          mma_tm<8>(tm + T_D1, zero, v, s0, BIG);
+          tc_commit(&sm.s0_free);
           bar_wait(&sm.ds_full, parity, a.status);
           tc_fence_after_sync();
           mma_km<8>(tm + T_D2, xu - BOX, BIG, ds, BIG, false);
           mma_km<8>(tm + T_D2, xu, BIG, ds, BIG, true);
+          tc_commit(&sm.ds_free);
+          bar_wait(&sm.s0_low, parity, a.status);
+          tc_fence_after_sync();
+          mma_km<8>(tm + T_D1, xo, BIG, s0, BIG, true);
+          bar_wait(&sm.ds_low, parity, a.status);
+          tc_fence_after_sync();
+          mma_km<8>(tm + T_D2, xu - BOX, BIG, ds, BIG, true);
           tc_commit(&sm.tiles_free);
           if (hr == 0) bar_wait(&sm.qk_full, i & 1, a.status);
           bar_wait(&sm.w_ready, parity, a.status);
           tc_fence_after_sync();
           mma_km<4>(tm + T_D4, w, 0, k, BOX, false);
           mma_km<4>(tm + T_D4, w + 2 * BOX, 0, k, BOX, true);
-          mma_tm(tm + T_D4, zero, w, q, BOX);
-          mma_tm(tm + T_D4, zero, w + 2 * BOX, q, BOX);
-          mma_tm(tm + T_D4, zero, w + BOX, k, BOX);
-          mma_tm(tm + T_D4, zero, w + 3 * BOX, k, BOX);
+          mma_tm<4>(tm + T_D4, zero, w, q, BOX);
+          mma_tm<4>(tm + T_D4, zero, w + 2 * BOX, q, BOX);
+          mma_tm<4>(tm + T_D4, zero, w + BOX, k, BOX);
+          mma_tm<4>(tm + T_D4, zero, w + 3 * BOX, k, BOX);
           tc_commit(&sm.d4_done);
         }
         ++i;

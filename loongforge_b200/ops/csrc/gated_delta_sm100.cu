@@ -36,15 +36,15 @@
 //
 // Precision. The state, U, X and all products along the chain carry 16 or more bits: an fp32 operand is cut into a bf16
 // high and low part (relative remainder 2^-18) and multiplied in two passes where the other operand is a bf16 input
-// (q, k, do), in three where both are cut. That keeps states, dg and dbeta at fp32 accuracy. dQ and dK are only needed to
-// bf16: there S0, dS1, dV and N enter with the high part alone (2^-9 relative each, in terms that decay has made small);
-// U and W, whose products can cancel to little when keys are alike, keep both parts.
+// (q, k, do), in three where both are cut, in dQ and dK too: with decays near one the terms of S0 and dS1 are the main ones
+// there. What is left out is 2^-18 of an operand: states, dg and dbeta come out within 2e-6 to 9e-6 (2-norm), where fp32
+// throughout has 2e-7 to 5e-7, and dq and dk as their rounding to bf16 leaves them.
 //
 // The chain is bound by latency: three dependent products of at most 64 x 128 x 16 per chunk, with a hand-over between
-// them, 5.8K cycles a chunk forward and 7K backward. mma.sync runs at a quarter of tcgen05's rate, but operands and results
+// them, 5.8K cycles a chunk forward and 7.5K backward. mma.sync runs at a quarter of tcgen05's rate, but operands and results
 // stay in registers, and 32 heads make 1024 warps of such work. One sequence of 4096 tokens with 32 heads of 128 x 128 (five
-// sequences of 16384): prepare 38 us (131), forward 190 (660), backward 238 (826), dqk 97 (364), gates 8 (16). Measured
-// against it: a whole unit in one warp 471 (959) forward and 620 (1278) backward; eight warps along the chain and eight
+// sequences of 16384): prepare 38 us (131), forward 190 (656), backward 257 (884; 238 and 826 without the low parts
+// that dqk reads), dqk 138 (520), gates 8 (16). Measured against it: a whole unit in one warp 471 (959) forward and 620 (1278) backward; eight warps along the chain and eight
 // beside it 208 (713) and 257 (874), bound by shared memory; a head as one 128-column product on tcgen05 11.7K cycles a
 // chunk, 5K of them the work on elements between the products, on an eighth as many blocks.
 #include "gated_delta.cuh"
@@ -975,21 +975,23 @@ backward_kernel(const DeltaArgs a) {
       bulk_copy(x.vec, a.vec + rec * DELTA_VEC, sizeof(x.vec), &sm.full[i & 1]);
     }
   };
-  // The gradient of the state behind a chunk: for the unit's other warps, and (keep_state, high part) for dqk.
-  uint32_t ph[KW][4];
+  // The gradient of the state behind a chunk: for the unit's other warps, and (keep_state) for dqk.
+  uint32_t ph[KW][4], pl[KW][4];
   auto publish_state = [&]() {
 #pragma unroll
     for (int k = 0; k < KW; ++k) {
-      uint32_t lo[4];
-      split_a(s[2 * k], s[2 * k + 1], ph[k], lo);
-      put(sm.state[unit][KW * w + k], ph[k], lo);
+      split_a(s[2 * k], s[2 * k + 1], ph[k], pl[k]);
+      put(sm.state[unit][KW * w + k], ph[k], pl[k]);
     }
     bar_arrive(&sm.state_ready[unit]);
   };
   auto keep_state = [&](int c) {
-    uint4* df = reinterpret_cast<uint4*>(a.dstates) + (((c0 + c) * a.Hv + h) * VT + vt) * KT * 32 + lane;
+    uint4* df = reinterpret_cast<uint4*>(a.dstates) + (((c0 + c) * a.Hv + h) * VT + vt) * 2 * KT * 32 + lane;
 #pragma unroll
-    for (int k = 0; k < KW; ++k) df[(KW * w + k) * 32] = make_uint4(ph[k][0], ph[k][1], ph[k][2], ph[k][3]);
+    for (int k = 0; k < KW; ++k) {
+      df[(KW * w + k) * 32] = make_uint4(ph[k][0], ph[k][1], ph[k][2], ph[k][3]);
+      df[(KT + KW * w + k) * 32] = make_uint4(pl[k][0], pl[k][1], pl[k][2], pl[k][3]);
+    }
   };
   // What a chunk's warp reads of the forward pass: its part of the state in front, and m, U, past of its tokens.
   struct Kept {
@@ -1208,6 +1210,11 @@ backward_kernel(const DeltaArgs a) {
     if (c > 0) keep_state(c - 1);
     store_tile(sm.out[warp], static_cast<bf16*>(a.dv_) + ((t0 + tok) * a.Hv + h) * a.dv + col0,
                static_cast<long long>(a.Hv) * a.dv, len - tok, u[0], u[1]);
+    {  // what that rounding left of dV, for dqk
+      uint32_t hi[4], lo[4];
+      split_a(u[0], u[1], hi, lo);
+      reinterpret_cast<uint4*>(a.dv_lo)[((rec * VT + vt) * 4 + w) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
     float* rd = a.rowdots + (rec * VT + vt) * 128 + tok + t2;
 #pragma unroll
     for (int q = 0; q < 2; ++q)
@@ -1237,22 +1244,24 @@ backward_kernel(const DeltaArgs a) {
 template <int DK, int DV>
 struct DqkSmem {
   static constexpr int P = DK + 8, VP = DV + 8;
-  bf16 q[C * P], k[C * P], dO[C * VP], dV[C * VP], u[DV * APITCH], ul[DV * APITCH], s0[DV * P], ds[DV * P];
-  bf16 w1[C * APITCH], w1l[C * APITCH], w2[C * APITCH];
+  // names in l: what the rounding to bf16 left
+  bf16 q[C * P], k[C * P], dO[C * VP], dV[C * VP], dVl[DV * APITCH], u[DV * APITCH], ul[DV * APITCH];
+  bf16 s0[DV * P], s0l[DV * P], ds[DV * P], dsl[DV * P];
+  bf16 w1[C * APITCH], w1l[C * APITCH], w2[C * APITCH], w2l[C * APITCH];
   float vec[8 * 64];
   float dots[2][2][C];
 };
 
 constexpr int DQK_THREADS = 256;
 
-// State fragments of all dv / 16 column tiles -> [DV][DK] rows of pitch DK + 8.
+// State fragments of all dv / 16 column tiles, high and low parts -> [DV][DK] rows of pitch DK + 8.
 template <int DK, int DV>
-__device__ __forceinline__ void load_fragments(bf16* dst, const uint4* src, int tile_stride) {
+__device__ __forceinline__ void load_fragments(bf16* hi, bf16* lo, const uint4* src) {
   constexpr int KT = DK / 16, P = DK + 8;
-  for (int i = threadIdx.x; i < DV / 16 * KT * 32; i += DQK_THREADS) {
-    const int lane = i & 31, kk = (i >> 5) % KT, vt = (i >> 5) / KT, g = lane >> 2, t2 = (lane & 3) * 2;
-    const uint4 f = src[static_cast<long long>(vt) * tile_stride + kk * 32 + lane];
-    bf16* p = dst + (vt * 16 + g) * P + kk * 16 + t2;
+  for (int i = threadIdx.x; i < DV / 16 * 2 * KT * 32; i += DQK_THREADS) {
+    const int lane = i & 31, kk = (i >> 5) % KT, part = (i >> 5) / KT & 1, vt = (i >> 5) / (2 * KT), g = lane >> 2, t2 = (lane & 3) * 2;
+    const uint4 f = src[i];
+    bf16* p = (part ? lo : hi) + (vt * 16 + g) * P + kk * 16 + t2;
     *reinterpret_cast<uint32_t*>(p) = f.x;
     *reinterpret_cast<uint32_t*>(p + 8 * P) = f.y;
     *reinterpret_cast<uint32_t*>(p + 8) = f.z;
@@ -1260,13 +1269,14 @@ __device__ __forceinline__ void load_fragments(bf16* dst, const uint4* src, int 
   }
 }
 
-// U^T and its remainder -> [DV][64 tokens] rows of pitch APITCH.
-template <int DV>
-__device__ __forceinline__ void load_u(bf16* hi, bf16* lo, const uint4* src) {
-  for (int i = threadIdx.x; i < DV / 16 * 256; i += DQK_THREADS) {
-    const int lane = i & 31, part = (i >> 5) & 1, w = (i >> 6) & 3, vt = i >> 8, g = lane >> 2, t2 = (lane & 3) * 2;
+// PARTS fragments of every 16 columns and 16 tokens -> [DV][64 tokens] rows of pitch APITCH: U^T and its remainder, or that
+// of dV^T alone.
+template <int DV, int PARTS>
+__device__ __forceinline__ void load_tokens(bf16* first, bf16* second, const uint4* src) {
+  for (int i = threadIdx.x; i < DV / 16 * 4 * PARTS * 32; i += DQK_THREADS) {
+    const int lane = i & 31, part = (i >> 5) % PARTS, w = (i >> 5) / PARTS & 3, vt = (i >> 5) / (4 * PARTS), g = lane >> 2, t2 = (lane & 3) * 2;
     const uint4 f = src[i];
-    bf16* p = (part ? lo : hi) + (vt * 16 + g) * APITCH + w * 16 + t2;
+    bf16* p = (part ? second : first) + (vt * 16 + g) * APITCH + w * 16 + t2;
     *reinterpret_cast<uint32_t*>(p) = f.x;
     *reinterpret_cast<uint32_t*>(p + 8 * APITCH) = f.y;
     *reinterpret_cast<uint32_t*>(p + 8) = f.z;
@@ -1303,9 +1313,10 @@ dqk_kernel(const DeltaArgs a) {
     load_rows<DV, DQK_THREADS>(x.dV, VP, static_cast<const bf16*>(a.dv_) + row, stride, sp.len);
     load_vec<DQK_THREADS>(x.vec, a.vec + rec * DELTA_VEC, 8);
     cp_commit();
-    load_u<DV>(x.u, x.ul, reinterpret_cast<const uint4*>(a.u) + rec * (DV / 16) * 256);
-    load_fragments<DK, DV>(x.s0, reinterpret_cast<const uint4*>(a.states) + rec * (DV / 16) * 2 * KT * 32, 2 * KT * 32);
-    load_fragments<DK, DV>(x.ds, reinterpret_cast<const uint4*>(a.dstates) + rec * (DV / 16) * KT * 32, KT * 32);
+    load_tokens<DV, 2>(x.u, x.ul, reinterpret_cast<const uint4*>(a.u) + rec * (DV / 16) * 256);
+    load_tokens<DV, 1>(x.dVl, nullptr, reinterpret_cast<const uint4*>(a.dv_lo) + rec * (DV / 16) * 128);
+    load_fragments<DK, DV>(x.s0, x.s0l, reinterpret_cast<const uint4*>(a.states) + rec * (DV / 16) * 2 * KT * 32);
+    load_fragments<DK, DV>(x.ds, x.dsl, reinterpret_cast<const uint4*>(a.dstates) + rec * (DV / 16) * 2 * KT * 32);
     cp_wait<0>();
     __syncthreads();
     // dO U^T and dV U^T, 16 x 32 of each per warp, lower part only
@@ -1316,9 +1327,10 @@ dqk_kernel(const DeltaArgs a) {
       for (int e = 0; e < 4; ++e) p[j][e] = nn[j][e] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < DV / 16; ++kk) {
-      uint32_t fo[4], fv[4], b[4], bl[4];
+      uint32_t fo[4], fv[4], fvl[4], b[4], bl[4];
       a_from_mk(fo, x.dO, VP, wm * 16, kk * 16);
       a_from_mk(fv, x.dV, VP, wm * 16, kk * 16);
+      a_from_km(fvl, x.dVl, APITCH, kk * 16, wm * 16);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (wn * 2 + j > wm) continue;
@@ -1330,6 +1342,10 @@ dqk_kernel(const DeltaArgs a) {
         b_from_kn(bl, x.ul, APITCH, kk * 16, wn * 32 + j * 16);
         mma(p[2 * j], fo, bl[0], bl[1]);
         mma(p[2 * j + 1], fo, bl[2], bl[3]);
+        mma(nn[2 * j], fv, bl[0], bl[1]);
+        mma(nn[2 * j + 1], fv, bl[2], bl[3]);
+        mma(nn[2 * j], fvl, b[0], b[1]);
+        mma(nn[2 * j + 1], fvl, b[2], b[3]);
       }
     }
 #pragma unroll
@@ -1348,8 +1364,9 @@ dqk_kernel(const DeltaArgs a) {
         x.w1[i * APITCH + jj] = w1h;
         x.w1l[i * APITCH + jj] = __float2bfloat16(w1 - __bfloat162float(w1h));
         if (i >= jj) {  // N + N^T
-          x.w2[i * APITCH + jj] = __float2bfloat16(w2);
-          x.w2[jj * APITCH + i] = __float2bfloat16(w2);
+          const bf16 w2h = __float2bfloat16(w2), w2r = __float2bfloat16(w2 - __bfloat162float(w2h));
+          x.w2[i * APITCH + jj] = x.w2[jj * APITCH + i] = w2h;
+          x.w2l[i * APITCH + jj] = x.w2l[jj * APITCH + i] = w2r;
         }
       }
     }
@@ -1362,7 +1379,6 @@ dqk_kernel(const DeltaArgs a) {
         for (int e = 0; e < 4; ++e) t[j][e] = 0.f;
     };
     auto product = [&](const bf16* rows, const bf16* state, bool transposed) {
-      clear();
 #pragma unroll
       for (int kk = 0; kk < DV / 16; ++kk) {
         uint32_t f[4], b[4];
@@ -1384,21 +1400,30 @@ dqk_kernel(const DeltaArgs a) {
         acc[j][3] += f1 * t[j][3];
       }
     };
+    clear();
     product(x.dO, x.s0, false);
+    product(x.dO, x.s0l, false);
     add(dq, x.vec[V_OQ * 64 + r0], x.vec[V_OQ * 64 + r0 + 8]);
+    clear();
     product(x.dV, x.s0, false);
+    product(x.dV, x.s0l, false);
+    product(x.dVl, x.s0, true);
     add(dk, -x.vec[V_YK * 64 + r0], -x.vec[V_YK * 64 + r0 + 8]);
+    clear();
     product(x.u, x.ds, true);
+    product(x.u, x.dsl, true);
+    product(x.ul, x.ds, true);
     add(dk, x.vec[V_SU * 64 + r0], x.vec[V_SU * 64 + r0 + 8]);
     __syncthreads();  // w1, w2
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      uint32_t f1[4], f1l[4], ft[4], ftl[4], f2[4], b[4];
+      uint32_t f1[4], f1l[4], ft[4], ftl[4], f2[4], f2l[4], b[4];
       a_from_mk(f1, x.w1, APITCH, wm * 16, kk * 16);
       a_from_mk(f1l, x.w1l, APITCH, wm * 16, kk * 16);
       a_from_km(ft, x.w1, APITCH, kk * 16, wm * 16);
       a_from_km(ftl, x.w1l, APITCH, kk * 16, wm * 16);
       a_from_mk(f2, x.w2, APITCH, wm * 16, kk * 16);
+      a_from_mk(f2l, x.w2l, APITCH, wm * 16, kk * 16);
 #pragma unroll
       for (int j = 0; j < NT / 2; ++j) {
         b_from_kn(b, x.k, P, kk * 16, n0 + j * 16);
@@ -1410,6 +1435,8 @@ dqk_kernel(const DeltaArgs a) {
         }
         mma(dk[2 * j], f2, b[0], b[1]);
         mma(dk[2 * j + 1], f2, b[2], b[3]);
+        mma(dk[2 * j], f2l, b[0], b[1]);
+        mma(dk[2 * j + 1], f2l, b[2], b[3]);
         if (kk >= wm) {
           b_from_kn(b, x.q, P, kk * 16, n0 + j * 16);
           mma(dk[2 * j], ft, b[0], b[1]);

@@ -34,7 +34,8 @@ struct DeltaArgs {
   const void* dout = nullptr;   // bf16 [T, Hv, dv], contiguous
   const float* ds_out = nullptr;  // gradient of s_out or null
   float* ds_in = nullptr;         // gradient of s_in or null
-  void* dstates = nullptr;      // bf16 fragments of the state gradients, half the size of `states`
+  void* dstates = nullptr;      // the gradients of the states behind every chunk, as `states`
+  void* dv_lo = nullptr;        // what the rounding of dv_ left, fragments of half the size of `u`
   float* rowdots = nullptr;     // fp32 [NC, Hv, dv / 16, 2, 64]
   float* sdots = nullptr;       // fp32 [NC, Hv, dv / 16, 4]
   void *dq = nullptr, *dkey = nullptr, *dv_ = nullptr;  // bf16, contiguous

@@ -109,6 +109,22 @@ def test_gated_delta_rule_head_dims(dk, dv):
     check([70, 130], 1, 3, dk, dv, state=True, final=True)
 
 
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128)])
+@pytest.mark.parametrize("decay", [1e-3, 1.0])
+def test_gated_delta_rule_key_and_query_gradients_element_by_element(dk, dv, decay):
+    """With decays near one most of dq and dk comes from the states in front of and behind a chunk. Every operand keeps 16
+    bits, so an element is off by its rounding and by 2^-17 of its terms, twice that where both operands are cut: the bound
+    of `close` with a second 2^-12 of the largest result."""
+    q, k, v, g, beta, do, cu = make([250], 2, 4, dk, dv, 11, decay=decay)
+    ins = [t.requires_grad_() for t in (q, k, v, g, beta)]
+    got = torch.autograd.grad(LA.gated_delta_rule(*ins, cu_seqlens=cu), ins[:2], do)
+    rins = [t.detach().double().requires_grad_() for t in ins]
+    want = torch.autograd.grad((oracle(*rins, [0, 250])[0] * do.double()).sum(), rins[:2])
+    for name, a, b in zip(("dq", "dk"), got, want):
+        off = (a.double() - b).abs() - b.abs() * 2.0 ** -8
+        assert (off <= b.abs().max() * 2.0 ** -11).all(), (name, (off.max() / b.abs().max()).item() * 2.0 ** 11)
+
+
 @pytest.mark.parametrize("hk,hv", [(1, 1), (3, 3), (2, 6)])
 def test_gated_delta_rule_states_and_shared_heads(hk, hv):
     check([100, 0, 37], hk, hv, state=True, final=True)

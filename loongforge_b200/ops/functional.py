@@ -34,6 +34,28 @@ def _C():
     return _ext.require()
 
 
+class _FirstOrder(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, name, n, *tensors):
+        ctx.name = name
+        return tuple(t.detach() for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name}: its kernels have no second derivative")
+
+
+def first_order(name: str, grads: tuple, *inputs) -> tuple:
+    """What a backward pass of kernels returns: `grads`, made of `inputs` (upstream gradients and what the forward pass took).
+    Kernels run outside autograd, so a second derivative would lack their part without a word; here it raises, by whatever
+    way it reaches an input."""
+    if not torch.is_grad_enabled():
+        return grads
+    made = [g for g in grads if g is not None]
+    out = iter(_FirstOrder.apply(name, len(made), *made, *(t for t in inputs if t is not None)))
+    return tuple(None if g is None else next(out) for g in grads)
+
+
 def use_native_gemm(x: torch.Tensor) -> bool:
     return x.is_cuda and x.dtype == torch.bfloat16
 
@@ -350,7 +372,7 @@ class _QKNormRopeFn(torch.autograd.Function):
         d = [g if g.data_ptr() % 16 == 0 else g.clone() for g in (g.contiguous() for g in grads)]
         dx, dqw, dkw = _C().qk_norm_rope_bwd(d[0], d[1], d[2], d[3] if gated else None, qkv, G, R, gated, qw, kw, freqs,
                                              inv_freq, pos, axis, *rot, _ext.status_tensor(qkv.device))
-        return (dx, dqw, dkw) + (None,) * 12
+        return first_order("qk_norm_rope", (dx, dqw, dkw), *grads, qkv, qw, kw) + (None,) * 12
 
 
 def qk_norm_rope_supported(qkv, groups: int, q_per_group: int, q_weight, rot_dim: Optional[int] = None, *,
@@ -379,7 +401,7 @@ def qk_norm_rope(qkv: torch.Tensor, groups: int, q_per_group: int, q_weight: tor
     (fp32 ``[rot_dim/2]``) with ``pos_ids [T]`` or ``[axes, T]`` and ``axis [rot_dim/2]`` naming each frequency's position
     axis (time / height / width of images and video): angle i of token t is ``pos_ids[axis[i], t] * inv_freq[i]``. The
     first `rot_dim` elements of a head rotate, pairs ``(i, i + rot_dim/2)`` or, interleaved, ``(2i, 2i + 1)``; cosine and
-    sine are scaled by `mscale`. On a GPU a table row or an axis out of range turns by zero and sets the status word.
+    sine are scaled by `mscale`. Differentiable in `qkv` and the weights, once on a GPU. On a GPU a table row or an axis out of range turns by zero and sets the status word.
     """
     if (freqs is None) == (inv_freq is None):
         raise ValueError("qk_norm_rope: give either `freqs` or `inv_freq`")

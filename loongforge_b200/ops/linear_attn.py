@@ -15,8 +15,9 @@ chunk-parallel form (WY representation inside a chunk, one state update per chun
 
 On a GPU bf16 inputs run on the kernels of ``csrc/gated_delta_sm100.cu``, ``csrc/gated_delta_step.cu`` and
 ``csrc/causal_conv.cu``: they read ``cu_seqlens`` on the device (no host synchronisation; capturable into a CUDA
-graph) and take fewer key heads than value heads as they are. Other devices, dtypes and head dims take the PyTorch
-formulation below, which is also what the kernels are tested against.
+graph) and take fewer key heads than value heads as they are. Their gradients can be taken once: a second derivative
+raises, and forward-mode derivatives and ``vmap`` are refused. Other devices, dtypes and head dims take the PyTorch
+formulation below, which is also what the kernels are tested against, and which has all of these.
 """
 from __future__ import annotations
 
@@ -26,6 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _ext
+from .functional import first_order
 
 
 def l2norm(x: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
@@ -108,11 +110,12 @@ class _GatedDeltaFn(torch.autograd.Function):
     def forward(ctx, q, k, v, g, beta, s_in, cu, scale, l2norm, want_state, keep):
         ctx.set_materialize_grads(False)
         C, status = _ext.require(), _status(v)
+        inputs = tuple(t if need else None for t, need in zip((q, k, v, g, beta, s_in), ctx.needs_input_grad))
         q, k, v, gf, bf = _rows16(q), _rows16(k), _rows16(v), _fp32(g), _fp32(beta)
         bounds, first = (None, None) if cu is None else C.delta_plan(cu, q.shape[0], status)
         o, s_out, kept = C.delta_fwd(q, k, v, gf, bf, bounds, first, scale, l2norm, s_in, want_state, keep, status)
         if keep:
-            ctx.save_for_backward(q, k, v, gf, bf, bounds, first, kept)
+            ctx.save_for_backward(*inputs, q, k, v, gf, bf, bounds, first, kept)
             ctx.cfg = (scale, l2norm, g.dtype, beta.dtype)
         if not want_state:
             ctx.mark_non_differentiable(s_out)
@@ -121,13 +124,15 @@ class _GatedDeltaFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do, ds_out):
         scale, l2norm, g_dtype, beta_dtype = ctx.cfg
-        q, k, v, g, beta, bounds, first, kept = ctx.saved_tensors
+        inputs, (q, k, v, g, beta, bounds, first, kept) = ctx.saved_tensors[:6], ctx.saved_tensors[6:]
         want_ds = ctx.needs_input_grad[5]
+        up = (do, ds_out)
         do = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if do is None else _dense16(do)
         dq, dk, dv, dg, dbeta, ds_in = _ext.require().delta_bwd(
             do, None if ds_out is None else _dense16(ds_out), q, k, v, g, beta, bounds, first, scale, l2norm, want_ds, kept,
             _status(v))
-        return (dq, dk, dv, dg.to(g_dtype), dbeta.to(beta_dtype), ds_in if want_ds else None) + (None,) * 5
+        grads = (dq, dk, dv, dg.to(g_dtype), dbeta.to(beta_dtype), ds_in if want_ds else None)
+        return first_order("gated_delta_rule", grads, *up, *inputs) + (None,) * 5
 
 
 def _status(t: torch.Tensor) -> torch.Tensor:
@@ -349,7 +354,7 @@ class _CausalConvFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, cu = ctx.saved_tensors
         dx, dw, db = _ext.require().conv1d_bwd(_dense16(dy), x, weight, bias, cu, ctx.silu)
-        return dx, dw, db if bias is not None else None, None, None
+        return first_order("causal_conv1d", (dx, dw, db if bias is not None else None), dy, x, weight, bias) + (None, None)
 
 
 _ACTIVATIONS = {None: False, "silu": True, "swish": True}

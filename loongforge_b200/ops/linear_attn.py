@@ -127,7 +127,7 @@ class _GatedDeltaFn(torch.autograd.Function):
         inputs, (q, k, v, g, beta, bounds, first, kept) = ctx.saved_tensors[:6], ctx.saved_tensors[6:]
         want_ds = ctx.needs_input_grad[5]
         up = (do, ds_out)
-        do = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if do is None else _dense16(do)
+        do = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if do is None else _rows16(do.contiguous())
         dq, dk, dv, dg, dbeta, ds_in = _ext.require().delta_bwd(
             do, None if ds_out is None else _dense16(ds_out), q, k, v, g, beta, bounds, first, scale, l2norm, want_ds, kept,
             _status(v))
@@ -145,13 +145,11 @@ def _fp32(t: torch.Tensor) -> torch.Tensor:
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """The tensor itself when its rows are unit-stride and 16-byte aligned (what the kernels read), else a copy."""
-    if t.data_ptr() % 16 == 0:
-        if t.is_contiguous():
-            return t
-        s = t.stride()
-        if s[-1] == 1 and all(x % 8 == 0 for x in s[:-1]):
-            return t
+    """The tensor itself when its rows are unit-stride and 16-byte aligned (what the kernels read), else a copy. A dimension
+    of one element may have any stride in a contiguous tensor: the strides themselves are looked at."""
+    s = t.stride()
+    if t.data_ptr() % 16 == 0 and s[-1] == 1 and all(x % 8 == 0 for x in s[:-1]):
+        return t
     return t.clone(memory_format=torch.contiguous_format)
 
 

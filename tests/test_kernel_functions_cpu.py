@@ -34,3 +34,13 @@ def test_second_derivatives_are_an_error_not_a_part_of_one(monkeypatch):
             for leaf in leaves:  # each reaches the loss by another way too
                 with pytest.raises(RuntimeError, match=f"{name}.*second derivative"):
                     torch.autograd.grad(sum(t.square().sum() for t in d), leaf, retain_graph=True)
+
+
+def test_rows_for_the_kernels_have_strides_of_whole_16_byte_pieces():
+    """A single row cut out of a wider one counts as contiguous whatever its row stride."""
+    wide = torch.randn(3, 65).bfloat16()
+    for t in (wide[:1, :64], wide[:, :64], wide[:1, :64].view(1, 1, 64), wide[:1, 1:], torch.randn(1, 67, dtype=torch.bfloat16)[:, None, :64]):
+        r = LA._rows16(t)
+        assert torch.equal(r, t) and r.stride(-1) == 1 and all(s % 8 == 0 for s in r.stride()[:-1]) and r.data_ptr() % 16 == 0
+    even = torch.randn(4, 72).bfloat16()[:, :64]
+    assert LA._rows16(even) is even

@@ -586,3 +586,37 @@ def test_wide_indices_do_not_wrap_into_range():
                     freqs=torch.rand(4, 32, device="cuda"), pos_ids=far)
     with pytest.raises(RuntimeError, match="out of range"):
         _ext.check_status()
+
+
+def test_one_row_out_of_a_wider_one():
+    """A single row whose stride is odd, as inputs of all four operators and as the gradient that comes back."""
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    d = 64
+
+    def odd(*shape):  # the first elements of a row that is three longer
+        n = shape[-1]
+        for s in shape[1:-1]:
+            n *= s
+        return randn(gen, 1, n + 3, dtype=BF16)[:, :n].unflatten(1, shape[1:]) if len(shape) > 2 else randn(gen, 1, n + 3, dtype=BF16)[:, :n]
+
+    for hv in (1, 2):
+        q, k, v, up = odd(1, 1, d), odd(1, 1, d), odd(1, hv, d), odd(1, hv, d)
+        g, beta = -torch.rand(1, hv, device="cuda"), torch.rand(1, hv, device="cuda")
+        rows = [t.detach().requires_grad_() for t in (q, k, v)]
+        same = [t.clone(memory_format=torch.contiguous_format).requires_grad_() for t in (q, k, v)]
+        a, b = (LA.gated_delta_rule(*t, g, beta) for t in (rows, same))
+        da, db = torch.autograd.grad(a, rows, up), torch.autograd.grad(b, same, up.clone(memory_format=torch.contiguous_format))
+        assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(da, db))
+        s1, s2 = torch.ones(1, hv, d, d, device="cuda"), torch.ones(1, hv, d, d, device="cuda")
+        with torch.no_grad():
+            assert torch.equal(LA.gated_delta_rule_step(q, k, v, g, beta, s1), LA.gated_delta_rule_step(*same, g, beta, s2))
+        assert torch.equal(s1, s2)
+    x, up, w = odd(1, d), odd(1, d), randn(gen, d, 4, dtype=BF16)
+    xs = [x.detach().requires_grad_(), x.clone(memory_format=torch.contiguous_format).requires_grad_()]
+    y = [LA.causal_conv1d(t, w) for t in xs]
+    dx = [torch.autograd.grad(t, u, up)[0] for t, u in zip(y, xs)]
+    assert torch.equal(*y) and torch.equal(*dx)
+    w1, w2 = (torch.ones(1, d, 3, device="cuda", dtype=BF16) for _ in range(2))
+    with torch.no_grad():
+        assert torch.equal(LA.causal_conv1d_step(x, w1, w), LA.causal_conv1d_step(xs[1], w2, w))
+    assert torch.equal(w1, w2)

@@ -178,9 +178,15 @@ class MLP(nn.Module):
         return self.linear_fc2(h, residual)
 
 
+def _watched(m: nn.Module) -> bool:
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
 def fused_qk_applies(attn, qkv, groups: int, q_per_group: int, rotary: Optional[RotaryInputs], *, gated: bool = False) -> bool:
-    """Whether `attn`'s per-head query / key norms and its rotation run as one kernel on the packed projection."""
-    return (rotary is not None and isinstance(attn.q_layernorm, Norm) and attn.q_layernorm.kind == "RMSNorm"
+    """Whether `attn`'s per-head query / key norms and its rotation run as one kernel on the packed projection. The kernel
+    takes the norms' weights and never calls them: modules that are watched (hooks), or that are not plain norms, are."""
+    norms = (attn.q_layernorm, attn.k_layernorm)
+    return (rotary is not None and all(type(n) is Norm and n.kind == "RMSNorm" and not _watched(n) for n in norms)
             and OF.qk_norm_rope_supported(qkv, groups, q_per_group, attn.q_layernorm.weight, attn.rot_dim, gated=gated))
 
 

@@ -331,12 +331,29 @@ def rope(x: torch.Tensor, freqs: torch.Tensor, *, pos_ids: Optional[torch.Tensor
 
 
 def _rot_angles(T, freqs, inv_freq, axis, pos_ids):
-    """Angles [T, rot_dim / 2]: rows of the table, or position times frequency of each frequency's axis."""
+    """Angles [T, rot_dim / 2]: rows of the table, or position times frequency of each frequency's axis. Rows and axes out of
+    range turn by zero and are reported, as the kernel does it: an index out of range would end a GPU's context, and one
+    below zero would wrap."""
     if freqs is not None:
-        return freqs[:T] if pos_ids is None else freqs[pos_ids.long()]
+        if pos_ids is None:
+            return freqs[:T]
+        row, n = pos_ids.long().to(freqs.device), freqs.shape[0]
+        known = (row >= 0) & (row < n)
+        _report_rows(known, "a row of the table in pos_ids")
+        return torch.where(known[:, None], freqs[row.clamp(0, n - 1)], 0.0) if n else freqs.new_zeros(T, freqs.shape[1])
     pos = pos_ids if pos_ids.dim() == 2 else pos_ids[None]
-    ax = torch.zeros(inv_freq.numel(), dtype=torch.long, device=pos.device) if axis is None else axis.long()
-    return (pos.double()[ax].t() * inv_freq.double()).float()
+    ax = torch.zeros(inv_freq.numel(), dtype=torch.long, device=pos.device) if axis is None else axis.long().to(pos.device)
+    known = (ax >= 0) & (ax < pos.shape[0])
+    _report_rows(known, "axis")
+    ang = (pos.double()[ax.clamp(0, pos.shape[0] - 1)].t() * inv_freq.double()).float()
+    return torch.where(known, ang, 0.0)
+
+
+def _report_rows(known: torch.Tensor, what: str):
+    if known.is_cuda:
+        _ext.status_tensor(known.device).masked_fill_(~known.all(), 7)
+    elif not known.all():
+        raise ValueError(f"qk_norm_rope: {what} is out of range")
 
 
 def qk_norm_rope_ref(qkv, groups, q_per_group, q_weight, k_weight, *, freqs=None, inv_freq=None, axis=None, pos_ids=None,
@@ -401,7 +418,8 @@ def qk_norm_rope(qkv: torch.Tensor, groups: int, q_per_group: int, q_weight: tor
     (fp32 ``[rot_dim/2]``) with ``pos_ids [T]`` or ``[axes, T]`` and ``axis [rot_dim/2]`` naming each frequency's position
     axis (time / height / width of images and video): angle i of token t is ``pos_ids[axis[i], t] * inv_freq[i]``. The
     first `rot_dim` elements of a head rotate, pairs ``(i, i + rot_dim/2)`` or, interleaved, ``(2i, 2i + 1)``; cosine and
-    sine are scaled by `mscale`. Differentiable in `qkv` and the weights, once on a GPU. On a GPU a table row or an axis out of range turns by zero and sets the status word.
+    sine are scaled by `mscale`. Differentiable in `qkv` and the weights, once on a GPU. On a GPU a table row or an axis out
+    of range turns by zero and sets the status word; elsewhere it raises.
     """
     if (freqs is None) == (inv_freq is None):
         raise ValueError("qk_norm_rope: give either `freqs` or `inv_freq`")

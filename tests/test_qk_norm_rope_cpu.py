@@ -105,3 +105,17 @@ def test_refusals():
         OF.qk_norm_rope(x, G, R, w[:8], w, freqs=f)
     with pytest.raises(ValueError, match="heads"):
         OF.qk_norm_rope(x[:, :-1], G, R, w, w, freqs=f)
+
+
+def test_rows_and_axes_out_of_range_are_refused():
+    """A row below zero is no row from the table's end."""
+    x, w, f = torch.randn(4, 4 * 16), torch.ones(16), torch.rand(5, 8)
+    for pos in ([0, 1, 2, -1], [0, 5, 0, 0], [2 ** 40, 0, 0, 0]):
+        with pytest.raises(ValueError, match="out of range"):
+            OF.qk_norm_rope(x, 1, 2, w, w, freqs=f, pos_ids=torch.tensor(pos))
+    with pytest.raises(ValueError, match="out of range"):
+        OF.qk_norm_rope(x, 1, 2, w, w, freqs=f[:0], pos_ids=torch.zeros(4, dtype=torch.long))
+    inv, pos = torch.rand(8), torch.arange(8).view(2, 4)
+    for ax in (-1, 2):
+        with pytest.raises(ValueError, match="out of range"):
+            OF.qk_norm_rope(x, 1, 2, w, w, inv_freq=inv, pos_ids=pos, axis=torch.full((8,), ax))

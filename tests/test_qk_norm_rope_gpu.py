@@ -205,3 +205,18 @@ def test_qk_norm_rope_upstream_layouts_streams_and_replay():
     torch.cuda.synchronize()
     want = run(*leaves(), ups)
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_qk_norm_rope_bad_rows_in_the_pytorch_form():
+    """Shapes without a kernel (head dim 48, fp32) treat rows and axes out of range as the kernel does."""
+    x, w, freqs = torch.randn(4, 4 * 48, device="cuda"), torch.ones(48, device="cuda"), torch.rand(10, 24, device="cuda") + 0.5
+    pos = torch.tensor([3, 10, -1, 1 << 40], device="cuda")
+    q, _, _ = OF.qk_norm_rope(x, 1, 2, w, w, freqs=freqs, pos_ids=pos)
+    with pytest.raises(RuntimeError, match="out of range"):
+        _ext.check_status()
+    still, _, _ = OF.qk_norm_rope(x, 1, 2, w, w, freqs=torch.zeros_like(freqs), pos_ids=pos.clamp(0, 9))
+    assert torch.equal(q[1:], still[1:]) and not torch.equal(q[0], still[0])
+    _ext.check_status()
+    OF.qk_norm_rope(x, 1, 2, w, w, inv_freq=freqs[0], axis=torch.full((24,), 2, device="cuda"), pos_ids=pos[:1].expand(2, 4))
+    with pytest.raises(RuntimeError, match="out of range"):
+        _ext.check_status()

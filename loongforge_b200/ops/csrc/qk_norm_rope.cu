@@ -491,7 +491,8 @@ qk_bwd_kernel(const QkNormRopeArgs a) {
         dots = fma2(d[j] * x[j], w[j], dots);
       }
       const float s = head_sum<LANES>(sum(ss)), dot = head_sum<LANES>(sum(dots));
-      const float rstd = rsqrtf(s * (1.f / D) + a.eps), m = dot * rstd * rstd * rstd * (1.f / D);
+      // a lane without a head works on zeros, whose root is zero when eps is: nothing of it may reach dw
+      const float rstd = mine ? rsqrtf(s * (1.f / D) + a.eps) : 0.f, m = dot * rstd * rstd * rstd * (1.f / D);
       const F2 rr = two(rstd, rstd), mm = two(m, m);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {

@@ -220,3 +220,19 @@ def test_qk_norm_rope_bad_rows_in_the_pytorch_form():
     OF.qk_norm_rope(x, 1, 2, w, w, inv_freq=freqs[0], axis=torch.full((24,), 2, device="cuda"), pos_ids=pos[:1].expand(2, 4))
     with pytest.raises(RuntimeError, match="out of range"):
         _ext.check_status()
+
+
+def test_qk_norm_rope_without_eps():
+    """Lanes that have no head or token left must not bring the root of nothing into the weights' gradients."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    for T, G, R, D in ((1, 1, 1, 64), (3, 2, 3, 128), (301, 1, 5, 256)):
+        x, w = (torch.randn(*s, generator=gen, device="cuda").to(BF16).requires_grad_() for s in ((T, G * (R + 2) * D), (D,)))
+        f = torch.rand(T, D // 2, device="cuda")
+        got = OF.qk_norm_rope(x, G, R, w, w, freqs=f, eps=0.0)
+        ups = [torch.randn(t.shape, generator=gen, device="cuda").to(BF16) for t in got]
+        rx, rw = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+        want = oracle(rx, rw, rw, G, R, False, f.double(), D, False, 1.0, 0.0, 0.0)
+        a, b = torch.autograd.grad(got, (x, w), ups), torch.autograd.grad(want, (rx, rw), [u.double() for u in ups])
+        near(a[0], b[0], "dqkv")
+        # dw of the queries and of the keys are each rounded, and their sum once more
+        assert ((a[1].double() - b[1]).abs() <= 3 * 2.0 ** -8 * b[1].abs().max()).all()

@@ -266,15 +266,15 @@ def _check_state(state, shape, device, name: str):
                          f"{state.device}")
 
 
-def _step_index(state_indices, rows: int, slots: int, device) -> Optional[torch.Tensor]:
-    """Slots of the rows as int32 on `device`. Indices on the host are checked here; those on the device are checked by
-    the kernel, which reports a bad one through the status word and leaves its row out."""
+def _step_index(state_indices, rows: int, slots: int, device, native: bool) -> Optional[torch.Tensor]:
+    """Slots of the rows as int32 on `device`. Indices on the host are checked here, and so are those that the PyTorch form
+    reads; those on the device are else checked by the kernel, which reports a bad one through the status word and leaves
+    its row out."""
     if state_indices is None:
         if rows > slots:
             raise ValueError(f"{rows} rows need {rows} state slots, there are {slots}")
         return None
-    on_device = torch.is_tensor(state_indices) and state_indices.is_cuda and device.type == "cuda"
-    if not on_device:
+    if not (native and torch.is_tensor(state_indices) and state_indices.is_cuda):
         idx = [int(i) for i in (state_indices.tolist() if torch.is_tensor(state_indices) else state_indices)]
         used = [i for i in idx if i >= 0]
         if len(idx) != rows or any(i >= slots for i in used) or len(set(used)) < len(used):
@@ -302,8 +302,9 @@ def gated_delta_rule_step(q, k, v, g, beta, state: torch.Tensor, *, state_indice
     """One token of the gated delta rule for each of B rows: q, k ``[B, Hk, dk]``, v ``[B, Hv, dv]``, g, beta ``[B, Hv]``;
     returns ``o [B, Hv, dv]``. ``state [slots, Hv, dk, dv]`` (fp32, contiguous) is updated IN PLACE: row b uses slot
     ``state_indices[b]`` (its own number without indices). A negative index is a padding row: zeros come back and no state
-    changes. Two rows on one slot, or a slot out of range, are an error: raised here for indices on the host; for indices
-    on the GPU the later row is left out as a padding row is and the status word is set (``_ext.check_status``).
+    changes. Two rows on one slot, or a slot out of range, are an error: raised here for indices on the host and where no
+    kernel covers the inputs; else, for indices on the GPU, the later row is left out as a padding row is and the status
+    word is set (``_ext.check_status``).
     """
     _check_delta(q, k, v, g, beta, "B")
     _no_gradient(q, k, v, g, beta, state)
@@ -315,8 +316,9 @@ def gated_delta_rule_step(q, k, v, g, beta, state: torch.Tensor, *, state_indice
     if not state.is_contiguous():
         raise ValueError("state is updated in place and must be contiguous")
     scale = float(scale) if scale is not None else dk ** -0.5
-    idx = _step_index(state_indices, B, state.shape[0], v.device)
-    if gated_delta_rule_native(q, k, v):
+    native = gated_delta_rule_native(q, k, v)
+    idx = _step_index(state_indices, B, state.shape[0], v.device, native)
+    if native:
         return _ext.require().delta_step(_rows16(q), _rows16(k), _rows16(v), g if g.dtype == torch.float32 and g.is_contiguous() else _fp32(g),
                                          beta if beta.dtype == torch.float32 and beta.is_contiguous() else _fp32(beta), state, idx,
                                          scale, qk_l2norm, _status(v))
@@ -413,8 +415,9 @@ def causal_conv1d_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tenso
     if state.dim() != 3 or state.shape[1:] != (C, K - 1) or state.dtype != x.dtype or state.device != x.device or not state.is_contiguous():
         raise ValueError(f"state must be contiguous {x.dtype} [slots, {C}, {K - 1}] on {x.device}, got {state.dtype} "
                          f"{list(state.shape)} on {state.device}")
-    idx = _step_index(state_indices, B, state.shape[0], x.device)
-    if _conv_native(x, weight):
+    native = _conv_native(x, weight)
+    idx = _step_index(state_indices, B, state.shape[0], x.device, native)
+    if native:
         return _ext.require().conv1d_step(_rows16(x), state, _plain16(weight), _plain16(bias), idx, _ACTIVATIONS[activation],
                                           _status(x))
     out = torch.zeros_like(x)

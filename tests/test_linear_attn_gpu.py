@@ -620,3 +620,22 @@ def test_one_row_out_of_a_wider_one():
     with torch.no_grad():
         assert torch.equal(LA.causal_conv1d_step(x, w1, w), LA.causal_conv1d_step(xs[1], w2, w))
     assert torch.equal(w1, w2)
+
+
+def test_bad_slots_where_no_kernel_covers_the_step():
+    """fp32 rows take the PyTorch form, which reads the slots: it refuses what the kernel would leave out."""
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    q, k, v = (randn(gen, 2, 1, 16) for _ in range(3))
+    g, x, w = torch.zeros(2, 1, device="cuda"), randn(gen, 2, 12), randn(gen, 12, 4)
+    pool, win = randn(gen, 3, 1, 16, 16), randn(gen, 3, 12, 3)
+    kept = pool.clone(), win.clone()
+    for bad in ([1, 1], [0, 3], [2 ** 32, 0]):
+        idx = torch.tensor(bad, device="cuda")
+        with pytest.raises(ValueError, match="state_indices"):
+            LA.gated_delta_rule_step(q, k, v, g, g + 1, pool, state_indices=idx)
+        with pytest.raises(ValueError, match="state_indices"):
+            LA.causal_conv1d_step(x, win, w, state_indices=idx)
+    assert torch.equal(pool, kept[0]) and torch.equal(win, kept[1])
+    idx = torch.tensor([2, -1], device="cuda")
+    o = LA.gated_delta_rule_step(q, k, v, g, g + 1, pool, state_indices=idx)
+    assert o[0].any() and not o[1].any() and torch.equal(pool[:2], kept[0][:2])

@@ -179,10 +179,16 @@ def _check_delta(q, k, v, g, beta, rows: str):
         raise ValueError("q, k, v, g and beta must be on one device")
 
 
+def _whole(t, name: str):
+    if torch.is_tensor(t) and (t.is_floating_point() or t.is_complex()):
+        raise ValueError(f"{name} must be whole numbers, got {t.dtype}")
+
+
 def _host_bounds(cu_seqlens, T: int) -> list:
     """Sequence boundaries as a list; every one of them inside [0, T] and none in front of the one before it."""
     if cu_seqlens is None:
         return [0, T]
+    _whole(cu_seqlens, "cu_seqlens")
     b = [int(x) for x in (cu_seqlens.tolist() if torch.is_tensor(cu_seqlens) else cu_seqlens)]
     if len(b) < 2 or b[0] < 0 or b[-1] > T or any(e < s for s, e in zip(b, b[1:])):
         raise ValueError(f"cu_seqlens must be at least two non-decreasing offsets within the {T} rows, got {b[:8]}...")
@@ -203,6 +209,7 @@ def _device_bounds(cu_seqlens, T: int, device) -> Optional[torch.Tensor]:
         return None
     if not torch.is_tensor(cu_seqlens) or not cu_seqlens.is_cuda:
         return torch.tensor(_host_bounds(cu_seqlens, T), dtype=torch.int32, device=device)
+    _whole(cu_seqlens, "cu_seqlens")
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
         raise ValueError("cu_seqlens must hold at least two offsets")
     if cu_seqlens.dtype == torch.int32 and cu_seqlens.device == device and cu_seqlens.is_contiguous():
@@ -274,6 +281,7 @@ def _step_index(state_indices, rows: int, slots: int, device, native: bool) -> O
         if rows > slots:
             raise ValueError(f"{rows} rows need {rows} state slots, there are {slots}")
         return None
+    _whole(state_indices, "state_indices")
     if not (native and torch.is_tensor(state_indices) and state_indices.is_cuda):
         idx = [int(i) for i in (state_indices.tolist() if torch.is_tensor(state_indices) else state_indices)]
         used = [i for i in idx if i >= 0]

@@ -111,3 +111,18 @@ def test_bad_slots_and_states_are_refused():
         LA.causal_conv1d(x, w[:5])
     with pytest.raises(ValueError, match="bias"):
         LA.causal_conv1d(x, w, torch.zeros(5))
+
+
+def test_numbers_that_are_not_whole_are_refused():
+    q, k, v, g, beta = make(T=3)
+    pool, x, w = torch.zeros(4, 4, 16, 8), torch.randn(3, 6), torch.randn(6, 4)
+    for idx in (torch.tensor([0.0, 1.0, 2.0]), torch.tensor([0.5, 1.5, 2.5], dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="state_indices must be whole"):
+            LA.gated_delta_rule_step(q, k, v, g, beta, pool, state_indices=idx)
+        with pytest.raises(ValueError, match="state_indices must be whole"):
+            LA.causal_conv1d_step(x, torch.zeros(3, 6, 3), w, state_indices=idx)
+    for cu in (torch.tensor([0.0, 3.0]), torch.tensor([0.0, 1.5, 3.0])):
+        with pytest.raises(ValueError, match="cu_seqlens must be whole"):
+            LA.gated_delta_rule(q, k, v, g, beta, cu_seqlens=cu)
+        with pytest.raises(ValueError, match="cu_seqlens must be whole"):
+            LA.causal_conv1d(x, w, cu_seqlens=cu)

@@ -639,3 +639,5 @@ def test_bad_slots_where_no_kernel_covers_the_step():
     idx = torch.tensor([2, -1], device="cuda")
     o = LA.gated_delta_rule_step(q, k, v, g, g + 1, pool, state_indices=idx)
     assert o[0].any() and not o[1].any() and torch.equal(pool[:2], kept[0][:2])
+    with pytest.raises(ValueError, match="whole"):
+        LA.causal_conv1d_step(x, win, w, state_indices=idx.float())

@@ -31,7 +31,7 @@
 //             mma.sync, and an accumulator tile is, register by register, the A operand of the next product. Four warps
 //             share a unit (by dk for the state, by tokens for the rest) and hand their operands to each other.
 //   backward  the same in reverse with dS^T.
-//   dqk       dQ and dK, parallel over chunks: here for a head dim of 64, in gated_delta_dqk_sm100.cu for 128.
+//   dqk       dQ and dK, parallel over chunks: in gated_delta_dqk_sm100.cu for dk = dv = 128, here where either is 64.
 //   gates     dg and dbeta.
 //
 // Precision. The state, U, X and all products along the chain carry 16 or more bits: an fp32 operand is cut into a bf16
@@ -44,9 +44,10 @@
 // them, 5.8K cycles a chunk forward and 7.5K backward. mma.sync runs at a quarter of tcgen05's rate, but operands and results
 // stay in registers, and 32 heads make 1024 warps of such work. One sequence of 4096 tokens with 32 heads of 128 x 128 (five
 // sequences of 16384): prepare 38 us (131), forward 190 (656), backward 257 (884; 238 and 826 without the low parts
-// that dqk reads), dqk 138 (520), gates 8 (16). Measured against it: a whole unit in one warp 471 (959) forward and 620 (1278) backward; eight warps along the chain and eight
-// beside it 208 (713) and 257 (874), bound by shared memory; a head as one 128-column product on tcgen05 11.7K cycles a
-// chunk, 5K of them the work on elements between the products, on an eighth as many blocks.
+// that dqk reads), dqk 138 (520), gates 8 (16). Measured against it: a whole unit in one warp 471 (959) forward and 620
+// (1278) backward; eight warps along the chain and eight beside it 208 (713) and 257 (874), bound by shared memory; a head
+// as one 128-column product on tcgen05 11.7K cycles a chunk, 5K of them the work on elements between the products, on an
+// eighth as many blocks.
 #include "gated_delta.cuh"
 
 namespace lf {
@@ -1595,8 +1596,9 @@ int backward_dk(const DeltaArgs& a, cudaStream_t s) {
   int rc = launch_backward<DK, 2>(a, s);
   if (rc) return rc;
   if (a.NC > 0) {
-    if (a.dk == 128 && a.dv == 128) rc = delta_tc_dqk(a, s);
-    else rc = a.dv == 64 ? launch_dqk<DK, 64>(a, s) : launch_dqk<DK, 128>(a, s);
+    if (a.dv == 64) rc = launch_dqk<DK, 64>(a, s);
+    else if constexpr (DK == 128) rc = delta_tc_dqk(a, s);
+    else rc = launch_dqk<DK, 128>(a, s);
     if (rc) return rc;
     gates_kernel<<<static_cast<unsigned>((a.NC * a.Hv + GATE_WARPS - 1) / GATE_WARPS), GATE_WARPS * 32, 0, s>>>(a);
   }

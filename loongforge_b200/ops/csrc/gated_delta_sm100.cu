@@ -19,9 +19,12 @@
 //
 //   dg_t = sum_{i >= t} (o~_i.do_i - m_i.dv_i) - sum_{j >= t} u_j.x~_j + sum_j e^{G_C - G_j} (K dS1)_j.u_j + e^{G_C} <dS1, S0>
 //
-// with sums over the chunk. Every term carries a decay, so strongly decaying heads keep the relative accuracy of their
-// (small) gradient; that is why A and P are kept as strict lower parts, their diagonals apart: o~, m and x~ are sums of
-// their own, never differences of larger numbers.
+// with sums over the chunk. Every term carries a decay, so heads that decay strongly throughout keep the relative accuracy
+// of their (small) gradient; that is why A and P are kept as strict lower parts, their diagonals apart: o~, m and x~ are
+// sums of their own, never differences of larger numbers. That does not hold for a single reset among mild decays: a pair
+// j < i of tokens that both lie behind t enters dg_t once through o~_i and m_i and once, negated, through x~_j, and neither
+// carries g_t. What is left of such a dg_t is the rounding of its neighbours' terms (2e-6 where they are of order one; 4e-7
+// in fp32 throughout).
 //
 // Kernels:
 //   prepare   one block per (chunk, key head): Q K^T and K K^T once, then A, P and the per-token factors of each of its

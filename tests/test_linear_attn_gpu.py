@@ -641,3 +641,30 @@ def test_bad_slots_where_no_kernel_covers_the_step():
     assert o[0].any() and not o[1].any() and torch.equal(pool[:2], kept[0][:2])
     with pytest.raises(ValueError, match="whole"):
         LA.causal_conv1d_step(x, win, w, state_indices=idx.float())
+
+
+@pytest.mark.parametrize("strong", [-30.0, -8.0])
+def test_gated_delta_rule_resets_among_mild_decays(strong):
+    """The gradient of a reset is next to nothing, and what comes back is the rounding of the terms that cancel in it: o . do
+    and v . dv of the tokens behind it, each off by up to 4 * 2^-17 of itself, independently, so their 2-norm. The gradient
+    of a rate that multiplies all decays weighs these with g."""
+    q, k, v, g, beta, do, cu = make([250], 2, 4, 128, 128, 21, decay=0.05)
+    hit = torch.rand(250, 4, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") < 0.06
+    g[hit] = strong
+    ins = [t.requires_grad_() for t in (q, k, v, g, beta)]
+    got = torch.autograd.grad(LA.gated_delta_rule(*ins, cu_seqlens=cu), ins, do)
+    rins = [t.detach().double().requires_grad_() for t in ins]
+    ro, _ = oracle(*rins, [0, 250])
+    want = torch.autograd.grad((ro * do.double()).sum(), rins)
+    terms = ((ro * do.double()).sum(-1).square() + (rins[2] * want[2]).sum(-1).square()).sum(0).sqrt()
+    lim = 4 * 2.0 ** -17 * terms
+    off = (got[3].double() - want[3]).abs()
+    assert (torch.where(hit, off, 0.0) <= lim).all(), (off[hit].max(), lim)
+    rate = (g.detach().double() * (got[3].double() - want[3])).sum(0).abs()
+    assert (rate <= lim * g.detach().double().norm(dim=0)).all(), (rate, lim)
+    assert rel(got[3], want[3]) < 4 * 2.0 ** -17
+
+
+def test_gated_delta_rule_long_memory():
+    """Heads as training leaves some: decays near one over thousands of tokens, where a state is the sum of hundreds."""
+    check([2100], 1, 2, decay=1e-3)

@@ -11,6 +11,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include "device_info.h"
 #include "linear_attn.h"
 
 namespace lf {
@@ -318,8 +319,9 @@ conv_dw_kernel(const float* __restrict__ partial, int blocks, int C, int K, bf16
 // enough that there are two blocks per SM.
 int row_span(long long T, int C, int v) {
   const long long cblocks = (C + 2 * v * THREADS - 1) / (2 * v * THREADS);
+  const int blocks = 2 * sm_count();
   int span = MAX_SPAN;
-  while (span > 16 && (T + span - 1) / span * cblocks < 2 * 148) span >>= 1;
+  while (span > 16 && (T + span - 1) / span * cblocks < blocks) span >>= 1;
   return span;
 }
 

@@ -23,6 +23,7 @@
 // products have read that, and a unit's loads begin when its predecessor's products are done. What bounds it are these two
 // rounds of loads, which alternate with the products: 18K cycles a unit.
 #include <atomic>
+#include "device_info.h"
 #include "gated_delta.cuh"
 #include "sm100_ptx.cuh"
 
@@ -448,8 +449,8 @@ int delta_tc_dqk(const DeltaArgs& a, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   const size_t bytes = sizeof(Smem) + 1024;
   if (!allow_smem(tc_dqk_kernel, bytes, allowed)) return -3;
-  const long long items = a.NC * a.Hk;
-  tc_dqk_kernel<<<static_cast<unsigned>(items < 148 ? items : 148), THREADS, bytes, s>>>(a);
+  const long long items = a.NC * a.Hk, sms = sm_count();
+  tc_dqk_kernel<<<static_cast<unsigned>(items < sms ? items : sms), THREADS, bytes, s>>>(a);
   return 0;
 }
 

@@ -177,8 +177,8 @@ __global__ void plan_kernel(const int* __restrict__ in, int N, long long T, int*
 }
 
 // Zeroes the rows that no sequence covers, [0, cu[0]) and [cu[N], T), of a row-major buffer. The kernels that run anyway do
-// it with their first blocks: a launch of its own costs a small call as much as its largest kernel.
-constexpr int ZERO_BLOCKS = 148;
+// it with their first blocks, whatever the device: a launch of its own costs a small call as much as its largest kernel.
+constexpr int ZERO_BLOCKS = 128;
 __device__ __forceinline__ void zero_rows(const DeltaArgs& a, long long first, long long last, void* buffer, long long words) {
   const long long n = (first + a.T - last) * words, step = static_cast<long long>(gridDim.x < ZERO_BLOCKS ? gridDim.x : ZERO_BLOCKS) * blockDim.x;
   for (long long w = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; w < n; w += step) {

@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include "device_info.h"
 #include "linear_attn.h"
 
 namespace lf {
@@ -140,8 +141,8 @@ delta_step_kernel(const DeltaStepArgs a) {
 template <int DK>
 int launch(const DeltaStepArgs& a, cudaStream_t s) {
   const long long heads = static_cast<long long>(a.B) * a.Hv;
-  // 32 columns a block while that leaves SMs without one: 128-byte pieces of a row. Full rows otherwise.
-  const int cols = heads * (a.dv / 64) < 2 * 148 ? 32 : 64;
+  // 32 columns a block, 128-byte pieces of a row, while 64 leave multiprocessors with less than two blocks; else 64.
+  const int cols = heads * (a.dv / 64) < 2 * sm_count() ? 32 : 64;
   const long long grid = heads * (a.dv / cols);
   if (grid > INT32_MAX) return -2;
   if (cols == 32) delta_step_kernel<DK, 32><<<static_cast<unsigned>(grid), THREADS, 0, s>>>(a);

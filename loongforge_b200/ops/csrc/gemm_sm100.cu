@@ -18,6 +18,7 @@
 // Replaces the cuBLASLt GEMMs behind TE's Column/RowParallelLinear in the
 // reference (loongforge/models/dispatch.py:45-54).
 #include "sm100_ptx.cuh"
+#include "device_info.h"
 #include "gemm_sm100.h"
 
 namespace lf {
@@ -390,19 +391,17 @@ static int launch_cfg(const GemmArgs& a, cudaStream_t stream) {
   p.alpha = a.alpha;
   p.status = a.status;
   auto kern = gemm_bf16_tcgen05_kernel<BN, A_MN, B_MN>;
-  // per device: the shared-memory opt-in of this instantiation and the SM count (a process may drive several GPUs)
+  // per device: the shared-memory opt-in of this instantiation (a process may drive several GPUs)
   constexpr int kMaxDev = 64;
   static bool attr_set[kMaxDev] = {};
-  static int num_sms[kMaxDev] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDev) return -4;
   if (!attr_set[dev]) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES);
     if (e != cudaSuccess) return -4;
-    cudaDeviceGetAttribute(&num_sms[dev], cudaDevAttrMultiProcessorCount, dev);
     attr_set[dev] = true;
   }
-  const int dev_sms = num_sms[dev];
+  const int dev_sms = sm_count();
   int sms = a.max_ctas > 0 ? (a.max_ctas < dev_sms ? a.max_ctas : dev_sms) : dev_sms;
   const int tiles = p.tiles_m * p.tiles_n;
   const int grid = tiles < sms ? tiles : sms;

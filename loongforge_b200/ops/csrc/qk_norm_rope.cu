@@ -21,6 +21,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include "device_info.h"
 #include "elementwise.h"
 
 namespace lf {
@@ -595,14 +596,14 @@ bool covered(const QkNormRopeArgs& a) { return (a.D == 64 || a.D == 128 || a.D =
 }  // namespace
 
 int qk_norm_rope_bwd_grid(QkNormRopeArgs& a) {
-  return a.T == 0 ? 0 : lay_out(a, 148 * 2);
+  return a.T == 0 ? 0 : lay_out(a, sm_count() * 2);
 }
 
 int qk_norm_rope_fwd(QkNormRopeArgs& a, cudaStream_t s) {
   if (!covered(a)) return -1;
   if (a.T > INT32_MAX / 2) return -2;
   if (a.T == 0) return 0;
-  const int blocks = lay_out(a, 148 * 3);
+  const int blocks = lay_out(a, sm_count() * 3);
   const int rc = a.D == 64 ? launch_fwd<4>(a, blocks, s) : a.D == 128 ? launch_fwd<8>(a, blocks, s) : launch_fwd<16>(a, blocks, s);
   if (rc != 0) return rc;
   return cudaGetLastError() == cudaSuccess ? 0 : -3;

@@ -21,6 +21,7 @@ formulation below, which is also what the kernels are tested against, and which 
 """
 from __future__ import annotations
 
+from operator import index
 from typing import Optional
 
 import torch
@@ -148,7 +149,7 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     """The tensor itself when its rows are unit-stride and 16-byte aligned (what the kernels read), else a copy. A dimension
     of one element may have any stride in a contiguous tensor: the strides themselves are looked at."""
     s = t.stride()
-    if t.data_ptr() % 16 == 0 and s[-1] == 1 and all(x % 8 == 0 for x in s[:-1]):
+    if s[-1] == 1 and not (s[0] | s[-2]) & 7 and t.data_ptr() % 16 == 0:  # two or three dimensions
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -189,7 +190,7 @@ def _host_bounds(cu_seqlens, T: int) -> list:
     if cu_seqlens is None:
         return [0, T]
     _whole(cu_seqlens, "cu_seqlens")
-    b = [int(x) for x in (cu_seqlens.tolist() if torch.is_tensor(cu_seqlens) else cu_seqlens)]
+    b = [index(x) for x in (cu_seqlens.tolist() if torch.is_tensor(cu_seqlens) else cu_seqlens)]
     if len(b) < 2 or b[0] < 0 or b[-1] > T or any(e < s for s, e in zip(b, b[1:])):
         raise ValueError(f"cu_seqlens must be at least two non-decreasing offsets within the {T} rows, got {b[:8]}...")
     return b
@@ -287,18 +288,19 @@ def _step_index(state_indices, rows: int, slots: int, device, native: bool) -> O
         if rows > slots:
             raise ValueError(f"{rows} rows need {rows} state slots, there are {slots}")
         return None
+    if native and torch.is_tensor(state_indices) and state_indices.is_cuda:
+        if state_indices.shape != (rows,):
+            raise ValueError(f"state_indices must hold one slot for each of the {rows} rows")
+        if state_indices.dtype == torch.int32 and state_indices.device == device and state_indices.is_contiguous():
+            return state_indices
+        _whole(state_indices, "state_indices")
+        return _int32(state_indices, device)
     _whole(state_indices, "state_indices")
-    if not (native and torch.is_tensor(state_indices) and state_indices.is_cuda):
-        idx = [int(i) for i in (state_indices.tolist() if torch.is_tensor(state_indices) else state_indices)]
-        used = [i for i in idx if i >= 0]
-        if len(idx) != rows or any(i >= slots for i in used) or len(set(used)) < len(used):
-            raise ValueError(f"state_indices must name {rows} different slots below {slots} (negative: no row)")
-        return torch.tensor(idx, dtype=torch.int32, device=device)
-    if state_indices.shape != (rows,):
-        raise ValueError(f"state_indices must hold one slot for each of the {rows} rows")
-    if state_indices.dtype == torch.int32 and state_indices.device == device and state_indices.is_contiguous():
-        return state_indices
-    return _int32(state_indices, device)
+    idx = [index(i) for i in (state_indices.tolist() if torch.is_tensor(state_indices) else state_indices)]
+    used = [i for i in idx if i >= 0]
+    if len(idx) != rows or any(i >= slots for i in used) or len(set(used)) < len(used):
+        raise ValueError(f"state_indices must name {rows} different slots below {slots} (negative: no row)")
+    return torch.tensor(idx, dtype=torch.int32, device=device)
 
 
 def _no_gradient(*tensors):

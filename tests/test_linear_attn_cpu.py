@@ -126,3 +126,7 @@ def test_numbers_that_are_not_whole_are_refused():
             LA.gated_delta_rule(q, k, v, g, beta, cu_seqlens=cu)
         with pytest.raises(ValueError, match="cu_seqlens must be whole"):
             LA.causal_conv1d(x, w, cu_seqlens=cu)
+    with pytest.raises(TypeError):
+        LA.gated_delta_rule_step(q, k, v, g, beta, pool, state_indices=[0, 1.5, 2])
+    with pytest.raises(TypeError):
+        LA.causal_conv1d(x, w, cu_seqlens=[0, 1.5, 3])

@@ -4,7 +4,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
-#include <atomic>
+#include "device_info.h"
 #include "linear_attn.h"
 
 namespace lf {
@@ -89,17 +89,6 @@ __device__ __forceinline__ void bar_wait(uint64_t* b, uint32_t parity, int* stat
     if (done) return;
   }
   *status = 1;
-}
-// Once per kernel and device: the call costs as much as a launch.
-template <typename K>
-bool allow_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return true;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess) return false;
-  done.fetch_or(bit, std::memory_order_relaxed);
-  return true;
 }
 
 }  // namespace delta

@@ -23,7 +23,6 @@
 // products have read that, and a unit's loads begin when its predecessor's products are done. What bounds it are these two
 // rounds of loads, which alternate with the products: 18K cycles a unit.
 #include <atomic>
-#include "device_info.h"
 #include "gated_delta.cuh"
 #include "sm100_ptx.cuh"
 

@@ -573,23 +573,24 @@ int lay_out(QkNormRopeArgs& a, int room) {
   return a.q_blocks + ks;
 }
 
-using Kernel = void (*)(QkNormRopeArgs);
-int launch(Kernel f, size_t bytes, const QkNormRopeArgs& a, int grid, cudaStream_t s) {
-  if (cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess) return -3;
-  f<<<static_cast<unsigned>(grid), THREADS, bytes, s>>>(a);
+template <auto KERNEL>
+int launch(size_t bytes, const QkNormRopeArgs& a, int grid, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed{0};
+  if (!allow_smem(KERNEL, bytes, allowed)) return -3;
+  KERNEL<<<static_cast<unsigned>(grid), THREADS, bytes, s>>>(a);
   return 0;
 }
 template <int LANES>
 int launch_fwd(const QkNormRopeArgs& a, int grid, cudaStream_t s) {
-  return launch(a.interleaved ? Kernel(qk_fwd_kernel<LANES, PAIRS>)
-                              : a.rot_dim % 16 == 0 ? Kernel(qk_fwd_kernel<LANES, HALVES>) : Kernel(qk_fwd_kernel<LANES, QUADS>),
-                sizeof(FwdSmem), a, grid, s);
+  if (a.interleaved) return launch<qk_fwd_kernel<LANES, PAIRS>>(sizeof(FwdSmem), a, grid, s);
+  if (a.rot_dim % 16 == 0) return launch<qk_fwd_kernel<LANES, HALVES>>(sizeof(FwdSmem), a, grid, s);
+  return launch<qk_fwd_kernel<LANES, QUADS>>(sizeof(FwdSmem), a, grid, s);
 }
 template <int LANES>
 int launch_bwd(const QkNormRopeArgs& a, int grid, cudaStream_t s) {
-  return launch(a.interleaved ? Kernel(qk_bwd_kernel<LANES, PAIRS>)
-                              : a.rot_dim % 16 == 0 ? Kernel(qk_bwd_kernel<LANES, HALVES>) : Kernel(qk_bwd_kernel<LANES, QUADS>),
-                sizeof(BwdSmem), a, grid, s);
+  if (a.interleaved) return launch<qk_bwd_kernel<LANES, PAIRS>>(sizeof(BwdSmem), a, grid, s);
+  if (a.rot_dim % 16 == 0) return launch<qk_bwd_kernel<LANES, HALVES>>(sizeof(BwdSmem), a, grid, s);
+  return launch<qk_bwd_kernel<LANES, QUADS>>(sizeof(BwdSmem), a, grid, s);
 }
 bool covered(const QkNormRopeArgs& a) { return (a.D == 64 || a.D == 128 || a.D == 256) && a.rot_dim <= a.D; }
 

@@ -64,3 +64,36 @@ def test_attention_layers_fused_norm_and_rotation(kind, monkeypatch):
     # ten such roundings relative to the probabilities, and as many again in the gradients
     for a, b in zip(fused, apart):
         assert (a.float() - b.float()).norm() < 20 * 2.0 ** -8 * b.float().norm()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_linear_attention_layer_trains_on_the_gpu(d, monkeypatch):
+    """Outputs and gradients of the layer over a packed row, on the kernels and with the delta rule and the convolution in
+    their PyTorch form on the same GPU, which differ by roundings to bf16."""
+    from loongforge_b200.models.transformer import PackedSeqParams
+    from loongforge_b200.ops import _ext
+    from loongforge_b200.ops import linear_attn as LA
+
+    cfg, net = layer("cuda", BF16, linear_key_head_dim=d, linear_value_head_dim=d)
+    torch.manual_seed(5)
+    lens = [70, 1, 130]
+    x, up = (torch.randn(sum(lens), cfg.hidden_size, device="cuda").to(BF16) for _ in range(2))
+    cu = torch.tensor([0] + lens).cumsum(0).to(device="cuda", dtype=torch.int32)
+
+    def run():
+        xi = x.clone().requires_grad_()
+        params = list(net.parameters())
+        y = net(xi, packed=PackedSeqParams(cu_seqlens=cu))
+        return [y.detach(), *torch.autograd.grad(y, [xi, *params], up)]
+
+    _ext.reset_launch_count()
+    on = run()
+    assert _ext.launch_count() >= 8  # convolution 1 + 2, delta rule 3 + 3 and their neighbours
+    _ext.check_status()
+    monkeypatch.setattr(LA, "gated_delta_rule_native", lambda *a: False)
+    monkeypatch.setattr(LA, "_conv_native", lambda *a: False)
+    off = run()
+    # the convolution's sum and its activation are rounded apart in the PyTorch form, q, k and v once more each; projections,
+    # norm and gates round in both: a handful of roundings of 2^-8, as in decoding, twice over on the way back
+    for n, a, b in zip(["y", "x"] + [n for n, _ in net.named_parameters()], on, off):
+        assert (a.float() - b.float()).norm() < 12 * 2.0 ** -8 * b.float().norm(), (n, (a.float() - b.float()).norm() / b.float().norm())

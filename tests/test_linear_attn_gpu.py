@@ -668,3 +668,20 @@ def test_gated_delta_rule_resets_among_mild_decays(strong):
 def test_gated_delta_rule_long_memory():
     """Heads as training leaves some: decays near one over thousands of tokens, where a state is the sum of hundreds."""
     check([2100], 1, 2, decay=1e-3)
+
+
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 64)])
+def test_gated_delta_rule_gradients_of_strided_rows(dk, dv):
+    """q, k and v as the layer cuts them out of the convolution's rows, and an upstream gradient laid out otherwise."""
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    T, hk, hv = 150, 2, 4
+    rows = randn(gen, T, 2 * hk * dk + hv * dv, dtype=BF16).requires_grad_()
+    g, beta = -torch.rand(T, hv, device="cuda"), torch.rand(T, hv, device="cuda")
+    cu = torch.tensor([0, 70, 150], device="cuda")
+    up = randn(gen, hv, T, dv, dtype=BF16).transpose(0, 1)
+    cut = lambda x: (x[:, :hk * dk].view(T, hk, dk), x[:, hk * dk:2 * hk * dk].view(T, hk, dk), x[:, 2 * hk * dk:].view(T, hv, dv))  # noqa: E731
+    o = LA.gated_delta_rule(*cut(rows), g, beta, cu_seqlens=cu)
+    got = torch.autograd.grad(o, rows, up)[0]
+    whole = [t.detach().contiguous().requires_grad_() for t in cut(rows)]
+    want = torch.autograd.grad(LA.gated_delta_rule(*whole, g, beta, cu_seqlens=cu), whole, up.contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(cut(got), want))

@@ -38,6 +38,14 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
   lo = pack2(x - lo_half(hi), y - hi_half(hi));
 }
+// With the remainder of the second rounding too: x and y but for 2^-26.
+__device__ __forceinline__ void split3(float x, float y, uint32_t& hi, uint32_t& lo, uint32_t& rest) {
+  asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+  x -= lo_half(hi);
+  y -= hi_half(hi);
+  lo = pack2(x, y);
+  rest = pack2(x - lo_half(lo), y - hi_half(lo));
+}
 struct Span {
   int n;            // sequence
   long long start;  // first token of the chunk

@@ -92,6 +92,14 @@ __device__ __forceinline__ void stsm_t(uint32_t addr, const uint4& r) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
 }
 
+// The two parts of eight fp32 values of U.
+__device__ __forceinline__ void split_u(const uint4& x, const uint4& y, uint4& hi, uint4& lo) {
+  split2(__uint_as_float(x.x), __uint_as_float(x.y), hi.x, lo.x);
+  split2(__uint_as_float(x.z), __uint_as_float(x.w), hi.y, lo.y);
+  split2(__uint_as_float(y.x), __uint_as_float(y.y), hi.z, lo.z);
+  split2(__uint_as_float(y.z), __uint_as_float(y.w), hi.w, lo.w);
+}
+
 // The block's (chunk, key head) pairs, every gridDim.x-th, without a division each.
 struct Item {
   int c, hk, dc, dh;
@@ -292,7 +300,7 @@ tc_dqk_kernel(const DeltaArgs a) {
       for (int hr = 0; hr < rep; ++hr, ++u) {
         const int h = hk * rep + hr;
         const long long rec = static_cast<long long>(c) * a.Hv + h;
-        // U: 8 tiles of columns x 4 of tokens x 2 parts; v the same of one part; the states: 8 tiles of columns x 2 parts x 8 of dk
+        // U, in fp32: 8 tiles of columns x 4 of tokens x 2; v the same, one each; the states: 8 tiles of columns x 2 parts x 8 of dk
         uint4 fu[MINE], fs[MINE];
         const uint4* us = reinterpret_cast<const uint4*>(a.u) + rec * 8 * 256 + lane;
         const uint4* vs = reinterpret_cast<const uint4*>(a.dv_lo) + rec * 8 * 128 + lane;
@@ -313,9 +321,12 @@ tc_dqk_kernel(const DeltaArgs a) {
           }
         };
 #pragma unroll
-        for (int j = 0; j < MINE; ++j) {
+        for (int j = 0; j < VMINE; ++j) {
           const int t = lw + LOAD_WARPS * j;
-          if (t < TILES) fu[j] = us[32 * t];
+          if (t < VTILES) {
+            fu[2 * j] = us[64 * t];
+            fu[2 * j + 1] = us[64 * t + 32];
+          }
         }
         take_state(fs, ss, 0);
         // the last head's products have read the tiles; D1 of it waited until the vec of two heads ago was read
@@ -334,10 +345,15 @@ tc_dqk_kernel(const DeltaArgs a) {
         if (tid < DELTA_VEC / 4) cp16(&sm.vec[u & 1][tid * 4], a.vec + rec * DELTA_VEC + tid * 4, true);
         cp_commit();
 #pragma unroll
-        for (int j = 0; j < MINE; ++j) {
-          const int f = lw + LOAD_WARPS * j;
-          const int t = 64 * (f & 1) + 16 * ((f >> 1) & 3) + (m >> 1) * 8 + l8, v = 16 * (f >> 3) + (m & 1) * 8;
-          if (f < TILES) stsm_t(xu + (v >> 6) * BIG + piece_at(t, (v >> 3) & 7), fu[j]);
+        for (int j = 0; j < VMINE; ++j) {
+          const int f = lw + LOAD_WARPS * j, t = 16 * (f & 3) + (m >> 1) * 8 + l8, v = 16 * (f >> 2) + (m & 1) * 8;
+          const uint32_t at = xu + (v >> 6) * BIG + piece_at(t, (v >> 3) & 7);
+          uint4 hi, lo;
+          split_u(fu[2 * j], fu[2 * j + 1], hi, lo);
+          if (f < VTILES) {
+            stsm_t(at, hi);
+            stsm_t(at + BOX, lo);  // 64 rows further on
+          }
         }
 #pragma unroll
         for (int j = 0; j < VMINE; ++j) {

@@ -37,16 +37,18 @@
 //   dqk       dQ and dK, parallel over chunks: in gated_delta_dqk_sm100.cu for dk = dv = 128, here where either is 64.
 //   gates     dg and dbeta.
 //
-// Precision. The state, U, X and all products along the chain carry 16 or more bits: an fp32 operand is cut into a bf16
-// high and low part (relative remainder 2^-18) and multiplied in two passes where the other operand is a bf16 input
-// (q, k, do), in three where both are cut, in dQ and dK too: with decays near one the terms of S0 and dS1 are the main ones
-// there. What is left out is 2^-18 of an operand: states, dg and dbeta come out within 2e-6 to 9e-6 (2-norm), where fp32
-// throughout has 2e-7 to 5e-7, and dq and dk as their rounding to bf16 leaves them.
+// Precision. Sums and the state are fp32. An fp32 operand of a product is cut into bf16 parts: r, U and its scaled copy, dU
+// and P into three (24 bits), since they make up the results as they are; the state, A, dS1 and what is added to it, whose
+// remainder of 2^-18 goes through a decay first, into two; dQ and dK take two parts of everything, which is far below their
+// rounding. Products of parts below 2^-24 are left out. The third parts of P lie in the blocks of its tiles that no product
+// reads, those of r, U and dU in shared memory of their own; they cost 22 us forward and 12 backward of what stands below at
+// 4096 tokens. With the gates of a new layer states, dg and dbeta come out within 1e-7, 5e-7 and 1.4e-7 (2-norm; 2e-6 to 6e-6
+// with two parts everywhere), as with fp32 products; with decays of 1e-3 a token, within 2e-6, 4e-6 and 4e-6.
 //
 // The chain is bound by latency: three dependent products of at most 64 x 128 x 16 per chunk, with a hand-over between
-// them, 5.8K cycles a chunk forward and 7.5K backward. mma.sync runs at a quarter of tcgen05's rate, but operands and results
+// them, 6.5K cycles a chunk forward and 8K backward. mma.sync runs at a quarter of tcgen05's rate, but operands and results
 // stay in registers, and 32 heads make 1024 warps of such work. One sequence of 4096 tokens with 32 heads of 128 x 128 (five
-// sequences of 16384): prepare 38 us (131), forward 190 (656), backward 257 (884; 238 and 826 without the low parts
+// sequences of 16384): prepare 39 us (137), forward 212 (750), backward 270 (920; 238 and 826 without the low parts
 // that dqk reads), dqk 138 (520), gates 8 (16). Measured against it: a whole unit in one warp 471 (959) forward and 620
 // (1278) backward; eight warps along the chain and eight beside it 208 (713) and 257 (874), bound by shared memory; a head
 // as one 128-column product on tcgen05 11.7K cycles a chunk, 5K of them the work on elements between the products, on an
@@ -103,6 +105,21 @@ __device__ __forceinline__ void split_a(const float (&c0)[4], const float (&c1)[
   split2(c0[2], c0[3], hi[1], lo[1]);
   split2(c1[0], c1[1], hi[2], lo[2]);
   split2(c1[2], c1[3], hi[3], lo[3]);
+}
+
+// The same with the remainder of the second rounding as a third part: the fp32 values themselves, but for 2^-26.
+__device__ __forceinline__ void split_a3(const float (&c0)[4], const float (&c1)[4], uint32_t (&hi)[4], uint32_t (&lo)[4], uint32_t (&rest)[4]) {
+  split3(c0[0], c0[1], hi[0], lo[0], rest[0]);
+  split3(c0[2], c0[3], hi[1], lo[1], rest[1]);
+  split3(c1[0], c1[1], hi[2], lo[2], rest[2]);
+  split3(c1[2], c1[3], hi[3], lo[3], rest[3]);
+}
+
+// A strictly lower 64 x 64 matrix in two tiles, high and low parts: the blocks of 16 x 16 above the diagonal are never read
+// as such, and hold what is left of the values, those of block (i, j) below the diagonal at (j, i) of the high parts' tile,
+// those of the diagonal ones in the low parts' tile. Returns the place of block (i, j), i >= j.
+__device__ __forceinline__ int rest_block(int i, int j) {
+  return i > j ? 16 * j * APITCH + 16 * i : C * APITCH + (i < 3 ? 16 * (i + 1) : 16 * APITCH + 32);
 }
 
 // acc[2 * NT] += (hi + lo) x B for 2 * NT column tiles: one pass over all of them, then the other, so that no product
@@ -438,10 +455,13 @@ prepare_kernel(const DeltaArgs a) {
           if (i == jj) vec[V_PD * 64 + i] = pv;
         }
         *reinterpret_cast<float2*>(M + i * MMP + j0) = make_float2(m[0], m[1]);
-        uint32_t hi, lo;
-        split2(p[0], p[1], hi, lo);
-        *reinterpret_cast<uint32_t*>(Ps + i * APITCH + j0) = hi;
-        *reinterpret_cast<uint32_t*>(Ps + C * APITCH + i * APITCH + j0) = lo;
+        if ((j >> 1) <= warp) {  // the block holds or meets the diagonal
+          uint32_t hi, lo, rest;
+          split3(p[0], p[1], hi, lo, rest);
+          *reinterpret_cast<uint32_t*>(Ps + i * APITCH + j0) = hi;
+          *reinterpret_cast<uint32_t*>(Ps + C * APITCH + i * APITCH + j0) = lo;
+          *reinterpret_cast<uint32_t*>(Ps + rest_block(warp, j >> 1) + (i & 15) * APITCH + (j0 & 15)) = rest;
+        }
       }
     }
     *reinterpret_cast<uint4*>(Ps + tid * APITCH + C) = make_uint4(0, 0, 0, 0);
@@ -511,7 +531,7 @@ __device__ __forceinline__ void load_vec(float* dst, const float* src, int rows)
 
 // A unit is 16 columns of dv of one head and four warps. Warp w holds columns [w dk/4, (w + 1) dk/4) of the unit's state
 // S^T [16, dk] in fp32, and makes everything that is per token for tokens [16 w, 16 w + 16) of a chunk. What the others
-// need of it (the state, R, U) goes through shared memory as ready A operands, high and low part, 16 bytes a lane.
+// need of it (the state, R, U) goes through shared memory as ready A operands, two or three parts, 16 bytes a lane each.
 struct Operands {  // one k step of 16
   uint4 hi[32], lo[32];
 };
@@ -519,6 +539,22 @@ __device__ __forceinline__ void put(Operands& x, const uint32_t (&hi)[4], const 
   const int lane = threadIdx.x & 31;
   x.hi[lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
   x.lo[lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+struct Operands3 {
+  uint4 hi[32], lo[32], rest[32];
+};
+__device__ __forceinline__ void put(Operands3& x, const uint32_t (&hi)[4], const uint32_t (&lo)[4], const uint32_t (&rest)[4]) {
+  const int lane = threadIdx.x & 31;
+  x.hi[lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  x.lo[lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  x.rest[lane] = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+}
+__device__ __forceinline__ void get(const Operands3& x, uint32_t (&hi)[4], uint32_t (&lo)[4], uint32_t (&rest)[4]) {
+  const int lane = threadIdx.x & 31;
+  const uint4 h = x.hi[lane], l = x.lo[lane], r = x.rest[lane];
+  hi[0] = h.x; hi[1] = h.y; hi[2] = h.z; hi[3] = h.w;
+  lo[0] = l.x; lo[1] = l.y; lo[2] = l.z; lo[3] = l.w;
+  rest[0] = r.x; rest[1] = r.y; rest[2] = r.z; rest[3] = r.w;
 }
 __device__ __forceinline__ void get(const Operands& x, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
   const int lane = threadIdx.x & 31;
@@ -560,19 +596,27 @@ __device__ __forceinline__ void store_tile(bf16* stage, bf16* out, long long str
   const int lane = threadIdx.x & 31, row = lane >> 1, v = (lane & 1) * 8;
   if (row < len) *reinterpret_cast<uint4*>(out + row * stride + v) = *reinterpret_cast<const uint4*>(stage + row * OUT_PITCH + v);
 }
-// U = beta (v - m) of two neighbouring tokens of one column, m from its parts.
-__device__ __forceinline__ void memory_term(uint32_t v, uint32_t mh, uint32_t ml, float2 beta, float& u0, float& u1) {
-  u0 = beta.x * (lo_half(v) - (lo_half(mh) + lo_half(ml)));
-  u1 = beta.y * (hi_half(v) - (hi_half(mh) + hi_half(ml)));
-}
-
-// The fp32 values of a fragment's two parts.
-__device__ __forceinline__ void join(const uint4& hi, const uint4& lo, float (&c)[2][4]) {
-  const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+// The fp32 values of a fragment's three parts.
+__device__ __forceinline__ void join(const uint32_t (&hi)[4], const uint32_t (&lo)[4], const uint32_t (&rest)[4], float (&c)[2][4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    c[i >> 1][2 * (i & 1)] = lo_half(h[i]) + lo_half(l[i]);
-    c[i >> 1][2 * (i & 1) + 1] = hi_half(h[i]) + hi_half(l[i]);
+    c[i >> 1][2 * (i & 1)] = lo_half(hi[i]) + (lo_half(lo[i]) + lo_half(rest[i]));
+    c[i >> 1][2 * (i & 1) + 1] = hi_half(hi[i]) + (hi_half(lo[i]) + hi_half(rest[i]));
+  }
+}
+// Accumulators as they are kept for the backward pass, and back.
+__device__ __forceinline__ void keep(uint4* dst, const float (&c)[2][4]) {
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+    dst[32 * f] = make_uint4(__float_as_uint(c[f][0]), __float_as_uint(c[f][1]), __float_as_uint(c[f][2]), __float_as_uint(c[f][3]));
+}
+__device__ __forceinline__ void kept(const uint4 (&x)[2], float (&c)[2][4]) {
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    c[f][0] = __uint_as_float(x[f].x);
+    c[f][1] = __uint_as_float(x[f].y);
+    c[f][2] = __uint_as_float(x[f].z);
+    c[f][3] = __uint_as_float(x[f].w);
   }
 }
 
@@ -620,7 +664,8 @@ struct FwdStage {
 template <int DK, int NU>
 struct FwdSmem {
   FwdStage<DK, NU> stage[2];
-  Operands state[NU][DK / 16], r[NU][4], u[NU][4], su[NU][4];
+  Operands state[NU][DK / 16];
+  Operands3 r[NU][4], u[NU][4], su[NU][4];
   bf16 out[NU * 4][16 * OUT_PITCH];
   uint64_t full[2], empty[2], state_ready[NU], r_ready[NU], u_ready[NU];
 };
@@ -747,9 +792,9 @@ forward_kernel(const DeltaArgs a) {
       u[f][2] = be[f].x * (lo_half(v[2 * f + 1]) - y[f][2]);
       u[f][3] = be[f].y * (hi_half(v[2 * f + 1]) - y[f][3]);
     }
-    uint32_t rh[4], rl[4];  // the warp's own part of r
-    split_a(u[0], u[1], rh, rl);
-    put(sm.r[unit][w], rh, rl);
+    uint32_t rh[4], rl[4], rr[4];  // the warp's own part of r
+    split_a3(u[0], u[1], rh, rl, rr);
+    put(sm.r[unit][w], rh, rl, rr);
     bar_arrive(&sm.r_ready[unit]);
     // while the others get there: (A - I) r with the warp's own part, the rest of A, and e^G Q S. The output is made for
     // tokens [tok2, tok2 + 16), mirrored: the warp with the most of A has the least of P.
@@ -773,24 +818,27 @@ forward_kernel(const DeltaArgs a) {
       mma_pair(m, rh, b);
       mma_pair(m2, rl, b);
       mma_pair(m3, rh, bl);
+      mma_pair(m2, rr, b);
+      mma_pair(m3, rl, bl);
     }
     float2 f2[2], ib[2];
 #pragma unroll
     for (int f = 0; f < 2; ++f) ib[f] = make_float2(__fdividef(1.f, be[f].x), __fdividef(1.f, be[f].y));
     factors(vec + V_SU * 64, f2);
     bar_wait(&sm.r_ready[unit], parity, a.status);
-    // (A - I) r; y becomes the memory read at each token, m = e^G K S - ((A - I) r) / beta, in 16 bits, and U is
-    // beta (V - m), made of the rounded m and used in two parts everywhere: the products of dg must see the same U.
+    // (A - I) r; the memory read at each token is m = e^G K S - ((A - I) r) / beta, and U = beta (V - m), which enters its
+    // products in three parts: what they and the sums of dg see of U must be the same to fp32.
 #pragma unroll
     for (int kk = 0; kk < 3; ++kk)
       if (kk < w) {
-        uint32_t hi[4], lo[4];
-        get(sm.r[unit][kk], hi, lo);
+        uint32_t hi[4], lo[4], rest[4];
+        get(sm.r[unit][kk], hi, lo, rest);
         mma_pair(m, hi, ab[kk][0]);
         mma_pair(m2, lo, ab[kk][0]);
         mma_pair(m3, hi, ab[kk][1]);
+        mma_pair(m2, rest, ab[kk][0]);
+        mma_pair(m3, lo, ab[kk][1]);
       }
-    uint32_t mh[4], ml[4], uh[4], ul[4];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
       m[f][0] = y[f][0] - (m[f][0] + (m2[f][0] + m3[f][0])) * ib[f].x;
@@ -798,22 +846,24 @@ forward_kernel(const DeltaArgs a) {
       m[f][2] = y[f][2] - (m[f][2] + (m2[f][2] + m3[f][2])) * ib[f].x;
       m[f][3] = y[f][3] - (m[f][3] + (m2[f][3] + m3[f][3])) * ib[f].y;
     }
-    split_a(m[0], m[1], mh, ml);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) memory_term(v[i], mh[i], ml[i], be[i >> 1], u[i >> 1][2 * (i & 1)], u[i >> 1][2 * (i & 1) + 1]);
+    for (int i = 0; i < 4; ++i) {
+      u[i >> 1][2 * (i & 1)] = be[i >> 1].x * (lo_half(v[i]) - m[i >> 1][2 * (i & 1)]);
+      u[i >> 1][2 * (i & 1) + 1] = be[i >> 1].y * (hi_half(v[i]) - m[i >> 1][2 * (i & 1) + 1]);
+    }
     {
       float su[2][4];
-      uint32_t hi[4], lo[4];
+      uint32_t hi[4], lo[4], rest[4];
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) su[f][e] = u[f][e];
       scale_tokens(su, f2);
-      split_a(su[0], su[1], hi, lo);
-      put(sm.su[unit][w], hi, lo);
+      split_a3(su[0], su[1], hi, lo, rest);
+      put(sm.su[unit][w], hi, lo, rest);
+      split_a3(u[0], u[1], hi, lo, rest);
+      put(sm.u[unit][w], hi, lo, rest);
     }
-    split_a(u[0], u[1], uh, ul);
-    put(sm.u[unit][w], uh, ul);
     bar_arrive(&sm.u_ready[unit]);
     // meanwhile: K for the state, e^G Q S, and what is kept
     const float ge = x.vec[V_END * 64];
@@ -840,13 +890,18 @@ forward_kernel(const DeltaArgs a) {
     // S^T <- e^{G_C} S^T + (e^{G_C - G} U)^T K, the warp's columns of dk
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
-      uint32_t hi[4], lo[4];
-      get(sm.su[unit][kk], hi, lo);
+      uint32_t hi[4], lo[4], rest[4];
+      get(sm.su[unit][kk], hi, lo, rest);
       mma2<KW>(s, hi, lo, bt[kk]);
+#pragma unroll
+      for (int j = 0; j < KW; ++j) {
+        mma(s[2 * j], rest, bt[kk][j][0], bt[kk][j][1]);
+        mma(s[2 * j + 1], rest, bt[kk][j][2], bt[kk][j][3]);
+      }
     }
     if (c + 1 < chunks) publish_state();
-    // what earlier tokens give to the output: + (P - diag P) U, with all four parts: the backward pass multiplies with
-    // this P and this U too
+    // what earlier tokens give to the output: + (P - diag P) U, but for what is below 2^-26 of it: the backward pass
+    // multiplies with this P too
     add_to(o, z);
     factors(vec2 + V_OQ * 64, f2);
     scale_tokens(o, f2);
@@ -856,35 +911,32 @@ forward_kernel(const DeltaArgs a) {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
       if (kk <= 3 - w) {
-        uint32_t hi[4], lo[4], b[4], bl[4];
+        uint32_t hi[4], lo[4], rest[4], b[4], bl[4];
         b_from_nk(b, phi, APITCH, tok2, 16 * kk);
         b_from_nk(bl, plo, APITCH, tok2, 16 * kk);
-        get(sm.u[unit][kk], hi, lo);
+        get(sm.u[unit][kk], hi, lo, rest);
         mma_pair(o, hi, b);
         mma_pair(z, lo, b);
         mma_pair(m2, hi, bl);
         mma_pair(m3, lo, bl);
+        mma_pair(m3, rest, b);
+        b_from_nk(b, phi + rest_block(3 - w, kk), APITCH, 0, 0);
+        mma_pair(m2, hi, b);
       }
     add_to(m2, m3);
     add_to(z, m2);
     add_to(o, z);
     if (KEEP) {
       const long long piece = (((c0 + c) * a.Hv + h) * (a.dv / 16) + (col0 >> 4)) * 4;
-      uint4* mf = reinterpret_cast<uint4*>(a.mem) + (piece + w) * 64 + lane;
-      mf[0] = make_uint4(mh[0], mh[1], mh[2], mh[3]);
-      mf[32] = make_uint4(ml[0], ml[1], ml[2], ml[3]);
-      uint4* uf = reinterpret_cast<uint4*>(a.u) + (piece + w) * 64 + lane;
-      uf[0] = make_uint4(uh[0], uh[1], uh[2], uh[3]);
-      uf[32] = make_uint4(ul[0], ul[1], ul[2], ul[3]);
-      uint4* pf = reinterpret_cast<uint4*>(a.past) + (piece + 3 - w) * 64 + lane;
-      pf[0] = make_uint4(__float_as_uint(o[0][0]), __float_as_uint(o[0][1]), __float_as_uint(o[0][2]), __float_as_uint(o[0][3]));
-      pf[32] = make_uint4(__float_as_uint(o[1][0]), __float_as_uint(o[1][1]), __float_as_uint(o[1][2]), __float_as_uint(o[1][3]));
+      keep(reinterpret_cast<uint4*>(a.mem) + (piece + w) * 64 + lane, m);
+      keep(reinterpret_cast<uint4*>(a.u) + (piece + w) * 64 + lane, u);
+      keep(reinterpret_cast<uint4*>(a.past) + (piece + 3 - w) * 64 + lane, o);
       if (c + 1 < chunks) keep_state(c + 1);
     }
     {
-      uint32_t hi[4], lo[4];
-      get(sm.u[unit][3 - w], hi, lo);
-      join(make_uint4(hi[0], hi[1], hi[2], hi[3]), make_uint4(lo[0], lo[1], lo[2], lo[3]), u);
+      uint32_t hi[4], lo[4], rest[4];
+      get(sm.u[unit][3 - w], hi, lo, rest);
+      join(hi, lo, rest, u);
     }
     factors(vec2 + V_PD * 64, f2);
 #pragma unroll
@@ -919,7 +971,8 @@ struct BwdStage {
 template <int DK, int NU>
 struct BwdSmem {
   BwdStage<DK, NU> stage[2];
-  Operands state[NU][DK / 16], du[NU][4], dv[NU][4], go[NU][4];
+  Operands state[NU][DK / 16], dv[NU][4], go[NU][4];
+  Operands3 du[NU][4];
   bf16 out[NU * 4][16 * OUT_PITCH];
   uint64_t full[2], empty[2], state_ready[NU], du_ready[NU], dv_ready[NU];
 };
@@ -1054,6 +1107,8 @@ backward_kernel(const DeltaArgs a) {
         b_from_kn(bl, plo, APITCH, 16 * kk, tok);
         mma_pair(u, f, b);
         mma_pair(z, f, bl);
+        b_from_kn(b, phi + rest_block(kk, w), APITCH, 0, 0);
+        mma_pair(z, f, b);
       }
     a_from_km(fo, x.dO, VP, tok, unit * 16);
     float2 f2[2], su[2], be[2];
@@ -1090,22 +1145,22 @@ backward_kernel(const DeltaArgs a) {
     scale_tokens(y, su);
     // dU^T = y + u + (diag P dO)^T
     add_to(u, y);
-    uint32_t dh[4], dl[4];
+    uint32_t dh[4], dl[4], dr[4];
     {
       float d[2][4];
 #pragma unroll
       for (int f = 0; f < 2; ++f)
 #pragma unroll
         for (int e = 0; e < 4; ++e) d[f][e] = u[f][e] + du[f][e];
-      split_a(d[0], d[1], dh, dl);
-      put(sm.du[unit][w], dh, dl);
+      split_a3(d[0], d[1], dh, dl, dr);
+      put(sm.du[unit][w], dh, dl, dr);
     }
     bar_arrive(&sm.du_ready[unit]);
     // while the others get there: U + dU^T (A - I) begins with the warp's own part
     const float ge = x.vec[V_END * 64];
     float mm[2][4], uu[2][4];
-    join(now.m[0], now.m[1], mm);
-    join(now.u[0], now.u[1], uu);
+    kept(now.m, mm);
+    kept(now.u, uu);
     float sdot = 0.f, bdot = 0.f;
 #pragma unroll
     for (int f = 0; f < 2; ++f)
@@ -1127,6 +1182,8 @@ backward_kernel(const DeltaArgs a) {
       mma_pair(u, dh, b);
       mma_pair(y, dl, b);
       mma_pair(z, dh, bl);
+      mma_pair(y, dr, b);
+      mma_pair(z, dl, bl);
     }
     factors(vec + V_BETA * 64, be);
     factors(vec + V_YK * 64, f2);
@@ -1135,11 +1192,13 @@ backward_kernel(const DeltaArgs a) {
 #pragma unroll
     for (int kk = 1; kk < 4; ++kk)
       if (kk > w) {
-        uint32_t hi[4], lo[4];
-        get(sm.du[unit][kk], hi, lo);
+        uint32_t hi[4], lo[4], rest[4];
+        get(sm.du[unit][kk], hi, lo, rest);
         mma_pair(u, hi, ab[kk - 1][0]);
         mma_pair(y, lo, ab[kk - 1][0]);
         mma_pair(z, hi, ab[kk - 1][1]);
+        mma_pair(y, rest, ab[kk - 1][0]);
+        mma_pair(z, lo, ab[kk - 1][1]);
       }
     add_to(y, z);
     add_to(u, y);
@@ -1273,18 +1332,28 @@ __device__ __forceinline__ void load_fragments(bf16* hi, bf16* lo, const uint4* 
   }
 }
 
-// PARTS fragments of every 16 columns and 16 tokens -> [DV][64 tokens] rows of pitch APITCH: U^T and its remainder, or that
-// of dV^T alone.
-template <int DV, int PARTS>
-__device__ __forceinline__ void load_tokens(bf16* first, bf16* second, const uint4* src) {
-  for (int i = threadIdx.x; i < DV / 16 * 4 * PARTS * 32; i += DQK_THREADS) {
-    const int lane = i & 31, part = (i >> 5) % PARTS, w = (i >> 5) / PARTS & 3, vt = (i >> 5) / (4 * PARTS), g = lane >> 2, t2 = (lane & 3) * 2;
-    const uint4 f = src[i];
-    bf16* p = (part ? second : first) + (vt * 16 + g) * APITCH + w * 16 + t2;
-    *reinterpret_cast<uint32_t*>(p) = f.x;
-    *reinterpret_cast<uint32_t*>(p + 8 * APITCH) = f.y;
-    *reinterpret_cast<uint32_t*>(p + 8) = f.z;
-    *reinterpret_cast<uint32_t*>(p + 8 * APITCH + 8) = f.w;
+// A fragment of 16 columns and 16 tokens to [DV][64 tokens] rows of pitch APITCH.
+__device__ __forceinline__ void put_tokens(bf16* tile, int vt, int w, int lane, const uint32_t (&f)[4]) {
+  bf16* p = tile + (vt * 16 + (lane >> 2)) * APITCH + w * 16 + (lane & 3) * 2;
+  *reinterpret_cast<uint32_t*>(p) = f[0];
+  *reinterpret_cast<uint32_t*>(p + 8 * APITCH) = f[1];
+  *reinterpret_cast<uint32_t*>(p + 8) = f[2];
+  *reinterpret_cast<uint32_t*>(p + 8 * APITCH + 8) = f[3];
+}
+// U^T, kept in fp32, in its two parts; and what the rounding of dV^T left.
+template <int DV>
+__device__ __forceinline__ void load_tokens(bf16* uh, bf16* ul, bf16* dvl, const uint4* u, const uint4* v) {
+  for (int i = threadIdx.x; i < DV / 16 * 128; i += DQK_THREADS) {
+    const int lane = i & 31, w = (i >> 5) & 3, vt = i >> 7;
+    const uint4 x[2] = {u[(i >> 5) * 64 + lane], u[(i >> 5) * 64 + 32 + lane]}, y = v[i];
+    float c[2][4];
+    kept(x, c);
+    uint32_t hi[4], lo[4];
+    split_a(c[0], c[1], hi, lo);
+    put_tokens(uh, vt, w, lane, hi);
+    put_tokens(ul, vt, w, lane, lo);
+    const uint32_t d[4] = {y.x, y.y, y.z, y.w};
+    put_tokens(dvl, vt, w, lane, d);
   }
 }
 
@@ -1317,8 +1386,8 @@ dqk_kernel(const DeltaArgs a) {
     load_rows<DV, DQK_THREADS>(x.dV, VP, static_cast<const bf16*>(a.dv_) + row, stride, sp.len);
     load_vec<DQK_THREADS>(x.vec, a.vec + rec * DELTA_VEC, 8);
     cp_commit();
-    load_tokens<DV, 2>(x.u, x.ul, reinterpret_cast<const uint4*>(a.u) + rec * (DV / 16) * 256);
-    load_tokens<DV, 1>(x.dVl, nullptr, reinterpret_cast<const uint4*>(a.dv_lo) + rec * (DV / 16) * 128);
+    load_tokens<DV>(x.u, x.ul, x.dVl, reinterpret_cast<const uint4*>(a.u) + rec * (DV / 16) * 256,
+                    reinterpret_cast<const uint4*>(a.dv_lo) + rec * (DV / 16) * 128);
     load_fragments<DK, DV>(x.s0, x.s0l, reinterpret_cast<const uint4*>(a.states) + rec * (DV / 16) * 2 * KT * 32);
     load_fragments<DK, DV>(x.ds, x.dsl, reinterpret_cast<const uint4*>(a.dstates) + rec * (DV / 16) * 2 * KT * 32);
     cp_wait<0>();

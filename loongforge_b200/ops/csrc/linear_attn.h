@@ -24,8 +24,8 @@ struct DeltaArgs {
   float* s_out = nullptr;       // [N, Hv, dk, dv] or null
   void *o = nullptr;            // bf16 [T, Hv, dv]
   // Kept for the backward pass (all or none), as the fragments that one warp's lanes hold, [NC, Hv, dv / 16, 4, ..., 32]:
-  // what o owes to earlier tokens (fp32), the memory read at each token and U (bf16 and the remainder of the rounding);
-  // and the state in front of every chunk.
+  // what o owes to earlier tokens, the memory read at each token and U (fp32); and the state in front of every chunk (bf16
+  // and the remainder of the rounding).
   void *past = nullptr, *mem = nullptr, *u = nullptr, *states = nullptr;
   void* qk = nullptr;    // bf16 [NC, Hk, 2, 64, dk + DELTA_ROW_PAD]: q and k of every chunk, rows behind its end zero
   void* ap = nullptr;    // bf16 [NC, Hv, DELTA_AP]
@@ -35,7 +35,7 @@ struct DeltaArgs {
   const float* ds_out = nullptr;  // gradient of s_out or null
   float* ds_in = nullptr;         // gradient of s_in or null
   void* dstates = nullptr;      // the gradients of the states behind every chunk, as `states`
-  void* dv_lo = nullptr;        // what the rounding of dv_ left, fragments of half the size of `u`
+  void* dv_lo = nullptr;        // what the rounding of dv_ left, in bf16: fragments of half the size of `u`
   float* rowdots = nullptr;     // fp32 [NC, Hv, dv / 16, 2, 64]
   float* sdots = nullptr;       // fp32 [NC, Hv, dv / 16, 4]
   void *dq = nullptr, *dkey = nullptr, *dv_ = nullptr;  // bf16, contiguous

@@ -235,9 +235,10 @@ def gated_delta_rule(q, k, v, g, beta, *, cu_seqlens=None, scale: Optional[float
     two states) are kept until the backward pass, which itself works on ``4 dk dv + 161 dv`` more. With 16 / 32 heads of 128
     that is 7 MB a chunk: 1.8 GB for one row of 16,384 tokens, 29 GB for 4,096 sequences of one token.
 
-    Precision there: sums and the state along the sequence are fp32; the products take operands of 16 bits (two bf16 parts)
-    or bf16 inputs as they are. Results in bf16 are as exact as their rounding; final states, dg and dbeta are within 1e-5
-    (2-norm), about 20 times what fp32 products give. Inputs in fp32 take the PyTorch form, in fp32 throughout.
+    Precision there: sums and the state along the sequence are fp32; the products take bf16 inputs as they are, and of fp32
+    operands 24 bits or, behind a decay, 16 (three or two bf16 parts). Results in bf16 are as exact as their rounding. Final
+    states, dg and dbeta are within 1e-6 (2-norm) for heads that forget within some hundred tokens, as fp32 products give
+    them, and within 5e-6, ten times that, for decays near one. Inputs in fp32 take the PyTorch form, in fp32 throughout.
     """
     _check_delta(q, k, v, g, beta, "T")
     T, _, dk = q.shape

@@ -125,6 +125,26 @@ def test_gated_delta_rule_key_and_query_gradients_element_by_element(dk, dv, dec
         assert (off <= b.abs().max() * 2.0 ** -11).all(), (name, (off.max() / b.abs().max()).item() * 2.0 ** 11)
 
 
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128)])
+def test_gated_delta_rule_fp32_results_with_the_gates_of_a_new_layer(dk, dv):
+    """Gradients of the gates and final states where heads forget within some tokens, as the layer starts: U, what it is made
+    of and P enter their products with 24 bits, and what is still cut to 16 (the state, the inverse, the state's gradient)
+    carries a decay, so that its 2^-18 counts half at most."""
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    q, k, v, _, _, do, cu = make([300, 64, 90], 2, 4, dk, dv, 15)
+    x = torch.nn.functional.softplus(torch.randn(454, 4, generator=gen, device="cuda") + 1)
+    g, beta = -x * torch.tensor([4.0, 8.0, 12.0, 16.0], device="cuda"), torch.rand(454, 4, generator=gen, device="cuda").sigmoid()
+    s0 = randn(gen, 3, 4, dk, dv, scale=0.1)
+    ins = [t.requires_grad_() for t in (q, k, v, g, beta)]
+    o, last = LA.gated_delta_rule(*ins, cu_seqlens=cu, initial_state=s0, output_final_state=True)
+    got = torch.autograd.grad(o, ins[3:], do)
+    rins = [t.detach().double().requires_grad_() for t in ins]
+    ro, rlast = oracle(*rins, cu.tolist(), s0)
+    want = torch.autograd.grad((ro * do.double()).sum(), rins[3:])
+    for name, a, b in (("last", last, rlast), ("dg", got[0], want[0]), ("dbeta", got[1], want[1])):
+        assert rel(a, b) < 2.0 ** -19, (name, rel(a, b))
+
+
 @pytest.mark.parametrize("hk,hv", [(1, 1), (3, 3), (2, 6)])
 def test_gated_delta_rule_states_and_shared_heads(hk, hv):
     check([100, 0, 37], hk, hv, state=True, final=True)
@@ -685,3 +705,34 @@ def test_gated_delta_rule_gradients_of_strided_rows(dk, dv):
     whole = [t.detach().contiguous().requires_grad_() for t in cut(rows)]
     want = torch.autograd.grad(LA.gated_delta_rule(*whole, g, beta, cu_seqlens=cu), whole, up.contiguous())
     assert all(torch.equal(a, b) for a, b in zip(cut(got), want))
+
+
+def test_gated_delta_rule_without_gradients_gives_the_same_bits():
+    q, k, v, g, beta, _, cu = make([100, 0, 130], 2, 4, 128, 128, 16)
+    s0 = torch.randn(3, 4, 128, 128, device="cuda")
+    with torch.no_grad():
+        a = LA.gated_delta_rule(q, k, v, g, beta, cu_seqlens=cu, initial_state=s0, output_final_state=True)
+    b = LA.gated_delta_rule(q.requires_grad_(), k, v, g, beta, cu_seqlens=cu, initial_state=s0, output_final_state=True)
+    assert b[0].requires_grad and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_gated_delta_rule_does_not_read_what_memory_held():
+    """Another call's buffers, and buffers full of NaN, where this call's come to lie."""
+    q, k, v, g, beta, do, cu = make([1, 2, 63, 64, 65, 130], 2, 4, 128, 128, 17)
+    other = make([200, 125], 2, 4, 128, 128, 18)
+
+    def run(q, k, v, g, beta, do, cu):
+        ins = [t.detach().requires_grad_() for t in (q, k, v, g, beta)]
+        o, last = LA.gated_delta_rule(*ins, cu_seqlens=cu, output_final_state=True)
+        return [o.detach(), last.detach(), *torch.autograd.grad(o, ins, do)]
+
+    want = run(q, k, v, g, beta, do, cu)
+    run(*other)
+    got = run(q, k, v, g, beta, do, cu)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for fill in (float("nan"), 3e38):
+        del got
+        junk = [torch.full((n,), fill, device="cuda") for n in (1 << 25, 1 << 23, 1 << 21, 1 << 19, 1 << 17) * 3]
+        del junk
+        got = run(q, k, v, g, beta, do, cu)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -194,7 +194,9 @@ class GatedDeltaNet(nn.Module):
     @torch.no_grad()
     def prefill(self, x, cache, slots, *, cu_seqlens=None, residual=None):
         """`forward` over new sequences, one per entry of `slots` (bounds in `cu_seqlens`; None = one sequence); leaves
-        their windows and states in those slots of `cache`. The slots are read on the host: they must differ and exist."""
+        their windows and states in those slots of `cache`. The slots are read on the host: they must differ and exist.
+        Every sequence begins here: what a slot holds is replaced, not continued. A later part of a sequence goes through
+        `step`, token by token."""
         self._check_decoding()
         windows, states = cache
         slots = [int(i) for i in (slots.tolist() if torch.is_tensor(slots) else slots)]

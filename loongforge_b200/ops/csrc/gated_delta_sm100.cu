@@ -38,9 +38,9 @@
 //   gates     dg and dbeta.
 //
 // Precision. Sums and the state are fp32. An fp32 operand of a product is cut into bf16 parts: r, U and its scaled copy, dU
-// and P into three (24 bits), since they make up the results as they are; the state, A, dS1 and what is added to it, whose
-// remainder of 2^-18 goes through a decay first, into two; dQ and dK take two parts of everything, which is far below their
-// rounding. Products of parts below 2^-24 are left out. The third parts of P lie in the blocks of its tiles that no product
+// and P into three (24 bits), since they make up the results as they are; the state, A, dS1 and what is added to it into two:
+// a decay lies between what they leave out, 2^-18, and the results, which makes it small unless it is near one; and dQ and
+// dK take two parts of everything, which is far below their rounding. Products of parts below 2^-24 are left out. The third parts of P lie in the blocks of its tiles that no product
 // reads, those of r, U and dU in shared memory of their own; they cost 22 us forward and 12 backward of what stands below at
 // 4096 tokens. With the gates of a new layer states, dg and dbeta come out within 1e-7, 5e-7 and 1.4e-7 (2-norm; 2e-6 to 6e-6
 // with two parts everywhere), as with fp32 products; with decays of 1e-3 a token, within 2e-6, 4e-6 and 4e-6.

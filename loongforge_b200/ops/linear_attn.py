@@ -401,7 +401,9 @@ def _plain16(t):
 def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, cu_seqlens=None,
                   activation: Optional[str] = "silu") -> torch.Tensor:
     """Depthwise causal convolution over packed tokens. x [T, C]; weight [C, K]. Token t sees t-K+1..t of
-    its own sequence only. Rows that no sequence covers come back as zeros."""
+    its own sequence only: every sequence begins here, inputs of an earlier part of it are not taken. Rows that no sequence
+    covers come back as zeros. ``activation`` is "silu" ("swish") or None, others are refused, and so are boundaries on the
+    host that leave the rows or go back; those on a GPU are clamped."""
     _check_conv(x, weight, bias, activation)
     T, C = x.shape
     K = weight.shape[-1]

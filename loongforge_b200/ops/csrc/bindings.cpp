@@ -1094,9 +1094,9 @@ std::vector<at::Tensor> delta_bwd(const at::Tensor& dout, c10::optional<at::Tens
   at::Tensor dq = at::empty(q.sizes(), bf), dk = at::empty(k.sizes(), bf), dv = at::empty(v.sizes(), bf);
   at::Tensor dg = at::empty_like(g), dbeta = at::empty_like(beta);
   at::Tensor ds_in = want_ds ? at::empty({a.N, a.Hv, a.dk, a.dv}, fl) : at::empty({0}, fl);
-  // [NC, Hv] x: dstates bf16 [2, dv, dk], dv_lo bf16 [dv, 64], rowdots fp32 [dv / 16, 2, 64], sdots fp32 [dv / 16, 4], all
+  // [NC, Hv] x: dstates bf16 [2, dv, dk], dv_lo bf16 [dv, 64], rowdots fp32 [dv / 16, 3, 64], sdots fp32 [dv / 16, 4], all
   // multiples of 64 bytes
-  const int64_t heads = a.NC * a.Hv, sbytes = heads * 2 * a.dv * a.dk * 2, lbytes = heads * a.dv * 64 * 2, rbytes = heads * (a.dv / 16) * 2 * 64 * 4;
+  const int64_t heads = a.NC * a.Hv, sbytes = heads * 2 * a.dv * a.dk * 2, lbytes = heads * a.dv * 64 * 2, rbytes = heads * (a.dv / 16) * 3 * 64 * 4;
   at::Tensor work = at::empty({sbytes + lbytes + rbytes + heads * (a.dv / 16) * 4 * 4}, bf.dtype(at::kByte));
   char* base = static_cast<char*>(work.data_ptr());
   a.dout = dout.data_ptr();

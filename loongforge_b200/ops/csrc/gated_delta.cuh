@@ -15,6 +15,7 @@ constexpr int C = DELTA_CHUNK;
 
 // Rows of a chunk's factor block, 64 floats each.
 enum { V_YK = 0, V_BETA, V_OQ, V_SU, V_GHI, V_GLO, V_QS, V_RK, V_END, V_PD, V_RQ };  // V_PD: diagonal of P
+constexpr int ROW_DOTS = 3;  // sums over the columns that the backward chain leaves for every token, per unit: see there
 constexpr int SEQ_ROWS = V_PD + 1;  // rows that the kernels along the sequence read
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -77,6 +78,16 @@ __device__ __forceinline__ Span chunk_span(const DeltaArgs& a, long long c) {
   const long long left = a.cu[lo + 1] - s.start;
   s.len = left < C ? static_cast<int>(left) : C;
   return s;
+}
+
+// W_ii = qs_i rk_i do_i.u_i, without the decay that the rest of W carries: the largest part of dq and dk in heads that forget
+// at once. From the sums of the backward chain, so that it is as exact as U.
+__device__ __forceinline__ float w_diagonal(const DeltaArgs& a, long long rec, int i, const float* vec) {
+  const float* rd = a.rowdots + (rec * (a.dv / 16) * ROW_DOTS + 2) * 64 + i;
+  float s = 0.f;
+#pragma unroll 8
+  for (int v = 0; v < a.dv / 16; ++v) s += rd[v * ROW_DOTS * 64];
+  return vec[V_QS * 64 + i] * vec[V_RK * 64 + i] * s;
 }
 
 // Barriers between the warps of a block and of a buffer's copies. They complete in every chunk, so a wait ends unless the

@@ -3,25 +3,26 @@
 // One (chunk, value head) is five products with 128 rows and 128 columns in TMEM. Tokens are rows, 0-63 for dq and
 // 64-127 for dk (or for what leads there):
 //
-//   D3 = [dO; dV] [U; u]^T + [0; v] [U; u]^T        -> W = lower(dO U^T) D and N = -strict_lower(dV U^T) D, in two parts each
+//   D3 = [dO; dV] [U; u]^T + [0; v] [U; u]^T        -> W = strict_lower(dO U^T) D and N = -strict_lower(dV U^T) D, in two parts each
 //   D1 = [dO; dV] (S0 + s0)^T + [0; v] S0^T         -> dq += e^G (.), dk -= e^G (.)
 //   D2 = [  ; U] (dS1 + ds1)^T + [  ; u] dS1^T      -> dk += e^{G_C - G} (.)
 //   D4 = [W; N] K + [0; W^T] Q + [0; N^T] K         -> dq += , dk +=
 //
 // with capitals for the bf16 high parts and v, u, s0, ds1 for what they leave of dV, U and the states; products of two such
-// remainders are left out (2^-18 of the term). Rows are scaled when the accumulators are read, so that every operand is a
+// remainders are left out (2^-18 of the term). The diagonal of W comes from the backward chain and is added to the rows in
+// fp32 at the end. Rows are scaled when the accumulators are read, so that every operand is a
 // bf16 tile as it lies in memory. An operand tile whose first 64 rows are not wanted starts 64 rows early: what lies there
 // ends in rows of D2 that nobody reads; where they have to be zeros, v, W and N lie columns first, so that their first 64
 // rows can come from a tile of zeros elsewhere.
 //
 // 208 KB a (chunk, value head) come in, 128 of them the two states in two parts each, and 48 a (chunk, key head): about
-// 290 us at 16384 tokens, 16 key and 32 value heads, where the kernel takes 520 (138 at 4096). With the high parts of S0, dS1
+// 290 us at 16384 tokens, 16 key and 32 value heads, where the kernel takes 540 (144 at 4096). With the high parts of S0, dS1
 // and dV alone it took 358 (97), and dq and dk were off by 2.4e-3 where decays are near one, instead of the 1.66e-3 of their
 // rounding. One block per SM goes through its share of (chunk, key head) pairs; seven warps bring tiles (fragments of
 // registers, turned by stmatrix on the way), one thread issues the products, eight warps make W and N, and add up rows over
 // the value heads of a key head. The tiles fill shared memory: a state's low part takes the place of its high part when the
 // products have read that, and a unit's loads begin when its predecessor's products are done. What bounds it are these two
-// rounds of loads, which alternate with the products: 18K cycles a unit.
+// rounds of loads, which alternate with the products: 19K cycles a unit.
 #include <atomic>
 #include "gated_delta.cuh"
 #include "sm100_ptx.cuh"
@@ -171,15 +172,14 @@ tc_dqk_kernel(const DeltaArgs a) {
       float acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = 0.f;
-      float norm = 1.f;
+      float norm = 1.f, wd = 0.f;  // wd: the diagonal of W in the thread's row
       for (int hr = 0; hr < rep; ++hr, ++u) {
         const float* vec = sm.vec[u & 1];
-        // W_ij = qs_i rk_j D_ij (dO U^T)_ij for i >= j, N_ij = -rk_i rk_j D_ij (dV U^T)_ij for i > j
+        // W_ij = qs_i rk_j D_ij (dO U^T)_ij, N_ij = -rk_i rk_j D_ij (dV U^T)_ij, i > j
         bar_wait(&sm.d3_done, u & 1, a.status);
         tc_fence_after_sync();
         const float gh = vec[V_GHI * 64 + tok], gl = vec[V_GLO * 64 + tok];
         const float f = key ? -vec[V_RK * 64 + tok] : vec[V_QS * 64 + tok];
-        const int last = key ? tok - 1 : tok;  // the last column that counts
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           // element by element the chain of latencies is long: sixteen at a time, made everywhere and selected at the end
@@ -202,7 +202,7 @@ tc_dqk_kernel(const DeltaArgs a) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             e[j] *= x[j] + __uint_as_float(y[j]);
-            e[j] = j0 + j <= last ? e[j] : 0.f;
+            e[j] = j0 + j < tok ? e[j] : 0.f;
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) split2(e[2 * j], e[2 * j + 1], ph[j], pl[j]);
@@ -216,6 +216,7 @@ tc_dqk_kernel(const DeltaArgs a) {
         fence_proxy_async_smem();
         tc_fence_before_sync();
         bar_arrive(&sm.w_ready);
+        wd += w_diagonal(a, static_cast<long long>(c) * a.Hv + hk * rep + hr, tok, vec);
         // the rows, scaled; D1 and D2 while D4 is under way
         const float f1 = key ? -vec[V_YK * 64 + tok] : vec[V_OQ * 64 + tok], f2 = vec[V_SU * 64 + tok];
         norm = vec[(key ? V_RK : V_RQ) * 64 + tok];
@@ -249,8 +250,18 @@ tc_dqk_kernel(const DeltaArgs a) {
         }
       }
       // The rows are r dq^ and r dk^ with r = 1 / norm, so that dq = r dq^ - q r^2 (q . r dq^), the same for k.
-      const unsigned char* tile = key ? sm.k : sm.q;
+      const unsigned char *tile = key ? sm.k : sm.q, *other = key ? sm.q : sm.k;
       bar_wait(&sm.qk_full, i & 1, a.status);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint4 y = *reinterpret_cast<const uint4*>(other + half * BOX + piece_at(tok, j));
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[8 * j + 2 * e] += wd * lo_half(w[e]);
+          acc[8 * j + 2 * e + 1] += wd * hi_half(w[e]);
+        }
+      }
       uint4 x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const uint4*>(tile + half * BOX + piece_at(tok, j));

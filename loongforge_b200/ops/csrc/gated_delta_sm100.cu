@@ -10,7 +10,7 @@
 //
 //   X = A^T (P^T dO + diag(e^{G_C - G}) K dS1),   dV = diag(beta) X,   dbeta = (X . U) / beta
 //   dS0 = e^{G_C} dS1 + Q^T diag(e^G) dO - K^T diag(e^G) dV
-//   dQ = diag(e^G) dO S0^T + W K,   W = lower(dO U^T) D
+//   dQ = diag(e^G) dO S0^T + W K,   W = lower(dO U^T) D   (its diagonal, do_i.u_i, apart and in fp32)
 //   dK = -diag(e^G) dV S0^T + diag(e^{G_C - G}) U dS1^T + W^T Q + (N + N^T) K,   N = -strict_lower(dV U^T) D
 //
 // The gradient of a log decay g_t gathers what every token or state in front of t gives to every token or state from t
@@ -40,16 +40,15 @@
 // Precision. Sums and the state are fp32. An fp32 operand of a product is cut into bf16 parts: r, U and its scaled copy, dU
 // and P into three (24 bits), since they make up the results as they are; the state, A, dS1 and what is added to it into two:
 // a decay lies between what they leave out, 2^-18, and the results, which makes it small unless it is near one; and dQ and
-// dK take two parts of everything, which is far below their rounding. Products of parts below 2^-24 are left out. The third parts of P lie in the blocks of its tiles that no product
-// reads, those of r, U and dU in shared memory of their own; they cost 22 us forward and 12 backward of what stands below at
-// 4096 tokens. With the gates of a new layer states, dg and dbeta come out within 1e-7, 5e-7 and 1.4e-7 (2-norm; 2e-6 to 6e-6
+// dK take two parts of everything but the diagonal of W, which is far below their rounding. Products of parts below 2^-24 are left out. The third parts of P lie in the blocks of its tiles that no product
+// reads, those of r, U and dU in shared memory of their own; they cost 22 us forward of what stands below at 4096 tokens. With the gates of a new layer states, dg and dbeta come out within 1e-7, 5e-7 and 1.4e-7 (2-norm; 2e-6 to 6e-6
 // with two parts everywhere), as with fp32 products; with decays of 1e-3 a token, within 2e-6, 4e-6 and 4e-6.
 //
 // The chain is bound by latency: three dependent products of at most 64 x 128 x 16 per chunk, with a hand-over between
 // them, 6.5K cycles a chunk forward and 8K backward. mma.sync runs at a quarter of tcgen05's rate, but operands and results
 // stay in registers, and 32 heads make 1024 warps of such work. One sequence of 4096 tokens with 32 heads of 128 x 128 (five
-// sequences of 16384): prepare 39 us (137), forward 212 (750), backward 270 (920; 238 and 826 without the low parts
-// that dqk reads), dqk 138 (520), gates 8 (16). Measured against it: a whole unit in one warp 471 (959) forward and 620
+// sequences of 16384): prepare 39 us (137), forward 212 (740), backward 261 (886; 238 and 826 without the low
+// parts that dqk reads and the third ones), dqk 144 (540), gates 8 (16). Measured against it: a whole unit in one warp 471 (959) forward and 620
 // (1278) backward; eight warps along the chain and eight beside it 208 (713) and 257 (874), bound by shared memory; a head
 // as one 128-column product on tcgen05 11.7K cycles a chunk, 5K of them the work on elements between the products, on an
 // eighth as many blocks.
@@ -1202,8 +1201,8 @@ backward_kernel(const DeltaArgs a) {
       }
     add_to(y, z);
     add_to(u, y);
-    // X = u + (diag P dO)^T, dV = beta X; row sums over the unit's 16 columns: past . dO - m . dV - U . u, and U . X
-    float d[2][4];
+    // X = u + (diag P dO)^T, dV = beta X; row sums over the unit's 16 columns: past . dO - m . dV - U . u, U . X and U . dO
+    float d[ROW_DOTS][4];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
       d[0][2 * f] = -(uu[f][0] * u[f][0] + uu[f][2] * u[f][2]);
@@ -1229,6 +1228,8 @@ backward_kernel(const DeltaArgs a) {
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
       const float* past = reinterpret_cast<const float*>(&now.past[f]);
+      d[2][2 * f] = uu[f][0] * lo_half(fo[2 * f]) + uu[f][2] * lo_half(fo[2 * f + 1]);
+      d[2][2 * f + 1] = uu[f][1] * hi_half(fo[2 * f]) + uu[f][3] * hi_half(fo[2 * f + 1]);
       d[0][2 * f] += past[0] * lo_half(fo[2 * f]) + past[2] * lo_half(fo[2 * f + 1]) - (mm[f][0] * u[f][0] + mm[f][2] * u[f][2]);
       d[0][2 * f + 1] += past[1] * hi_half(fo[2 * f]) + past[3] * hi_half(fo[2 * f + 1]) - (mm[f][1] * u[f][1] + mm[f][3] * u[f][3]);
     }
@@ -1278,9 +1279,9 @@ backward_kernel(const DeltaArgs a) {
       split_a(u[0], u[1], hi, lo);
       reinterpret_cast<uint4*>(a.dv_lo)[((rec * VT + vt) * 4 + w) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
-    float* rd = a.rowdots + (rec * VT + vt) * 128 + tok + t2;
+    float* rd = a.rowdots + (rec * VT + vt) * ROW_DOTS * 64 + tok + t2;
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+    for (int q = 0; q < ROW_DOTS; ++q)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float r = d[q][e];
@@ -1377,6 +1378,7 @@ dqk_kernel(const DeltaArgs a) {
   for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) dq[j][e] = dk[j][e] = 0.f;
+  float wd[2] = {0.f, 0.f};  // diagonal of W in the thread's rows
   for (int hr = 0; hr < rep; ++hr) {
     const int h = hk * rep + hr;
     const long long rec = c * a.Hv + h;
@@ -1428,10 +1430,10 @@ dqk_kernel(const DeltaArgs a) {
       for (int e = 0; e < 4; ++e) {
         const int i = r0 + 8 * (e >> 1), jj = wn * 32 + j * 8 + t2 + (e & 1);
         float w1 = 0.f, w2 = 0.f;
-        if (i >= jj) {
+        if (i > jj) {
           const float d = x.vec[V_RK * 64 + jj] * __expf((x.vec[V_GHI * 64 + i] - x.vec[V_GHI * 64 + jj]) + (x.vec[V_GLO * 64 + i] - x.vec[V_GLO * 64 + jj]));
           w1 = x.vec[V_QS * 64 + i] * d * p[j][e];
-          if (i > jj) w2 = -x.vec[V_RK * 64 + i] * d * nn[j][e];
+          w2 = -x.vec[V_RK * 64 + i] * d * nn[j][e];
         }
         const bf16 w1h = __float2bfloat16(w1);
         x.w1[i * APITCH + jj] = w1h;
@@ -1443,6 +1445,8 @@ dqk_kernel(const DeltaArgs a) {
         }
       }
     }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) wd[e] += w_diagonal(a, rec, r0 + 8 * e, x.vec);
     // the products with the states: rows scaled afterwards
     float t[NT][4];
     auto clear = [&]() {
@@ -1521,6 +1525,17 @@ dqk_kernel(const DeltaArgs a) {
     }
   }
   __syncthreads();
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int at = (r0 + 8 * e) * P + n0 + 8 * j + t2;
+      const uint32_t kw = *reinterpret_cast<const uint32_t*>(x.k + at), qw = *reinterpret_cast<const uint32_t*>(x.q + at);
+      dq[j][2 * e] += wd[e] * lo_half(kw);
+      dq[j][2 * e + 1] += wd[e] * hi_half(kw);
+      dk[j][2 * e] += wd[e] * lo_half(qw);
+      dk[j][2 * e + 1] += wd[e] * hi_half(qw);
+    }
   // The accumulators hold r dq^ and r dk^ with r = 1 / norm, so that dq = r dq^ - q r^2 (q . r dq^), the same for k.
   auto finish = [&](float(&acc)[NT][4], bf16* tile, int which, const float* r) {
     if (a.l2norm) {
@@ -1590,7 +1605,7 @@ gates_kernel(const DeltaArgs a) {
   const Span sp = chunk_span(a, c);
   if (sp.len == 0) return;
   const int lane = threadIdx.x & 31, VT = a.dv / 16;
-  const float* rd = a.rowdots + rec * VT * 128;
+  const float* rd = a.rowdots + rec * VT * ROW_DOTS * 64;
   double carry = lane < 4 * VT ? a.sdots[rec * 4 * VT + lane] : 0.f;  // dv / 4 <= 32 of them
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) carry += __shfl_xor_sync(0xffffffffu, carry, o);
@@ -1599,8 +1614,8 @@ gates_kernel(const DeltaArgs a) {
     const int i = half * 32 + lane;
     double s = 0.0, xu = 0.0;
     for (int v = 0; v < VT; ++v) {
-      s += rd[v * 128 + i];
-      xu += rd[v * 128 + 64 + i];
+      s += rd[v * ROW_DOTS * 64 + i];
+      xu += rd[(v * ROW_DOTS + 1) * 64 + i];
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

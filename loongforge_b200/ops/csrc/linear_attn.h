@@ -36,7 +36,7 @@ struct DeltaArgs {
   float* ds_in = nullptr;         // gradient of s_in or null
   void* dstates = nullptr;      // the gradients of the states behind every chunk, as `states`
   void* dv_lo = nullptr;        // what the rounding of dv_ left, in bf16: fragments of half the size of `u`
-  float* rowdots = nullptr;     // fp32 [NC, Hv, dv / 16, 2, 64]
+  float* rowdots = nullptr;     // fp32 [NC, Hv, dv / 16, 3, 64]
   float* sdots = nullptr;       // fp32 [NC, Hv, dv / 16, 4]
   void *dq = nullptr, *dkey = nullptr, *dv_ = nullptr;  // bf16, contiguous
   float *dg = nullptr, *dbeta = nullptr;                // fp32 [T, Hv]

@@ -232,7 +232,7 @@ def gated_delta_rule(q, k, v, g, beta, *, cu_seqlens=None, scale: Optional[float
     as zero there. Memory goes by chunks, each of up to 64 tokens of ONE sequence: they are taken as ``T / 64 + N``, so that
     many short sequences cost more than their tokens. A chunk takes 39,680 bytes a value head and ``256 (dk + 8)`` a key
     head while the call runs; with gradients enabled these and ``768 dv + 4 dk dv`` bytes a value head (partial results and
-    two states) are kept until the backward pass, which itself works on ``4 dk dv + 161 dv`` more. With 16 / 32 heads of 128
+    two states) are kept until the backward pass, which itself works on ``4 dk dv + 177 dv`` more. With 16 / 32 heads of 128
     that is 7 MB a chunk: 1.8 GB for one row of 16,384 tokens, 29 GB for 4,096 sequences of one token.
 
     Precision there: sums and the state along the sequence are fp32; the products take bf16 inputs as they are, and of fp32

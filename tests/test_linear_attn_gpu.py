@@ -145,6 +145,26 @@ def test_gated_delta_rule_fp32_results_with_the_gates_of_a_new_layer(dk, dv):
         assert rel(a, b) < 2.0 ** -19, (name, rel(a, b))
 
 
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128)])
+def test_gated_delta_rule_bf16_results_are_the_rounded_values(dk, dv):
+    """With the gates of a new layer the part of a result that no decay has made small keeps 24 bits, and the rest is off by
+    2^-18 of a part that counts half at most: a result lies that near to a border between two bf16 values, 2^-8 apart, with
+    a chance of 2^-10 at most, counted half since the values spread over twice their lowest. dq and dk add heads and take
+    the norm's part off, each of the same kind."""
+    gen = torch.Generator(device="cuda").manual_seed(19)
+    q, k, v, _, _, do, cu = make([300, 64, 90], 2, 4, dk, dv, 19)
+    g = -torch.nn.functional.softplus(torch.randn(454, 4, generator=gen, device="cuda") + 1) * torch.tensor([4.0, 8.0, 12.0, 16.0], device="cuda")
+    ins = [t.requires_grad_() for t in (q, k, v, g, torch.rand(454, 4, generator=gen, device="cuda"))]
+    o = LA.gated_delta_rule(*ins, cu_seqlens=cu)
+    got = [o.detach(), *torch.autograd.grad(o, ins[:3], do)]
+    rins = [t.detach().double().requires_grad_() for t in ins]
+    ro, _ = oracle(*rins, cu.tolist())
+    want = [ro.detach(), *torch.autograd.grad((ro * do.double()).sum(), rins[:3])]
+    for name, a, b in zip(("o", "dq", "dk", "dv"), got, want):
+        other = (a != b.to(BF16)).double().mean().item()
+        assert other < 2.0 ** -11, (name, other * 2.0 ** 11)
+
+
 @pytest.mark.parametrize("hk,hv", [(1, 1), (3, 3), (2, 6)])
 def test_gated_delta_rule_states_and_shared_heads(hk, hv):
     check([100, 0, 37], hk, hv, state=True, final=True)

@@ -6,8 +6,8 @@
 //
 // Bound by memory: x is read and y written once. A thread owns a few neighbouring channels and walks down the tokens
 // with the window in registers, so every row is read once plus a halo of K - 1 rows per block of tokens.
-// 16384 x 8192: forward 96 us (5.6 TB/s), backward 175 us (4.6 TB/s, 60 % of the issue slots) + 7 for dw; 2047 x 6144: 15,
-// 25 and 3 us.
+// 16384 x 8192: forward 98 us (5.5 TB/s), backward 180 us (4.5 TB/s, 60 % of the issue slots) + 7 for dw; 2047 x 6144: 15,
+// 24 and 3 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

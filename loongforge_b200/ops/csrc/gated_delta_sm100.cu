@@ -23,8 +23,8 @@
 // of their (small) gradient; that is why A and P are kept as strict lower parts, their diagonals apart: o~, m and x~ are
 // sums of their own, never differences of larger numbers. That does not hold for a single reset among mild decays: a pair
 // j < i of tokens that both lie behind t enters dg_t once through o~_i and m_i and once, negated, through x~_j, and neither
-// carries g_t. What is left of such a dg_t is the rounding of its neighbours' terms (2e-6 where they are of order one; 4e-7
-// in fp32 throughout).
+// carries g_t. What is left of such a dg_t is the rounding of its neighbours' terms (3e-7 where they are of order one, as
+// with fp32 products).
 //
 // Kernels:
 //   prepare   one block per (chunk, key head): Q K^T and K K^T once, then A, P and the per-token factors of each of its
@@ -40,18 +40,20 @@
 // Precision. Sums and the state are fp32. An fp32 operand of a product is cut into bf16 parts: r, U and its scaled copy, dU
 // and P into three (24 bits), since they make up the results as they are; the state, A, dS1 and what is added to it into two:
 // a decay lies between what they leave out, 2^-18, and the results, which makes it small unless it is near one; and dQ and
-// dK take two parts of everything but the diagonal of W, which is far below their rounding. Products of parts below 2^-24 are left out. The third parts of P lie in the blocks of its tiles that no product
-// reads, those of r, U and dU in shared memory of their own; they cost 22 us forward of what stands below at 4096 tokens. With the gates of a new layer states, dg and dbeta come out within 1e-7, 5e-7 and 1.4e-7 (2-norm; 2e-6 to 6e-6
-// with two parts everywhere), as with fp32 products; with decays of 1e-3 a token, within 2e-6, 4e-6 and 4e-6.
+// dK take two parts of everything but the diagonal of W, which is far below their rounding. Products of parts below 2^-24
+// are left out. The third parts of P lie in the blocks of its tiles that no product reads, those of r, U and dU in shared
+// memory of their own; they cost 22 us forward of what stands below at 4096 tokens. With the gates of a new layer states, dg
+// and dbeta come out within 1e-7, 5e-7 and 1.4e-7 (2-norm; 2e-6 to 6e-6 with two parts everywhere), as with fp32 products;
+// with decays of 1e-3 a token, within 2e-6, 4e-6 and 4e-6.
 //
 // The chain is bound by latency: three dependent products of at most 64 x 128 x 16 per chunk, with a hand-over between
 // them, 6.5K cycles a chunk forward and 8K backward. mma.sync runs at a quarter of tcgen05's rate, but operands and results
 // stay in registers, and 32 heads make 1024 warps of such work. One sequence of 4096 tokens with 32 heads of 128 x 128 (five
-// sequences of 16384): prepare 39 us (137), forward 212 (740), backward 261 (886; 238 and 826 without the low
-// parts that dqk reads and the third ones), dqk 144 (540), gates 8 (16). Measured against it: a whole unit in one warp 471 (959) forward and 620
-// (1278) backward; eight warps along the chain and eight beside it 208 (713) and 257 (874), bound by shared memory; a head
-// as one 128-column product on tcgen05 11.7K cycles a chunk, 5K of them the work on elements between the products, on an
-// eighth as many blocks.
+// sequences of 16384): prepare 39 us (137), forward 212 (740), backward 261 (886), dqk 144 (540), gates 8 (16); 190 (656)
+// and 238 (826) before the third parts and the low ones that dqk reads. Measured against that: a whole unit in one warp 471
+// (959) forward and 620 (1278) backward; eight warps along the chain and eight beside it 208 (713) and 257 (874), bound by
+// shared memory; a head as one 128-column product on tcgen05 11.7K cycles a chunk, 5K of them the work on elements between
+// the products, on an eighth as many blocks.
 #include "gated_delta.cuh"
 
 namespace lf {

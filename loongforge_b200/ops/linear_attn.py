@@ -111,8 +111,10 @@ class _GatedDeltaFn(torch.autograd.Function):
     def forward(ctx, q, k, v, g, beta, s_in, cu, scale, l2norm, want_state, keep):
         ctx.set_materialize_grads(False)
         C, status = _ext.require(), _status(v)
-        inputs = tuple(t if need else None for t, need in zip((q, k, v, g, beta, s_in), ctx.needs_input_grad))
+        inputs = (q, k, v, g, beta, s_in)
         q, k, v, gf, bf = _rows16(q), _rows16(k), _rows16(v), _fp32(g), _fp32(beta)
+        # what has a gradient and is not saved as it is below: see first_order
+        inputs = tuple(t if need and t is not x else None for t, x, need in zip(inputs, (q, k, v, gf, bf, None), ctx.needs_input_grad))
         bounds, first = (None, None) if cu is None else C.delta_plan(cu, q.shape[0], status)
         o, s_out, kept = C.delta_fwd(q, k, v, gf, bf, bounds, first, scale, l2norm, s_in, want_state, keep, status)
         if keep:
@@ -133,7 +135,7 @@ class _GatedDeltaFn(torch.autograd.Function):
             do, None if ds_out is None else _dense16(ds_out), q, k, v, g, beta, bounds, first, scale, l2norm, want_ds, kept,
             _status(v))
         grads = (dq, dk, dv, dg.to(g_dtype), dbeta.to(beta_dtype), ds_in if want_ds else None)
-        return first_order("gated_delta_rule", grads, *up, *inputs) + (None,) * 5
+        return first_order("gated_delta_rule", grads, *up, *inputs, q, k, v) + (None,) * 5
 
 
 def _status(t: torch.Tensor) -> torch.Tensor:

@@ -44,3 +44,15 @@ def test_rows_for_the_kernels_have_strides_of_whole_16_byte_pieces():
         assert torch.equal(r, t) and r.stride(-1) == 1 and all(s % 8 == 0 for s in r.stride()[:-1]) and r.data_ptr() % 16 == 0
     even = torch.randn(4, 72).bfloat16()[:, :64]
     assert LA._rows16(even) is even
+
+
+def test_inputs_are_saved_once(monkeypatch):
+    """What offloads saved tensors moves each of them as often as it is saved."""
+    fake = SimpleNamespace(delta_fwd=lambda q, k, v, *a: (v.clone(), torch.zeros(0), torch.zeros(1)))
+    monkeypatch.setattr(_ext, "require", lambda: fake)
+    monkeypatch.setattr(LA, "_status", lambda t: torch.zeros(1, dtype=torch.int32))
+    q, k, v = (torch.randn(6, 1, 8, requires_grad=True) for _ in range(3))
+    g, seen = torch.randn(6, 1, requires_grad=True), []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.data_ptr()) or t, lambda t: t):
+        LA._GatedDeltaFn.apply(q, k, v, g, g, None, None, 1.0, True, False, True)
+    assert [seen.count(t.data_ptr()) for t in (q, k, v)] == [1, 1, 1]

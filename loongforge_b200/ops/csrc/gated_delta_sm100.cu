@@ -44,7 +44,8 @@
 // are left out. The third parts of P lie in the blocks of its tiles that no product reads, those of r, U and dU in shared
 // memory of their own; they cost 22 us forward of what stands below at 4096 tokens. With the gates of a new layer states, dg
 // and dbeta come out within 1e-7, 5e-7 and 1.4e-7 (2-norm; 2e-6 to 6e-6 with two parts everywhere), as with fp32 products;
-// with decays of 1e-3 a token, within 2e-6, 4e-6 and 4e-6.
+// with decays of 1e-3 a token, within 2e-6, 4e-6 and 4e-6. Exponentials are the fast ones: 2^-22 of a decay near one, and
+// 2^-20 of e^-10.
 //
 // The chain is bound by latency: three dependent products of at most 64 x 128 x 16 per chunk, with a hand-over between
 // them, 6.5K cycles a chunk forward and 8K backward. mma.sync runs at a quarter of tcgen05's rate, but operands and results

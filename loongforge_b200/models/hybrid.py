@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import math
 import zlib
+from operator import index
 from typing import Optional
 
 import torch
@@ -199,7 +200,7 @@ class GatedDeltaNet(nn.Module):
         `step`, token by token."""
         self._check_decoding()
         windows, states = cache
-        slots = [int(i) for i in (slots.tolist() if torch.is_tensor(slots) else slots)]
+        slots = [index(i) for i in (slots.tolist() if torch.is_tensor(slots) else slots)]
         n = 1 if cu_seqlens is None else len(cu_seqlens) - 1
         if len(slots) != n:
             raise ValueError(f"{n} sequences need as many slots, got {len(slots)}")

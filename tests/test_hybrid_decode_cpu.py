@@ -81,3 +81,12 @@ def test_gated_attention_and_mrope_inputs_agree_on_the_angles():
         r = RotaryEmbedding(cfg, 16).mrope(torch.randint(0, 1000, (3, 20)))
         ang = r.axis_pos.double()[r.axis.long()].t() * r.inv_freq.double()
         assert torch.allclose(ang.float(), r.freqs, rtol=2.0 ** -23, atol=0)
+
+
+def test_prefill_refuses_slots_that_are_not_whole():
+    cfg, net = layer()
+    cache = net.new_cache(4)
+    for slots in ([0, 1.5], torch.tensor([0.0, 1.0])):
+        with pytest.raises(TypeError):
+            net.prefill(torch.randn(8, cfg.hidden_size), cache, slots, cu_seqlens=[0, 3, 8])
+    assert not cache[0].any() and not cache[1].any()
